@@ -238,9 +238,16 @@ hipError_t launch_large(int v, int dtype, bool gated, fsw::GemmArgs& a, hipStrea
 
 }  // namespace
 
+namespace fsw {
+
+int device_status() { return check_device(); }
+int launch_status(hipError_t e) { return finish(e); }
+
+}  // namespace fsw
+
 extern "C" {
 
-int fsw_version(void) { return 2000; }
+int fsw_version(void) { return 2001; }
 
 const char* fsw_strerror(int code) {
   switch (code) {

@@ -144,3 +144,12 @@ hipError_t launch_decode_mlp(int dtype, const DecodeArgs& a, hipStream_t stream,
 hipError_t decode_barrier_failures(int* count);
 
 }  // namespace fsw
+
+namespace fsw {
+
+// For entry points outside fsw_api.hip: FSW_OK or FSW_E_DEVICE for the current device; FSW_OK or FSW_E_LAUNCH, keeping the
+// error for fsw_last_hip_error.
+int device_status();
+int launch_status(hipError_t e);
+
+}  // namespace fsw

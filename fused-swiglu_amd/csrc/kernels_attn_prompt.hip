@@ -1,0 +1,307 @@
+// Causal attention of packed prompts: o_i = sum_j p_ij v_j / sum_j p_ij, p_ij = 2^(c s_ij - c m_i), s = q k^T, in one pass
+// over the keys with a running maximum m and running sums (fp32).
+//
+// A workgroup owns BM rows of one sequence and key-value head. A row is a (token, query head of the group) pair: the group's heads of a token are
+// neighbouring rows, so they share the keys and values that the workgroup copies to LDS, short prompts fill their tiles, and the
+// triangle's edge cuts fewer tiles. Four waves own 32 NQ rows each and walk the same tiles of 64 keys.
+// The score tile is computed transposed, S^T = K Q^T (v_mfma_f32_32x32x16): lane l holds query row l % 32 and, of 32 keys, 8 (r / 4) + 4
+// (l / 32) + r % 4 in register r, so a row's maximum and sum are in-lane sums and one exchange with lane l ^ 32, and
+// eight registers in a row, rounded to the element type, are the B operand of O^T = V^T P^T if its 16 keys are numbered {4 h .. 4 h + 3, 8 + 4 h .. 8 + 4 h + 3}
+// (h = l / 32). The A operand has V's channels as rows and the same order of keys: two transposing reads of 4 keys x 16
+// channels (ds_read_b64_tr_b16) deliver it from V as it lies.
+#include "attn.h"
+#include "fsw_device.h"
+#include "fsw_internal.h"
+
+namespace fsw {
+namespace {
+
+typedef __attribute__((ext_vector_type(16))) float f32x16;
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+typedef __attribute__((address_space(3))) void lds_void;
+typedef __attribute__((address_space(3))) unsigned char lds_byte;
+
+constexpr float NEG_INF = -__builtin_inff();
+constexpr float SLACK = 8.0f;  // the maximum moves only when a score passes it by this much (powers of two): p < 2^8
+constexpr int KEYS = 64;
+
+template <class T>
+__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c);
+template <>
+__device__ __forceinline__ f32x16 mfma32<Bf16>(u32x4 a, u32x4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+template <>
+__device__ __forceinline__ f32x16 mfma32<Fp16>(u32x4 a, u32x4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+// c + lo + hi of a packed pair
+template <class T>
+__device__ __forceinline__ float add2(unsigned p, float c);
+template <>
+__device__ __forceinline__ float add2<Bf16>(unsigned p, float c) {
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, p), __builtin_bit_cast(bf16x2, 0x3f803f80u), c, false);
+}
+template <>
+__device__ __forceinline__ float add2<Fp16>(unsigned p, float c) {
+  return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, p), __builtin_bit_cast(f16x2, 0x3c003c00u), c, false);
+}
+
+__device__ __forceinline__ u32x2 read_tr(const unsigned char* p) {
+  return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
+}
+
+// Position of 16-byte vector c of key row `key` in its LDS row: the 16 rows of a K fragment read, and the 4 rows x 64
+// bytes that a half wave of a transposing V read covers, each fall on all 64 banks once.
+template <int DP>
+__device__ __forceinline__ int k_swizzle(int key) {
+  return DP == 64 ? (key >> 1) & 7 : key & 15;
+}
+template <int DP>
+__device__ __forceinline__ int v_swizzle(int key) {
+  return DP == 64 ? ((key >> 1) & 1) << 2 : (key & 3) << 2;
+}
+
+template <class T, int DP, int NQ>
+__global__ __launch_bounds__(256, 1) void attn_prompt_kernel(PromptArgs a, int slots) {
+  constexpr int RB = DP * 2, TILE = KEYS * RB, LOADS = TILE / 4096;  // copies per wave and tile
+  constexpr int KSTEPS = DP / 16, DB = DP / 32, BM = 128 * NQ;
+  __shared__ __align__(1024) unsigned char k0s[TILE];
+  __shared__ __align__(1024) unsigned char k1s[TILE];
+  __shared__ __align__(1024) unsigned char v0s[TILE];
+  __shared__ __align__(1024) unsigned char v1s[TILE];
+
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int col = lane & 31, half = lane >> 5;
+  const int kvh = (int)blockIdx.x % a.hkv, slot = slots - 1 - (int)blockIdx.x / a.hkv;
+  const int group = a.hq / a.hkv;
+
+  // Sequence s owns the slots from rows_before(s) / BM + s on, which leaves it enough for its rows whatever their remainder; slot -> s by
+  // a search of 64 entries at a time. Entry a.seqs is the rows behind the last sequence.
+  auto start_q = [&](int s) -> int {
+    const int x = a.cu_q[s];
+    return x < 0 ? 0 : x > a.tq ? a.tq : x;
+  };
+  auto base = [&](int s) -> int { return (int)((long long)start_q(s) * group / BM) + s; };
+  int seq = 0;
+  for (int n = a.seqs + 1; n > 1;) {
+    const int step = (n + 63) / 64, idx = lane * step;
+    const int below = __popcll(__ballot(idx < n && base(seq + (idx < n ? idx : 0)) <= slot));
+    const int skip = (below > 0 ? below - 1 : 0) * step;
+    seq += skip;
+    n = n - skip < step ? n - skip : step;
+  }
+  seq = __builtin_amdgcn_readfirstlane(seq);
+  const int tile = slot - __builtin_amdgcn_readfirstlane(base(seq));
+  const bool behind = seq == a.seqs;
+  const int q_at = start_q(seq), q_to = behind ? a.tq : start_q(seq + 1);
+  const int nq = q_to > q_at ? q_to - q_at : 0;
+  int k_at = 0, nk = 0;
+  if (!behind) {
+    const int x = a.cu_k[seq], y = a.cu_k[seq + 1];
+    k_at = x < 0 ? 0 : x > a.tk ? a.tk : x;
+    const int k_to = y < 0 ? 0 : y > a.tk ? a.tk : y;
+    nk = k_to > k_at ? k_to - k_at : 0;
+  }
+  const int rows = __builtin_amdgcn_readfirstlane(nq) * group;  // <= 2^30: at most 2^20 tokens of 1024 heads
+  const int row0 = tile * BM;
+  if (tile < 0 || row0 >= rows) return;
+  k_at = __builtin_amdgcn_readfirstlane(k_at);
+  nk = __builtin_amdgcn_readfirstlane(nk);
+  const int shift = nk - __builtin_amdgcn_readfirstlane(nq) + 1;
+  // keys that a row sees
+  auto sees = [&](int row) -> int {
+    const int v = (row < rows ? row : rows - 1) / group + shift;
+    return v < 0 ? 0 : v < nk ? v : nk;
+  };
+  const int wrow = row0 + wave * 32 * NQ;
+  const int block_keys = sees(row0 + BM - 1);
+  int vis[NQ];
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) vis[n] = sees(wrow + 32 * n + col);
+  const int wave_first = __builtin_amdgcn_readfirstlane(sees(wrow));
+  const int wave_last = __builtin_amdgcn_readfirstlane(sees(wrow + 32 * NQ - 1));
+
+  u32x4 qf[NQ][KSTEPS];
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    const int row = wrow + 32 * n + col < rows ? wrow + 32 * n + col : rows - 1;
+    const int token = row / group;
+    const unsigned short* p = (const unsigned short*)a.q.p + (q_at + token) * a.q.token +
+                              (long long)(kvh * group + row - token * group) * a.q.head;
+#pragma unroll
+    for (int s = 0; s < KSTEPS; ++s) {
+      const int ch = s * 16 + half * 8;
+      qf[n][s] = u32x4{0, 0, 0, 0};
+      if (ch < a.d) qf[n][s] = *(const u32x4*)(p + ch);
+    }
+  }
+
+  f32x16 o[DB][NQ];
+  float m[NQ], sum[NQ];
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    m[n] = NEG_INF;
+    sum[n] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < DB; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[i][n][r] = 0.0f;
+  }
+
+  // copies: lane -> 16 bytes of LDS, from the vector of the key row that belongs there
+  const unsigned char* kp = (const unsigned char*)a.k.p + (k_at * a.k.token + kvh * a.k.head) * 2;
+  const unsigned char* vp = (const unsigned char*)a.v.p + (k_at * a.v.token + kvh * a.v.head) * 2;
+  unsigned koff[LOADS], voff[LOADS];
+#pragma unroll
+  for (int j = 0; j < LOADS; ++j) {
+    const int byte = (j * 4 + wave) * 1024 + lane * 16, key = byte / RB, pos = (byte % RB) / 16;
+    const int kc = pos ^ k_swizzle<DP>(key), vc = pos ^ v_swizzle<DP>(key);
+    koff[j] = kc * 8 < a.d ? (unsigned)(key * (int)a.k.token * 2 + kc * 16) : OOB_OFFSET;
+    voff[j] = vc * 8 < a.d ? (unsigned)(key * (int)a.v.token * 2 + vc * 16) : OOB_OFFSET;
+  }
+  auto copy = [&](int at, unsigned char* ks, unsigned char* vs) {
+    const int left = nk - at < KEYS ? nk - at : KEYS;  // rows behind the sequence's end read as zero
+    const auto kr = make_rsrc(kp + at * a.k.token * 2, left > 0 ? (left - 1) * a.k.token * 2 + a.d * 2 : 0);
+    const auto vr = make_rsrc(vp + at * a.v.token * 2, left > 0 ? (left - 1) * a.v.token * 2 + a.d * 2 : 0);
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, (lds_void*)(ks + (j * 4 + wave) * 1024), 16, (int)koff[j], 0, 0, 0);
+#pragma unroll
+    for (int j = 0; j < LOADS; ++j)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, (lds_void*)(vs + (j * 4 + wave) * 1024), 16, (int)voff[j], 0, 0, 0);
+  };
+
+  const float c = a.scale_log2, slack = SLACK / c;
+  auto attend = [&](int at, const unsigned char* ks, const unsigned char* vs) {
+    if (at >= wave_last) return;
+    f32x16 s[2][NQ];
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+#pragma unroll
+      for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[kb][n][r] = 0.0f;
+      const int key = kb * 32 + col;
+#pragma unroll
+      for (int st = 0; st < KSTEPS; ++st) {
+        const u32x4 kf = *(const u32x4*)(ks + key * RB + ((2 * st + half) ^ k_swizzle<DP>(key)) * 16);
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) s[kb][n] = mfma32<T>(kf, qf[n][st], s[kb][n]);
+      }
+    }
+    if (at + KEYS > wave_first) {
+#pragma unroll
+      for (int n = 0; n < NQ; ++n) {
+        const int left = vis[n] - at - 4 * half;
+#pragma unroll
+        for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            if (kb * 32 + (r / 4) * 8 + r % 4 >= left) s[kb][n][r] = NEG_INF;
+      }
+    }
+    unsigned p[NQ][2][8];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+      float top = s[0][n][0];
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[kb][n][r]);
+      top = fmaxf(top, __shfl_xor(top, 32));
+      if (__any(top > m[n] + slack)) {
+        const float now = fmaxf(m[n], top);
+        const float alpha = now == m[n] ? 1.0f : __builtin_amdgcn_exp2f((m[n] - now) * c);
+        m[n] = now;
+        sum[n] *= alpha;
+#pragma unroll
+        for (int i = 0; i < DB; ++i)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[i][n][r] *= alpha;
+      }
+      const float mc = m[n] == NEG_INF ? 0.0f : m[n] * c;
+#pragma unroll
+      for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+        for (int r = 0; r < 16; r += 2) {
+          const float lo = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][n][r], c, -mc));
+          const float hi = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][n][r + 1], c, -mc));
+          p[n][kb][r / 2] = T::pack2(lo, hi);
+          sum[n] = add2<T>(p[n][kb][r / 2], sum[n]);
+        }
+    }
+    const int i16 = lane & 15, sub = (lane >> 4) & 1;
+#pragma unroll
+    for (int st = 0; st < 4; ++st) {
+#pragma unroll
+      for (int i = 0; i < DB; ++i) {
+        const int key = st * 16 + 4 * half + (i16 >> 2);
+        const int ch = i * 4 + sub * 2 + ((i16 & 3) >> 1);
+        const u32x2 lo = read_tr(vs + key * RB + (ch ^ v_swizzle<DP>(key)) * 16 + (i16 & 1) * 8);
+        const u32x2 hi = read_tr(vs + (key + 8) * RB + (ch ^ v_swizzle<DP>(key + 8)) * 16 + (i16 & 1) * 8);
+        const u32x4 vf = {lo[0], lo[1], hi[0], hi[1]};
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+          const unsigned* pp = &p[n][st >> 1][(st & 1) * 4];
+          o[i][n] = mfma32<T>(vf, u32x4{pp[0], pp[1], pp[2], pp[3]}, o[i][n]);
+        }
+      }
+    }
+  };
+
+  // tile t is in buffer t % 2; copies of tile t + 1 are under way while tile t is worked on
+  if (block_keys > 0) copy(0, k0s, v0s);
+  for (int at = 0; at < block_keys; at += 2 * KEYS) {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (at + KEYS < block_keys) copy(at + KEYS, k1s, v1s);
+    attend(at, k0s, v0s);
+    if (at + KEYS >= block_keys) break;
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (at + 2 * KEYS < block_keys) copy(at + 2 * KEYS, k0s, v0s);
+    attend(at + KEYS, k1s, v1s);
+  }
+
+#pragma unroll
+  for (int n = 0; n < NQ; ++n) {
+    const int row = wrow + 32 * n + col;
+    const float total = sum[n] + __shfl_xor(sum[n], 32);
+    if (row >= rows) continue;
+    const float inv = vis[n] > 0 ? 1.0f / total : 0.0f;
+    const int token = row / group;
+    unsigned short* p = (unsigned short*)a.o.p + (q_at + token) * a.o.token +
+                        (long long)(kvh * group + row - token * group) * a.o.head;
+#pragma unroll
+    for (int i = 0; i < DB; ++i)
+#pragma unroll
+      for (int r = 0; r < 16; r += 4) {
+        const int ch = i * 32 + (r / 4) * 8 + 4 * half;
+        if (ch < a.d)
+          *(u32x2*)(p + ch) = u32x2{T::pack2(o[i][n][r] * inv, o[i][n][r + 1] * inv),
+                                    T::pack2(o[i][n][r + 2] * inv, o[i][n][r + 3] * inv)};
+      }
+  }
+}
+
+template <class T, int DP, int NQ>
+hipError_t launch(const PromptArgs& a, hipStream_t stream) {
+  const long long rows = (long long)a.tq * (a.hq / a.hkv);
+  const long long slots = rows / (128 * NQ) + a.seqs + 1;
+  attn_prompt_kernel<T, DP, NQ><<<(unsigned)(slots * a.hkv), 256, 0, stream>>>(a, (int)slots);
+  return hipGetLastError();
+}
+
+template <class T>
+hipError_t launch_typed(const PromptArgs& a, hipStream_t stream) {
+  if (a.d <= 64) return launch<T, 64, 1>(a, stream);
+  if (a.d <= 128) return launch<T, 128, 1>(a, stream);
+  return launch<T, 256, 1>(a, stream);
+}
+
+}  // namespace
+
+hipError_t launch_attn_prompt(int dtype, const PromptArgs& a, hipStream_t stream) {
+  return dtype == FSW_BF16 ? launch_typed<Bf16>(a, stream) : launch_typed<Fp16>(a, stream);
+}
+
+}  // namespace fsw

@@ -190,6 +190,8 @@ void meta_swiglu_fwd_bf16(int64_t, int64_t, int64_t, Tensor const&, int64_t, Ten
 
 }  // namespace
 
+void bind_attention(pybind11::module_& m);  // attn_bindings.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("fused_swiglu_bf16", &fused_swiglu_bf16, "fused SwiGLU for bf16");
   m.def("swiglu_fwd_bf16", &swiglu_fwd_bf16, "SwiGLU fwd bf16");
@@ -203,6 +205,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("variant_name", [](int family, int64_t M, int64_t n, int64_t k) {
     return std::string(fsw_variant_name(family, FSW_BF16, M, n, k));
   }, "kernel variant the dispatcher picks (family 0 = gate/up, 1 = down)");
+  bind_attention(m);
 }
 
 TORCH_LIBRARY(ASMLLM, m) {

@@ -16,6 +16,16 @@ E_NULL, E_DTYPE, E_SHAPE, E_LD, E_ALIGN, E_WORKSPACE, E_LAUNCH, E_DEVICE, E_VARI
 
 # name -> (restype, argtypes); the list the loader test checks against include/fsw.h
 _i, _i64, _vp, _sz, _cp = ctypes.c_int, ctypes.c_int64, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_char_p
+_rows = [_vp, _i64, _i64]  # rows [token][head][channel]: base, token stride, head stride
+
+
+class KvCache(ctypes.Structure):
+    """fsw_kv_cache of include/fsw.h."""
+    _fields_ = [("k", _vp), ("v", _vp), ("pages", _i64), ("page_size", _i64), ("page_stride", _i64), ("head_stride", _i64),
+                ("token_stride", _i64)]
+
+
+_kvp = ctypes.POINTER(KvCache)
 PROTOTYPES = {
     "fsw_validate_gateup": (_i, [_i, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64]),
     "fsw_gateup": (_i, [_i, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp]),
@@ -36,6 +46,13 @@ PROTOTYPES = {
     "fsw_down_blocked": (_i, [_i, _i64, _i64, _i64, _vp, _vp, _i64, _i, _vp, _i64, _vp]),
     "fsw_gateup_workspace_bytes": (_sz, [_i, _i64, _i64, _i64]),
     "fsw_gateup_ws": (_i, [_i, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp, _sz, _vp]),
+    "fsw_validate_kv_append": (_i, [_i] + [_i64] * 5 + _rows * 3 + [_vp, _i64, _vp, _vp] + _rows * 2 + [_kvp]),
+    "fsw_kv_append": (_i, [_i] + [_i64] * 5 + [_i] + _rows * 3 + [_vp, _i64, _vp, _vp] + _rows * 2 + [_kvp, _vp]),
+    "fsw_validate_attn_decode": (_i, [_i] + [_i64] * 4 + _rows + [_kvp, _vp, _i64, _vp, _i64, ctypes.c_float] + _rows),
+    "fsw_attn_decode_workspace_bytes": (_sz, [_i] + [_i64] * 5),
+    "fsw_attn_decode": (_i, [_i] + [_i64] * 4 + _rows + [_kvp, _vp, _i64, _vp, _i64, ctypes.c_float] + _rows + [_vp, _sz, _vp]),
+    "fsw_validate_attn_prompt": (_i, [_i] + [_i64] * 6 + _rows * 3 + [_vp, _vp, ctypes.c_float] + _rows),
+    "fsw_attn_prompt": (_i, [_i] + [_i64] * 6 + _rows * 3 + [_vp, _vp, ctypes.c_float] + _rows + [_vp]),
     "fsw_strerror": (_cp, [_i]),
     "fsw_last_hip_error": (_i, []),
     "fsw_decode_barrier_failures": (_i, []),
@@ -350,6 +367,138 @@ def down_blocked(Hb, W2, out=None):
     with torch.cuda.device(like.device):
         check(lib().fsw_down_blocked(code, Hb.rows, D, Hb.k, Hb.data_ptr(), W2.data_ptr(), 0 if wb else _ld(W2),
                                      1 if wb else 0, out.data_ptr(), _ld(out), _stream(like)))
+    return out
+
+
+def _row_args(t):
+    """Base, token stride and head stride of a [tokens, heads, channels] device tensor."""
+    return t.data_ptr(), _step(t, 0), _step(t, 1)
+
+
+def _step(t, dim):
+    """Stride of a dimension; one that is never stepped along may hold anything."""
+    return t.stride(dim) if t.shape[dim] > 1 else 0
+
+
+def _check_rows(first, *others):
+    for t in (first,) + others:
+        if t.dim() != 3:
+            raise FswError(E_SHAPE, "fsw: rows must be [tokens, heads, channels]")
+        if not t.is_cuda or t.device != first.device:
+            raise FswError(E_DEVICE, "fsw: operands must be device tensors on one device")
+        if t.dtype != first.dtype:
+            raise FswError(E_DTYPE, "fsw: operands differ in element type")
+        if t.shape[2] > 1 and t.stride(2) != 1:
+            raise FswError(E_LD, "fsw: channels must be contiguous")
+
+
+def _check_int32(like, *arrays):
+    import torch
+    for t in arrays:
+        if t.dtype != torch.int32:
+            raise FswError(E_DTYPE, "fsw: positions, slots, pages, lengths and offsets are int32")
+        if not t.is_cuda or t.device != like.device:
+            raise FswError(E_DEVICE, "fsw: operands must be device tensors on one device")
+        if t.shape[-1] > 1 and t.stride(-1) != 1:
+            raise FswError(E_LD, "fsw: int32 arrays must be contiguous")
+
+
+def kv_cache(k_cache, v_cache):
+    """fsw_kv_cache of two [pages, heads, page_size, channels] device tensors with the same strides (any order of dimensions
+    whose channels are contiguous)."""
+    if k_cache.dim() != 4 or v_cache.shape != k_cache.shape or \
+            any(_step(k_cache, i) != _step(v_cache, i) for i in range(3)):
+        raise FswError(E_SHAPE, "fsw: the caches must be [pages, heads, page_size, channels] with the same strides")
+    if k_cache.shape[3] > 1 and k_cache.stride(3) != 1:
+        raise FswError(E_LD, "fsw: channels must be contiguous")
+    return KvCache(k_cache.data_ptr(), v_cache.data_ptr(), k_cache.shape[0], k_cache.shape[2], _step(k_cache, 0),
+                   _step(k_cache, 1), _step(k_cache, 2))
+
+
+def kv_append(q, k, v, cos_sin, positions, slots, k_cache, v_cache, interleaved=False, q_out=None, k_out=None):
+    """Rotated copies of q [T, Hq, D] and k [T, Hkv, D]; rotated k, and v, go to their slots of the caches (fsw_kv_append)."""
+    import torch
+    code = dtype_code(q)
+    _check_rows(q, k, v)
+    _check_int32(q, positions, slots)
+    cache = kv_cache(k_cache, v_cache)
+    T, Hq, D = q.shape
+    Hkv = k.shape[1]
+    if k.shape != (T, Hkv, D) or v.shape != k.shape or tuple(k_cache.shape[1::2]) != (Hkv, D):
+        raise FswError(E_SHAPE, "fsw: q is [T, Hq, D], k and v are [T, Hkv, D], the caches [pages, Hkv, page_size, D]")
+    if positions.shape != (T,) or slots.shape != (T,) or cos_sin.dim() != 2:
+        raise FswError(E_SHAPE, "fsw: positions and slots are [T], cos_sin is [rows, rot]")
+    if cos_sin.dtype != torch.float32 or k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
+        raise FswError(E_DTYPE, "fsw: cos_sin is float32, the caches have the rows' element type")
+    if any(t.device != q.device for t in (cos_sin, k_cache, v_cache)):
+        raise FswError(E_DEVICE, "fsw: operands live on different devices")
+    if not cos_sin.is_contiguous():
+        raise FswError(E_LD, "fsw: cos_sin must be contiguous")
+    q_out = torch.empty((T, Hq, D), dtype=q.dtype, device=q.device) if q_out is None else q_out
+    k_out = torch.empty((T, Hkv, D), dtype=q.dtype, device=q.device) if k_out is None else k_out
+    _check_rows(q, q_out, k_out)
+    if q_out.shape != q.shape or k_out.shape != k.shape:
+        raise FswError(E_SHAPE, "fsw: q_out and k_out have the shapes of q and k")
+    with torch.cuda.device(q.device):
+        check(lib().fsw_kv_append(code, T, Hq, Hkv, D, cos_sin.shape[1], int(interleaved), *_row_args(q), *_row_args(k),
+                                  *_row_args(v), cos_sin.data_ptr(), cos_sin.shape[0], positions.data_ptr(), slots.data_ptr(),
+                                  *_row_args(q_out), *_row_args(k_out), ctypes.byref(cache), _stream(q)))
+    return q_out, k_out
+
+
+def attn_decode(q, k_cache, v_cache, block_table, lengths, max_len, scale, out=None, workspace=None):
+    """Attention of one token per sequence, q [B, Hq, D], over the paged caches (fsw_attn_decode). `workspace` (uint8 device
+    tensor) may be reused."""
+    import torch
+    code = dtype_code(q)
+    _check_rows(q)
+    _check_int32(q, block_table, lengths)
+    cache = kv_cache(k_cache, v_cache)
+    B, Hq, D = q.shape
+    Hkv = k_cache.shape[1]
+    if k_cache.shape[3] != D or block_table.dim() != 2 or block_table.shape[0] != B or lengths.shape != (B,):
+        raise FswError(E_SHAPE, "fsw: q is [B, Hq, D], the caches [pages, Hkv, page_size, D], block_table [B, width], lengths [B]")
+    if k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
+        raise FswError(E_DTYPE, "fsw: the caches have the queries' element type")
+    if k_cache.device != q.device or v_cache.device != q.device:
+        raise FswError(E_DEVICE, "fsw: operands live on different devices")
+    if block_table.shape[1] * k_cache.shape[2] < max_len:
+        raise FswError(E_LD, "fsw: block_table is narrower than max_len")
+    out = torch.empty((B, Hq, D), dtype=q.dtype, device=q.device) if out is None else out
+    _check_rows(q, out)
+    if out.shape != q.shape:
+        raise FswError(E_SHAPE, "fsw: `out` has the shape of q")
+    nbytes = lib().fsw_attn_decode_workspace_bytes(code, B, Hq, Hkv, D, max_len)
+    if workspace is None and nbytes:
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    if workspace is not None and (workspace.dtype != torch.uint8 or workspace.device != q.device or not workspace.is_contiguous()):
+        raise FswError(E_WORKSPACE, "fsw: workspace must be a contiguous uint8 tensor on the operands' device")
+    ld = block_table.stride(0) if B > 1 else block_table.shape[1]
+    with torch.cuda.device(q.device):
+        check(lib().fsw_attn_decode(code, B, Hq, Hkv, D, *_row_args(q), ctypes.byref(cache), block_table.data_ptr(), ld,
+                                    lengths.data_ptr(), max_len, scale, *_row_args(out),
+                                    workspace.data_ptr() if workspace is not None else None,
+                                    workspace.numel() if workspace is not None else 0, _stream(q)))
+    return out
+
+
+def attn_prompt(q, k, v, cu_q, cu_k, scale, out=None):
+    """Causal attention of packed sequences, q [Tq, Hq, D], k and v [Tk, Hkv, D], offsets [B + 1] (fsw_attn_prompt)."""
+    import torch
+    code = dtype_code(q)
+    _check_rows(q, k, v)
+    _check_int32(q, cu_q, cu_k)
+    Tq, Hq, D = q.shape
+    Tk, Hkv = k.shape[:2]
+    if k.shape[2] != D or v.shape != k.shape or cu_q.dim() != 1 or cu_q.numel() < 1 or cu_k.shape != cu_q.shape:
+        raise FswError(E_SHAPE, "fsw: q is [Tq, Hq, D], k and v are [Tk, Hkv, D], offsets are [B + 1]")
+    out = torch.empty((Tq, Hq, D), dtype=q.dtype, device=q.device) if out is None else out
+    _check_rows(q, out)
+    if out.shape != q.shape:
+        raise FswError(E_SHAPE, "fsw: `out` has the shape of q")
+    with torch.cuda.device(q.device):
+        check(lib().fsw_attn_prompt(code, Tq, Tk, cu_q.numel() - 1, Hq, Hkv, D, *_row_args(q), *_row_args(k), *_row_args(v),
+                                    cu_q.data_ptr(), cu_k.data_ptr(), scale, *_row_args(out), _stream(q)))
     return out
 
 

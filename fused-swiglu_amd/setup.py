@@ -5,7 +5,7 @@ Counterpart of the reference's setup.py:12-45 (CUDAExtension + nvcc sm_80), in t
   1. the HIP kernels and the C-ABI dispatcher (csrc/*.hip) are compiled by hipcc for gfx950 into
      `libfsw_hip.so`, which exports only the C symbols declared in include/fsw.h (and the benchmark's two
      measurement kernels, csrc/probes.hip, into `libfsw_probe.so`, include/fsw_probe.h);
-  2. csrc/torch_bindings.cpp is built as a host-only C++ extension (`CppExtension`, so torch's source
+  2. csrc/torch_bindings.cpp (and attn_bindings.cpp) is built as a host-only C++ extension (`CppExtension`, so torch's source
      translation pass for CUDA extensions never runs) that links `libfsw_hip.so`.
 
 Usage (in this directory):  python setup.py build_ext --inplace
@@ -22,7 +22,8 @@ INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 OBJ_DIR = os.path.join(HERE, "build", "hip_obj")
 LIB_NAME = "libfsw_hip.so"
 HIP_SOURCES = ["kernels_pair16.hip", "kernels_mid_bf16_gateup.hip", "kernels_mid_bf16_down.hip",
-               "kernels_mid_fp16_gateup.hip", "kernels_mid_fp16_down.hip", "kernels_mid.hip", "kernels_tiled.hip", "kernels_skinny.hip", "kernels_stream.hip", "kernels_decode.hip", "fsw_api.hip"]
+               "kernels_mid_fp16_gateup.hip", "kernels_mid_fp16_down.hip", "kernels_mid.hip", "kernels_tiled.hip", "kernels_skinny.hip", "kernels_stream.hip", "kernels_decode.hip", "fsw_api.hip",
+               "kernels_kv_append.hip", "kernels_attn_decode.hip", "kernels_attn_prompt.hip", "attn_api.hip"]
 PROBE_LIB_NAME = "libfsw_probe.so"  # measurement kernels of the benchmark (include/fsw_probe.h): not part of the product
 PROBE_SOURCES = ["probes.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
@@ -79,7 +80,7 @@ def main():
         ext_modules=[
             CppExtension(
                 name="fused_mlp_module",
-                sources=[os.path.join("csrc", "torch_bindings.cpp")],
+                sources=[os.path.join("csrc", "torch_bindings.cpp"), os.path.join("csrc", "attn_bindings.cpp")],
                 include_dirs=include_paths("cuda") + [INCLUDE, os.path.join(rocm, "include")],
                 define_macros=[("__HIP_PLATFORM_AMD__", "1"), ("USE_ROCM", "1")],
                 extra_compile_args=["-O3", "-Wall", "-std=c++17", "-Wno-unused-function"],

@@ -180,11 +180,90 @@ FSW_API size_t fsw_gateup_workspace_bytes(int dtype, int64_t M, int64_t N, int64
 FSW_API int fsw_gateup_ws(int dtype, int64_t M, int64_t N, int64_t K, const void* X, int64_t ldx, const void* W13,
                           int64_t ldw, void* H, int64_t ldh, void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * Attention beside the MLP (no counterpart in the reference, whose extension ends at the MLP): the other half of a decoder layer that is being
+ * served. Hq query heads share Hkv key-value heads (Hq a multiple of Hkv, both at most 1024; query head h reads head
+ * h / (Hq / Hkv)) of D channels (a multiple of 8, 8 .. 256). Rows of queries, keys, values and outputs are addressed by a token and a
+ * head stride in elements, multiples of 8 and not negative, with D contiguous channels from a 16-byte aligned base: the slices of a fused
+ * projection's output are such rows. Rows of an output must not overlap. At most 2^20 tokens per call.
+ * Whole numbers on the device (positions, slots, pages, lengths, offsets) are int32. The host cannot check them, so the
+ * kernels do: nothing outside the described arrays is ever read or written, and what each kernel does instead is said below.
+ */
+
+/* A paged cache of one layer. Token t of a page holds its head h at element page * page_stride + h * head_stride +
+ * t * token_stride of k, and of v likewise. Strides are multiples of 8 below 2^40 (token_stride: at most 2^24); pages * page_size < 2^31. */
+typedef struct fsw_kv_cache {
+  void* k;
+  void* v;
+  int64_t pages, page_size;
+  int64_t page_stride, head_stride, token_stride;
+} fsw_kv_cache;
+
+/* Host-only validation of fsw_kv_append. 0 <= rot <= D, rot even. */
+FSW_API int fsw_validate_kv_append(int dtype, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t rot,
+                                   const void* Q, int64_t q_token, int64_t q_head, const void* K, int64_t k_token, int64_t k_head,
+                                   const void* V, int64_t v_token, int64_t v_head, const float* cos_sin, int64_t table_rows,
+                                   const int32_t* positions, const int32_t* slots, const void* Qout, int64_t qo_token,
+                                   int64_t qo_head, const void* Kout, int64_t ko_token, int64_t ko_head,
+                                   const fsw_kv_cache* cache);
+
+/*
+ * Rotates queries and keys by their positions and appends keys and values to the cache. The first `rot` channels are turned in pairs (a, b) =
+ * (x[i], x[i + rot/2]), or (x[2i], x[2i+1]) if `interleaved`: a cos - b sin, b cos + a sin in fp32, one rounding. Row p of
+ * cos_sin [table_rows, rot] holds position p's rot/2 cosines, then its sines (16-byte aligned; 4-byte where rot is no multiple of 8). Qout may be Q itself, Kout K itself or NULL.
+ * Token t goes to slot slots[t] = page * page_size + place in the page; a slot outside the cache appends nothing (padding). Slots of one
+ * call must differ. A position outside the table gives NaN in the turned channels.
+ */
+FSW_API int fsw_kv_append(int dtype, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t rot, int interleaved,
+                          const void* Q, int64_t q_token, int64_t q_head, const void* K, int64_t k_token, int64_t k_head,
+                          const void* V, int64_t v_token, int64_t v_head, const float* cos_sin, int64_t table_rows,
+                          const int32_t* positions, const int32_t* slots, void* Qout, int64_t qo_token, int64_t qo_head,
+                          void* Kout, int64_t ko_token, int64_t ko_head, const fsw_kv_cache* cache, void* stream);
+
+/* Host-only validation of fsw_attn_decode (all but the workspace). B <= 2^20; scale finite and positive (a normal number); table_ld >= ceil(max_len / page_size). */
+FSW_API int fsw_validate_attn_decode(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, const void* Q, int64_t q_seq,
+                                     int64_t q_head, const fsw_kv_cache* cache, const int32_t* block_table, int64_t table_ld,
+                                     const int32_t* lengths, int64_t max_len, float scale, const void* O, int64_t o_seq,
+                                     int64_t o_head);
+
+/* Bytes of device scratch fsw_attn_decode needs (FSW_E_WORKSPACE without them): the float32 sums of the parts that long sequences are
+ * split into where there are few of them, else 0. Need not be initialised. */
+FSW_API size_t fsw_attn_decode_workspace_bytes(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_len);
+
+/*
+ * O[b, h] = softmax_j(scale * Q[b, h] . k_j) . v_j over the keys j < lengths[b] of sequence b, which lie in pages
+ * block_table[b * table_ld + j / page_size]: one new token per sequence. fp32 scores, weights and sums, one rounding. max_len: the host's bound of the lengths, which sets
+ * the launch's shape. A length of 0 gives zeros; a length below 0 or above max_len, or a page outside the cache among a sequence's pages, gives NaN for that
+ * sequence. What the cache holds behind a length is never used.
+ */
+FSW_API int fsw_attn_decode(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, const void* Q, int64_t q_seq, int64_t q_head,
+                            const fsw_kv_cache* cache, const int32_t* block_table, int64_t table_ld, const int32_t* lengths,
+                            int64_t max_len, float scale, void* O, int64_t o_seq, int64_t o_head, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
+/* Host-only validation of fsw_attn_prompt. B <= 2^20; k_token, v_token between D and 2^21; scale finite and positive (a normal number). */
+FSW_API int fsw_validate_attn_prompt(int dtype, int64_t Tq, int64_t Tk, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, const void* Q,
+                                     int64_t q_token, int64_t q_head, const void* K, int64_t k_token, int64_t k_head,
+                                     const void* V, int64_t v_token, int64_t v_head, const int32_t* cu_q, const int32_t* cu_k,
+                                     float scale, const void* O, int64_t o_token, int64_t o_head);
+
+/*
+ * Causal attention of B packed sequences: sequence b is rows cu_q[b] .. cu_q[b + 1] - 1 of Q and O and rows cu_k[b] .. cu_k[b + 1] - 1 of
+ * K and V (B + 1 offsets each, ascending from 0; for whole prompts both are one array). Ends are aligned: query i of nq sees the keys
+ * j <= i + nk - nq. A query that sees no key, and a row of Q behind the last sequence, gives zeros. Scores, sums and the
+ * normalisation are fp32; the weights 2^(c s - m) are rounded to the element type once, for the matrix product with V, and their sum is taken of the rounded values.
+ */
+FSW_API int fsw_attn_prompt(int dtype, int64_t Tq, int64_t Tk, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, const void* Q,
+                            int64_t q_token, int64_t q_head, const void* K, int64_t k_token, int64_t k_head, const void* V,
+                            int64_t v_token, int64_t v_head, const int32_t* cu_q, const int32_t* cu_k, float scale, void* O,
+                            int64_t o_token, int64_t o_head, void* stream);
+
 /* The hipError_t (as int) of the most recent failed launch on the calling thread, 0 if none. */
 FSW_API int fsw_last_hip_error(void);
 
 /* ABI version: major * 1000 + minor. 2000: the measurement kernels fsw_probe_* left this library (libfsw_probe.so,
- * fsw_probe.h); fsw_gateup_f32out and fsw_gateup_hblocked joined it; fsw_gateup_workspace_bytes returns 0. */
+ * fsw_probe.h); fsw_gateup_f32out and fsw_gateup_hblocked joined it; fsw_gateup_workspace_bytes returns 0. 2001: the attention
+ * entry points. */
 FSW_API int fsw_version(void);
 
 /*
