@@ -9,6 +9,23 @@
 
 namespace fsw {
 
+// Division of a whole number below 2^30 by a divisor known on the host: n / d = mulhi(4 n, ceil(2^(30 + s) / d)) >> s with s =
+// ceil(log2 d). The multiplier exceeds 2^(30 + s) / d by less than 1 <= 2^s / d, so the quotient's error is below n 2^-30 / d < 1 / d.
+struct Divisor {
+  unsigned d, mul;
+  int shift;
+  Divisor() = default;
+  explicit Divisor(unsigned by) : d(by), shift(0) {
+    while ((1ull << shift) < by) ++shift;
+    mul = (unsigned)(((1ull << (30 + shift)) + by - 1) / by);
+  }
+#ifdef __HIP_DEVICE_COMPILE__
+  __device__ __forceinline__ int quotient(int n) const { return (int)(__umulhi((unsigned)n << 2, mul) >> shift); }
+#else
+  __host__ __device__ int quotient(int n) const { return (int)((((unsigned long long)((unsigned)n << 2) * mul) >> 32) >> shift); }
+#endif
+};
+
 // [tokens][heads][channels], unit stride over the channels; strides in elements
 struct Rows {
   const void* p;
@@ -25,6 +42,7 @@ struct PagedKv {
   void* v;
   int pages, page_size;
   long long page, head, token;
+  Divisor per_page;  // by page_size
 };
 
 struct AppendArgs {
@@ -54,6 +72,7 @@ struct PagedAttnArgs {
 struct PagedAttnPlan {
   int splits;  // workgroups that share the keys of one sequence and key-value head
   int chunk;   // keys of each
+  int waves;   // of a workgroup
   size_t workspace_bytes;
 };
 PagedAttnPlan paged_attn_plan(int seqs, int hq, int hkv, int d, int max_len);

@@ -9,7 +9,7 @@
 
 namespace {
 
-constexpr int64_t MAX_TOKENS = 1 << 20, MAX_SEQS = 1 << 20, MAX_HEADS = 1024, MAX_CHANNELS = 256;
+constexpr int64_t MAX_TOKENS = 1 << 20, MAX_SEQS = 65535, MAX_HEADS = 1024, MAX_CHANNELS = 256;
 constexpr int64_t MAX_STRIDE = 1LL << 40;        // elements; times 2^20 tokens stays far below 2^63
 constexpr int64_t MAX_PAGE_TOKEN = 1LL << 24;    // token stride inside a page
 constexpr int64_t MAX_TILE_TOKEN = 1LL << 21;    // token stride of keys and values that are read through a buffer descriptor
@@ -64,7 +64,8 @@ int check_cache(const fsw_kv_cache* c, int64_t d, int64_t heads) {
 }
 
 fsw::PagedKv paged(const fsw_kv_cache* c) {
-  return fsw::PagedKv{c->k, c->v, (int)c->pages, (int)c->page_size, c->page_stride, c->head_stride, c->token_stride};
+  return fsw::PagedKv{c->k, c->v, (int)c->pages, (int)c->page_size, c->page_stride, c->head_stride, c->token_stride,
+                      fsw::Divisor((unsigned)c->page_size)};
 }
 
 // (the kernels multiply scores by it before they are compared: a masked score, -inf, has to stay one)
@@ -150,7 +151,7 @@ int fsw_attn_decode(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, co
   fsw::PagedAttnArgs a;
   a.seqs = (int)B, a.hq = (int)Hq, a.hkv = (int)Hkv, a.d = (int)D;
   a.q = {Q, q_seq, q_head};
-  a.cache = max_len > 0 ? paged(cache) : fsw::PagedKv{nullptr, nullptr, 0, 16, 0, 0, 0};
+  a.cache = max_len > 0 ? paged(cache) : fsw::PagedKv{nullptr, nullptr, 0, 16, 0, 0, 0, fsw::Divisor(16)};
   a.block_table = block_table, a.table_ld = table_ld, a.lengths = lengths, a.max_len = (int)max_len;
   a.scale_log2 = scale * LOG2E;
   a.o = {O, o_seq, o_head};

@@ -4,14 +4,13 @@
 //
 // Every key and value is read once for all the query heads that share it, and 4 to 64 operations are done per byte: memory
 // bounds it, so the kernel is laid out for loads. Query heads are the columns of every matrix instruction, up to 16 at a
-// time. Keys are the rows: a wave reads 16 keys of 64 bytes per load, straight into the A operand of
+// time. Keys are the rows: a wave reads 16 keys, 64 bytes of each per load, straight into the A operand of
 // v_mfma_f32_16x16x32, and gets S^T: lane l holds head l % 16 and keys 4 (l / 16) + r. That is just what the B
-// operand of v_mfma_f32_16x16x4_f32 wants (head l % 16, k = l / 16) when step r takes the keys {4 g + r}, and its A operand
-// (channel l % 16, k = l / 16) is a value row read as it lies, 16 lanes with 8 consecutive channels each of which instruction
-// j takes the j-th. So neither P nor V crosses lanes, nothing goes through LDS, P is not rounded at all, and the output is O^T:
-// maximum, sum and rescaling of a head live in the lanes of its accumulators. fp32 matrix instructions run at a
-// sixteenth of the bf16 rate; the 64 KB of keys and values that four waves of a CU hold take them about 4100 cycles, a third of the time in which
-// HBM delivers them.
+// operand of v_mfma_f32_16x16x16 wants (head l % 16, k = 4 (l / 16) + r), and its A operand (channel l % 16, the same keys) comes out of
+// value rows that are read as they lie: 16 lanes with 8 consecutive channels each, four rows per lane, of which instruction j
+// takes the j-th channels, put side by side by two byte permutations. So neither P nor V crosses lanes, nothing goes through LDS before the end, and
+// the output is O^T: maximum, sum and rescaling of a head live in the lanes of its accumulators. P is not rounded to the element type but
+// split into two elements, whose products both are added.
 #include "attn.h"
 #include "fsw_device.h"
 #include "fsw_internal.h"
@@ -22,8 +21,21 @@ namespace {
 constexpr float NEG_INF = -__builtin_inff();
 // The running maximum of a head moves only when a score passes it by this much (in powers of two): p stays below 2^8.
 constexpr float SLACK = 8.0f;
-constexpr int WAVES = 4;
 
+typedef __attribute__((ext_vector_type(4))) short s16x4;
+typedef __attribute__((ext_vector_type(4))) _Float16 f16x4;
+
+// 16 x 16 x 16: lane l holds row (column) l % 16, k = 4 (l / 16) + j of A (B)
+template <class T>
+__device__ __forceinline__ f32x4 mfma_k16(u32x2 a, u32x2 b, f32x4 c);
+template <>
+__device__ __forceinline__ f32x4 mfma_k16<Bf16>(u32x2 a, u32x2 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(s16x4, a), __builtin_bit_cast(s16x4, b), c, 0, 0, 0);
+}
+template <>
+__device__ __forceinline__ f32x4 mfma_k16<Fp16>(u32x2 a, u32x2 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, a), __builtin_bit_cast(f16x4, b), c, 0, 0, 0);
+}
 template <class T>
 __device__ __forceinline__ void unpack2(unsigned u, float& lo, float& hi);
 template <>
@@ -37,10 +49,18 @@ __device__ __forceinline__ void unpack2<Fp16>(unsigned u, float& lo, float& hi) 
   lo = (float)v[0];
   hi = (float)v[1];
 }
+// the low (high) halves of a and b side by side
+__device__ __forceinline__ unsigned lows(unsigned a, unsigned b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
+__device__ __forceinline__ unsigned highs(unsigned a, unsigned b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
 
-__device__ __forceinline__ float max_over_groups(float x) {  // over lanes l, l ^ 16, l ^ 32, l ^ 48
-  x = fmaxf(x, __shfl_xor(x, 16));
-  return fmaxf(x, __shfl_xor(x, 32));
+// over lanes l, l ^ 16, l ^ 32, l ^ 48: a lane swap of a register with a copy of itself leaves the two halves' values side by side
+__device__ __forceinline__ float max_over_groups(float x) {
+  const unsigned u = __builtin_bit_cast(unsigned, x);
+  const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const float y = fmaxf(__builtin_bit_cast(float, a[0]), __builtin_bit_cast(float, a[1]));
+  const unsigned w = __builtin_bit_cast(unsigned, y);
+  const auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+  return fmaxf(__builtin_bit_cast(float, b[0]), __builtin_bit_cast(float, b[1]));
 }
 __device__ __forceinline__ float sum_over_groups(float x) {
   x += __shfl_xor(x, 16);
@@ -54,296 +74,296 @@ __device__ __forceinline__ float scale_of(float a, float b) {
 
 // DP: channels, padded to 64, 128 or 256; a row of values is NV vectors of VL elements on 16 lanes.
 // WHOLE: page_size % 16 == 0, so 16 keys in a row lie in one page and the page's address is wave-uniform.
-template <class T, int DP, bool WHOLE>
-__global__ __launch_bounds__(64 * WAVES, 2) void attn_decode_kernel(PagedAttnArgs a, int chunk, int splits, int head_tiles,
-                                                                    float* partial) {
+template <class T, int DP, bool WHOLE, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, DP == 256 ? 2 : 4) void attn_decode_kernel(PagedAttnArgs a, int chunk, int group, int head_tiles,
+                                                                                    float* partial) {
   constexpr int KS = DP / 32;                  // steps over the channels
   constexpr int VL = DP == 64 ? 4 : 8, NV = DP / (16 * VL), NA = NV * VL;
-  constexpr int TT = DP == 256 ? 2 : 4;        // tiles of 16 keys in flight
-  constexpr int KEYS = 16 * TT;
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, grp = lane >> 4;
-  const int items = a.seqs * a.hkv * head_tiles;
-  const int split = blockIdx.x / items, item = blockIdx.x % items;
-  const int seq = item / (a.hkv * head_tiles), rest = item % (a.hkv * head_tiles);
-  const int kvh = rest / head_tiles, group = a.hq / a.hkv, first = (rest % head_tiles) * 16;
-  const int head = kvh * group + first + col;  // this lane's query head
-  const bool real = first + col < group;
+  const int split = blockIdx.z, splits = gridDim.z, seq = blockIdx.y;
+  int kvh = blockIdx.x, first = 0;
+  if (head_tiles > 1) {
+    kvh = (int)blockIdx.x / head_tiles;
+    first = ((int)blockIdx.x - kvh * head_tiles) * 16;
+  }
+  const int here = group - first < 16 ? group - first : 16;  // query heads of this workgroup
+  const int head0 = kvh * group + first, head = head0 + col;  // this lane's
+  const bool real = col < here;
+  const int begin = split * chunk;
 
+  const unsigned short* kc = (const unsigned short*)a.cache.k + kvh * a.cache.head;
+  const unsigned short* vc = (const unsigned short*)a.cache.v + kvh * a.cache.head;
+  const int* table = a.block_table + (long long)seq * a.table_ld;
+  // page and place of this lane's key of the tile that begins at `at`; below max_len, whatever the length is
+  int page, place;
+  auto locate = [&](int at) {
+    int key = at + col;
+    key = key < a.max_len ? key : a.max_len - 1;
+    const int idx = a.cache.per_page.quotient(key);
+    page = table[idx];
+    place = key - idx * a.cache.page_size;
+  };
+  int at = begin + wave * 16;
+  if (at < a.max_len) locate(at);  // before the length is known: three trips to memory (length, page, keys) become two
+
+  u32x4 qf[KS];
+  const unsigned short* qp = (const unsigned short*)a.q.p + (long long)seq * a.q.token + (long long)head * a.q.head;
+#pragma unroll
+  for (int s = 0; s < KS; ++s) {
+    const int ch = s * 32 + grp * 8;
+    qf[s] = u32x4{0, 0, 0, 0};
+    if (real && ch < a.d) qf[s] = *(const u32x4*)(qp + ch);
+  }
   const int len = a.lengths[seq];
   const bool bad_len = len < 0 || len > a.max_len;
-  const int begin = split * chunk;
   const int end = bad_len ? 0 : (len - begin < chunk ? len : begin + chunk);
-
-  // a share without keys writes nothing (share 0 of an invalid length does: NaN)
-  if (splits > 1 && begin >= end && !(bad_len && split == 0)) return;
+  // a share without keys: nothing to do, unless it is the first of an empty sequence or of one of invalid length
+  if (split > 0 && begin >= end) return;
 
   f32x4 acc[NA];
 #pragma unroll
   for (int i = 0; i < NA; ++i) acc[i] = f32x4{0, 0, 0, 0};
   float m = NEG_INF, sum = 0.0f;
+  bool bad_page = false;
 
-  if (begin < end) {
-    u32x4 qf[KS];
-    const unsigned short* qp = (const unsigned short*)a.q.p + (long long)seq * a.q.token + (long long)head * a.q.head;
+  for (; at < end; at += 16 * WAVES) {
+    const bool part = at + 16 > end;
+    // a page outside the cache is an error where a key lies in it, and read as page 0
+    const bool inside = (unsigned)page < (unsigned)a.cache.pages;
+    bad_page |= !inside && at + col < end;
+    const long long where = (long long)(inside ? page : 0) * a.cache.page + (long long)place * a.cache.token;
+    u32x4 kf[KS];
+    u32x4 vf[4][NV];
+    const unsigned short* tile = nullptr;
+    if constexpr (WHOLE) {
+      const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)where);
+      const unsigned hi = __builtin_amdgcn_readfirstlane((unsigned)((unsigned long long)where >> 32));
+      tile = vc + (long long)(((unsigned long long)hi << 32) | lo);
+    }
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
       const int ch = s * 32 + grp * 8;
-      qf[s] = u32x4{0, 0, 0, 0};
-      if (real && ch < a.d) qf[s] = *(const u32x4*)(qp + ch);
+      kf[s] = u32x4{0, 0, 0, 0};
+      if (ch < a.d) kf[s] = __builtin_nontemporal_load((const u32x4*)(kc + where + ch));
     }
-    const unsigned short* kc = (const unsigned short*)a.cache.k + kvh * a.cache.head;
-    const unsigned short* vc = (const unsigned short*)a.cache.v + kvh * a.cache.head;
-    const int* table = a.block_table + (long long)seq * a.table_ld;
-    bool bad_page = false;
-
-    // element offset of this lane's key (lane % KEYS of the tile that begins at `at`); keys past the end repeat the last one
-    auto locate = [&](int at) -> long long {
-      int key = at + lane % KEYS;
-      key = key < end ? key : end - 1;
-      const int idx = key / a.cache.page_size;
-      int page = table[idx];
-      if (page < 0 || page >= a.cache.pages) {
-        bad_page = true;
-        page = 0;
-      }
-      return (long long)page * a.cache.page + (long long)(key - idx * a.cache.page_size) * a.cache.token;
-    };
-    auto from = [&](long long x, int src) -> long long { return __shfl(x, src); };
-    auto uniform = [&](long long x, int src) -> long long {
-      const unsigned lo = __builtin_amdgcn_readlane((unsigned)x, src);
-      const unsigned hi = __builtin_amdgcn_readlane((unsigned)((unsigned long long)x >> 32), src);
-      return (long long)(((unsigned long long)hi << 32) | lo);
-    };
-
-    int at = begin + wave * KEYS;
-    long long where = at < end ? locate(at) : 0;
-    for (; at < end; at += WAVES * KEYS) {
-      const bool part = at + KEYS > end;
-      u32x4 kf[TT][KS];
-      u32x4 vf[TT][4][NV];
 #pragma unroll
-      for (int t = 0; t < TT; ++t) {
-        const unsigned short* p;
-        if constexpr (WHOLE) {
-          int in = col;  // a tile's keys past the end: its last one (a tile wholly past the end repeats key end - 1)
-          const int left = end - 1 - (at + 16 * t);
-          in = left < 0 ? 0 : in < left ? in : left;
-          p = kc + uniform(where, 16 * t) + (long long)in * a.cache.token;
-        } else {
-          p = kc + from(where, 16 * t + col);
-        }
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-          const int ch = s * 32 + grp * 8;
-          kf[t][s] = u32x4{0, 0, 0, 0};
-          if (ch < a.d) kf[t][s] = *(const u32x4*)(p + ch);
-        }
+    for (int r = 0; r < 4; ++r) {
+      const int k = 4 * grp + r;
+      const unsigned short* p;
+      if constexpr (WHOLE) {
+        p = tile + k * (int)a.cache.token;  // the page has room for all 16, keys or not
+      } else {
+        p = vc + __shfl(where, k);
       }
 #pragma unroll
-      for (int t = 0; t < TT; ++t) {
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          const int k = 4 * grp + r;
-          const unsigned short* p;
-          if constexpr (WHOLE) {
-            const int left = end - 1 - (at + 16 * t);
-            const int in = left < 0 ? 0 : k < left ? k : left;
-            p = vc + uniform(where, 16 * t) + (long long)in * a.cache.token;
+      for (int v = 0; v < NV; ++v) {
+        const int ch = (v * 16 + col) * VL;
+        vf[r][v] = u32x4{0, 0, 0, 0};
+        if (ch < a.d) {
+          if constexpr (VL == 8) {
+            vf[r][v] = __builtin_nontemporal_load((const u32x4*)(p + ch));
           } else {
-            p = vc + from(where, 16 * t + k);
-          }
-#pragma unroll
-          for (int v = 0; v < NV; ++v) {
-            const int ch = (v * 16 + col) * VL;
-            vf[t][r][v] = u32x4{0, 0, 0, 0};
-            if (ch < a.d) {
-              if constexpr (VL == 8) {
-                vf[t][r][v] = *(const u32x4*)(p + ch);
-              } else {
-                const u32x2 w = *(const u32x2*)(p + ch);
-                vf[t][r][v][0] = w[0], vf[t][r][v][1] = w[1];
-              }
-            }
-            // what lies behind the end weighs nothing, whatever it holds
-            if (part && at + 16 * t + k >= end) vf[t][r][v] = u32x4{0, 0, 0, 0};
+            const u32x2 w = __builtin_nontemporal_load((const u32x2*)(p + ch));
+            vf[r][v][0] = w[0], vf[r][v][1] = w[1];
           }
         }
+        // what lies behind the end weighs nothing, whatever it holds
+        if (part && at + k >= end) vf[r][v] = u32x4{0, 0, 0, 0};
       }
-      if (at + WAVES * KEYS < end) where = locate(at + WAVES * KEYS);
-
-      f32x4 s[TT];
-      float top = NEG_INF;
-#pragma unroll
-      for (int t = 0; t < TT; ++t) {
-        s[t] = f32x4{0, 0, 0, 0};
-#pragma unroll
-        for (int i = 0; i < KS; ++i) s[t] = T::mfma16(kf[t][i], qf[i], s[t]);
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          s[t][r] *= a.scale_log2;
-          if (part && at + 16 * t + 4 * grp + r >= end) s[t][r] = NEG_INF;
-          top = fmaxf(top, s[t][r]);
-        }
-      }
-      top = max_over_groups(top);
-      if (__any(top > m + SLACK)) {
-        const float now = fmaxf(m, top), alpha = scale_of(m, now);
-        m = now;
-        sum *= alpha;
-#pragma unroll
-        for (int i = 0; i < NA; ++i)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) acc[i][r] *= alpha;
-      }
-      const float base = m == NEG_INF ? 0.0f : m;
-#pragma unroll
-      for (int t = 0; t < TT; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          s[t][r] = __builtin_amdgcn_exp2f(s[t][r] - base);
-          sum += s[t][r];
-        }
-#pragma unroll
-      for (int t = 0; t < TT; ++t)
-#pragma unroll
-        for (int r = 0; r < 4; ++r)
-#pragma unroll
-          for (int v = 0; v < NV; ++v)
-#pragma unroll
-            for (int j = 0; j < VL / 2; ++j) {
-              float lo, hi;
-              unpack2<T>(vf[t][r][v][j], lo, hi);
-              acc[v * VL + 2 * j] = __builtin_amdgcn_mfma_f32_16x16x4f32(lo, s[t][r], acc[v * VL + 2 * j], 0, 0, 0);
-              acc[v * VL + 2 * j + 1] = __builtin_amdgcn_mfma_f32_16x16x4f32(hi, s[t][r], acc[v * VL + 2 * j + 1], 0, 0, 0);
-            }
     }
-    if (__any(bad_page)) sum = __builtin_nanf("");
-    sum = sum_over_groups(sum);
-  }
-  if (bad_len) sum = __builtin_nanf("");
+    if (at + 16 * WAVES < end) locate(at + 16 * WAVES);
 
-  // the waves' shares of the keys: weights relative to the largest maximum, then their sums
+    f32x4 s = {0, 0, 0, 0};
+#pragma unroll
+    for (int i = 0; i < KS; ++i) s = T::mfma16(kf[i], qf[i], s);
+    float top = NEG_INF;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      s[r] *= a.scale_log2;
+      if (part && at + 4 * grp + r >= end) s[r] = NEG_INF;
+      top = fmaxf(top, s[r]);
+    }
+    top = max_over_groups(top);
+    if (__any(top > m + SLACK)) {
+      const float now = fmaxf(m, top), alpha = scale_of(m, now);
+      m = now;
+      sum *= alpha;
+#pragma unroll
+      for (int i = 0; i < NA; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[i][r] *= alpha;
+    }
+    const float base = m == NEG_INF ? 0.0f : m;
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+      s[r] = __builtin_amdgcn_exp2f(s[r] - base);
+      sum += s[r];
+    }
+    // weights as the sum of two elements, so that they carry twice the bits: the product is as good as one in fp32
+    u32x2 p1, p2;
+#pragma unroll
+    for (int r = 0; r < 4; r += 2) {
+      float lo, hi;
+      p1[r / 2] = T::pack2(s[r], s[r + 1]);
+      unpack2<T>(p1[r / 2], lo, hi);
+      p2[r / 2] = T::pack2(s[r] - lo, s[r + 1] - hi);
+    }
+#pragma unroll
+    for (int v = 0; v < NV; ++v)
+#pragma unroll
+      for (int j = 0; j < VL / 2; ++j) {
+        const u32x2 even = {lows(vf[0][v][j], vf[1][v][j]), lows(vf[2][v][j], vf[3][v][j])};
+        const u32x2 odd = {highs(vf[0][v][j], vf[1][v][j]), highs(vf[2][v][j], vf[3][v][j])};
+        f32x4& x = acc[v * VL + 2 * j];
+        f32x4& y = acc[v * VL + 2 * j + 1];
+        x = mfma_k16<T>(even, p1, x);
+        y = mfma_k16<T>(odd, p1, y);
+        x = mfma_k16<T>(even, p2, x);
+        y = mfma_k16<T>(odd, p2, y);
+      }
+  }
+  if (__any(bad_page) || bad_len) sum = __builtin_nanf("");
+  sum = sum_over_groups(sum);
+
+  // The waves' shares of the keys, joined through LDS: rows of the real heads, each wave's scaled to the largest maximum. Four
+  // channels of padding spread the rows of 16 heads over the banks.
+  constexpr int ROW = DP + 4, WIDE = DP / 4;
+  extern __shared__ __align__(16) float shares[];  // [WAVES][here][ROW]
   __shared__ float stats[WAVES][2][16];
-  __shared__ f32x4 shares[WAVES - 1][NA][64];
   if (grp == 0) {
     stats[wave][0][col] = m;
     stats[wave][1][col] = sum;
   }
   __syncthreads();
-  float top = NEG_INF, total = 0.0f;
+  float top = NEG_INF;
 #pragma unroll
   for (int w = 0; w < WAVES; ++w) top = fmaxf(top, stats[w][0][col]);
-#pragma unroll
-  for (int w = 0; w < WAVES; ++w) total += stats[w][1][col] * scale_of(stats[w][0][col], top);
-  const float mine = scale_of(m, top);
-#pragma unroll
-  for (int i = 0; i < NA; ++i)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) acc[i][r] *= mine;
-  if (wave > 0) {
-#pragma unroll
-    for (int i = 0; i < NA; ++i) shares[wave - 1][i][lane] = acc[i];
-  }
-  __syncthreads();
-  if (wave > 0 || !real) return;
-#pragma unroll
-  for (int i = 0; i < NA; ++i)
-#pragma unroll
-    for (int w = 0; w < WAVES - 1; ++w) acc[i] += shares[w][i][lane];
-
-  if (splits > 1) {  // unnormalised sums, maximum and sum of this share: attn_join_kernel
-    const long long row = ((long long)seq * a.hq + head) * splits + split;
-    if (grp == 0) {
-      float* ml = partial + (long long)a.seqs * a.hq * splits * a.d + row * 2;
-      ml[0] = top;
-      ml[1] = total;
-    }
+  if (real) {
+    const float mine = scale_of(m, top);
+    float* row = shares + (wave * here + col) * ROW;
 #pragma unroll
     for (int v = 0; v < NV; ++v)
 #pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int ch = (v * 16 + 4 * grp + r) * VL;
-        if (ch >= a.d) continue;
+      for (int r = 0; r < 4; ++r)
 #pragma unroll
         for (int j = 0; j < VL; j += 4) {
-          const f32x4 x = {acc[v * VL + j][r], acc[v * VL + j + 1][r], acc[v * VL + j + 2][r], acc[v * VL + j + 3][r]};
-          *(f32x4*)(partial + row * a.d + ch + j) = x;
+          f32x4 x;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[i] = acc[v * VL + j + i][r] * mine;
+          *(f32x4*)(row + (v * 16 + 4 * grp + r) * VL + j) = x;
         }
-      }
-    return;
   }
-  const float inv = len == 0 ? 0.0f : 1.0f / total;
-  unsigned short* op = (unsigned short*)a.o.p + (long long)seq * a.o.token + (long long)head * a.o.head;
+  __syncthreads();
+  const bool parted = len > chunk && !bad_len;
+  for (int t = threadIdx.x; t < here * WIDE; t += 64 * WAVES) {
+    const int h = t / WIDE, ch = (t % WIDE) * 4;
+    if (ch >= a.d) continue;
+    float most = NEG_INF, total = 0.0f;
 #pragma unroll
-  for (int v = 0; v < NV; ++v)
+    for (int w = 0; w < WAVES; ++w) most = fmaxf(most, stats[w][0][h]);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int ch = (v * 16 + 4 * grp + r) * VL;
-      if (ch >= a.d) continue;
-      unsigned w[VL / 2];
+    for (int w = 0; w < WAVES; ++w) total += stats[w][1][h] * scale_of(stats[w][0][h], most);
+    f32x4 x = {0, 0, 0, 0};
 #pragma unroll
-      for (int j = 0; j < VL / 2; ++j) w[j] = T::pack2(acc[v * VL + 2 * j][r] * inv, acc[v * VL + 2 * j + 1][r] * inv);
-      if constexpr (VL == 8) {
-        *(u32x4*)(op + ch) = u32x4{w[0], w[1], w[2], w[3]};
-      } else {
-        *(u32x2*)(op + ch) = u32x2{w[0], w[1]};
+    for (int w = 0; w < WAVES; ++w) x += *(const f32x4*)(shares + (w * here + h) * ROW + ch);
+    if (parted) {  // unnormalised sums, maximum and sum of this share: attn_join_kernel
+      const long long row = ((long long)seq * a.hq + head0 + h) * splits + split;
+      *(f32x4*)(partial + row * a.d + ch) = x;
+      if (ch == 0) {
+        float* ml = partial + (long long)a.seqs * a.hq * splits * a.d + row * 2;
+        ml[0] = most;
+        ml[1] = total;
       }
+    } else {
+      const float inv = len == 0 ? 0.0f : 1.0f / total;
+      unsigned short* op = (unsigned short*)a.o.p + (long long)seq * a.o.token + (long long)(head0 + h) * a.o.head;
+      *(u32x2*)(op + ch) = u32x2{T::pack2(x[0] * inv, x[1] * inv), T::pack2(x[2] * inv, x[3] * inv)};
     }
+  }
 }
 
-// The shares of one query head's keys, joined: weights 2^(m_i - m), one normalisation, one rounding. A workgroup per head;
-// d / 4 threads stand side by side on a share's channels, 256 / (d / 4) shares at a time.
-template <class T>
+// The shares of one query head's keys, joined where there is more than one: weights 2^(m_i - m), one normalisation, one
+// rounding. TH threads per head: d / 4 of them stand side by side on a share's channels, TH / (d / 4) shares at a time, and
+// every thread keeps a running maximum of its own, so that all loads are one trip to memory.
+template <class T, int TH>
 __global__ __launch_bounds__(256) void attn_join_kernel(PagedAttnArgs a, int chunk, int splits, const float* partial) {
-  const int seq = blockIdx.x / a.hq, head = blockIdx.x % a.hq;
+  const int seq = blockIdx.y, lane = threadIdx.x % TH, first = threadIdx.x - lane;
+  const int head = (int)blockIdx.x * (256 / TH) + (int)threadIdx.x / TH;
+  const int width = a.d / 4, rows = TH / width, part = lane / width, at = lane % width;
   const int len = a.lengths[seq];
-  const bool bad_len = len < 0 || len > a.max_len;
-  const int used = bad_len ? 1 : (len + chunk - 1) / chunk;  // <= splits: len <= max_len
+  if (len <= chunk || len > a.max_len) return;
+  const int used = (len + chunk - 1) / chunk;  // <= splits: len <= max_len
   const long long row = ((long long)seq * a.hq + head) * splits;
   const float* ml = partial + (long long)a.seqs * a.hq * splits * a.d + row * 2;
-  const int width = a.d / 4, rows = 256 / width, part = threadIdx.x / width, at = threadIdx.x % width;
+  const float* po = partial + row * a.d + 4 * at;
 
-  float top = NEG_INF;
-  for (int i = 0; i < used; ++i) top = fmaxf(top, ml[2 * i]);
   f32x4 o = {0, 0, 0, 0};
-  float total = 0.0f;
-  if (part < rows) {
-    for (int i = part; i < used; i += rows) {
-      const float w = scale_of(ml[2 * i], top);
-      const f32x4 x = *(const f32x4*)(partial + (row + i) * a.d + 4 * at);
+  float top = NEG_INF, total = 0.0f;
+  auto add = [&](float m, float sum, f32x4 x) {
+    const float now = fmaxf(top, m), old = scale_of(top, now), w = scale_of(m, now);
+    top = now;
+    total = total * old + sum * w;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) o[j] += w * x[j];
-      total += w * ml[2 * i + 1];
+    for (int j = 0; j < 4; ++j) o[j] = o[j] * old + x[j] * w;
+  };
+  constexpr int BATCH = 4;
+  if (part < rows && head < a.hq) {
+    for (int i = part; i < used; i += rows * BATCH) {
+      f32x4 x[BATCH];
+      float m[BATCH], s[BATCH];
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k) {
+        const int n = i + k * rows < used ? i + k * rows : i;
+        x[k] = *(const f32x4*)(po + (long long)n * a.d);
+        m[k] = ml[2 * n];
+        s[k] = ml[2 * n + 1];
+      }
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k)
+        if (i + k * rows < used) add(m[k], s[k], x[k]);
     }
   }
   __shared__ f32x4 os[256];
-  __shared__ float ts[256];
+  __shared__ float ms[256], ts[256];
   os[threadIdx.x] = o;
+  ms[threadIdx.x] = top;
   ts[threadIdx.x] = total;
   __syncthreads();
-  if (part > 0) return;
-  for (int i = 1; i < rows; ++i) {
-    o += os[i * width + at];
-    total += ts[i * width + at];
+  if (part > 0 || head >= a.hq) return;
+  for (int i = 1; i < rows && i < used; ++i) {
+    const int n = first + i * width + at;
+    add(ms[n], ts[n], os[n]);
   }
-  const float inv = len == 0 ? 0.0f : 1.0f / total;
+  const float inv = 1.0f / total;
   unsigned short* op = (unsigned short*)a.o.p + (long long)seq * a.o.token + (long long)head * a.o.head;
   *(u32x2*)(op + 4 * at) = u32x2{T::pack2(o[0] * inv, o[1] * inv), T::pack2(o[2] * inv, o[3] * inv)};
 }
 
 int head_tiles(int hq, int hkv) { return (hq / hkv + 15) / 16; }
 
+template <class T, int DP, int WAVES>
+hipError_t launch_waves(const PagedAttnArgs& a, const PagedAttnPlan& p, float* partial, hipStream_t stream) {
+  const int tiles = head_tiles(a.hq, a.hkv);
+  const int group = a.hq / a.hkv;
+  const dim3 grid(a.hkv * tiles, a.seqs, p.splits);
+  const size_t lds = (size_t)WAVES * (group < 16 ? group : 16) * (DP + 4) * sizeof(float);
+  const auto kernel = a.cache.page_size % 16 == 0 ? attn_decode_kernel<T, DP, true, WAVES> : attn_decode_kernel<T, DP, false, WAVES>;
+  kernel<<<grid, 64 * WAVES, lds, stream>>>(a, p.chunk, group, tiles, partial);
+  return hipGetLastError();
+}
+
+template <int DP>
+constexpr int MANY_WAVES = DP == 256 ? 8 : 16;
+
 template <class T, int DP>
 hipError_t launch_dp(const PagedAttnArgs& a, const PagedAttnPlan& p, float* partial, hipStream_t stream) {
-  const int tiles = head_tiles(a.hq, a.hkv);
-  const unsigned blocks = (unsigned)a.seqs * a.hkv * tiles * p.splits;
-  if (a.cache.page_size % 16 == 0)
-    attn_decode_kernel<T, DP, true><<<blocks, 64 * WAVES, 0, stream>>>(a, p.chunk, p.splits, tiles, partial);
-  else
-    attn_decode_kernel<T, DP, false><<<blocks, 64 * WAVES, 0, stream>>>(a, p.chunk, p.splits, tiles, partial);
-  hipError_t e = hipGetLastError();
+  const hipError_t e = p.waves == 4 ? launch_waves<T, DP, 4>(a, p, partial, stream)
+                                    : launch_waves<T, DP, MANY_WAVES<DP>>(a, p, partial, stream);
   if (e != hipSuccess || p.splits == 1) return e;
-  attn_join_kernel<T><<<(unsigned)(a.seqs * a.hq), 256, 0, stream>>>(a, p.chunk, p.splits, partial);
+  if (p.splits > 8)
+    attn_join_kernel<T, 256><<<dim3(a.hq, a.seqs), 256, 0, stream>>>(a, p.chunk, p.splits, partial);
+  else
+    attn_join_kernel<T, 64><<<dim3((a.hq + 3) / 4, a.seqs), 256, 0, stream>>>(a, p.chunk, p.splits, partial);
   return hipGetLastError();
 }
 
@@ -356,22 +376,33 @@ hipError_t launch_typed(const PagedAttnArgs& a, const PagedAttnPlan& p, float* p
 
 }  // namespace
 
+// Shares of the keys. Where (sequence, key-value head, 16 query heads) items alone do not fill the card, as many workgroups of many waves as do,
+// of at least 512 keys: the shares' launch that joins them costs 4.5 us, and the keys that a workgroup saves by it have to take
+// longer. (One sequence of 131071 keys, 8 key-value heads: 87.5 + 4.6 us; four waves a workgroup and 128 shares 91.2 + 5.5.) Where they do, shares level batches of
+// uneven lengths, of which the host knows only the bound: 40 x 40 items of 1 .. 4096 keys take 196 us unsplit, 132 in
+// shares of 2048 and 113 of 1024, + 4.6 for the join. Even batches lose by it: 128 x 8 items of 1700 .. 2300 keys take
+// 174 us unsplit, 186 in two shares, 196 in three; so a bound of up to 2560 keys is left whole. From 8192 items on the card's dynamic
+// assignment levels them.
 PagedAttnPlan paged_attn_plan(int seqs, int hq, int hkv, int d, int max_len) {
   const long long items = (long long)seqs * hkv * head_tiles(hq, hkv);
-  const long long unit = 256;  // keys that the four waves of a workgroup take in one turn
-  long long splits = items > 0 ? (1024 + items - 1) / items : 1;
-  const long long most = (max_len + unit - 1) / unit;
-  if (splits > most) splits = most;
-  if (splits < 1) splits = 1;
-  const long long per = (max_len + splits - 1) / splits;
-  long long chunk = (per + unit - 1) / unit * unit;
-  if (chunk < unit) chunk = unit;
-  splits = (max_len + chunk - 1) / chunk;
-  if (splits < 1) splits = 1;
   PagedAttnPlan p;
-  p.splits = (int)splits;
-  p.chunk = (int)chunk;
-  p.workspace_bytes = splits > 1 ? (size_t)seqs * hq * splits * (size_t)(d + 2) * 4 : 0;
+  const bool few = items < 128;
+  p.waves = few ? (d > 128 ? 8 : 16) : 4;
+  const long long unit = 16 * p.waves;  // keys of a workgroup's turn
+  long long wanted = 1;
+  if (few)
+    wanted = items > 0 ? (4096 / p.waves + items - 1) / items : 1;
+  else if (items < 8192 && max_len > 2560)
+    wanted = 8;
+  const long long least = few ? 512 : 1024;
+  long long splits = (max_len + least - 1) / least;
+  if (splits > wanted) splits = wanted;
+  if (splits < 1) splits = 1;
+  const long long chunk = ((max_len + splits - 1) / splits + unit - 1) / unit * unit;
+  p.chunk = (int)(chunk < unit ? unit : chunk);
+  p.splits = (int)((max_len + p.chunk - 1) / p.chunk);
+  if (p.splits < 1) p.splits = 1;
+  p.workspace_bytes = p.splits > 1 ? (size_t)seqs * hq * p.splits * (size_t)(d + 2) * 4 : 0;
   return p;
 }
 

@@ -185,6 +185,23 @@ def test_decode_joined_parts(capi, lengths, max_len, Hq, Hkv, D, page):
     check_decode(capi, gen, lengths, Hq, Hkv, D, page, BF, max_len=max_len)
 
 
+@pytest.mark.parametrize("Hq,Hkv,D,page", [(6, 6, 128, 16), (20, 10, 64, 5), (17, 1, 128, 3), (16, 8, 256, 32), (5, 5, 80, 24)])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_decode_of_many_sequences(capi, Hq, Hkv, D, page, dtype):
+    """128 (sequence, key-value head) items and more: workgroups of four waves."""
+    gen = torch.Generator().manual_seed(Hq + D)
+    lengths = [1, 0, 17, 64, 65, 130] * (1 + 128 // (6 * Hkv))
+    check_decode(capi, gen, lengths, Hq, Hkv, D, page, dtype)
+
+
+@pytest.mark.parametrize("Hq,Hkv,D,page", [(128, 128, 16, 16), (160, 130, 8, 7)])
+def test_decode_joined_parts_of_many_items(capi, Hq, Hkv, D, page):
+    gen = torch.Generator().manual_seed(Hq)
+    Hq = Hkv if Hq % Hkv else Hq
+    assert capi.lib().fsw_attn_decode_workspace_bytes(0, 2, Hq, Hkv, D, 2600) > 0
+    check_decode(capi, gen, [2600, 1030], Hq, Hkv, D, page, BF)
+
+
 @pytest.mark.parametrize("holes", [float("inf"), float("-inf"), NAN, torch.finfo(BF).min])
 def test_decode_ignores_what_lies_behind_a_length(capi, holes):
     gen = torch.Generator().manual_seed(9)

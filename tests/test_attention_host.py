@@ -55,7 +55,7 @@ def test_attn_decode_codes(capi, cache):
         return capi.lib().fsw_validate_attn_decode(dtype, B, Hq, Hkv, D, *q, c or cache(), table, ld, lengths, max_len, scale, *o)
     assert v() == v(B=0, q=(None, 0, 0)) == v(max_len=0, table=None, ld=0) == capi.OK
     assert v(dtype=5) == capi.E_DTYPE
-    for kw in (dict(B=-1), dict(B=(1 << 20) + 1), dict(max_len=-1), dict(max_len=(1 << 30) + 1), dict(scale=0.0), dict(scale=-1.0),
+    for kw in (dict(B=-1), dict(B=65536), dict(max_len=-1), dict(max_len=(1 << 30) + 1), dict(scale=0.0), dict(scale=-1.0),
                dict(scale=float("nan")), dict(scale=float("inf")), dict(scale=1e-40), dict(Hq=5), dict(c=cache(pages=0))):
         assert v(**kw) == capi.E_SHAPE, kw
     for kw in (dict(q=(None, 256, 64)), dict(table=None), dict(lengths=None), dict(o=(None, 256, 64)), dict(c=cache(k=None))):
@@ -76,8 +76,9 @@ def test_attn_decode_scratch(capi):
     ws = capi.lib().fsw_attn_decode_workspace_bytes
     assert ws(0, 0, 4, 2, 64, 1000) == ws(0, 4, 4, 2, 64, 0) == ws(7, 4, 4, 2, 64, 1000) == 0
     assert ws(0, 1024, 8, 8, 128, 100000) == 0                        # sequences enough: none is split
+    assert ws(0, 128, 64, 8, 128, 2560) == 0 < ws(0, 128, 64, 8, 128, 2561)
     assert ws(0, 1, 32, 8, 128, 131072) % (32 * (128 + 2) * 4) == 0   # float32 sums, maximum and sum of each part and head
-    for B, n in ((1, 1 << 30), (1 << 20, 1 << 30), (7, 12345)):
+    for B, n in ((1, 1 << 30), (65535, 1 << 30), (7, 12345)):
         assert 0 <= ws(0, B, 1024, 1024, 256, n) < 1 << 42
 
 
