@@ -63,7 +63,7 @@ __device__ __forceinline__ int v_swizzle(int key) {
 }
 
 template <class T, int DP, int NQ>
-__global__ __launch_bounds__(256, 1) void attn_prompt_kernel(PromptArgs a, int slots) {
+__global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prompt_kernel(PromptArgs a, int slots) {
   constexpr int RB = DP * 2, TILE = KEYS * RB, LOADS = TILE / 4096;  // copies per wave and tile
   constexpr int KSTEPS = DP / 16, DB = DP / 32, BM = 128 * NQ;
   __shared__ __align__(1024) unsigned char k0s[TILE];
