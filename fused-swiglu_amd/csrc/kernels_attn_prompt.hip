@@ -16,7 +16,6 @@
 namespace fsw {
 namespace {
 
-typedef __attribute__((ext_vector_type(16))) float f32x16;
 typedef __attribute__((ext_vector_type(4))) short s16x4;
 typedef __attribute__((address_space(3))) void lds_void;
 typedef __attribute__((address_space(3))) unsigned char lds_byte;
@@ -25,16 +24,6 @@ constexpr float NEG_INF = -__builtin_inff();
 constexpr float SLACK = 8.0f;  // the maximum moves only when a score passes it by this much (powers of two): p < 2^8
 constexpr int KEYS = 64;
 
-template <class T>
-__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c);
-template <>
-__device__ __forceinline__ f32x16 mfma32<Bf16>(u32x4 a, u32x4 b, f32x16 c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
-template <>
-__device__ __forceinline__ f32x16 mfma32<Fp16>(u32x4 a, u32x4 b, f32x16 c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-}
 // c + lo + hi of a packed pair
 template <class T>
 __device__ __forceinline__ float add2(unsigned p, float c);
@@ -51,7 +40,7 @@ __device__ __forceinline__ u32x2 read_tr(const unsigned char* p) {
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
 }
 
-// Position of 16-byte vector c of key row `key` in its LDS row: the 16 rows of a K fragment read, and the 4 rows x 64
+// Position of 16-byte vector c of key row `key` in its LDS row: the 16 rows of a K fragment read, and the 8 rows x 32
 // bytes that a half wave of a transposing V read covers, each fall on all 64 banks once.
 template <int DP>
 __device__ __forceinline__ int k_swizzle(int key) {
@@ -59,22 +48,33 @@ __device__ __forceinline__ int k_swizzle(int key) {
 }
 template <int DP>
 __device__ __forceinline__ int v_swizzle(int key) {
-  return DP == 64 ? ((key >> 1) & 1) << 2 : (key & 3) << 2;
+  return DP == 64 ? ((key >> 1) & 3) << 1 : (key & 7) << 1;
 }
 
-template <class T, int DP, int NQ>
-__global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prompt_kernel(PromptArgs a, int slots) {
+// over lanes l, l ^ 16, l ^ 32, l ^ 48: a swap of a register with its copy leaves two groups' values side by side
+__device__ __forceinline__ float max_of_groups(float x) {
+  const unsigned u = __builtin_bit_cast(unsigned, x);
+  const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+  const float y = fmaxf(__builtin_bit_cast(float, a[0]), __builtin_bit_cast(float, a[1]));
+  const unsigned w = __builtin_bit_cast(unsigned, y);
+  const auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
+  return fmaxf(__builtin_bit_cast(float, b[0]), __builtin_bit_cast(float, b[1]));
+}
+
+template <class T, int DP>
+__global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prompt_kernel(PromptArgs a, Divisor by_group, Divisor by_hkv,
+                                                                                  int slots) {
   constexpr int RB = DP * 2, TILE = KEYS * RB, LOADS = TILE / 4096;  // copies per wave and tile
-  constexpr int KSTEPS = DP / 16, DB = DP / 32, BM = 128 * NQ;
+  constexpr int KSTEPS = DP / 32, DB = DP / 16, KB = KEYS / 16, BM = 128;
   __shared__ __align__(1024) unsigned char k0s[TILE];
   __shared__ __align__(1024) unsigned char k1s[TILE];
   __shared__ __align__(1024) unsigned char v0s[TILE];
   __shared__ __align__(1024) unsigned char v1s[TILE];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int col = lane & 31, half = lane >> 5;
-  const int kvh = (int)blockIdx.x % a.hkv, slot = slots - 1 - (int)blockIdx.x / a.hkv;
-  const int group = a.hq / a.hkv;
+  const int col = lane & 15, grp = lane >> 4;
+  const int rank = by_hkv.quotient(blockIdx.x), kvh = (int)blockIdx.x - rank * a.hkv, slot = slots - 1 - rank;
+  const int group = (int)by_group.d;
 
   // Sequence s owns the slots from rows_before(s) / BM + s on, which leaves it enough for its rows whatever their remainder; slot -> s by
   // a search of 64 entries at a time. Entry a.seqs is the rows behind the last sequence.
@@ -111,43 +111,34 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prompt_kernel(Pro
   const int shift = nk - __builtin_amdgcn_readfirstlane(nq) + 1;
   // keys that a row sees
   auto sees = [&](int row) -> int {
-    const int v = (row < rows ? row : rows - 1) / group + shift;
+    const int v = by_group.quotient(row < rows ? row : rows - 1) + shift;
     return v < 0 ? 0 : v < nk ? v : nk;
   };
-  const int wrow = row0 + wave * 32 * NQ;
+  const int wrow = row0 + wave * 32;
   const int block_keys = sees(row0 + BM - 1);
-  int vis[NQ];
-#pragma unroll
-  for (int n = 0; n < NQ; ++n) vis[n] = sees(wrow + 32 * n + col);
   const int wave_first = __builtin_amdgcn_readfirstlane(sees(wrow));
-  const int wave_last = __builtin_amdgcn_readfirstlane(sees(wrow + 32 * NQ - 1));
-
-  u32x4 qf[NQ][KSTEPS];
+  const int wave_last = __builtin_amdgcn_readfirstlane(sees(wrow + 31));
+  int vis[2], tokens[2], heads[2];  // of this lane's rows (one past the sequence repeats its last)
+  u32x4 qf[2][KSTEPS];
 #pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    const int row = wrow + 32 * n + col < rows ? wrow + 32 * n + col : rows - 1;
-    const int token = row / group;
-    const unsigned short* p = (const unsigned short*)a.q.p + (q_at + token) * a.q.token +
-                              (long long)(kvh * group + row - token * group) * a.q.head;
+  for (int n = 0; n < 2; ++n) {
+    const int row = wrow + 16 * n + col < rows ? wrow + 16 * n + col : rows - 1;
+    vis[n] = sees(row);
+    tokens[n] = by_group.quotient(row);
+    heads[n] = kvh * group + row - tokens[n] * group;
+    const unsigned short* p = (const unsigned short*)a.q.p + (q_at + tokens[n]) * a.q.token + heads[n] * a.q.head;
 #pragma unroll
     for (int s = 0; s < KSTEPS; ++s) {
-      const int ch = s * 16 + half * 8;
+      const int ch = s * 32 + grp * 8;
       qf[n][s] = u32x4{0, 0, 0, 0};
       if (ch < a.d) qf[n][s] = *(const u32x4*)(p + ch);
     }
   }
 
-  f32x16 o[DB][NQ];
-  float m[NQ], sum[NQ];
+  f32x4 o[DB][2];
+  float m[2] = {NEG_INF, NEG_INF}, sum[2] = {0.0f, 0.0f};
 #pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    m[n] = NEG_INF;
-    sum[n] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < DB; ++i)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) o[i][n][r] = 0.0f;
-  }
+  for (int i = 0; i < DB; ++i) o[i][0] = o[i][1] = f32x4{0, 0, 0, 0};
 
   // copies: lane -> 16 bytes of LDS, from the vector of the key row that belongs there
   const unsigned char* kp = (const unsigned char*)a.k.p + (k_at * a.k.token + kvh * a.k.head) * 2;
@@ -160,142 +151,138 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prompt_kernel(Pro
     koff[j] = kc * 8 < a.d ? (unsigned)(key * (int)a.k.token * 2 + kc * 16) : OOB_OFFSET;
     voff[j] = vc * 8 < a.d ? (unsigned)(key * (int)a.v.token * 2 + vc * 16) : OOB_OFFSET;
   }
-  auto copy = [&](int at, unsigned char* ks, unsigned char* vs) {
-    const int left = nk - at < KEYS ? nk - at : KEYS;  // rows behind the sequence's end read as zero
-    const auto kr = make_rsrc(kp + at * a.k.token * 2, left > 0 ? (left - 1) * a.k.token * 2 + a.d * 2 : 0);
-    const auto vr = make_rsrc(vp + at * a.v.token * 2, left > 0 ? (left - 1) * a.v.token * 2 + a.d * 2 : 0);
+  // rows behind the sequence's end read as zero
+  auto copy = [&](int at, const unsigned char* p, long long token_stride, const unsigned (&offs)[LOADS], unsigned char* to) {
+    const int left = nk - at < KEYS ? nk - at : KEYS;
+    const auto rsrc = make_rsrc(p + at * token_stride * 2, left > 0 ? (left - 1) * token_stride * 2 + a.d * 2 : 0);
 #pragma unroll
     for (int j = 0; j < LOADS; ++j)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(kr, (lds_void*)(ks + (j * 4 + wave) * 1024), 16, (int)koff[j], 0, 0, 0);
-#pragma unroll
-    for (int j = 0; j < LOADS; ++j)
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(vr, (lds_void*)(vs + (j * 4 + wave) * 1024), 16, (int)voff[j], 0, 0, 0);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void*)(to + (j * 4 + wave) * 1024), 16, (int)offs[j], 0, 0, 0);
   };
+  auto copy_k = [&](int at, unsigned char* to) { copy(at, kp, a.k.token, koff, to); };
+  auto copy_v = [&](int at, unsigned char* to) { copy(at, vp, a.v.token, voff, to); };
 
   const float c = a.scale_log2, slack = SLACK / c;
   auto attend = [&](int at, const unsigned char* ks, const unsigned char* vs) {
     if (at >= wave_last) return;
-    f32x16 s[2][NQ];
+    f32x4 s[KB][2];
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
-#pragma unroll
-      for (int n = 0; n < NQ; ++n)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[kb][n][r] = 0.0f;
-      const int key = kb * 32 + col;
+    for (int kb = 0; kb < KB; ++kb) {
+      s[kb][0] = s[kb][1] = f32x4{0, 0, 0, 0};
+      const int key = kb * 16 + col;
 #pragma unroll
       for (int st = 0; st < KSTEPS; ++st) {
-        const u32x4 kf = *(const u32x4*)(ks + key * RB + ((2 * st + half) ^ k_swizzle<DP>(key)) * 16);
+        const u32x4 kf = *(const u32x4*)(ks + key * RB + ((4 * st + grp) ^ k_swizzle<DP>(key)) * 16);
 #pragma unroll
-        for (int n = 0; n < NQ; ++n) s[kb][n] = mfma32<T>(kf, qf[n][st], s[kb][n]);
+        for (int n = 0; n < 2; ++n) s[kb][n] = T::mfma16(kf, qf[n][st], s[kb][n]);
       }
     }
     if (at + KEYS > wave_first) {
 #pragma unroll
-      for (int n = 0; n < NQ; ++n) {
-        const int left = vis[n] - at - 4 * half;
+      for (int n = 0; n < 2; ++n) {
+        const int left = vis[n] - at - 4 * grp;
 #pragma unroll
-        for (int kb = 0; kb < 2; ++kb)
+        for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-          for (int r = 0; r < 16; ++r)
-            if (kb * 32 + (r / 4) * 8 + r % 4 >= left) s[kb][n][r] = NEG_INF;
+          for (int r = 0; r < 4; ++r)
+            if (kb * 16 + r >= left) s[kb][n][r] = NEG_INF;
       }
     }
-    unsigned p[NQ][2][8];
+    float top[2];
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-      float top = s[0][n][0];
+    for (int n = 0; n < 2; ++n) {
+      float t[KB];
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
+      for (int kb = 0; kb < KB; ++kb) t[kb] = fmaxf(fmaxf(s[kb][n][0], s[kb][n][1]), fmaxf(s[kb][n][2], s[kb][n][3]));
+      top[n] = max_of_groups(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])));
+    }
+    if (__any(top[0] > m[0] + slack || top[1] > m[1] + slack)) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) top = fmaxf(top, s[kb][n][r]);
-      top = fmaxf(top, __shfl_xor(top, 32));
-      if (__any(top > m[n] + slack)) {
-        const float now = fmaxf(m[n], top);
+      for (int n = 0; n < 2; ++n) {
+        const float now = fmaxf(m[n], top[n]);
         const float alpha = now == m[n] ? 1.0f : __builtin_amdgcn_exp2f((m[n] - now) * c);
         m[n] = now;
         sum[n] *= alpha;
 #pragma unroll
         for (int i = 0; i < DB; ++i)
 #pragma unroll
-          for (int r = 0; r < 16; ++r) o[i][n][r] *= alpha;
+          for (int r = 0; r < 4; ++r) o[i][n][r] *= alpha;
       }
+    }
+    unsigned p[2][KB][2];
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
       const float mc = m[n] == NEG_INF ? 0.0f : m[n] * c;
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
+      for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-        for (int r = 0; r < 16; r += 2) {
+        for (int r = 0; r < 4; r += 2) {
           const float lo = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][n][r], c, -mc));
           const float hi = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][n][r + 1], c, -mc));
           p[n][kb][r / 2] = T::pack2(lo, hi);
           sum[n] = add2<T>(p[n][kb][r / 2], sum[n]);
         }
     }
-    const int i16 = lane & 15, sub = (lane >> 4) & 1;
 #pragma unroll
-    for (int st = 0; st < 4; ++st) {
+    for (int st = 0; st < KB / 2; ++st) {
 #pragma unroll
       for (int i = 0; i < DB; ++i) {
-        const int key = st * 16 + 4 * half + (i16 >> 2);
-        const int ch = i * 4 + sub * 2 + ((i16 & 3) >> 1);
-        const u32x2 lo = read_tr(vs + key * RB + (ch ^ v_swizzle<DP>(key)) * 16 + (i16 & 1) * 8);
-        const u32x2 hi = read_tr(vs + (key + 8) * RB + (ch ^ v_swizzle<DP>(key + 8)) * 16 + (i16 & 1) * 8);
-        const u32x4 vf = {lo[0], lo[1], hi[0], hi[1]};
+        const int key = st * 32 + 4 * grp + (col >> 2), ch = i * 2 + ((col & 3) >> 1);
+        const u32x2 lo = read_tr(vs + key * RB + (ch ^ v_swizzle<DP>(key)) * 16 + (col & 1) * 8);
+        const u32x2 hi = read_tr(vs + (key + 16) * RB + (ch ^ v_swizzle<DP>(key + 16)) * 16 + (col & 1) * 8);
 #pragma unroll
-        for (int n = 0; n < NQ; ++n) {
-          const unsigned* pp = &p[n][st >> 1][(st & 1) * 4];
-          o[i][n] = mfma32<T>(vf, u32x4{pp[0], pp[1], pp[2], pp[3]}, o[i][n]);
-        }
+        for (int n = 0; n < 2; ++n)
+          o[i][n] = T::mfma16(u32x4{lo[0], lo[1], hi[0], hi[1]},
+                              u32x4{p[n][2 * st][0], p[n][2 * st][1], p[n][2 * st + 1][0], p[n][2 * st + 1][1]}, o[i][n]);
       }
     }
   };
 
   // tile t is in buffer t % 2; copies of tile t + 1 are under way while tile t is worked on
-  if (block_keys > 0) copy(0, k0s, v0s);
+  auto copy_both = [&](int at, unsigned char* ks, unsigned char* vs) {
+    copy_k(at, ks);
+    copy_v(at, vs);
+  };
+  if (block_keys > 0) copy_both(0, k0s, v0s);
   for (int at = 0; at < block_keys; at += 2 * KEYS) {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (at + KEYS < block_keys) copy(at + KEYS, k1s, v1s);
+    if (at + KEYS < block_keys) copy_both(at + KEYS, k1s, v1s);
     attend(at, k0s, v0s);
     if (at + KEYS >= block_keys) break;
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (at + 2 * KEYS < block_keys) copy(at + 2 * KEYS, k0s, v0s);
+    if (at + 2 * KEYS < block_keys) copy_both(at + 2 * KEYS, k0s, v0s);
     attend(at + KEYS, k1s, v1s);
   }
 
 #pragma unroll
-  for (int n = 0; n < NQ; ++n) {
-    const int row = wrow + 32 * n + col;
-    const float total = sum[n] + __shfl_xor(sum[n], 32);
-    if (row >= rows) continue;
+  for (int n = 0; n < 2; ++n) {
+    float total = sum[n] + __shfl_xor(sum[n], 16);
+    total += __shfl_xor(total, 32);
+    if (wrow + 16 * n + col >= rows) continue;
     const float inv = vis[n] > 0 ? 1.0f / total : 0.0f;
-    const int token = row / group;
-    unsigned short* p = (unsigned short*)a.o.p + (q_at + token) * a.o.token +
-                        (long long)(kvh * group + row - token * group) * a.o.head;
+    unsigned short* p = (unsigned short*)a.o.p + (q_at + tokens[n]) * a.o.token + heads[n] * a.o.head;
 #pragma unroll
-    for (int i = 0; i < DB; ++i)
-#pragma unroll
-      for (int r = 0; r < 16; r += 4) {
-        const int ch = i * 32 + (r / 4) * 8 + 4 * half;
-        if (ch < a.d)
-          *(u32x2*)(p + ch) = u32x2{T::pack2(o[i][n][r] * inv, o[i][n][r + 1] * inv),
-                                    T::pack2(o[i][n][r + 2] * inv, o[i][n][r + 3] * inv)};
-      }
+    for (int i = 0; i < DB; ++i) {
+      const int ch = i * 16 + 4 * grp;
+      if (ch < a.d)
+        *(u32x2*)(p + ch) = u32x2{T::pack2(o[i][n][0] * inv, o[i][n][1] * inv), T::pack2(o[i][n][2] * inv, o[i][n][3] * inv)};
+    }
   }
 }
 
-template <class T, int DP, int NQ>
+template <class T, int DP>
 hipError_t launch(const PromptArgs& a, hipStream_t stream) {
   const long long rows = (long long)a.tq * (a.hq / a.hkv);
-  const long long slots = rows / (128 * NQ) + a.seqs + 1;
-  attn_prompt_kernel<T, DP, NQ><<<(unsigned)(slots * a.hkv), 256, 0, stream>>>(a, (int)slots);
+  const long long slots = rows / 128 + a.seqs + 1;
+  attn_prompt_kernel<T, DP><<<(unsigned)(slots * a.hkv), 256, 0, stream>>>(a, Divisor(a.hq / a.hkv), Divisor(a.hkv), (int)slots);
   return hipGetLastError();
 }
 
 template <class T>
 hipError_t launch_typed(const PromptArgs& a, hipStream_t stream) {
-  if (a.d <= 64) return launch<T, 64, 1>(a, stream);
-  if (a.d <= 128) return launch<T, 128, 1>(a, stream);
-  return launch<T, 256, 1>(a, stream);
+  if (a.d <= 64) return launch<T, 64>(a, stream);
+  if (a.d <= 128) return launch<T, 128>(a, stream);
+  return launch<T, 256>(a, stream);
 }
 
 }  // namespace
