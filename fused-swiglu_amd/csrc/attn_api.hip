@@ -50,7 +50,7 @@ int check_out(const void* p, int64_t n, int64_t token, int64_t heads, int64_t he
 int check_cache(const fsw_kv_cache* c, int64_t d, int64_t heads) {
   if (!c || !c->k || !c->v) return FSW_E_NULL;
   if (c->pages < 1 || c->page_size < 1 || c->pages > 0x7fffffff || c->page_size > 0x7fffffff ||
-      c->pages * c->page_size > 0x7fffffff)
+      c->pages * c->page_size > MAX_LEN)
     return FSW_E_SHAPE;
   const int64_t strides[3] = {c->page_stride, c->head_stride, c->token_stride}, n[3] = {c->pages, heads, c->page_size};
   for (int i = 0; i < 3; ++i) {

@@ -61,11 +61,11 @@ __device__ __forceinline__ float max_of_groups(float x) {
   return fmaxf(__builtin_bit_cast(float, b[0]), __builtin_bit_cast(float, b[1]));
 }
 
-template <class T, int DP>
+template <class T, int DP, int NB>
 __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prompt_kernel(PromptArgs a, Divisor by_group, Divisor by_hkv,
                                                                                   int slots) {
   constexpr int RB = DP * 2, TILE = KEYS * RB, LOADS = TILE / 4096;  // copies per wave and tile
-  constexpr int KSTEPS = DP / 32, DB = DP / 16, KB = KEYS / 16, BM = 128;
+  constexpr int KSTEPS = DP / 32, DB = DP / 16, KB = KEYS / 16, WM = 16 * NB, BM = 4 * WM;
   __shared__ __align__(1024) unsigned char k0s[TILE];
   __shared__ __align__(1024) unsigned char k1s[TILE];
   __shared__ __align__(1024) unsigned char v0s[TILE];
@@ -114,14 +114,14 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prompt_kernel(Pro
     const int v = by_group.quotient(row < rows ? row : rows - 1) + shift;
     return v < 0 ? 0 : v < nk ? v : nk;
   };
-  const int wrow = row0 + wave * 32;
+  const int wrow = row0 + wave * WM;
   const int block_keys = sees(row0 + BM - 1);
   const int wave_first = __builtin_amdgcn_readfirstlane(sees(wrow));
-  const int wave_last = __builtin_amdgcn_readfirstlane(sees(wrow + 31));
-  int vis[2], tokens[2], heads[2];  // of this lane's rows (one past the sequence repeats its last)
-  u32x4 qf[2][KSTEPS];
+  const int wave_last = __builtin_amdgcn_readfirstlane(sees(wrow + WM - 1));
+  int vis[NB], tokens[NB], heads[NB];  // of this lane's rows (one past the sequence repeats its last)
+  u32x4 qf[NB][KSTEPS];
 #pragma unroll
-  for (int n = 0; n < 2; ++n) {
+  for (int n = 0; n < NB; ++n) {
     const int row = wrow + 16 * n + col < rows ? wrow + 16 * n + col : rows - 1;
     vis[n] = sees(row);
     tokens[n] = by_group.quotient(row);
@@ -135,10 +135,15 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prompt_kernel(Pro
     }
   }
 
-  f32x4 o[DB][2];
-  float m[2] = {NEG_INF, NEG_INF}, sum[2] = {0.0f, 0.0f};
+  f32x4 o[DB][NB];
+  float m[NB], sum[NB];
 #pragma unroll
-  for (int i = 0; i < DB; ++i) o[i][0] = o[i][1] = f32x4{0, 0, 0, 0};
+  for (int n = 0; n < NB; ++n) {
+    m[n] = NEG_INF;
+    sum[n] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < DB; ++i) o[i][n] = f32x4{0, 0, 0, 0};
+  }
 
   // copies: lane -> 16 bytes of LDS, from the vector of the key row that belongs there
   const unsigned char* kp = (const unsigned char*)a.k.p + (k_at * a.k.token + kvh * a.k.head) * 2;
@@ -165,21 +170,22 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prompt_kernel(Pro
   const float c = a.scale_log2, slack = SLACK / c;
   auto attend = [&](int at, const unsigned char* ks, const unsigned char* vs) {
     if (at >= wave_last) return;
-    f32x4 s[KB][2];
+    f32x4 s[KB][NB];
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
-      s[kb][0] = s[kb][1] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int n = 0; n < NB; ++n) s[kb][n] = f32x4{0, 0, 0, 0};
       const int key = kb * 16 + col;
 #pragma unroll
       for (int st = 0; st < KSTEPS; ++st) {
         const u32x4 kf = *(const u32x4*)(ks + key * RB + ((4 * st + grp) ^ k_swizzle<DP>(key)) * 16);
 #pragma unroll
-        for (int n = 0; n < 2; ++n) s[kb][n] = T::mfma16(kf, qf[n][st], s[kb][n]);
+        for (int n = 0; n < NB; ++n) s[kb][n] = T::mfma16(kf, qf[n][st], s[kb][n]);
       }
     }
     if (at + KEYS > wave_first) {
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
+      for (int n = 0; n < NB; ++n) {
         const int left = vis[n] - at - 4 * grp;
 #pragma unroll
         for (int kb = 0; kb < KB; ++kb)
@@ -188,17 +194,19 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prompt_kernel(Pro
             if (kb * 16 + r >= left) s[kb][n][r] = NEG_INF;
       }
     }
-    float top[2];
+    float top[NB];
+    bool above = false;
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
+    for (int n = 0; n < NB; ++n) {
       float t[KB];
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) t[kb] = fmaxf(fmaxf(s[kb][n][0], s[kb][n][1]), fmaxf(s[kb][n][2], s[kb][n][3]));
       top[n] = max_of_groups(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])));
+      above |= top[n] > m[n] + slack;
     }
-    if (__any(top[0] > m[0] + slack || top[1] > m[1] + slack)) {
+    if (__any(above)) {
 #pragma unroll
-      for (int n = 0; n < 2; ++n) {
+      for (int n = 0; n < NB; ++n) {
         const float now = fmaxf(m[n], top[n]);
         const float alpha = now == m[n] ? 1.0f : __builtin_amdgcn_exp2f((m[n] - now) * c);
         m[n] = now;
@@ -209,9 +217,9 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prompt_kernel(Pro
           for (int r = 0; r < 4; ++r) o[i][n][r] *= alpha;
       }
     }
-    unsigned p[2][KB][2];
+    unsigned p[NB][KB][2];
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
+    for (int n = 0; n < NB; ++n) {
       const float mc = m[n] == NEG_INF ? 0.0f : m[n] * c;
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
@@ -231,31 +239,35 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prompt_kernel(Pro
         const u32x2 lo = read_tr(vs + key * RB + (ch ^ v_swizzle<DP>(key)) * 16 + (col & 1) * 8);
         const u32x2 hi = read_tr(vs + (key + 16) * RB + (ch ^ v_swizzle<DP>(key + 16)) * 16 + (col & 1) * 8);
 #pragma unroll
-        for (int n = 0; n < 2; ++n)
+        for (int n = 0; n < NB; ++n)
           o[i][n] = T::mfma16(u32x4{lo[0], lo[1], hi[0], hi[1]},
                               u32x4{p[n][2 * st][0], p[n][2 * st][1], p[n][2 * st + 1][0], p[n][2 * st + 1][1]}, o[i][n]);
       }
     }
   };
 
-  // tile t is in buffer t % 2; copies of tile t + 1 are under way while tile t is worked on
-  auto copy_both = [&](int at, unsigned char* ks, unsigned char* vs) {
-    copy_k(at, ks);
-    copy_v(at, vs);
+  // Tile t is in buffer t % 2; copies of tile t + 1 are under way while tile t is worked on. They are issued whether or not there
+  // is one (a descriptor of no bytes reads zeros and touches no memory): behind a branch the compiler no longer knows how many copies are
+  // younger than the tile that it is about to read, and waits for all of them.
+  auto turn = [&](int at, const unsigned char* ks, const unsigned char* vs, unsigned char* knext, unsigned char* vnext) {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    copy_k(at + KEYS, knext);
+    copy_v(at + KEYS, vnext);
+    attend(at, ks, vs);
   };
-  if (block_keys > 0) copy_both(0, k0s, v0s);
-  for (int at = 0; at < block_keys; at += 2 * KEYS) {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (at + KEYS < block_keys) copy_both(at + KEYS, k1s, v1s);
-    attend(at, k0s, v0s);
-    if (at + KEYS >= block_keys) break;
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (at + 2 * KEYS < block_keys) copy_both(at + 2 * KEYS, k0s, v0s);
-    attend(at + KEYS, k1s, v1s);
+  if (block_keys > 0) {
+    copy_k(0, k0s);
+    copy_v(0, v0s);
+    for (int at = 0; at < block_keys; at += 2 * KEYS) {
+      turn(at, k0s, v0s, k1s, v1s);
+      if (at + KEYS >= block_keys) break;
+      turn(at + KEYS, k1s, v1s, k0s, v0s);
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no copy is under way when the LDS becomes another workgroup's
   }
 
 #pragma unroll
-  for (int n = 0; n < 2; ++n) {
+  for (int n = 0; n < NB; ++n) {
     float total = sum[n] + __shfl_xor(sum[n], 16);
     total += __shfl_xor(total, 32);
     if (wrow + 16 * n + col >= rows) continue;
@@ -270,19 +282,31 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prompt_kernel(Pro
   }
 }
 
-template <class T, int DP>
+template <class T, int DP, int NB>
 hipError_t launch(const PromptArgs& a, hipStream_t stream) {
   const long long rows = (long long)a.tq * (a.hq / a.hkv);
-  const long long slots = rows / 128 + a.seqs + 1;
-  attn_prompt_kernel<T, DP><<<(unsigned)(slots * a.hkv), 256, 0, stream>>>(a, Divisor(a.hq / a.hkv), Divisor(a.hkv), (int)slots);
+  const long long slots = rows / (64 * NB) + a.seqs + 1;
+  attn_prompt_kernel<T, DP, NB><<<(unsigned)(slots * a.hkv), 256, 0, stream>>>(a, Divisor(a.hq / a.hkv), Divisor(a.hkv), (int)slots);
   return hipGetLastError();
+}
+
+// 64 rows a workgroup (16 a wave) where workgroups of 128 (32 a wave) would all be resident at once: half the rows are then not half the
+// rate, because no second round follows, and the longest workgroup's walk is what the launch takes. Above that 32 rows a wave
+// share each fragment that is read from LDS. 128 against 64 rows, us, 128 channels: 1000 tokens of 32 heads on 8 (252 workgroups of 128
+// rows) 27.4 | 22.8, 2000 (504) 56.2 | 55.3, 3000 (752) 92 | 110, 8192 of 64 heads 1096 | 1425; 64 channels: 2000 tokens of 16
+// heads on 4 (252) 33.6 | 25.5, 6000 (752) 115 | 107; 256 channels: 1000 tokens of 16 heads on 8 (128) 49 | 34, 4000 (500) 199 | 250.
+template <class T, int DP>
+hipError_t launch_dp(const PromptArgs& a, hipStream_t stream) {
+  constexpr int resident = 256 * (DP == 64 ? 3 : DP == 128 ? 2 : 1);  // workgroups of 128 rows, by LDS and registers
+  const long long rows = (long long)a.tq * (a.hq / a.hkv);
+  return (rows / 128 + a.seqs) * a.hkv <= resident ? launch<T, DP, 1>(a, stream) : launch<T, DP, 2>(a, stream);
 }
 
 template <class T>
 hipError_t launch_typed(const PromptArgs& a, hipStream_t stream) {
-  if (a.d <= 64) return launch<T, 64>(a, stream);
-  if (a.d <= 128) return launch<T, 128>(a, stream);
-  return launch<T, 256>(a, stream);
+  if (a.d <= 64) return launch_dp<T, 64>(a, stream);
+  if (a.d <= 128) return launch_dp<T, 128>(a, stream);
+  return launch_dp<T, 256>(a, stream);
 }
 
 }  // namespace

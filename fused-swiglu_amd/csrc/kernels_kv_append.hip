@@ -55,26 +55,19 @@ struct Dest {
 };
 
 template <class T, int STYLE, int HEADS>
-__global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a, int units, int groups, int tokens_per_block,
-                                                        int blocks_per_token) {
-  const int per_token = units * groups;
-  int token, item;
-  if (blocks_per_token == 1) {
-    const int local = (int)threadIdx.x / per_token;
-    if (local >= tokens_per_block) return;
-    token = (int)blockIdx.x * tokens_per_block + local;
-    item = (int)threadIdx.x - local * per_token;
-  } else {
-    token = (int)blockIdx.x / blocks_per_token;
-    item = ((int)blockIdx.x - token * blocks_per_token) * 256 + (int)threadIdx.x;
-  }
-  if (token >= a.tokens || item >= per_token) return;
-  const int unit = item % units, first = (item / units) * HEADS;
+__global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a, Divisor units, Divisor per_token, int tokens_per_block) {
+  // blockIdx.y = 256 threads of a token that needs more, else the block has several tokens
+  const int local = gridDim.y == 1 ? per_token.quotient(threadIdx.x) : 0;
+  if (local >= tokens_per_block) return;
+  const int token = (int)blockIdx.x * tokens_per_block + local;
+  const int item = (int)blockIdx.y * 256 + (int)threadIdx.x - local * (int)per_token.d;
+  if (token >= a.tokens || item >= (int)per_token.d) return;
+  const int set = units.quotient(item), unit = item - set * (int)units.d, first = set * HEADS;
   const int heads = a.hq + 2 * a.hkv, half = a.rot / 2;
 
   const int slot = a.slots[token], pos = a.positions[token];
   const bool stored = slot >= 0 && slot < a.cache.pages * a.cache.page_size;
-  const int page = stored ? slot / a.cache.page_size : 0;
+  const int page = stored ? a.cache.per_page.quotient(slot) : 0;
   const long long cell = (long long)page * a.cache.page + (long long)(slot - page * a.cache.page_size) * a.cache.token;
   const bool known = pos >= 0 && pos < a.table_rows;
   const float* cs = a.cos_sin + (long long)(known ? pos : 0) * a.rot;
@@ -188,10 +181,9 @@ __global__ __launch_bounds__(256) void kv_append_kernel(AppendArgs a, int units,
 template <class T, int STYLE, int HEADS>
 hipError_t launch(const AppendArgs& a, hipStream_t stream) {
   const int units = units_of(STYLE, a.d, a.rot), groups = (a.hq + 2 * a.hkv + HEADS - 1) / HEADS;
-  const int per_token = units * groups;
-  const int tpb = per_token < 256 ? 256 / per_token : 1, bpt = (per_token + 255) / 256;
-  const unsigned blocks = bpt == 1 ? (unsigned)((a.tokens + tpb - 1) / tpb) : (unsigned)a.tokens * (unsigned)bpt;
-  kv_append_kernel<T, STYLE, HEADS><<<blocks, 256, 0, stream>>>(a, units, groups, tpb, bpt);
+  const int per_token = units * groups, per_block = per_token <= 256 ? 256 / per_token : 1;
+  const dim3 grid((a.tokens + per_block - 1) / per_block, (per_token + 255) / 256);
+  kv_append_kernel<T, STYLE, HEADS><<<grid, 256, 0, stream>>>(a, Divisor(units), Divisor(per_token), per_block);
   return hipGetLastError();
 }
 
