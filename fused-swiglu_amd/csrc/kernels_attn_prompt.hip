@@ -24,6 +24,8 @@ constexpr float NEG_INF = -__builtin_inff();
 constexpr float SLACK = 8.0f;  // the maximum moves only when a score passes it by this much (powers of two): p < 2^8
 constexpr int KEYS = 64;
 
+#define INLINE __attribute__((always_inline))
+
 // c + lo + hi of a packed pair
 template <class T>
 __device__ __forceinline__ float add2(unsigned p, float c);
@@ -35,6 +37,14 @@ template <>
 __device__ __forceinline__ float add2<Fp16>(unsigned p, float c) {
   return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, p), __builtin_bit_cast(f16x2, 0x3c003c00u), c, false);
 }
+
+// exponent of infinities and NaN; sizes above it are NaN
+template <class T>
+constexpr unsigned INF_BITS = 0;
+template <>
+constexpr unsigned INF_BITS<Bf16> = 0x7f80;
+template <>
+constexpr unsigned INF_BITS<Fp16> = 0x7c00;
 
 __device__ __forceinline__ u32x2 read_tr(const unsigned char* p) {
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
@@ -70,6 +80,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prompt_kernel(Pro
   __shared__ __align__(1024) unsigned char k1s[TILE];
   __shared__ __align__(1024) unsigned char v0s[TILE];
   __shared__ __align__(1024) unsigned char v1s[TILE];
+  __shared__ int odd_sums[4];
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, grp = lane >> 4;
@@ -137,13 +148,6 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prompt_kernel(Pro
 
   f32x4 o[DB][NB];
   float m[NB], sum[NB];
-#pragma unroll
-  for (int n = 0; n < NB; ++n) {
-    m[n] = NEG_INF;
-    sum[n] = 0.0f;
-#pragma unroll
-    for (int i = 0; i < DB; ++i) o[i][n] = f32x4{0, 0, 0, 0};
-  }
 
   // copies: lane -> 16 bytes of LDS, from the vector of the key row that belongs there
   const unsigned char* kp = (const unsigned char*)a.k.p + (k_at * a.k.token + kvh * a.k.head) * 2;
@@ -157,18 +161,25 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prompt_kernel(Pro
     voff[j] = vc * 8 < a.d ? (unsigned)(key * (int)a.v.token * 2 + vc * 16) : OOB_OFFSET;
   }
   // rows behind the sequence's end read as zero
-  auto copy = [&](int at, const unsigned char* p, long long token_stride, const unsigned (&offs)[LOADS], unsigned char* to) {
+  auto copy = [&](int at, const unsigned char* p, long long token_stride, const unsigned (&offs)[LOADS], unsigned char* to) INLINE {
     const int left = nk - at < KEYS ? nk - at : KEYS;
     const auto rsrc = make_rsrc(p + at * token_stride * 2, left > 0 ? (left - 1) * token_stride * 2 + a.d * 2 : 0);
 #pragma unroll
     for (int j = 0; j < LOADS; ++j)
       __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (lds_void*)(to + (j * 4 + wave) * 1024), 16, (int)offs[j], 0, 0, 0);
   };
-  auto copy_k = [&](int at, unsigned char* to) { copy(at, kp, a.k.token, koff, to); };
-  auto copy_v = [&](int at, unsigned char* to) { copy(at, vp, a.v.token, voff, to); };
+  auto copy_k = [&](int at, unsigned char* to) INLINE { copy(at, kp, a.k.token, koff, to); };
+  auto copy_v = [&](int at, unsigned char* to) INLINE { copy(at, vp, a.v.token, voff, to); };
 
   const float c = a.scale_log2, slack = SLACK / c;
-  auto attend = [&](int at, const unsigned char* ks, const unsigned char* vs) {
+  // 16 channels x 32 keys: keys 4 g .. 4 g + 3 and 16 + 4 g .. 19 + 4 g of lane group g
+  auto value_fragment = [&](const unsigned char* vs, int st, int i) INLINE -> u32x4 {
+    const int key = st * 32 + 4 * grp + (col >> 2), ch = i * 2 + ((col & 3) >> 1);
+    const u32x2 lo = read_tr(vs + key * RB + (ch ^ v_swizzle<DP>(key)) * 16 + (col & 1) * 8);
+    const u32x2 hi = read_tr(vs + (key + 16) * RB + (ch ^ v_swizzle<DP>(key + 16)) * 16 + (col & 1) * 8);
+    return u32x4{lo[0], lo[1], hi[0], hi[1]};
+  };
+  auto attend = [&](int at, const unsigned char* ks, const unsigned char* vs) INLINE {
     if (at >= wave_last) return;
     f32x4 s[KB][NB];
 #pragma unroll
@@ -232,30 +243,51 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prompt_kernel(Pro
         }
     }
 #pragma unroll
-    for (int st = 0; st < KB / 2; ++st) {
+    for (int st = 0; st < KB / 2; ++st)
 #pragma unroll
       for (int i = 0; i < DB; ++i) {
-        const int key = st * 32 + 4 * grp + (col >> 2), ch = i * 2 + ((col & 3) >> 1);
-        const u32x2 lo = read_tr(vs + key * RB + (ch ^ v_swizzle<DP>(key)) * 16 + (col & 1) * 8);
-        const u32x2 hi = read_tr(vs + (key + 16) * RB + (ch ^ v_swizzle<DP>(key + 16)) * 16 + (col & 1) * 8);
+        const u32x4 vf = value_fragment(vs, st, i);
 #pragma unroll
         for (int n = 0; n < NB; ++n)
-          o[i][n] = T::mfma16(u32x4{lo[0], lo[1], hi[0], hi[1]},
-                              u32x4{p[n][2 * st][0], p[n][2 * st][1], p[n][2 * st + 1][0], p[n][2 * st + 1][1]}, o[i][n]);
+          o[i][n] = T::mfma16(vf, u32x4{p[n][2 * st][0], p[n][2 * st][1], p[n][2 * st + 1][0], p[n][2 * st + 1][1]}, o[i][n]);
       }
-    }
   };
 
   // Tile t is in buffer t % 2; copies of tile t + 1 are under way while tile t is worked on. They are issued whether or not there
   // is one (a descriptor of no bytes reads zeros and touches no memory): behind a branch the compiler no longer knows how many copies are
   // younger than the tile that it is about to read, and waits for all of them.
-  auto turn = [&](int at, const unsigned char* ks, const unsigned char* vs, unsigned char* knext, unsigned char* vnext) {
+  // A weight of zero does not silence an infinity or a NaN: where the diagonal cuts a tile, a value that a row does not see could
+  // reach it. That is rare, so it is noticed at the end, by a sum that is not finite, and all keys are taken once more with zeros in
+  // place of such values (which gives the other sums bit for bit as before); what each row sees of them is added to its output then.
+  auto silence = [&](unsigned char* vs) INLINE {
+#pragma unroll 1
+    for (int byte = (int)threadIdx.x * 16; byte < TILE; byte += 4096) {
+      u32x4 x = *(u32x4*)(vs + byte);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if ((x[j] & INF_BITS<T>) == INF_BITS<T>) x[j] &= 0xffff0000u;
+        if ((x[j] >> 16 & INF_BITS<T>) == INF_BITS<T>) x[j] &= 0xffffu;
+      }
+      *(u32x4*)(vs + byte) = x;
+    }
+    __syncthreads();
+  };
+  bool again = false;
+  auto turn = [&](int at, const unsigned char* ks, unsigned char* vs, unsigned char* knext, unsigned char* vnext) INLINE {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     copy_k(at + KEYS, knext);
     copy_v(at + KEYS, vnext);
+    if (__builtin_expect(again, 0)) silence(vs);
     attend(at, ks, vs);
   };
-  if (block_keys > 0) {
+  while (true) {
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      m[n] = NEG_INF;
+      sum[n] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < DB; ++i) o[i][n] = f32x4{0, 0, 0, 0};
+    }
     copy_k(0, k0s);
     copy_v(0, v0s);
     for (int at = 0; at < block_keys; at += 2 * KEYS) {
@@ -263,7 +295,19 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prompt_kernel(Pro
       if (at + KEYS >= block_keys) break;
       turn(at + KEYS, k1s, v1s, k0s, v0s);
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // no copy is under way when the LDS becomes another workgroup's
+    float probe = 0.0f;
+#pragma unroll
+    for (int n = 0; n < NB; ++n)
+#pragma unroll
+      for (int i = 0; i < DB; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) probe += o[i][n][r] * 0.0f;
+    const int odd = __any(!(probe == 0.0f));
+    if (lane == 0) odd_sums[wave] = odd;
+    // also: no copy is under way, and no read, when the LDS is filled again or becomes another workgroup's
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (again || __builtin_expect(!(odd_sums[0] | odd_sums[1] | odd_sums[2] | odd_sums[3]), 1)) break;
+    again = true;
   }
 
 #pragma unroll
@@ -278,6 +322,34 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prompt_kernel(Pro
       const int ch = i * 16 + 4 * grp;
       if (ch < a.d)
         *(u32x2*)(p + ch) = u32x2{T::pack2(o[i][n][0] * inv, o[i][n][1] * inv), T::pack2(o[i][n][2] * inv, o[i][n][3] * inv)};
+    }
+  }
+  if (__builtin_expect(!again, 1)) return;
+  // A lane owns a channel and walks the values in the order in which the wave's rows come to see them.
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the rows above are written
+#pragma unroll 1
+  for (int ch = lane; ch < a.d; ch += 64) {
+    const unsigned short* v = (const unsigned short*)vp + ch;
+    bool up = false, down = false, none = false;
+    int key = 0;
+#pragma unroll 1
+    for (int row = wrow; row < wrow + WM && row < rows; ++row) {
+      const int end = sees(row);
+#pragma unroll 8
+      for (; key < end; ++key) {
+        const unsigned x = v[key * a.v.token], size = x & 0x7fffu;
+        none |= size > INF_BITS<T>;
+        up |= x == INF_BITS<T>;
+        down |= size == INF_BITS<T> && x != size;
+      }
+      if (!(up || down || none)) continue;
+      const int token = by_group.quotient(row);
+      unsigned short* p = (unsigned short*)a.o.p + (q_at + token) * a.o.token +
+                          (long long)(kvh * group + row - token * group) * a.o.head + ch;
+      const float add = none || (up && down) ? __builtin_nanf("") : up ? -NEG_INF : NEG_INF;
+      const unsigned was = __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      const bool is_nan = (was & 0x7fffu) > INF_BITS<T>;  // of its scores
+      *p = is_nan ? (unsigned short)was : T::cvt1(add);
     }
   }
 }

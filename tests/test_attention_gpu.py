@@ -345,6 +345,31 @@ def test_prompt_is_not_touched_by_other_sequences(capi):
         assert torch.isnan(out[cu[2] + 128:]).all()
 
 
+@pytest.mark.parametrize("Hq,Hkv,D,n", [(2, 1, 64, 90), (4, 4, 128, 70), (3, 1, 256, 40), (16, 2, 72, 130), (8, 1, 128, 1500)])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_prompt_rows_are_not_touched_by_later_values(capi, Hq, Hkv, D, n, dtype):
+    """An infinity or NaN in a later token's value or key does not reach the rows before it, in the same tile either; the rows that
+    see it get what the weighted sum gives."""
+    gen = torch.Generator().manual_seed(n + D)
+    q, k, v = (randn(gen, n, h, D, dtype=dtype) for h in (Hq, Hkv, Hkv))
+    cu = int32([0, n])
+    clean = capi.attn_prompt(q.to(DEV), k.to(DEV), v.to(DEV), cu, cu, D ** -0.5).cpu()
+    at, late = n // 2, n - 2
+    v2 = v.clone()
+    v2[at, :, 3], v2[at, :, 4], v2[late, :, 3], v2[late, :, 5] = float("inf"), float("-inf"), float("-inf"), NAN
+    out = capi.attn_prompt(q.to(DEV), k.to(DEV), v2.to(DEV), cu, cu, D ** -0.5).cpu()
+    assert torch.equal(out[:at], clean[:at])
+    keep = [c for c in range(D) if c not in (3, 4, 5)]
+    assert torch.equal(out[..., keep], clean[..., keep])
+    assert torch.equal(out[:late, :, 5], clean[:late, :, 5]) and torch.isnan(out[late:, :, 5]).all()
+    assert (out[at:late, :, 3] == float("inf")).all() and torch.isnan(out[late:, :, 3]).all()
+    assert (out[at:, :, 4] == float("-inf")).all()
+    k2 = k.clone()
+    k2[at] = NAN
+    out = capi.attn_prompt(q.to(DEV), k2.to(DEV), v.to(DEV), cu, cu, D ** -0.5).cpu()
+    assert torch.equal(out[:at], clean[:at]) and torch.isnan(out[at:]).all()
+
+
 def test_prompt_scores_far_apart(capi):
     gen = torch.Generator().manual_seed(12)
     n, D = 400, 64
