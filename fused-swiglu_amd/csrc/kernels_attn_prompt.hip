@@ -1,14 +1,25 @@
 // Causal attention of packed prompts: o_i = sum_j p_ij v_j / sum_j p_ij, p_ij = 2^(c s_ij - c m_i), s = q k^T, in one pass
 // over the keys with a running maximum m and running sums (fp32).
 //
-// A workgroup owns BM rows of one sequence and key-value head. A row is a (token, query head of the group) pair: the group's heads of a token are
-// neighbouring rows, so they share the keys and values that the workgroup copies to LDS, short prompts fill their tiles, and the
-// triangle's edge cuts fewer tiles. Four waves own 32 NQ rows each and walk the same tiles of 64 keys.
-// The score tile is computed transposed, S^T = K Q^T (v_mfma_f32_32x32x16): lane l holds query row l % 32 and, of 32 keys, 8 (r / 4) + 4
-// (l / 32) + r % 4 in register r, so a row's maximum and sum are in-lane sums and one exchange with lane l ^ 32, and
-// eight registers in a row, rounded to the element type, are the B operand of O^T = V^T P^T if its 16 keys are numbered {4 h .. 4 h + 3, 8 + 4 h .. 8 + 4 h + 3}
-// (h = l / 32). The A operand has V's channels as rows and the same order of keys: two transposing reads of 4 keys x 16
-// channels (ds_read_b64_tr_b16) deliver it from V as it lies.
+// A workgroup owns 128 (or 64) rows of one sequence and key-value head. A row is a (token, query head of the group) pair: the group's
+// heads of a token are neighbouring rows, so they share the keys and values that the workgroup copies to LDS, short prompts fill their
+// tiles, and the triangle's edge cuts fewer tiles. Four waves own 32 (16) rows each and walk the same tiles of 64 keys, which come in by
+// LDS copies, two tiles of each kind in turn; workgroups with the longest walks start first, those of one key-value head on one XCD where
+// there are 8 heads.
+// The score tile is computed transposed, S^T = K Q^T (v_mfma_f32_16x16x32): lane l holds query row l % 16 and, of 16 keys, 4 (l / 16) + r in
+// register r, so a row's maximum and sum are in-lane ones and two lane swaps, and the registers of two blocks of 16 keys, rounded to the
+// element type, are the B operand of O^T = V^T P^T if its 32 keys are numbered {4 g .. 4 g + 3, 16 + 4 g .. 19 + 4 g} (g = l / 16). The A
+// operand has V's channels as rows and the same order of keys: two transposing reads of 4 keys x 16 channels (ds_read_b64_tr_b16) deliver
+// it from V as it lies. P never leaves its lanes.
+// The weights are rounded once, to the operand's type, as the matrix unit wants them; the sum is taken of the rounded ones (v_dot2), so the
+// normalisation is consistent: error against 64 bits 2.1e-3 on bf16 where one rounding of the output alone is 1.6e-3.
+// Bound: the matrix units, and the exponentials and moves that one instruction port per SIMD has to issue beside them. 8192 tokens of 64
+// heads of 128 on 8: 1017 .. 1100 us = 1.0 .. 1.08 PFLOP/s of what is under the diagonal, at the clock that the board's power leaves (about 1.9
+// GHz; a plain product of 8192 reaches 1.2); matrix units 48 % busy, no LDS bank conflicts. What that took: two waves a SIMD, by 211 registers
+// instead of 276 (1582 -> 1150 us); 16 x 16 instead of 32 x 32 instructions, which move half the accumulators a flop (1127 -> 1104);
+// copies issued without a branch (1104 -> 1065). What did not pay: the scores of the next keys beside the weights of these (1172),
+// keys and values copied one and a half turns ahead with a barrier more (1162), wave priorities (1136), eight waves on every other tile of
+// the same rows (1243).
 #include "attn.h"
 #include "fsw_device.h"
 #include "fsw_internal.h"
@@ -22,7 +33,7 @@ typedef __attribute__((address_space(3))) unsigned char lds_byte;
 
 constexpr float NEG_INF = -__builtin_inff();
 constexpr float SLACK = 8.0f;  // the maximum moves only when a score passes it by this much (powers of two): p < 2^8
-constexpr int KEYS = 64;
+constexpr int KEYS = 64;       // of a tile
 
 #define INLINE __attribute__((always_inline))
 
