@@ -18,6 +18,7 @@
 // number is looked up a turn ahead, and the first before the length is known. Measured: 131071 keys of 8 heads of 128 channels 86 us (6.2 TB/s) + 4.6 for the join;
 // 128 sequences of about 2000 keys 174 us (6.0 TB/s); HBM traffic is the keys and values once. A plain streaming read reaches 7.05 TB/s.
 #include "attn.h"
+#include "attn_device.h"
 #include "fsw_device.h"
 #include "fsw_internal.h"
 
@@ -59,15 +60,6 @@ __device__ __forceinline__ void unpack2<Fp16>(unsigned u, float& lo, float& hi) 
 __device__ __forceinline__ unsigned lows(unsigned a, unsigned b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
 __device__ __forceinline__ unsigned highs(unsigned a, unsigned b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
 
-// over lanes l, l ^ 16, l ^ 32, l ^ 48: a lane swap of a register with a copy of itself leaves the two halves' values side by side
-__device__ __forceinline__ float max_over_groups(float x) {
-  const unsigned u = __builtin_bit_cast(unsigned, x);
-  const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-  const float y = fmaxf(__builtin_bit_cast(float, a[0]), __builtin_bit_cast(float, a[1]));
-  const unsigned w = __builtin_bit_cast(unsigned, y);
-  const auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
-  return fmaxf(__builtin_bit_cast(float, b[0]), __builtin_bit_cast(float, b[1]));
-}
 __device__ __forceinline__ float sum_over_groups(float x) {
   x += __shfl_xor(x, 16);
   return x + __shfl_xor(x, 32);
@@ -387,8 +379,10 @@ hipError_t launch_typed(const PagedAttnArgs& a, const PagedAttnPlan& p, float* p
 // longer. (One sequence of 131071 keys, 8 key-value heads: 87.5 + 4.6 us; four waves a workgroup and 128 shares 91.2 + 5.5.) Where they do, shares level batches of
 // uneven lengths, of which the host knows only the bound: 40 x 40 items of 1 .. 4096 keys take 196 us unsplit, 132 in
 // shares of 2048 and 113 of 1024, + 4.6 for the join. Even batches lose by it: 128 x 8 items of 1700 .. 2300 keys take
-// 174 us unsplit, 186 in two shares, 196 in three; so a bound of up to 2560 keys is left whole. From 8192 items on the card's dynamic
-// assignment levels them.
+// 174 us unsplit, 186 in two shares, 196 in three; so a bound of up to 2560 keys is left whole. The farther the bound, the more shares, up to
+// 8192 of all items together (32 x 8 items of 1 .. 32768 keys: 225 us in 8 shares, 150 in 27): most of the short sequences' are empty and end at
+// once. From 8192 items on the card's dynamic assignment levels them. Where items are few and a workgroup has 16 waves, empty ones cost more than
+// they level (four sequences of 20 .. 32000 keys: 68 us in 8 shares, 81 in 32, 96 in 63).
 PagedAttnPlan paged_attn_plan(int seqs, int hq, int hkv, int d, int max_len) {
   const long long items = (long long)seqs * hkv * head_tiles(hq, hkv);
   PagedAttnPlan p;
@@ -399,7 +393,7 @@ PagedAttnPlan paged_attn_plan(int seqs, int hq, int hkv, int d, int max_len) {
   if (few)
     wanted = items > 0 ? (4096 / p.waves + items - 1) / items : 1;
   else if (items < 8192 && max_len > 2560)
-    wanted = 8;
+    wanted = 8192 / items > 8 ? 8192 / items : 8;
   const long long least = few ? 512 : 1024;
   long long splits = (max_len + least - 1) / least;
   if (splits > wanted) splits = wanted;

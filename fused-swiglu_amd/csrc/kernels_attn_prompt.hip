@@ -21,6 +21,7 @@
 // keys and values copied one and a half turns ahead with a barrier more (1162), wave priorities (1136), eight waves on every other tile of
 // the same rows (1243).
 #include "attn.h"
+#include "attn_device.h"
 #include "fsw_device.h"
 #include "fsw_internal.h"
 
@@ -72,21 +73,16 @@ __device__ __forceinline__ int v_swizzle(int key) {
   return DP == 64 ? ((key >> 1) & 3) << 1 : (key & 7) << 1;
 }
 
-// over lanes l, l ^ 16, l ^ 32, l ^ 48: a swap of a register with its copy leaves two groups' values side by side
-__device__ __forceinline__ float max_of_groups(float x) {
-  const unsigned u = __builtin_bit_cast(unsigned, x);
-  const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-  const float y = fmaxf(__builtin_bit_cast(float, a[0]), __builtin_bit_cast(float, a[1]));
-  const unsigned w = __builtin_bit_cast(unsigned, y);
-  const auto b = __builtin_amdgcn_permlane32_swap(w, w, false, false);
-  return fmaxf(__builtin_bit_cast(float, b[0]), __builtin_bit_cast(float, b[1]));
-}
-
 template <class T, int DP, int NB>
 __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prompt_kernel(PromptArgs a, Divisor by_group, Divisor by_hkv,
                                                                                   int slots) {
   constexpr int RB = DP * 2, TILE = KEYS * RB, LOADS = TILE / 4096;  // copies per wave and tile
   constexpr int KSTEPS = DP / 32, DB = DP / 16, KB = KEYS / 16, WM = 16 * NB, BM = 4 * WM;
+  // Fragments of keys and values are read ahead of the matrix instructions that take them, a block of 16 keys and four value fragments
+  // (1000 tokens 23.4 -> 22.1 us, 2000 56.6 -> 53.0, 8192 of 64 heads 1090 -> 1063; all of a tile's at once, with 16 rows a wave: 22.8 and 54.7);
+  // not at 256 channels and 32 rows, whose registers are full (4000 tokens of 16 heads: 200 us, 235 with spills).
+  constexpr bool AHEAD = DP < 256 || NB == 1;
+  constexpr int VBUF = AHEAD ? 2 : 1, VG = AHEAD ? 4 : 1;
   __shared__ __align__(1024) unsigned char k0s[TILE];
   __shared__ __align__(1024) unsigned char k1s[TILE];
   __shared__ __align__(1024) unsigned char v0s[TILE];
@@ -193,16 +189,27 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prompt_kernel(Pro
   auto attend = [&](int at, const unsigned char* ks, const unsigned char* vs) INLINE {
     if (at >= wave_last) return;
     f32x4 s[KB][NB];
+    u32x4 kf[2][KSTEPS];
+    auto key_fragment = [&](int kb, int st) INLINE -> u32x4 {
+      const int key = kb * 16 + col;
+      return *(const u32x4*)(ks + key * RB + ((4 * st + grp) ^ k_swizzle<DP>(key)) * 16);
+    };
+    auto key_fragments = [&](int kb) INLINE {
+#pragma unroll
+      for (int st = 0; st < KSTEPS; ++st) kf[kb & 1][st] = key_fragment(kb, st);
+    };
+    if (AHEAD) key_fragments(0);
 #pragma unroll
     for (int kb = 0; kb < KB; ++kb) {
+      if (AHEAD && kb + 1 < KB) key_fragments(kb + 1);
+      if (AHEAD) __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int n = 0; n < NB; ++n) s[kb][n] = f32x4{0, 0, 0, 0};
-      const int key = kb * 16 + col;
 #pragma unroll
       for (int st = 0; st < KSTEPS; ++st) {
-        const u32x4 kf = *(const u32x4*)(ks + key * RB + ((4 * st + grp) ^ k_swizzle<DP>(key)) * 16);
+        const u32x4 f = AHEAD ? kf[kb & 1][st] : key_fragment(kb, st);
 #pragma unroll
-        for (int n = 0; n < NB; ++n) s[kb][n] = T::mfma16(kf, qf[n][st], s[kb][n]);
+        for (int n = 0; n < NB; ++n) s[kb][n] = T::mfma16(f, qf[n][st], s[kb][n]);
       }
     }
     if (at + KEYS > wave_first) {
@@ -223,7 +230,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prompt_kernel(Pro
       float t[KB];
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) t[kb] = fmaxf(fmaxf(s[kb][n][0], s[kb][n][1]), fmaxf(s[kb][n][2], s[kb][n][3]));
-      top[n] = max_of_groups(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])));
+      top[n] = max_over_groups(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])));
       above |= top[n] > m[n] + slack;
     }
     if (__any(above)) {
@@ -253,15 +260,25 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prompt_kernel(Pro
           sum[n] = add2<T>(p[n][kb][r / 2], sum[n]);
         }
     }
+    constexpr int GROUPS = KB / 2 * DB / VG;
+    u32x4 vf[VBUF][VG];
+    auto value_group = [&](int g) INLINE {
 #pragma unroll
-    for (int st = 0; st < KB / 2; ++st)
+      for (int x = 0; x < VG; ++x) vf[g % VBUF][x] = value_fragment(vs, (g * VG + x) / DB, (g * VG + x) % DB);
+    };
+    if (AHEAD) value_group(0);
 #pragma unroll
-      for (int i = 0; i < DB; ++i) {
-        const u32x4 vf = value_fragment(vs, st, i);
+    for (int g = 0; g < GROUPS; ++g) {
+      if (g + VBUF - 1 < GROUPS) value_group(g + VBUF - 1);
+      if (AHEAD) __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int x = 0; x < VG; ++x) {
+        const int st = (g * VG + x) / DB, i = (g * VG + x) % DB;
 #pragma unroll
         for (int n = 0; n < NB; ++n)
-          o[i][n] = T::mfma16(vf, u32x4{p[n][2 * st][0], p[n][2 * st][1], p[n][2 * st + 1][0], p[n][2 * st + 1][1]}, o[i][n]);
+          o[i][n] = T::mfma16(vf[g % VBUF][x], u32x4{p[n][2 * st][0], p[n][2 * st][1], p[n][2 * st + 1][0], p[n][2 * st + 1][1]}, o[i][n]);
       }
+    }
   };
 
   // Tile t is in buffer t % 2; copies of tile t + 1 are under way while tile t is worked on. They are issued whether or not there
@@ -373,16 +390,18 @@ hipError_t launch(const PromptArgs& a, hipStream_t stream) {
   return hipGetLastError();
 }
 
-// 64 rows a workgroup (16 a wave) where workgroups of 128 (32 a wave) would all be resident at once: half the rows are then not half the
+// 64 rows a workgroup (16 a wave) where workgroups of 128 (32 a wave) would (nearly) all be resident at once: half the rows are then not half the
 // rate, because no second round follows, and the longest workgroup's walk is what the launch takes. Above that 32 rows a wave
 // share each fragment that is read from LDS. 128 against 64 rows, us, 128 channels: 1000 tokens of 32 heads on 8 (252 workgroups of 128
-// rows) 27.4 | 22.8, 2000 (504) 56.2 | 55.3, 3000 (752) 92 | 110, 8192 of 64 heads 1096 | 1425; 64 channels: 2000 tokens of 16
+// rows) 27.4 | 22.2, 2000 (504) 56.2 | 53.5, 13 prompts of 1 .. 777 tokens and 40 heads (about 540) 25.3 | 22.4, 3000 tokens (752) 92 | 110, 8192 of 64
+// heads 1080 | 1425; 64 channels: 2000 tokens of 16
 // heads on 4 (252) 33.6 | 25.5, 6000 (752) 115 | 107; 256 channels: 1000 tokens of 16 heads on 8 (128) 49 | 34, 4000 (500) 199 | 250.
 template <class T, int DP>
 hipError_t launch_dp(const PromptArgs& a, hipStream_t stream) {
   constexpr int resident = 256 * (DP == 64 ? 3 : DP == 128 ? 2 : 1);  // workgroups of 128 rows, by LDS and registers
   const long long rows = (long long)a.tq * (a.hq / a.hkv);
-  return (rows / 128 + a.seqs) * a.hkv <= resident ? launch<T, DP, 1>(a, stream) : launch<T, DP, 2>(a, stream);
+  const long long about = (rows / 128 + a.seqs / 2) * a.hkv;  // a sequence's last rows fill half a workgroup
+  return about <= resident + resident / 8 ? launch<T, DP, 1>(a, stream) : launch<T, DP, 2>(a, stream);
 }
 
 template <class T>

@@ -382,6 +382,29 @@ def test_prompt_scores_far_apart(capi):
         assert ((out.cpu().double() - ref).abs() <= attention.tolerance(ref, mag, BF, True, n)).all()
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("high", [0, 3, 4, 9, 14, 17, 40, 63, 70, 130])
+def test_one_key_far_above_the_others(capi, dtype, high):
+    """A key whose score lies 2^30 above all others, wherever it stands in a tile: the running maximum has to be its score, or the
+    weights of fp16 overflow. Prompts and single tokens."""
+    gen = torch.Generator().manual_seed(high)
+    n, D, page = 140, 64, 16
+    q, k, v = torch.zeros(n, 2, D), torch.zeros(n, 1, D), randn(gen, n, 1, D, dtype=dtype)
+    q[..., 0], k[:, 0, 0], k[high, 0, 0] = 4.0, -2.5, 2.5
+    q, k = q.to(dtype), k.to(dtype)
+    out = capi.attn_prompt(q.to(DEV), k.to(DEV), v.to(DEV), int32([0, n]), int32([0, n]), 1.0)
+    ref, mag = attention.prompt(q, k, v, [0, n], [0, n], 1.0)
+    assert ((out.cpu().double() - ref).abs() <= attention.tolerance(ref, mag, dtype, True, n)).all()
+    pages = -(-n // page)
+    caches = [torch.zeros(pages * page, D, dtype=dtype) for _ in range(2)]
+    caches[0][:n], caches[1][:n] = k[:, 0], v[:, 0]
+    devs = [c.view(pages, 1, page, D).to(DEV) for c in caches]
+    table = torch.arange(pages, dtype=torch.int32).view(1, -1)
+    out = capi.attn_decode(q[:1].to(DEV), *devs, table.to(DEV), int32([n]), n, 1.0)
+    ref, mag = attention.decode(q[:1], *devs, table, [n], 1.0)
+    assert ((out.cpu().double() - ref).abs() <= attention.tolerance(ref, mag, dtype, False, n)).all()
+
+
 def test_prompt_rows_in_other_orders(capi):
     """Head-major rows, a query stride of its own, one key-value head of a wider row."""
     gen = torch.Generator().manual_seed(13)
