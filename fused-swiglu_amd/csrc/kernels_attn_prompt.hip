@@ -15,7 +15,7 @@
 // normalisation is consistent: error against 64 bits 2.1e-3 on bf16 where one rounding of the output alone is 1.6e-3.
 // Bound: the matrix units, and the exponentials and moves that one instruction port per SIMD has to issue beside them. 8192 tokens of 64
 // heads of 128 on 8: 1017 .. 1100 us = 1.0 .. 1.08 PFLOP/s of what is under the diagonal, at the clock that the board's power leaves (about 1.9
-// GHz; a plain product of 8192 reaches 1.2); matrix units 48 % busy, no LDS bank conflicts. What that took: two waves a SIMD, by 211 registers
+// GHz; a plain product of 8192 reaches 1.2); matrix units 48 % busy, no LDS bank conflicts. What that took: two waves a SIMD, by at most 256 registers
 // instead of 276 (1582 -> 1150 us); 16 x 16 instead of 32 x 32 instructions, which move half the accumulators a flop (1127 -> 1104);
 // copies issued without a branch (1104 -> 1065). What did not pay: the scores of the next keys beside the weights of these (1172),
 // keys and values copied one and a half turns ahead with a barrier more (1162), wave priorities (1136), eight waves on every other tile of
@@ -79,7 +79,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prompt_kernel(Pro
   constexpr int RB = DP * 2, TILE = KEYS * RB, LOADS = TILE / 4096;  // copies per wave and tile
   constexpr int KSTEPS = DP / 32, DB = DP / 16, KB = KEYS / 16, WM = 16 * NB, BM = 4 * WM;
   // Fragments of keys and values are read ahead of the matrix instructions that take them, a block of 16 keys and four value fragments
-  // (1000 tokens 23.4 -> 22.1 us, 2000 56.6 -> 53.0, 8192 of 64 heads 1090 -> 1063; all of a tile's at once, with 16 rows a wave: 22.8 and 54.7);
+  // (1000 tokens 23.4 -> 22.1 us, 2000 56.6 -> 51.4, 8192 of 64 heads 1090 -> 1063; all of a tile's at once, with 16 rows a wave: 22.8 and 54.7);
   // not at 256 channels and 32 rows, whose registers are full (4000 tokens of 16 heads: 200 us, 235 with spills).
   constexpr bool AHEAD = DP < 256 || NB == 1;
   constexpr int VBUF = AHEAD ? 2 : 1, VG = AHEAD ? 4 : 1;
