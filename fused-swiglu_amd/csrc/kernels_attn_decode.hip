@@ -17,6 +17,10 @@
 // a quarter of the waves and gains nothing (112 against 100 us, 131071 keys). Loads are non-temporal, since every byte is read once: 100 -> 91 us. The page
 // number is looked up a turn ahead, and the first before the length is known. Measured: 131071 keys of 8 heads of 128 channels 86 us (6.2 TB/s) + 4.6 for the join;
 // 128 sequences of about 2000 keys 174 us (6.0 TB/s); HBM traffic is the keys and values once. A plain streaming read reaches 7.05 TB/s.
+#include <float.h>
+
+#include <type_traits>
+
 #include "attn.h"
 #include "attn_device.h"
 #include "fsw_device.h"
@@ -65,10 +69,13 @@ __device__ __forceinline__ float sum_over_groups(float x) {
   return x + __shfl_xor(x, 32);
 }
 
-// 2^(a - b) for a <= b, with -inf - -inf = 0 (nothing seen yet)
+// 2^(a - b) for a <= b, with -inf - -inf = 0 (nothing seen yet). Never zero, so that an infinity that has been summed up stays one; what
+// that adds to other sums is below 2^-126 of the values.
 __device__ __forceinline__ float scale_of(float a, float b) {
-  return a == b ? 1.0f : __builtin_amdgcn_exp2f(a - b);
+  return a == b ? 1.0f : fmaxf(__builtin_amdgcn_exp2f(a - b), FLT_MIN);
 }
+
+#define INLINE __attribute__((always_inline))
 
 // DP: channels, padded to 64, 128 or 256; a row of values is NV vectors of VL elements on 16 lanes.
 // WHOLE: page_size % 16 == 0, so 16 keys in a row lie in one page and the page's address is wave-uniform.
@@ -119,106 +126,129 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 2 : 4) void attn_decode_ker
   if (split > 0 && begin >= end) return;
 
   f32x4 acc[NA];
-#pragma unroll
-  for (int i = 0; i < NA; ++i) acc[i] = f32x4{0, 0, 0, 0};
-  float m = NEG_INF, sum = 0.0f;
+  float m, sum;
   bool bad_page = false;
 
-  for (; at < end; at += 16 * WAVES) {
-    const bool part = at + 16 > end;
-    // a page outside the cache is an error where a key lies in it, and read as page 0
-    const bool inside = (unsigned)page < (unsigned)a.cache.pages;
-    bad_page |= !inside && at + col < end;
-    const long long where = (long long)(inside ? page : 0) * a.cache.page + (long long)place * a.cache.token;
-    u32x4 kf[KS];
-    u32x4 vf[4][NV];
-    const unsigned short* tile = nullptr;
-    if constexpr (WHOLE) {
-      const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)where);
-      const unsigned hi = __builtin_amdgcn_readfirstlane((unsigned)((unsigned long long)where >> 32));
-      tile = vc + (long long)(((unsigned long long)hi << 32) | lo);
-    }
+  // finite: infinities and NaN among the values are taken as zeros
+  auto walk = [&](auto finite) INLINE {
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      const int ch = s * 32 + grp * 8;
-      kf[s] = u32x4{0, 0, 0, 0};
-      if (ch < a.d) kf[s] = __builtin_nontemporal_load((const u32x4*)(kc + where + ch));
-    }
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      const int k = 4 * grp + r;
-      const unsigned short* p;
+    for (int i = 0; i < NA; ++i) acc[i] = f32x4{0, 0, 0, 0};
+    m = NEG_INF, sum = 0.0f;
+    for (; at < end; at += 16 * WAVES) {
+      const bool part = at + 16 > end;
+      // a page outside the cache is an error where a key lies in it, and read as page 0
+      const bool inside = (unsigned)page < (unsigned)a.cache.pages;
+      bad_page |= !inside && at + col < end;
+      const long long where = (long long)(inside ? page : 0) * a.cache.page + (long long)place * a.cache.token;
+      u32x4 kf[KS];
+      u32x4 vf[4][NV];
+      const unsigned short* tile = nullptr;
       if constexpr (WHOLE) {
-        p = tile + k * (int)a.cache.token;  // the page has room for all 16, keys or not
-      } else {
-        p = vc + __shfl(where, k);
+        const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)where);
+        const unsigned hi = __builtin_amdgcn_readfirstlane((unsigned)((unsigned long long)where >> 32));
+        tile = vc + (long long)(((unsigned long long)hi << 32) | lo);
       }
 #pragma unroll
-      for (int v = 0; v < NV; ++v) {
-        const int ch = (v * 16 + col) * VL;
-        vf[r][v] = u32x4{0, 0, 0, 0};
-        if (ch < a.d) {
-          if constexpr (VL == 8) {
-            vf[r][v] = __builtin_nontemporal_load((const u32x4*)(p + ch));
-          } else {
-            const u32x2 w = __builtin_nontemporal_load((const u32x2*)(p + ch));
-            vf[r][v][0] = w[0], vf[r][v][1] = w[1];
+      for (int s = 0; s < KS; ++s) {
+        const int ch = s * 32 + grp * 8;
+        kf[s] = u32x4{0, 0, 0, 0};
+        if (ch < a.d) kf[s] = __builtin_nontemporal_load((const u32x4*)(kc + where + ch));
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int k = 4 * grp + r;
+        const unsigned short* p;
+        if constexpr (WHOLE) {
+          p = tile + k * (int)a.cache.token;  // the page has room for all 16, keys or not
+        } else {
+          p = vc + __shfl(where, k);
+        }
+#pragma unroll
+        for (int v = 0; v < NV; ++v) {
+          const int ch = (v * 16 + col) * VL;
+          vf[r][v] = u32x4{0, 0, 0, 0};
+          if (ch < a.d) {
+            if constexpr (VL == 8) {
+              vf[r][v] = __builtin_nontemporal_load((const u32x4*)(p + ch));
+            } else {
+              const u32x2 w = __builtin_nontemporal_load((const u32x2*)(p + ch));
+              vf[r][v][0] = w[0], vf[r][v][1] = w[1];
+            }
+          }
+          // what lies behind the end weighs nothing, whatever it holds
+          if (part && at + k >= end) vf[r][v] = u32x4{0, 0, 0, 0};
+          if constexpr (decltype(finite)::value) {
+#pragma unroll
+            for (int j = 0; j < VL / 2; ++j) vf[r][v][j] = finite2<T>(vf[r][v][j]);
           }
         }
-        // what lies behind the end weighs nothing, whatever it holds
-        if (part && at + k >= end) vf[r][v] = u32x4{0, 0, 0, 0};
       }
-    }
-    if (at + 16 * WAVES < end) locate(at + 16 * WAVES);
+      if (at + 16 * WAVES < end) locate(at + 16 * WAVES);
 
-    f32x4 s = {0, 0, 0, 0};
+      f32x4 s = {0, 0, 0, 0};
 #pragma unroll
-    for (int i = 0; i < KS; ++i) s = T::mfma16(kf[i], qf[i], s);
-    float top = NEG_INF;
+      for (int i = 0; i < KS; ++i) s = T::mfma16(kf[i], qf[i], s);
+      float top = NEG_INF;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      s[r] *= a.scale_log2;
-      if (part && at + 4 * grp + r >= end) s[r] = NEG_INF;
-      top = fmaxf(top, s[r]);
-    }
-    top = max_over_groups(top);
-    if (__any(top > m + SLACK)) {
-      const float now = fmaxf(m, top), alpha = scale_of(m, now);
-      m = now;
-      sum *= alpha;
-#pragma unroll
-      for (int i = 0; i < NA; ++i)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) acc[i][r] *= alpha;
-    }
-    const float base = m == NEG_INF ? 0.0f : m;
-#pragma unroll
-    for (int r = 0; r < 4; ++r) {
-      s[r] = __builtin_amdgcn_exp2f(s[r] - base);
-      sum += s[r];
-    }
-    // weights as the sum of two elements, so that they carry twice the bits: the product is as good as one in fp32
-    u32x2 p1, p2;
-#pragma unroll
-    for (int r = 0; r < 4; r += 2) {
-      float lo, hi;
-      p1[r / 2] = T::pack2(s[r], s[r + 1]);
-      unpack2<T>(p1[r / 2], lo, hi);
-      p2[r / 2] = T::pack2(s[r] - lo, s[r + 1] - hi);
-    }
-#pragma unroll
-    for (int v = 0; v < NV; ++v)
-#pragma unroll
-      for (int j = 0; j < VL / 2; ++j) {
-        const u32x2 even = {lows(vf[0][v][j], vf[1][v][j]), lows(vf[2][v][j], vf[3][v][j])};
-        const u32x2 odd = {highs(vf[0][v][j], vf[1][v][j]), highs(vf[2][v][j], vf[3][v][j])};
-        f32x4& x = acc[v * VL + 2 * j];
-        f32x4& y = acc[v * VL + 2 * j + 1];
-        x = mfma_k16<T>(even, p1, x);
-        y = mfma_k16<T>(odd, p1, y);
-        x = mfma_k16<T>(even, p2, x);
-        y = mfma_k16<T>(odd, p2, y);
+      for (int r = 0; r < 4; ++r) {
+        s[r] *= a.scale_log2;
+        if (part && at + 4 * grp + r >= end) s[r] = NEG_INF;
+        top = fmaxf(top, s[r]);
       }
+      top = max_over_groups(top);
+      if (__any(top > m + SLACK)) {
+        const float now = fmaxf(m, top), alpha = scale_of(m, now);
+        m = now;
+        sum *= alpha;
+#pragma unroll
+        for (int i = 0; i < NA; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) acc[i][r] *= alpha;
+      }
+      const float base = m == NEG_INF ? 0.0f : m;
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        s[r] = __builtin_amdgcn_exp2f(s[r] - base);
+        sum += s[r];
+      }
+      // weights as the sum of two elements, so that they carry twice the bits: the product is as good as one in fp32
+      u32x2 p1, p2;
+#pragma unroll
+      for (int r = 0; r < 4; r += 2) {
+        float lo, hi;
+        p1[r / 2] = T::pack2(s[r], s[r + 1]);
+        unpack2<T>(p1[r / 2], lo, hi);
+        p2[r / 2] = T::pack2(s[r] - lo, s[r + 1] - hi);
+      }
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int j = 0; j < VL / 2; ++j) {
+          const u32x2 even = {lows(vf[0][v][j], vf[1][v][j]), lows(vf[2][v][j], vf[3][v][j])};
+          const u32x2 odd = {highs(vf[0][v][j], vf[1][v][j]), highs(vf[2][v][j], vf[3][v][j])};
+          f32x4& x = acc[v * VL + 2 * j];
+          f32x4& y = acc[v * VL + 2 * j + 1];
+          x = mfma_k16<T>(even, p1, x);
+          y = mfma_k16<T>(odd, p1, y);
+          x = mfma_k16<T>(even, p2, x);
+          y = mfma_k16<T>(odd, p2, y);
+        }
+    }
+  };
+  walk(std::false_type());
+  // An infinity times the second part of a weight, which may be zero or negative, is no infinity, and a weight that has underflowed
+  // silences none. That is rare, so it is noticed here, by a sum that is not finite: the wave takes its keys once more with zeros in
+  // place of infinities and NaN, and puts what their weighted sum is over its sums below. Every key that is seen weighs more than nothing.
+  float probe = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NA; ++i)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) probe += acc[i][r] * 0.0f;
+  const bool again = __any(!(probe == 0.0f));
+  if (__builtin_expect(again, 0)) {
+    at = begin + wave * 16;
+    locate(at);
+    walk(std::true_type());
   }
   if (__any(bad_page) || bad_len) sum = __builtin_nanf("");
   sum = sum_over_groups(sum);
@@ -250,6 +280,23 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 2 : 4) void attn_decode_ker
           for (int i = 0; i < 4; ++i) x[i] = acc[v * VL + j + i][r] * mine;
           *(f32x4*)(row + (v * 16 + 4 * grp + r) * VL + j) = x;
         }
+  }
+  if (__builtin_expect(again, 0)) {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // the wave's rows above are written
+#pragma unroll 1
+    for (int ch = lane; ch < a.d; ch += 64) {
+      Extremes<T> seen;
+#pragma unroll 1
+      for (int turn = begin + wave * 16; turn < end; turn += 16 * WAVES)
+#pragma unroll 1
+        for (int key = turn; key < turn + 16 && key < end; ++key) {
+          const int idx = a.cache.per_page.quotient(key), n = table[idx];
+          const long long at_page = (long long)((unsigned)n < (unsigned)a.cache.pages ? n : 0) * a.cache.page;
+          seen.add(vc[at_page + (long long)(key - idx * a.cache.page_size) * a.cache.token + ch]);
+        }
+      if (seen.any())
+        for (int h = 0; h < here; ++h) shares[(wave * here + h) * ROW + ch] = seen.sum();
+    }
   }
   __syncthreads();
   const bool parted = len > chunk && !bad_len;

@@ -50,14 +50,6 @@ __device__ __forceinline__ float add2<Fp16>(unsigned p, float c) {
   return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, p), __builtin_bit_cast(f16x2, 0x3c003c00u), c, false);
 }
 
-// exponent of infinities and NaN; sizes above it are NaN
-template <class T>
-constexpr unsigned INF_BITS = 0;
-template <>
-constexpr unsigned INF_BITS<Bf16> = 0x7f80;
-template <>
-constexpr unsigned INF_BITS<Fp16> = 0x7c00;
-
 __device__ __forceinline__ u32x2 read_tr(const unsigned char* p) {
   return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p));
 }
@@ -292,10 +284,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prompt_kernel(Pro
     for (int byte = (int)threadIdx.x * 16; byte < TILE; byte += 4096) {
       u32x4 x = *(u32x4*)(vs + byte);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if ((x[j] & INF_BITS<T>) == INF_BITS<T>) x[j] &= 0xffff0000u;
-        if ((x[j] >> 16 & INF_BITS<T>) == INF_BITS<T>) x[j] &= 0xffffu;
-      }
+      for (int j = 0; j < 4; ++j) x[j] = finite2<T>(x[j]);
       *(u32x4*)(vs + byte) = x;
     }
     __syncthreads();
@@ -358,26 +347,20 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prompt_kernel(Pro
 #pragma unroll 1
   for (int ch = lane; ch < a.d; ch += 64) {
     const unsigned short* v = (const unsigned short*)vp + ch;
-    bool up = false, down = false, none = false;
+    Extremes<T> seen;
     int key = 0;
 #pragma unroll 1
     for (int row = wrow; row < wrow + WM && row < rows; ++row) {
       const int end = sees(row);
 #pragma unroll 8
-      for (; key < end; ++key) {
-        const unsigned x = v[key * a.v.token], size = x & 0x7fffu;
-        none |= size > INF_BITS<T>;
-        up |= x == INF_BITS<T>;
-        down |= size == INF_BITS<T> && x != size;
-      }
-      if (!(up || down || none)) continue;
+      for (; key < end; ++key) seen.add(v[key * a.v.token]);
+      if (!seen.any()) continue;
       const int token = by_group.quotient(row);
       unsigned short* p = (unsigned short*)a.o.p + (q_at + token) * a.o.token +
                           (long long)(kvh * group + row - token * group) * a.o.head + ch;
-      const float add = none || (up && down) ? __builtin_nanf("") : up ? -NEG_INF : NEG_INF;
       const unsigned was = __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       const bool is_nan = (was & 0x7fffu) > INF_BITS<T>;  // of its scores
-      *p = is_nan ? (unsigned short)was : T::cvt1(add);
+      *p = is_nan ? (unsigned short)was : T::cvt1(seen.sum());
     }
   }
 }

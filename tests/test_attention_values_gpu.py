@@ -1,0 +1,76 @@
+"""The attention operators where values and weights come to the edges of their types: infinities and NaN that are seen, weights
+far below the largest, sums beyond fp32. Against the definition in float64 (oracle/attention.py), which answers these too."""
+import pytest
+import torch
+
+from oracle import attention
+from test_attention_gpu import BF, DEV, HF, int32, paged, randn
+
+pytestmark = pytest.mark.gpu
+INF, NAN = float("inf"), float("nan")
+
+
+def agrees(out, ref, mag, dtype, weights_rounded, keys):
+    """Finite where the definition is, within the tolerance; the same infinities and NaN elsewhere."""
+    out, finite = out.cpu().double(), torch.isfinite(ref)
+    tol = attention.tolerance(ref, mag, dtype, weights_rounded, keys)
+    return bool(((out - ref).abs() <= tol)[finite].all()) and torch.equal(out[~finite].nan_to_num(7.0, INF, -INF),
+                                                                          ref[~finite].nan_to_num(7.0, INF, -INF))
+
+
+def put(cache, table, page, seq, key, channel, value):
+    cache[int(table[seq, key // page]), :, key % page, channel] = value
+
+
+@pytest.mark.parametrize("lengths,max_len,Hq,Hkv,D,page", [
+    ([40, 1, 17, 300], None, 4, 2, 64, 16),        # one share, sixteen waves
+    ([40, 1, 17, 300], None, 3, 1, 80, 5),         # pages that 16 keys do not fit
+    ([40, 1, 17, 300], None, 17, 1, 128, 32),      # two tiles of heads
+    ([40, 2, 33], None, 4, 4, 256, 16),
+    ([1300, 40, 700], None, 4, 2, 128, 16),        # shares that are joined
+    ([1300, 40, 700], None, 2, 1, 256, 7),
+    ([9000, 600], None, 2, 1, 64, 64),             # more than eight of them
+    ([70, 1, 130], None, 64, 64, 64, 16)])         # many items: four waves
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_decode_infinities_that_are_seen(capi, lengths, max_len, Hq, Hkv, D, page, dtype):
+    """What the weighted sum gives: the infinity, NaN where both signs or a NaN are seen; other channels and sequences as before."""
+    gen = torch.Generator().manual_seed(sum(lengths) + D)
+    caches, table = paged(gen, lengths, Hkv, D, page, dtype)
+    q = randn(gen, len(lengths), Hq, D, dtype=dtype, scale=1.5)
+    most, scale = max_len or max(lengths), D ** -0.5
+    args = (table.to(DEV), int32(lengths), most, scale)
+    clean = capi.attn_decode(q.to(DEV), *caches, *args)
+    v = caches[1].clone()
+    for seq in (0, len(lengths) - 1):
+        n = lengths[seq]
+        put(v, table, page, seq, n // 2, 3, INF)
+        put(v, table, page, seq, n - 1, 4, -INF)
+        put(v, table, page, seq, 0, 5, NAN)
+        put(v, table, page, seq, n // 3, 6, INF)
+        put(v, table, page, seq, n - 2, 6, -INF)
+        put(v, table, page, seq, n // 4, D - 1, INF)
+        put(v, table, page, seq, n // 4 + 1, D - 1, INF)
+    out = capi.attn_decode(q.to(DEV), caches[0], v, *args)
+    ref, mag = attention.decode(q, caches[0], v, table, lengths, scale)
+    assert (ref[0, :, 3] == INF).all() and torch.isnan(ref[0, :, 6]).all()
+    assert agrees(out, ref, mag, dtype, False, most)
+    assert torch.equal(out[1:-1], clean[1:-1])
+
+
+@pytest.mark.parametrize("n,page", [(81, 16), (90, 9), (4097, 16)])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_decode_infinity_of_a_key_that_weighs_little(capi, n, page, dtype):
+    """A key whose score lies 2^288 below the others' weighs more than nothing, also where it has a share to itself."""
+    D, pages = 64, -(-n // page)
+    gen = torch.Generator().manual_seed(n)
+    k, v = torch.zeros(pages * page, D), randn(gen, pages * page, D, dtype=dtype)
+    k[n - 1, 0] = -10.0
+    v[n - 1, 2] = -INF
+    q = torch.zeros(1, 1, D)
+    q[..., 0] = 20.0
+    q = q.to(dtype)
+    table = torch.arange(pages, dtype=torch.int32).view(1, -1)
+    caches = [c.to(dtype).view(pages, 1, page, D).to(DEV) for c in (k, v)]
+    out = capi.attn_decode(q.to(DEV), *caches, table.to(DEV), int32([n]), n, 1.0)
+    ref, mag = attention.decode(q, *caches, table, [n], 1.0)
+    assert ref[0, 0, 2] == -INF and agrees(out, ref, mag, dtype, False, n)
