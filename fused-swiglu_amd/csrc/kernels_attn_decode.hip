@@ -239,12 +239,12 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 2 : 4) void attn_decode_ker
   // An infinity times the second part of a weight, which may be zero or negative, is no infinity, and a weight that has underflowed
   // silences none. That is rare, so it is noticed here, by a sum that is not finite: the wave takes its keys once more with zeros in
   // place of infinities and NaN, and puts what their weighted sum is over its sums below. Every key that is seen weighs more than nothing.
-  float probe = 0.0f;
+  f32x4 probe = {0, 0, 0, 0};
 #pragma unroll
   for (int i = 0; i < NA; ++i)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) probe += acc[i][r] * 0.0f;
-  const bool again = __any(!(probe == 0.0f));
+    for (int r = 0; r < 4; ++r) probe[r] += acc[i][r] * 0.0f;
+  const bool again = __any(!(probe[0] + probe[1] + probe[2] + probe[3] == 0.0f));
   if (__builtin_expect(again, 0)) {
     at = begin + wave * 16;
     locate(at);
