@@ -10,7 +10,7 @@
 // value rows that are read as they lie: 16 lanes with 8 consecutive channels each, four rows per lane, of which instruction j
 // takes the j-th channels, put side by side by two byte permutations. So neither P nor V crosses lanes, nothing goes through LDS before the end, and
 // the output is O^T: maximum, sum and rescaling of a head live in the lanes of its accumulators. P is not rounded to the element type but
-// split into two elements, whose products both are added (v_mfma_f32_16x16x4_f32 on fp32 values does the same at an eighth of the rate: 512 keys of
+// split into two elements, whose products both are added (fp16, which has few exponents, takes them relative to the largest of 16 keys) (v_mfma_f32_16x16x4_f32 on fp32 values does the same at an eighth of the rate: 512 keys of
 // one sequence 12.5 against 10.6 us).
 // A wave takes 16 keys a turn, 8 KB, so 16 waves fit on a CU and keep 128 KB under way; tiles of 64 keys a wave, eight waves, were no faster on long
 // caches and slower on mixed ones (40 sequences of 1 .. 4096 keys: 153 against 113 us). A second set of registers for the next turn's keys and values costs
@@ -30,7 +30,8 @@ namespace fsw {
 namespace {
 
 constexpr float NEG_INF = -__builtin_inff();
-// The running maximum of a head moves only when a score passes it by this much (in powers of two): p stays below 2^8.
+// The running maximum of a head moves only when a score passes it by this much (in powers of two): sums stay near 1, the accumulators
+// are seldom rescaled.
 constexpr float SLACK = 8.0f;
 
 typedef __attribute__((ext_vector_type(4))) short s16x4;
@@ -84,6 +85,7 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 2 : 4) void attn_decode_ker
                                                                                     float* partial) {
   constexpr int KS = DP / 32;                  // steps over the channels
   constexpr int VL = DP == 64 ? 4 : 8, NV = DP / (16 * VL), NA = NV * VL;
+  constexpr bool BY_TURN = std::is_same<T, Fp16>::value;  // weights relative to the largest of 16 keys
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, grp = lane >> 4;
   const int split = blockIdx.z, splits = gridDim.z, seq = blockIdx.y;
   int kvh = blockIdx.x, first = 0;
@@ -205,12 +207,24 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 2 : 4) void attn_decode_ker
 #pragma unroll
           for (int r = 0; r < 4; ++r) acc[i][r] *= alpha;
       }
-      const float base = m == NEG_INF ? 0.0f : m;
+      // fp16 holds weights down to 2^-24 only. They are taken relative to the largest of their own 16 keys there, which weighs 2^15, and the
+      // products scaled to the running maximum in fp32: what a key loses is 2^-40 of its turn's largest, however many keys there are.
+      float base = m, weight = 1.0f;
+      if constexpr (BY_TURN) {
+        base = top - 15.0f;
+        weight = top == NEG_INF ? 0.0f : __builtin_amdgcn_exp2f(base - m);
+      }
+      if (base == NEG_INF) base = 0.0f;
+      float turn_sum = 0.0f;
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
         s[r] = __builtin_amdgcn_exp2f(s[r] - base);
-        sum += s[r];
+        if constexpr (BY_TURN)
+          turn_sum += s[r];
+        else
+          sum += s[r];
       }
+      if constexpr (BY_TURN) sum += turn_sum * weight;
       // weights as the sum of two elements, so that they carry twice the bits: the product is as good as one in fp32
       u32x2 p1, p2;
 #pragma unroll
@@ -226,12 +240,21 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 2 : 4) void attn_decode_ker
         for (int j = 0; j < VL / 2; ++j) {
           const u32x2 even = {lows(vf[0][v][j], vf[1][v][j]), lows(vf[2][v][j], vf[3][v][j])};
           const u32x2 odd = {highs(vf[0][v][j], vf[1][v][j]), highs(vf[2][v][j], vf[3][v][j])};
-          f32x4& x = acc[v * VL + 2 * j];
-          f32x4& y = acc[v * VL + 2 * j + 1];
+          f32x4 x = BY_TURN ? f32x4{0, 0, 0, 0} : acc[v * VL + 2 * j];
+          f32x4 y = BY_TURN ? f32x4{0, 0, 0, 0} : acc[v * VL + 2 * j + 1];
           x = mfma_k16<T>(even, p1, x);
           y = mfma_k16<T>(odd, p1, y);
           x = mfma_k16<T>(even, p2, x);
           y = mfma_k16<T>(odd, p2, y);
+          if constexpr (BY_TURN) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+              x[r] = __builtin_fmaf(x[r], weight, acc[v * VL + 2 * j][r]);
+              y[r] = __builtin_fmaf(y[r], weight, acc[v * VL + 2 * j + 1][r]);
+            }
+          }
+          acc[v * VL + 2 * j] = x;
+          acc[v * VL + 2 * j + 1] = y;
         }
     }
   };

@@ -232,7 +232,8 @@ FSW_API size_t fsw_attn_decode_workspace_bytes(int dtype, int64_t B, int64_t Hq,
 
 /*
  * O[b, h] = softmax_j(scale * Q[b, h] . k_j) . v_j over the keys j < lengths[b] of sequence b, which lie in pages
- * block_table[b * table_ld + j / page_size]: one new token per sequence. fp32 scores, weights and sums, one rounding. max_len: the host's bound of the lengths, which sets
+ * block_table[b * table_ld + j / page_size]: one new token per sequence. fp32 scores and sums, weights in two elements
+ * that hold 16 bits (bf16) or 22 (fp16) of them, one rounding. max_len: the host's bound of the lengths, which sets
  * the launch's shape. A length of 0 gives zeros; a length below 0 or above max_len, or a page outside the cache among a sequence's pages, gives NaN for that
  * sequence. What the cache holds behind a length is never used. Every key before it weighs more than nothing: an infinity among their values gives that
  * infinity, both signs or a NaN give NaN, in their channel.

@@ -74,3 +74,52 @@ def test_decode_infinity_of_a_key_that_weighs_little(capi, n, page, dtype):
     out = capi.attn_decode(q.to(DEV), *caches, table.to(DEV), int32([n]), n, 1.0)
     ref, mag = attention.decode(q, *caches, table, [n], 1.0)
     assert ref[0, 0, 2] == -INF and agrees(out, ref, mag, dtype, False, n)
+
+
+def one_above_the_others(gen, n, D, bits, dtype):
+    """q [1, 2, D], k and v [n, D]: at scale 1 a key's weight is 2^bits times that of each of the others, wherever it stands (here: first).
+    Channel 0 of the values is one everywhere, channel 1 one but for that key's zero, so that its sum is what the others weigh."""
+    k, v = torch.zeros(n, D), randn(gen, n, D, dtype=dtype)
+    k[:, 0], k[0, 0] = -bits * 0.6931472 / 4, bits * 0.6931472 / 4
+    v[:, :2], v[0, 1] = 1.0, 0.0
+    q = torch.zeros(1, 2, D)
+    q[..., 0] = 2.0
+    return q.to(dtype), k.to(dtype), v
+
+
+@pytest.mark.parametrize("bits", [12.0, 20.4, 24.4, 24.8, 25.1, 30.0])
+@pytest.mark.parametrize("n,D,page", [(131071, 64, 64), (40000, 128, 9)])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_decode_many_small_weights_beside_a_large_one(capi, n, D, page, bits, dtype):
+    """A long context whose first key outweighs each of the others by far, but not all of them together: no weight may be lost, and the
+    sum that normalises has to be the sum of the weights that were used."""
+    gen = torch.Generator().manual_seed(n)
+    q, k, v = one_above_the_others(gen, n, D, bits, dtype)
+    pages = -(-n // page)
+    caches = [torch.cat([c, c.new_zeros(pages * page - n, D)]).view(pages, 1, page, D) for c in (k, v)]
+    table = torch.arange(pages, dtype=torch.int32).view(1, -1)
+    out = capi.attn_decode(q.to(DEV), *(c.to(DEV) for c in caches), table.to(DEV), int32([n]), n, 1.0).cpu().double()
+    for h in range(2):
+        ref, mag = attention.attend(q[:, h], k, v, 1.0, [n])
+        assert ((out[:, h] - ref).abs() <= attention.tolerance(ref, mag, dtype, False, n)).all()
+
+
+@pytest.mark.parametrize("bits", [20.4, 24.8, 25.1, 30.0])
+@pytest.mark.parametrize("page", [64, 9])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_decode_many_small_weights_in_one_share(capi, page, bits, dtype):
+    """The same where sequences are so many that none is split: a wave takes a quarter of the keys beside the large one."""
+    n, D, B = 131071, 16, 8192
+    gen = torch.Generator().manual_seed(n)
+    q, k, v = one_above_the_others(gen, n, D, bits, dtype)
+    pages = -(-n // page)
+    caches = [torch.cat([c, c.new_zeros(pages * page - n, D)]).view(pages, 1, page, D).to(DEV) for c in (k, v)]
+    table = torch.arange(pages, dtype=torch.int32, device=DEV).repeat(B, 1)
+    lengths = torch.full((B,), 1, dtype=torch.int32, device=DEV)
+    lengths[5] = n
+    assert capi.lib().fsw_attn_decode_workspace_bytes(0, B, 2, 1, D, n) == 0
+    out = capi.attn_decode(q.to(DEV).repeat(B, 1, 1), *caches, table, lengths, n, 1.0).cpu().double()
+    for h in range(2):
+        ref, mag = attention.attend(q[:, h], k, v, 1.0, [n])
+        assert ((out[5, h] - ref[0]).abs() <= attention.tolerance(ref, mag, dtype, False, n)[0]).all()
+    assert torch.equal(out[:5], v[0].double().expand(5, 2, D)) and torch.equal(out[6:], v[0].double().expand(B - 6, 2, D))
