@@ -33,7 +33,17 @@ typedef __attribute__((address_space(3))) void lds_void;
 typedef __attribute__((address_space(3))) unsigned char lds_byte;
 
 constexpr float NEG_INF = -__builtin_inff();
-constexpr float SLACK = 8.0f;  // the maximum moves only when a score passes it by this much (powers of two): p < 2^8
+// m is the score that weighs 1. It moves when a score would weigh more than 2^(SHIFT + SLACK), so that this score weighs 2^SHIFT. fp16 has weights
+// from 2^-24 to 2^16, all of which are used: one is rounded like any other down to 2^-25 of the maximum's, and 2^-36 of that is what a
+// smaller one may lose. The kernel has both divided by c, in units of its scores.
+template <class T>
+constexpr float SLACK = 8.0f;
+template <class T>
+constexpr float SHIFT = 0.0f;
+template <>
+inline constexpr float SLACK<Fp16> = 4.0f;
+template <>
+inline constexpr float SHIFT<Fp16> = 11.0f;
 constexpr int KEYS = 64;       // of a tile
 
 #define INLINE __attribute__((always_inline))
@@ -67,7 +77,7 @@ __device__ __forceinline__ int v_swizzle(int key) {
 
 template <class T, int DP, int NB>
 __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prompt_kernel(PromptArgs a, Divisor by_group, Divisor by_hkv,
-                                                                                  int slots) {
+                                                                                  int slots, float lower, float limit) {
   constexpr int RB = DP * 2, TILE = KEYS * RB, LOADS = TILE / 4096;  // copies per wave and tile
   constexpr int KSTEPS = DP / 32, DB = DP / 16, KB = KEYS / 16, WM = 16 * NB, BM = 4 * WM;
   // Fragments of keys and values are read ahead of the matrix instructions that take them, a block of 16 keys and four value fragments
@@ -170,7 +180,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prompt_kernel(Pro
   auto copy_k = [&](int at, unsigned char* to) INLINE { copy(at, kp, a.k.token, koff, to); };
   auto copy_v = [&](int at, unsigned char* to) INLINE { copy(at, vp, a.v.token, voff, to); };
 
-  const float c = a.scale_log2, slack = SLACK / c;
+  const float c = a.scale_log2;
   // 16 channels x 32 keys: keys 4 g .. 4 g + 3 and 16 + 4 g .. 19 + 4 g of lane group g
   auto value_fragment = [&](const unsigned char* vs, int st, int i) INLINE -> u32x4 {
     const int key = st * 32 + 4 * grp + (col >> 2), ch = i * 2 + ((col & 3) >> 1);
@@ -223,12 +233,12 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prompt_kernel(Pro
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) t[kb] = fmaxf(fmaxf(s[kb][n][0], s[kb][n][1]), fmaxf(s[kb][n][2], s[kb][n][3]));
       top[n] = max_over_groups(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])));
-      above |= top[n] > m[n] + slack;
+      above |= top[n] > m[n] + limit;
     }
     if (__any(above)) {
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
-        const float now = fmaxf(m[n], top[n]);
+        const float now = fmaxf(m[n], top[n] - lower);
         const float alpha = now == m[n] ? 1.0f : __builtin_amdgcn_exp2f((m[n] - now) * c);
         m[n] = now;
         sum[n] *= alpha;
@@ -369,7 +379,8 @@ template <class T, int DP, int NB>
 hipError_t launch(const PromptArgs& a, hipStream_t stream) {
   const long long rows = (long long)a.tq * (a.hq / a.hkv);
   const long long slots = rows / (64 * NB) + a.seqs + 1;
-  attn_prompt_kernel<T, DP, NB><<<(unsigned)(slots * a.hkv), 256, 0, stream>>>(a, Divisor(a.hq / a.hkv), Divisor(a.hkv), (int)slots);
+  const float lower = SHIFT<T> / a.scale_log2, limit = (SHIFT<T> + SLACK<T>) / a.scale_log2;
+  attn_prompt_kernel<T, DP, NB><<<(unsigned)(slots * a.hkv), 256, 0, stream>>>(a, Divisor(a.hq / a.hkv), Divisor(a.hkv), (int)slots, lower, limit);
   return hipGetLastError();
 }
 

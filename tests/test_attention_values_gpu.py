@@ -123,3 +123,24 @@ def test_decode_many_small_weights_in_one_share(capi, page, bits, dtype):
         ref, mag = attention.attend(q[:, h], k, v, 1.0, [n])
         assert ((out[5, h] - ref[0]).abs() <= attention.tolerance(ref, mag, dtype, False, n)[0]).all()
     assert torch.equal(out[:5], v[0].double().expand(5, 2, D)) and torch.equal(out[6:], v[0].double().expand(B - 6, 2, D))
+
+
+@pytest.mark.parametrize("bits", [12.0, 20.4, 24.8, 25.1, 30.0])
+@pytest.mark.parametrize("nq,D", [(1, 64), (3, 128), (2, 256)])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_prompt_many_small_weights_beside_a_large_one(capi, nq, D, bits, dtype):
+    """The last rows of a long prompt, whose first key outweighs each of the others by far. Weights are rounded once, to u of their size. fp16 has
+    none below 2^-24; a kernel that lets a weight reach 2^15 where the running maximum's is at least 2^11 loses at most 2^-25 / 2^11 of each."""
+    n = 131071
+    gen = torch.Generator().manual_seed(n)
+    q, k, v = one_above_the_others(gen, n, D, bits, dtype)
+    q = q.repeat(nq, 1, 1)
+    out = capi.attn_prompt(q.to(DEV), k.to(DEV).view(n, 1, D), v.to(DEV).view(n, 1, D), int32([0, nq]), int32([0, n]), 1.0).cpu().double()
+    u = attention.U[dtype]
+    for i in range(nq):
+        ref, mag = attention.attend(q[i, :1], k, v, 1.0, [n - nq + 1 + i])
+        tol = u * ref.abs() + 2 * (2.0 ** -12 + u) * mag + 2.0 ** -24
+        if dtype == HF:
+            tol += n * 2.0 ** -36 * v.abs().max()
+        for h in range(2):
+            assert ((out[i, h] - ref[0]).abs() <= tol[0]).all()
