@@ -9,14 +9,19 @@
 
 namespace fsw {
 
+inline int ceil_log2(long long n) {
+  int bits = 0;
+  while ((1LL << bits) < n) ++bits;
+  return bits;
+}
+
 // Division of a whole number below 2^30 by a divisor known on the host: n / d = mulhi(4 n, ceil(2^(30 + s) / d)) >> s with s =
 // ceil(log2 d). The multiplier exceeds 2^(30 + s) / d by less than 1 <= 2^s / d, so the quotient's error is below n 2^-30 / d < 1 / d.
 struct Divisor {
   unsigned d, mul;
   int shift;
   Divisor() = default;
-  explicit Divisor(unsigned by) : d(by), shift(0) {
-    while ((1ull << shift) < by) ++shift;
+  explicit Divisor(unsigned by) : d(by), shift(ceil_log2(by)) {
     mul = (unsigned)(((1ull << (30 + shift)) + by - 1) / by);
   }
 #ifdef __HIP_DEVICE_COMPILE__

@@ -30,8 +30,8 @@ namespace fsw {
 namespace {
 
 constexpr float NEG_INF = -__builtin_inff();
-// The running maximum of a head moves only when a score passes it by this much (in powers of two): sums stay near 1, the accumulators
-// are seldom rescaled.
+// A head's m is the score that weighs 1 (in powers of two). It moves when a score passes m - lift by SLACK, and is that score plus the lift then, so the
+// accumulators are seldom rescaled.
 constexpr float SLACK = 8.0f;
 
 typedef __attribute__((ext_vector_type(4))) short s16x4;
@@ -71,7 +71,7 @@ __device__ __forceinline__ float sum_over_groups(float x) {
 }
 
 // 2^(a - b) for a <= b, with -inf - -inf = 0 (nothing seen yet). Never zero, so that an infinity that has been summed up stays one; what
-// that adds to other sums is below 2^-126 of the values.
+// that adds to other sums is below 2^-126 of the values, in units in which all weights are 2^-38 at least.
 __device__ __forceinline__ float scale_of(float a, float b) {
   return a == b ? 1.0f : fmaxf(__builtin_amdgcn_exp2f(a - b), FLT_MIN);
 }
@@ -81,7 +81,7 @@ __device__ __forceinline__ float scale_of(float a, float b) {
 // DP: channels, padded to 64, 128 or 256; a row of values is NV vectors of VL elements on 16 lanes.
 // WHOLE: page_size % 16 == 0, so 16 keys in a row lie in one page and the page's address is wave-uniform.
 template <class T, int DP, bool WHOLE, int WAVES>
-__global__ __launch_bounds__(64 * WAVES, DP == 256 ? 2 : 4) void attn_decode_kernel(PagedAttnArgs a, int chunk, int group, int head_tiles,
+__global__ __launch_bounds__(64 * WAVES, DP == 256 ? 2 : 4) void attn_decode_kernel(PagedAttnArgs a, float lift, int chunk, int group, int head_tiles,
                                                                                     float* partial) {
   constexpr int KS = DP / 32;                  // steps over the channels
   constexpr int VL = DP == 64 ? 4 : 8, NV = DP / (16 * VL), NA = NV * VL;
@@ -198,8 +198,8 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 2 : 4) void attn_decode_ker
         top = fmaxf(top, s[r]);
       }
       top = max_over_groups(top);
-      if (__any(top > m + SLACK)) {
-        const float now = fmaxf(m, top), alpha = scale_of(m, now);
+      if (__any(top > m + (SLACK - lift))) {
+        const float now = fmaxf(m, top + lift), alpha = scale_of(m, now);
         m = now;
         sum *= alpha;
 #pragma unroll
@@ -407,6 +407,13 @@ __global__ __launch_bounds__(256) void attn_join_kernel(PagedAttnArgs a, int chu
   *(u32x2*)(op + 4 * at) = u32x2{T::pack2(o[0] * inv, o[1] * inv), T::pack2(o[2] * inv, o[3] * inv)};
 }
 
+// bf16 has values as large as fp32's: there the weights of all keys together stay below 1, so that no sum of finite values overflows before it is
+// normalised, here or in the join. What that costs is fp32's smallest number, 2^-149, over the largest weight.
+template <class T>
+float lift_of(int keys) {
+  return std::is_same<T, Bf16>::value ? SLACK + ceil_log2(keys) : 0.0f;
+}
+
 int head_tiles(int hq, int hkv) { return (hq / hkv + 15) / 16; }
 
 template <class T, int DP, int WAVES>
@@ -416,7 +423,7 @@ hipError_t launch_waves(const PagedAttnArgs& a, const PagedAttnPlan& p, float* p
   const dim3 grid(a.hkv * tiles, a.seqs, p.splits);
   const size_t lds = (size_t)WAVES * (group < 16 ? group : 16) * (DP + 4) * sizeof(float);
   const auto kernel = a.cache.page_size % 16 == 0 ? attn_decode_kernel<T, DP, true, WAVES> : attn_decode_kernel<T, DP, false, WAVES>;
-  kernel<<<grid, 64 * WAVES, lds, stream>>>(a, p.chunk, group, tiles, partial);
+  kernel<<<grid, 64 * WAVES, lds, stream>>>(a, lift_of<T>(a.max_len), p.chunk, group, tiles, partial);
   return hipGetLastError();
 }
 

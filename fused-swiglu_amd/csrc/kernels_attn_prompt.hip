@@ -20,6 +20,8 @@
 // copies issued without a branch (1104 -> 1065). What did not pay: the scores of the next keys beside the weights of these (1172),
 // keys and values copied one and a half turns ahead with a barrier more (1162), wave priorities (1136), eight waves on every other tile of
 // the same rows (1243).
+#include <float.h>
+
 #include "attn.h"
 #include "attn_device.h"
 #include "fsw_device.h"
@@ -33,17 +35,24 @@ typedef __attribute__((address_space(3))) void lds_void;
 typedef __attribute__((address_space(3))) unsigned char lds_byte;
 
 constexpr float NEG_INF = -__builtin_inff();
-// m is the score that weighs 1. It moves when a score would weigh more than 2^(SHIFT + SLACK), so that this score weighs 2^SHIFT. fp16 has weights
-// from 2^-24 to 2^16, all of which are used: one is rounded like any other down to 2^-25 of the maximum's, and 2^-36 of that is what a
-// smaller one may lose. The kernel has both divided by c, in units of its scores.
+// m is the score that weighs 1. It moves when a score would weigh more than 2^(shift + SLACK), so that this score weighs 2^shift; the kernel has
+// both limits divided by c, in units of its scores. fp16 has weights from 2^-24 to 2^16, all of which are used: one is rounded like any
+// other down to 2^-25 of the maximum's, and 2^-36 of that is what a smaller one may lose. bf16 has fp32's exponents, and values as large as fp32's: all weights
+// of a row together stay below 1, so that no sum of finite values overflows before it is normalised (what that costs is fp32's smallest number, 2^-149, over the largest weight).
 template <class T>
 constexpr float SLACK = 8.0f;
-template <class T>
-constexpr float SHIFT = 0.0f;
 template <>
 inline constexpr float SLACK<Fp16> = 4.0f;
+template <class T>
+float shift_of(int keys);
 template <>
-inline constexpr float SHIFT<Fp16> = 11.0f;
+float shift_of<Bf16>(int keys) {
+  return -SLACK<Bf16> - ceil_log2(keys);
+}
+template <>
+float shift_of<Fp16>(int) {
+  return 11.0f;
+}
 constexpr int KEYS = 64;       // of a tile
 
 #define INLINE __attribute__((always_inline))
@@ -379,7 +388,8 @@ template <class T, int DP, int NB>
 hipError_t launch(const PromptArgs& a, hipStream_t stream) {
   const long long rows = (long long)a.tq * (a.hq / a.hkv);
   const long long slots = rows / (64 * NB) + a.seqs + 1;
-  const float lower = SHIFT<T> / a.scale_log2, limit = (SHIFT<T> + SLACK<T>) / a.scale_log2;
+  // (the smallest scales do without: a score that is no finite number is none)
+  const float shift = shift_of<T>(a.tk), lower = fmaxf(shift / a.scale_log2, -FLT_MAX / 4), limit = fmaxf((shift + SLACK<T>) / a.scale_log2, -FLT_MAX / 4);
   attn_prompt_kernel<T, DP, NB><<<(unsigned)(slots * a.hkv), 256, 0, stream>>>(a, Divisor(a.hq / a.hkv), Divisor(a.hkv), (int)slots, lower, limit);
   return hipGetLastError();
 }

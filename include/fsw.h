@@ -236,7 +236,7 @@ FSW_API size_t fsw_attn_decode_workspace_bytes(int dtype, int64_t B, int64_t Hq,
  * that hold 16 bits (bf16) or 22 (fp16) of them, one rounding. max_len: the host's bound of the lengths, which sets
  * the launch's shape. A length of 0 gives zeros; a length below 0 or above max_len, or a page outside the cache among a sequence's pages, gives NaN for that
  * sequence. What the cache holds behind a length is never used. Every key before it weighs more than nothing: an infinity among their values gives that
- * infinity, both signs or a NaN give NaN, in their channel.
+ * infinity, both signs or a NaN give NaN, in their channel. Finite values give finite sums, however large they are.
  */
 FSW_API int fsw_attn_decode(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, const void* Q, int64_t q_seq, int64_t q_head,
                             const fsw_kv_cache* cache, const int32_t* block_table, int64_t table_ld, const int32_t* lengths,
@@ -253,7 +253,8 @@ FSW_API int fsw_validate_attn_prompt(int dtype, int64_t Tq, int64_t Tk, int64_t 
  * Causal attention of B packed sequences: sequence b is rows cu_q[b] .. cu_q[b + 1] - 1 of Q and O and rows cu_k[b] .. cu_k[b + 1] - 1 of
  * K and V (B + 1 offsets each, ascending from 0; for whole prompts both are one array). Ends are aligned: query i of nq sees the keys
  * j <= i + nk - nq. A query that sees no key, and a row of Q behind the last sequence, gives zeros. Scores, sums and the
- * normalisation are fp32; infinities and NaN among the values are as for fsw_attn_decode, and do not reach rows that do not see them; the weights 2^(c s - m) are rounded to the element type once, for the matrix product with V, and their sum is taken of the rounded values.
+ * normalisation are fp32; values of any size, infinities and NaN among them are as for fsw_attn_decode, and do not reach rows that do not see them;
+ * the weights 2^(c s - m) are rounded to the element type once, for the matrix product with V, and their sum is taken of the rounded values.
  */
 FSW_API int fsw_attn_prompt(int dtype, int64_t Tq, int64_t Tk, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, const void* Q,
                             int64_t q_token, int64_t q_head, const void* K, int64_t k_token, int64_t k_head, const void* V,

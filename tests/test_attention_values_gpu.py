@@ -144,3 +144,73 @@ def test_prompt_many_small_weights_beside_a_large_one(capi, nq, D, bits, dtype):
             tol += n * 2.0 ** -36 * v.abs().max()
         for h in range(2):
             assert ((out[i, h] - ref[0]).abs() <= tol[0]).all()
+
+
+def huge(x, dtype, size):
+    """x of the order of one, scaled to the largest finite values there are (fp16: 60000)."""
+    return (x.float().clamp(-1, 1) * (size if dtype == BF else 60000.0)).to(dtype)
+
+
+@pytest.mark.parametrize("size", [3.3e38, 1e37])
+@pytest.mark.parametrize("n,Hq,Hkv,D,page,max_len", [(40, 2, 1, 64, 16, None), (700, 4, 2, 128, 9, None), (9000, 2, 1, 64, 64, None),
+                                                     (2600, 130, 130, 8, 16, None), (300, 2, 1, 256, 16, 20000)])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_decode_values_as_large_as_the_type_has(capi, n, Hq, Hkv, D, page, max_len, dtype, size):
+    """A mean of finite values is finite, whatever their size and number."""
+    gen = torch.Generator().manual_seed(n)
+    caches, table = paged(gen, [n], Hkv, D, page, dtype)
+    most = max_len or n
+    table = torch.cat([table, table[:, :1].expand(1, -(-most // page) - table.shape[1])], 1)
+    v = caches[1].cpu()
+    v = huge(torch.where(torch.isnan(v), v, v.abs() + 0.5), dtype, size)  # of one sign: nothing cancels
+    q = randn(gen, 1, Hq, D, dtype=dtype)
+    out = capi.attn_decode(q.to(DEV), caches[0], v.to(DEV), table.to(DEV), int32([n]), most, 0.3).cpu().double()
+    ref, mag = attention.decode(q, caches[0], v, table, [n], 0.3)
+    assert torch.isfinite(ref).all() and ((out - ref).abs() <= attention.tolerance(ref, mag, dtype, False, n)).all()
+
+
+@pytest.mark.parametrize("size", [3.3e38, 1e37])
+@pytest.mark.parametrize("n,Hq,Hkv,D", [(40, 2, 1, 64), (300, 4, 2, 128), (130, 2, 1, 256), (700, 1, 1, 16)])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_prompt_values_as_large_as_the_type_has(capi, n, Hq, Hkv, D, dtype, size):
+    gen = torch.Generator().manual_seed(n)
+    q, k, v = (randn(gen, n, h, D, dtype=dtype) for h in (Hq, Hkv, Hkv))
+    v = huge(v.abs() + 0.5, dtype, size)
+    out = capi.attn_prompt(q.to(DEV), k.to(DEV), v.to(DEV), int32([0, n]), int32([0, n]), 0.3).cpu().double()
+    ref, mag = attention.prompt(q, k, v, [0, n], [0, n], 0.3)
+    assert torch.isfinite(ref).all() and ((out - ref).abs() <= attention.tolerance(ref, mag, dtype, True, n)).all()
+
+
+@pytest.mark.parametrize("size", [1e-33, 1e-30])
+def test_values_as_small_as_bf16_has(capi, size):
+    """What keeps large values finite costs small ones little: sums are off by less than 2^-149 (fp32's smallest) over the largest weight, which is
+    at least 2^-8 over twice the number of keys the launch counts with."""
+    gen = torch.Generator().manual_seed(1)
+    n, D = 500, 64
+    q, k, v = (randn(gen, n, 1, D) for _ in range(3))
+    v = (v.float() * size).to(BF)
+    least = n * 2.0 ** -149 * 2 ** 8 * 2 * n
+    out = capi.attn_prompt(q.to(DEV), k.to(DEV), v.to(DEV), int32([0, n]), int32([0, n]), 0.1).cpu().double()
+    ref, mag = attention.prompt(q, k, v, [0, n], [0, n], 0.1)
+    assert ((out - ref).abs() <= 2.0 ** -8 * ref.abs() + 2 * (2.0 ** -12 + 2.0 ** -8) * mag + least).all()
+    caches = [torch.cat([c, c.new_zeros(12, 1, D)]).view(32, 16, 1, D).transpose(1, 2).to(DEV) for c in (k, v)]
+    table = torch.arange(32, dtype=torch.int32).view(1, -1)
+    out = capi.attn_decode(q[:1].to(DEV), *caches, table.to(DEV), int32([n]), n, 0.1).cpu().double()
+    ref, mag = attention.decode(q[:1], *caches, table, [n], 0.1)
+    assert ((out - ref).abs() <= 2.0 ** -8 * ref.abs() + 2 * 2.0 ** -12 * mag + least).all()
+
+
+@pytest.mark.parametrize("scale", [2.0 ** -126, 2.0 ** -125, 2.0 ** -120])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_smallest_scales_weigh_all_keys_alike(capi, dtype, scale):
+    gen = torch.Generator().manual_seed(2)
+    n, D = 200, 64
+    q, k, v = (randn(gen, n, 1, D, dtype=dtype) for _ in range(3))
+    out = capi.attn_prompt(q.to(DEV), k.to(DEV), v.to(DEV), int32([0, n]), int32([0, n]), scale).cpu().double()
+    ref, mag = attention.prompt(q, k, v, [0, n], [0, n], scale)
+    assert ((out - ref).abs() <= attention.tolerance(ref, mag, dtype, True, n)).all()
+    caches = [torch.cat([c, c.new_zeros(8, 1, D)]).view(13, 16, 1, D).transpose(1, 2).to(DEV) for c in (k, v)]
+    table = torch.arange(13, dtype=torch.int32).view(1, -1)
+    out = capi.attn_decode(q[:1].to(DEV), *caches, table.to(DEV), int32([n]), n, scale).cpu().double()
+    ref, mag = attention.decode(q[:1], *caches, table, [n], scale)
+    assert ((out - ref).abs() <= attention.tolerance(ref, mag, dtype, False, n)).all()
