@@ -102,7 +102,9 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prompt_kernel(Pro
 
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, grp = lane >> 4;
-  const int rank = by_hkv.quotient(blockIdx.x), kvh = (int)blockIdx.x - rank * a.hkv, slot = slots - 1 - rank;
+  const int block = (int)(blockIdx.y * gridDim.x + blockIdx.x);  // below 2^27: 2^30 rows / 64 + 2^26 (sequence, key-value head) pairs
+  const int rank = by_hkv.quotient(block), kvh = block - rank * a.hkv, slot = slots - 1 - rank;
+  if (slot < 0) return;
   const int group = (int)by_group.d;
 
   // Sequence s owns the slots from rows_before(s) / BM + s on, which leaves it enough for its rows whatever their remainder; slot -> s by
@@ -390,7 +392,9 @@ hipError_t launch(const PromptArgs& a, hipStream_t stream) {
   const long long slots = rows / (64 * NB) + a.seqs + 1;
   // (the smallest scales do without: a score that is no finite number is none)
   const float shift = shift_of<T>(a.tk), lower = fmaxf(shift / a.scale_log2, -FLT_MAX / 4), limit = fmaxf((shift + SLACK<T>) / a.scale_log2, -FLT_MAX / 4);
-  attn_prompt_kernel<T, DP, NB><<<(unsigned)(slots * a.hkv), 256, 0, stream>>>(a, Divisor(a.hq / a.hkv), Divisor(a.hkv), (int)slots, lower, limit);
+  const long long blocks = slots * a.hkv, most = 1 << 22;  // a launch has less than 2^32 threads along x
+  const dim3 grid((unsigned)(blocks < most ? blocks : most), (unsigned)((blocks + most - 1) / most));
+  attn_prompt_kernel<T, DP, NB><<<grid, 256, 0, stream>>>(a, Divisor(a.hq / a.hkv), Divisor(a.hkv), (int)slots, lower, limit);
   return hipGetLastError();
 }
 
