@@ -132,7 +132,8 @@ int fsw_validate_attn_decode(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int6
   CHECK(check_cache(cache, D, Hkv));
   if (!block_table) return FSW_E_NULL;
   if (table_ld > MAX_STRIDE) return FSW_E_SHAPE;
-  if (table_ld < (max_len + cache->page_size - 1) / cache->page_size) return FSW_E_LD;
+  // 0: one row for all sequences
+  if (table_ld < (max_len + cache->page_size - 1) / cache->page_size && !(table_ld == 0 && B > 1)) return FSW_E_LD;
   return aligned(block_table, 4) ? FSW_OK : FSW_E_ALIGN;
 }
 

@@ -220,7 +220,8 @@ FSW_API int fsw_kv_append(int dtype, int64_t T, int64_t Hq, int64_t Hkv, int64_t
                           const int32_t* positions, const int32_t* slots, void* Qout, int64_t qo_token, int64_t qo_head,
                           void* Kout, int64_t ko_token, int64_t ko_head, const fsw_kv_cache* cache, void* stream);
 
-/* Host-only validation of fsw_attn_decode (all but the workspace). B <= 65535; scale finite and positive (a normal number); table_ld >= ceil(max_len / page_size). */
+/* Host-only validation of fsw_attn_decode (all but the workspace). B <= 65535; scale finite and positive (a normal number); table_ld >=
+ * ceil(max_len / page_size), or 0: all sequences have the same pages. */
 FSW_API int fsw_validate_attn_decode(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, const void* Q, int64_t q_seq,
                                      int64_t q_head, const fsw_kv_cache* cache, const int32_t* block_table, int64_t table_ld,
                                      const int32_t* lengths, int64_t max_len, float scale, const void* O, int64_t o_seq,

@@ -24,3 +24,17 @@ def test_prompt_of_most_sequences_and_many_heads(capi, B, H):
     seqs = starts(list(at.values()))
     ref, mag = attention.prompt(q[:, some], k[:, some], v[:, some], seqs, seqs, 0.35)
     assert ((out[:, some].cpu().double() - ref).abs() <= attention.tolerance(ref, mag, BF, True, 70)).all()
+
+
+@pytest.mark.parametrize("lengths", [[70, 1, 64, 33], [1100, 3]])
+def test_decode_of_sequences_that_share_their_pages(capi, ext, lengths):
+    """A block table made by expand(): one row for all sequences, lengths of their own."""
+    gen = torch.Generator().manual_seed(5)
+    caches, table = paged(gen, [max(lengths)], 2, 64, 16, BF)
+    q, B = randn(gen, len(lengths), 4, 64), len(lengths)
+    args = (q.to(DEV), *caches, table.to(DEV).expand(B, -1), int32(lengths), max(lengths), 0.125)
+    want = capi.attn_decode(*args[:3], table.to(DEV).repeat(B, 1), *args[4:])
+    for got in (capi.attn_decode(*args), ext.attn_decode_bf16(*args), torch.ops.ASMLLM.attn_decode_bf16(*args)):
+        assert torch.equal(got, want)
+    ref, mag = attention.decode(q, *caches, table.expand(B, -1), lengths, 0.125)
+    assert ((want.cpu().double() - ref).abs() <= attention.tolerance(ref, mag, BF, False, max(lengths))).all()
