@@ -416,7 +416,8 @@ def kv_cache(k_cache, v_cache):
 
 
 def kv_append(q, k, v, cos_sin, positions, slots, k_cache, v_cache, interleaved=False, q_out=None, k_out=None):
-    """Rotated copies of q [T, Hq, D] and k [T, Hkv, D]; rotated k, and v, go to their slots of the caches (fsw_kv_append)."""
+    """Rotated copies of q [T, Hq, D] and k [T, Hkv, D]; rotated k, and v, go to their slots of the caches (fsw_kv_append).
+    k_out=False: rotated keys go to the cache only, the second result is None."""
     import torch
     code = dtype_code(q)
     _check_rows(q, k, v)
@@ -435,14 +436,18 @@ def kv_append(q, k, v, cos_sin, positions, slots, k_cache, v_cache, interleaved=
     if not cos_sin.is_contiguous():
         raise FswError(E_LD, "fsw: cos_sin must be contiguous")
     q_out = torch.empty((T, Hq, D), dtype=q.dtype, device=q.device) if q_out is None else q_out
-    k_out = torch.empty((T, Hkv, D), dtype=q.dtype, device=q.device) if k_out is None else k_out
-    _check_rows(q, q_out, k_out)
-    if q_out.shape != q.shape or k_out.shape != k.shape:
+    if k_out is False:
+        k_out = None
+    elif k_out is None:
+        k_out = torch.empty((T, Hkv, D), dtype=q.dtype, device=q.device)
+    _check_rows(q, q_out, *([] if k_out is None else [k_out]))
+    if q_out.shape != q.shape or (k_out is not None and k_out.shape != k.shape):
         raise FswError(E_SHAPE, "fsw: q_out and k_out have the shapes of q and k")
     with torch.cuda.device(q.device):
         check(lib().fsw_kv_append(code, T, Hq, Hkv, D, cos_sin.shape[1], int(interleaved), *_row_args(q), *_row_args(k),
                                   *_row_args(v), cos_sin.data_ptr(), cos_sin.shape[0], positions.data_ptr(), slots.data_ptr(),
-                                  *_row_args(q_out), *_row_args(k_out), ctypes.byref(cache), _stream(q)))
+                                  *_row_args(q_out), *((None, 0, 0) if k_out is None else _row_args(k_out)), ctypes.byref(cache),
+                                  _stream(q)))
     return q_out, k_out
 
 

@@ -38,3 +38,16 @@ def test_decode_of_sequences_that_share_their_pages(capi, ext, lengths):
         assert torch.equal(got, want)
     ref, mag = attention.decode(q, *caches, table.expand(B, -1), lengths, 0.125)
     assert ((want.cpu().double() - ref).abs() <= attention.tolerance(ref, mag, BF, False, max(lengths))).all()
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_append_without_rotated_keys(capi, dtype):
+    """k_out=False: the caches and the queries as with them, nothing else."""
+    gen = torch.Generator().manual_seed(6)
+    T, D = 9, 64
+    q, k, v = (randn(gen, T, h, D, dtype=dtype).to(DEV) for h in (4, 2, 2))
+    args = (angles(gen, T, D).to(DEV), int32(list(range(T))), int32(list(range(T))))
+    a, b = ([torch.zeros(2, 2, 8, D, dtype=dtype, device=DEV) for _ in range(2)] for _ in range(2))
+    want, _ = capi.kv_append(q, k, v, *args, *a)
+    got, none = capi.kv_append(q, k, v, *args, *b, k_out=False)
+    assert none is None and torch.equal(got, want) and all(torch.equal(x, y) for x, y in zip(a, b))
