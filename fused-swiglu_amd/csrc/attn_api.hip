@@ -68,8 +68,8 @@ fsw::PagedKv paged(const fsw_kv_cache* c) {
                       fsw::Divisor((unsigned)c->page_size)};
 }
 
-// (the kernels multiply scores by it before they are compared: a masked score, -inf, has to stay one)
-bool good_scale(float s) { return isfinite(s) && s >= FLT_MIN; }
+// (the kernels multiply scores by it and log2(e) before they are compared: a masked score, -inf, has to stay one, and zero zero)
+bool good_scale(float s) { return s >= FLT_MIN && isfinite(s * LOG2E); }
 
 #define CHECK(e)                    \
   do {                              \

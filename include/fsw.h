@@ -220,7 +220,7 @@ FSW_API int fsw_kv_append(int dtype, int64_t T, int64_t Hq, int64_t Hkv, int64_t
                           const int32_t* positions, const int32_t* slots, void* Qout, int64_t qo_token, int64_t qo_head,
                           void* Kout, int64_t ko_token, int64_t ko_head, const fsw_kv_cache* cache, void* stream);
 
-/* Host-only validation of fsw_attn_decode (all but the workspace). B <= 65535; scale finite and positive (a normal number); table_ld >=
+/* Host-only validation of fsw_attn_decode (all but the workspace). B <= 65535; scale a positive normal number, finite also times log2(e); table_ld >=
  * ceil(max_len / page_size), or 0: all sequences have the same pages. */
 FSW_API int fsw_validate_attn_decode(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, const void* Q, int64_t q_seq,
                                      int64_t q_head, const fsw_kv_cache* cache, const int32_t* block_table, int64_t table_ld,
@@ -244,7 +244,7 @@ FSW_API int fsw_attn_decode(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64
                             int64_t max_len, float scale, void* O, int64_t o_seq, int64_t o_head, void* workspace,
                             size_t workspace_bytes, void* stream);
 
-/* Host-only validation of fsw_attn_prompt. B <= 65535; k_token, v_token between D and 2^21; scale finite and positive (a normal number). */
+/* Host-only validation of fsw_attn_prompt. B <= 65535; k_token, v_token between D and 2^21; scale a positive normal number, finite also times log2(e). */
 FSW_API int fsw_validate_attn_prompt(int dtype, int64_t Tq, int64_t Tk, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, const void* Q,
                                      int64_t q_token, int64_t q_head, const void* K, int64_t k_token, int64_t k_head,
                                      const void* V, int64_t v_token, int64_t v_head, const int32_t* cu_q, const int32_t* cu_k,
