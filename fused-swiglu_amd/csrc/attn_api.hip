@@ -3,6 +3,8 @@
 #include <float.h>
 #include <math.h>
 
+#include <algorithm>
+
 #include "attn.h"
 #include "fsw.h"
 #include "fsw_internal.h"
@@ -63,6 +65,21 @@ int check_cache(const fsw_kv_cache* c, int64_t d, int64_t heads) {
   return FSW_OK;
 }
 
+// cells that are written: each dimension lies inside the stride of the next larger one
+bool cells_apart(const fsw_kv_cache* c, int64_t d, int64_t heads) {
+  struct Dim {
+    int64_t n, stride;
+  } dims[3] = {{c->pages, c->page_stride}, {heads, c->head_stride}, {c->page_size, c->token_stride}};
+  std::sort(dims, dims + 3, [](const Dim& a, const Dim& b) { return a.stride < b.stride; });
+  __int128 extent = d;  // up to 2^30 strides of up to 2^40 elements
+  for (const Dim& x : dims) {
+    if (x.n <= 1) continue;
+    if (x.stride < extent) return false;
+    extent += (__int128)(x.n - 1) * x.stride;
+  }
+  return true;
+}
+
 fsw::PagedKv paged(const fsw_kv_cache* c) {
   return fsw::PagedKv{c->k, c->v, (int)c->pages, (int)c->page_size, c->page_stride, c->head_stride, c->token_stride,
                       fsw::Divisor((unsigned)c->page_size)};
@@ -97,7 +114,8 @@ int fsw_validate_kv_append(int dtype, int64_t T, int64_t Hq, int64_t Hkv, int64_
   if (!positions || !slots || (rot > 0 && !cos_sin)) return FSW_E_NULL;
   if (rot > 0 && table_rows < 1) return FSW_E_SHAPE;
   if (!aligned(positions, 4) || !aligned(slots, 4) || !aligned(cos_sin, rot % 8 ? 4 : 16)) return FSW_E_ALIGN;
-  return check_cache(cache, D, Hkv);
+  CHECK(check_cache(cache, D, Hkv));
+  return cells_apart(cache, D, Hkv) ? FSW_OK : FSW_E_LD;
 }
 
 int fsw_kv_append(int dtype, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t rot, int interleaved, const void* Q,

@@ -191,7 +191,8 @@ FSW_API int fsw_gateup_ws(int dtype, int64_t M, int64_t N, int64_t K, const void
  */
 
 /* A paged cache of one layer. Token t of a page holds its head h at element page * page_stride + h * head_stride +
- * t * token_stride of k, and of v likewise. Strides are multiples of 8 below 2^40 (token_stride: at most 2^24); pages * page_size <= 2^30. */
+ * t * token_stride of k, and of v likewise. Strides are multiples of 8 below 2^40 (token_stride: at most 2^24); pages * page_size <= 2^30.
+ * A cache that is written has cells that do not overlap, each dimension inside the next larger stride. */
 typedef struct fsw_kv_cache {
   void* k;
   void* v;

@@ -27,3 +27,20 @@ def test_scales_that_are_finite_times_log2_e(capi):
         assert decode(capi, scale=scale) == prompt(capi, scale) == capi.OK
     for scale in (2.4e38, 3.4e38, float("inf"), float("nan"), 2.0 ** -127, 0.0, -1.0):
         assert decode(capi, scale=scale) == prompt(capi, scale) == capi.E_SHAPE
+
+
+def test_caches_whose_cells_overlap_are_not_written(capi):
+    """Any order of the dimensions, but each inside the next larger stride; reading does not mind."""
+    def append(strides, pages=4, page_size=16):
+        return capi.lib().fsw_validate_kv_append(0, 4, 4, 2, 64, 64, P, 256, 64, P, 128, 64, P, 128, 64, P, 8, P, P, P, 256, 64,
+                                                 P, 128, 64, cache_of(capi, pages, page_size, strides))
+    for strides in ((2048, 1024, 64), (2048, 64, 128), (64, 4096, 256), (4096, 2048, 64), (2056, 1032, 64)):
+        assert append(strides) == capi.OK, strides
+    assert append((0, 1024, 64), pages=1) == append((128, 64, 0), page_size=1) == capi.OK
+    assert append((1 << 40, 64, 128), pages=1 << 26) == append((64, 1 << 40, 1 << 24), page_size=1 << 16) == capi.OK
+    for strides in ((64, 64, 64), (1024, 1024, 64), (2040, 1024, 64), (2048, 1032, 64), (2048, 960, 64), (2048, 64, 64), (2048, 64, 120), (64, 4096, 248),
+                    (64, 1016, 256)):
+        assert append(strides) == capi.E_LD, strides
+        assert capi.lib().fsw_validate_attn_decode(0, 3, 4, 2, 64, P, 256, 64, cache_of(capi, strides=strides), P, 4, P, 64, 0.125, P, 256,
+                                                   64) == capi.OK
+    assert append((1 << 24, 64, 1 << 24), pages=1 << 26) == append((1 << 40, 1 << 40, 64), pages=1 << 26) == capi.E_LD
