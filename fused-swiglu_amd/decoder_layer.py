@@ -23,7 +23,7 @@ class PagedCache:
 
     def __init__(self, seqs, longest, kv_heads, channels, page, dtype, device):
         per_seq = -(-longest // page)
-        self.page, self.device = page, device
+        self.page, self.longest, self.device = page, longest, device
         self.k = torch.empty(seqs * per_seq, kv_heads, page, channels, dtype=dtype, device=device)
         self.v = torch.empty_like(self.k)
         self.free = list(range(seqs * per_seq))
@@ -33,6 +33,9 @@ class PagedCache:
 
     def grow(self, counts):
         """Room for counts[b] more tokens of sequence b -> positions and slots of the new tokens, packed, on the device."""
+        for b, n in enumerate(counts):
+            if self.lengths[b] + n > self.longest:
+                raise ValueError("sequence %d would have %d tokens, the cache was made for %d" % (b, self.lengths[b] + n, self.longest))
         positions, slots = [], []
         for b, n in enumerate(counts):
             for t in range(self.lengths[b], self.lengths[b] + n):
