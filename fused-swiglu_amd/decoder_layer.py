@@ -89,6 +89,9 @@ class DecoderLayer:
 
     def prefill(self, x, lengths, cache):
         """x: the packed rows of new sequences' prompts."""
+        for b, n in enumerate(lengths):
+            if n and cache.lengths[b]:
+                raise ValueError("sequence %d has tokens in the cache already" % b)
         q, k, v = self._qkv(x)
         positions, slots = cache.grow(lengths)
         q, k = self.append(q, k, v, self.cos_sin, positions, slots, cache.k, cache.v)

@@ -33,3 +33,12 @@ def test_a_sequence_grows_no_longer_than_the_cache_was_made_for():
             cache.grow(counts)
         assert state == (cache.lengths, cache.free, cache.pages)
     cache.grow([0, 36, 37])
+
+
+def test_prompts_are_of_sequences_that_have_no_tokens():
+    """prefill attends within the rows that it is given: a sequence that has tokens in the cache would lose them."""
+    layer, cache = decoder_layer.DecoderLayer.__new__(decoder_layer.DecoderLayer), new()
+    cache.grow([3, 0, 0])
+    with pytest.raises(ValueError, match="sequence 0"):
+        layer.prefill(torch.zeros(5, 16), [2, 3, 0], cache)
+    assert cache.lengths == [3, 0, 0]
