@@ -91,6 +91,7 @@ struct PromptArgs {
   float scale_log2;
   RowsOut o;
 };
+int attn_prompt_rows(int tq, int seqs, int hq, int hkv, int d);  // of a workgroup: 64 or 128
 hipError_t launch_attn_prompt(int dtype, const PromptArgs& a, hipStream_t stream);
 
 }  // namespace fsw

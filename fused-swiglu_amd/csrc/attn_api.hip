@@ -200,6 +200,11 @@ int fsw_validate_attn_prompt(int dtype, int64_t Tq, int64_t Tk, int64_t B, int64
   return k_token > MAX_TILE_TOKEN || v_token > MAX_TILE_TOKEN ? FSW_E_SHAPE : FSW_OK;
 }
 
+int fsw_attn_prompt_rows(int dtype, int64_t Tq, int64_t B, int64_t Hq, int64_t Hkv, int64_t D) {
+  if (check_heads(dtype, Hq, Hkv, D) != FSW_OK || Tq < 1 || Tq > MAX_TOKENS || B < 0 || B > MAX_SEQS) return 0;
+  return fsw::attn_prompt_rows((int)Tq, (int)B, (int)Hq, (int)Hkv, (int)D);
+}
+
 int fsw_attn_prompt(int dtype, int64_t Tq, int64_t Tk, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, const void* Q,
                     int64_t q_token, int64_t q_head, const void* K, int64_t k_token, int64_t k_head, const void* V,
                     int64_t v_token, int64_t v_head, const int32_t* cu_q, const int32_t* cu_k, float scale, void* O,

@@ -247,7 +247,7 @@ int launch_status(hipError_t e) { return finish(e); }
 
 extern "C" {
 
-int fsw_version(void) { return 2001; }
+int fsw_version(void) { return 2002; }
 
 const char* fsw_strerror(int code) {
   switch (code) {

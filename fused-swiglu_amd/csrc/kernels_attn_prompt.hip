@@ -404,12 +404,16 @@ hipError_t launch(const PromptArgs& a, hipStream_t stream) {
 // rows) 27.4 | 22.2, 2000 (504) 56.2 | 53.5, 13 prompts of 1 .. 777 tokens and 40 heads (about 540) 25.3 | 22.4, 3000 tokens (752) 92 | 110, 8192 of 64
 // heads 1080 | 1425; 64 channels: 2000 tokens of 16
 // heads on 4 (252) 33.6 | 25.5, 6000 (752) 115 | 107; 256 channels: 1000 tokens of 16 heads on 8 (128) 49 | 34, 4000 (500) 199 | 250.
+int rows_of(int tq, int seqs, int hq, int hkv, int d) {
+  const int resident = 256 * (d <= 64 ? 3 : d <= 128 ? 2 : 1);  // workgroups of 128 rows, by LDS and registers
+  const long long rows = (long long)tq * (hq / hkv);
+  const long long about = (rows / 128 + seqs / 2) * hkv;  // a sequence's last rows fill half a workgroup
+  return about <= resident + resident / 8 ? 64 : 128;
+}
+
 template <class T, int DP>
 hipError_t launch_dp(const PromptArgs& a, hipStream_t stream) {
-  constexpr int resident = 256 * (DP == 64 ? 3 : DP == 128 ? 2 : 1);  // workgroups of 128 rows, by LDS and registers
-  const long long rows = (long long)a.tq * (a.hq / a.hkv);
-  const long long about = (rows / 128 + a.seqs / 2) * a.hkv;  // a sequence's last rows fill half a workgroup
-  return about <= resident + resident / 8 ? launch<T, DP, 1>(a, stream) : launch<T, DP, 2>(a, stream);
+  return rows_of(a.tq, a.seqs, a.hq, a.hkv, a.d) == 64 ? launch<T, DP, 1>(a, stream) : launch<T, DP, 2>(a, stream);
 }
 
 template <class T>
@@ -420,6 +424,8 @@ hipError_t launch_typed(const PromptArgs& a, hipStream_t stream) {
 }
 
 }  // namespace
+
+int attn_prompt_rows(int tq, int seqs, int hq, int hkv, int d) { return rows_of(tq, seqs, hq, hkv, d); }
 
 hipError_t launch_attn_prompt(int dtype, const PromptArgs& a, hipStream_t stream) {
   return dtype == FSW_BF16 ? launch_typed<Bf16>(a, stream) : launch_typed<Fp16>(a, stream);

@@ -52,6 +52,7 @@ PROTOTYPES = {
     "fsw_attn_decode_workspace_bytes": (_sz, [_i] + [_i64] * 5),
     "fsw_attn_decode": (_i, [_i] + [_i64] * 4 + _rows + [_kvp, _vp, _i64, _vp, _i64, ctypes.c_float] + _rows + [_vp, _sz, _vp]),
     "fsw_validate_attn_prompt": (_i, [_i] + [_i64] * 6 + _rows * 3 + [_vp, _vp, ctypes.c_float] + _rows),
+    "fsw_attn_prompt_rows": (_i, [_i] + [_i64] * 5),
     "fsw_attn_prompt": (_i, [_i] + [_i64] * 6 + _rows * 3 + [_vp, _vp, ctypes.c_float] + _rows + [_vp]),
     "fsw_strerror": (_cp, [_i]),
     "fsw_last_hip_error": (_i, []),

@@ -263,12 +263,16 @@ FSW_API int fsw_attn_prompt(int dtype, int64_t Tq, int64_t Tk, int64_t B, int64_
                             int64_t v_token, int64_t v_head, const int32_t* cu_q, const int32_t* cu_k, float scale, void* O,
                             int64_t o_token, int64_t o_head, void* stream);
 
+/* Rows, (token, query head of a key-value head) pairs, of a workgroup of fsw_attn_prompt: 64 where the launch is small, else 128; 0 for what it refuses or where
+ * there is nothing to launch. For tests and benchmarks. */
+FSW_API int fsw_attn_prompt_rows(int dtype, int64_t Tq, int64_t B, int64_t Hq, int64_t Hkv, int64_t D);
+
 /* The hipError_t (as int) of the most recent failed launch on the calling thread, 0 if none. */
 FSW_API int fsw_last_hip_error(void);
 
 /* ABI version: major * 1000 + minor. 2000: the measurement kernels fsw_probe_* left this library (libfsw_probe.so,
  * fsw_probe.h); fsw_gateup_f32out and fsw_gateup_hblocked joined it; fsw_gateup_workspace_bytes returns 0. 2001: the attention
- * entry points. */
+ * entry points. 2002: fsw_attn_prompt_rows. */
 FSW_API int fsw_version(void);
 
 /*

@@ -44,3 +44,10 @@ def test_caches_whose_cells_overlap_are_not_written(capi):
         assert capi.lib().fsw_validate_attn_decode(0, 3, 4, 2, 64, P, 256, 64, cache_of(capi, strides=strides), P, 4, P, 64, 0.125, P, 256,
                                                    64) == capi.OK
     assert append((1 << 24, 64, 1 << 24), pages=1 << 26) == append((1 << 40, 1 << 40, 64), pages=1 << 26) == capi.E_LD
+
+
+def test_rows_of_a_prompts_workgroup(capi):
+    rows = capi.lib().fsw_attn_prompt_rows
+    assert rows(0, 24, 1, 16, 4, 64) == rows(1, 2000, 1, 32, 8, 128) == 64
+    assert rows(0, 8192, 1, 64, 8, 128) == rows(1, 1 << 20, 65535, 1024, 1024, 256) == 128
+    assert rows(0, 0, 1, 4, 2, 64) == rows(2, 9, 1, 4, 2, 64) == rows(0, 9, 1, 4, 3, 64) == rows(0, 9, -1, 4, 2, 64) == rows(0, 9, 1, 4, 2, 12) == 0
