@@ -451,25 +451,32 @@ hipError_t launch_typed(const PagedAttnArgs& a, const PagedAttnPlan& p, float* p
 
 }  // namespace
 
-// Shares of the keys. Where (sequence, key-value head, 16 query heads) items alone do not fill the card, as many workgroups of many waves as do,
-// of at least 512 keys: the shares' launch that joins them costs 4.5 us, and the keys that a workgroup saves by it have to take
-// longer. (One sequence of 131071 keys, 8 key-value heads: 87.5 + 4.6 us; four waves a workgroup and 128 shares 91.2 + 5.5.) Where they do, shares level batches of
-// uneven lengths, of which the host knows only the bound: 40 x 40 items of 1 .. 4096 keys take 196 us unsplit, 132 in
-// shares of 2048 and 113 of 1024, + 4.6 for the join. Even batches lose by it: 128 x 8 items of 1700 .. 2300 keys take
-// 174 us unsplit, 186 in two shares, 196 in three; so a bound of up to 2560 keys is left whole. The farther the bound, the more shares, up to
-// 8192 of all items together (32 x 8 items of 1 .. 32768 keys: 225 us in 8 shares, 150 in 27): most of the short sequences' are empty and end at
-// once. From 8192 items on the card's dynamic assignment levels them. Where items are few and a workgroup has 16 waves, empty ones cost more than
-// they level (four sequences of 20 .. 32000 keys: 68 us in 8 shares, 81 in 32, 96 in 63).
+// Shares of the keys, and waves of a workgroup.
+// Few (sequence, key-value head, 16 query heads) items: workgroups of many waves, of which a CU holds one; as many shares as give every CU one, of
+// at least 512 keys, because the launch that joins them costs 4.5 us. (One sequence of 131071 keys, 8 key-value heads: 87 + 4.6 us; four
+// waves a workgroup and 128 shares 91 + 5.5.) Empty shares cost more there than they level (four sequences of 20 .. 32000 keys: 68 us in 8
+// shares, 81 in 32, 96 in 63).
+// Many items: four waves, of which a CU holds four workgroups, so 1024 fill the card. Below that they do so only if they are split, and
+// bounds of up to 2560 keys are not; many waves serve those as long as items are no more than the CUs, or twice as many where the walk is long. us, many
+// waves | four, 8 key-value heads of 128 channels, bounds of 60, 300, 1000, 2560 keys: 128 items 6.5 | 5.0, 10.6 | 14.5, 17 | 41, 34 | 101;
+// 256 items 7.6 | 6.5, 12.5 | 16.6, 23 | 42, 58 | 108; 512 items 13.6 | 7.4, 22.9 | 21.2, 40 | 51, 116 | 141; 768 items 20 | 9, 33 | 25, 59 | 59, 170 | 173.
+// Above 2560, in shares: bounds of 4096, 128 items 50 | 61, 192 items 85 | 74, 256 items 89 | 90.
+// Shares level batches of uneven lengths, of which the host knows only the bound, and cost even ones. us, unsplit | in shares of 1024 keys:
+// 40 x 40 items of 1 .. 2000 keys 184 | 160, 2560 206 | 185, 3000 260 | 221, 4096 362 | 318; 128 x 8 items of 1700 .. 2300 keys 183 | 208, 1900 .. 2560
+// 200 | 224, 2200 .. 3000 234 | 258, 3000 .. 4096 319 | 351. Which of them a batch is cannot be told here: 2560 is where the uneven one's gain begins to outgrow the even one's
+// loss. The farther the bound, the more shares, up to 8192 of all items together (32 x 8 items of 1 .. 32768 keys: 225 us in 8 shares, 150 in
+// 27): most of the short sequences' are empty and end at once. From 8192 items on the card's dynamic assignment levels them.
 PagedAttnPlan paged_attn_plan(int seqs, int hq, int hkv, int d, int max_len) {
   const long long items = (long long)seqs * hkv * head_tiles(hq, hkv);
   PagedAttnPlan p;
-  const bool few = items < 128;
+  const bool whole = max_len <= 2560;  // not split where items are many
+  const bool few = items < 128 || (whole && (items <= 256 ? max_len > 64 : items <= 512 && max_len > 512));
   p.waves = few ? (d > 128 ? 8 : 16) : 4;
   const long long unit = 16 * p.waves;  // keys of a workgroup's turn
   long long wanted = 1;
   if (few)
     wanted = items > 0 ? (4096 / p.waves + items - 1) / items : 1;
-  else if (items < 8192 && max_len > 2560)
+  else if (items < 8192 && !whole)
     wanted = 8192 / items > 8 ? 8192 / items : 8;
   const long long least = few ? 512 : 1024;
   long long splits = (max_len + least - 1) / least;

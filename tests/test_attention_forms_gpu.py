@@ -222,3 +222,28 @@ def test_the_dispatcher_calls_the_kernels_in_both_types(capi):
         got = getattr(torch.ops.ASMLLM, "kv_append_" + name)(args[0], k, v, *rest, *a, True)
         want = capi.kv_append(args[0], k, v, *rest, *b, True)
         assert all(torch.equal(x, y) for x, y in zip(list(got) + a, list(want) + b))
+
+
+@pytest.mark.parametrize("Hq,Hkv,D,page", [(64, 64, 128, 16), (160, 80, 64, 16), (66, 66, 80, 5), (72, 72, 256, 16), (64, 64, 136, 24), (1024, 64, 16, 7)])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_decode_of_more_than_512_items(capi, Hq, Hkv, D, page, dtype):
+    """Workgroups of four waves whose sequences are whole."""
+    gen = torch.Generator().manual_seed(Hq + D)
+    lengths = [1, 0, 17, 64, 65, 130, 300, 33, 257]
+    assert len(lengths) * Hkv > 512 and parts(capi, len(lengths), Hq, Hkv, D, 300) == 0
+    q, rows, caches, table = decode_case(gen, lengths, Hq, Hkv, D, page, dtype, 300)
+    out = capi.attn_decode(q.to(DEV), *caches, table.to(DEV), int32(lengths), 300, D ** -0.5)
+    some, heads = sampled(Hq, Hkv)
+    check_shares(out[:, heads], q[:, heads], [[x[:, some] for x in kv] for kv in rows], lengths, D ** -0.5, dtype, 300)
+
+
+@pytest.mark.parametrize("B,Hkv", [(16, 8), (43, 6), (64, 8), (65, 8)])
+@pytest.mark.parametrize("most", [64, 65, 512, 513, 2560, 2561])
+def test_decode_on_both_sides_of_the_rules(capi, B, Hkv, most):
+    """Numbers of items and bounds where the workgroups and the shares change."""
+    gen = torch.Generator().manual_seed(B + most)
+    lengths = [3] * B
+    lengths[0], lengths[1], lengths[B - 1] = most, most - 1, 0
+    q, rows, caches, table = decode_case(gen, lengths, Hkv, Hkv, 16, 16, BF, most)
+    out = capi.attn_decode(q.to(DEV), *caches, table.to(DEV), int32(lengths), most, 0.25)
+    check_shares(out, q, rows, lengths, 0.25, BF, most, [0, 1, 2, B - 1])

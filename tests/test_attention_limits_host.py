@@ -51,3 +51,11 @@ def test_rows_of_a_prompts_workgroup(capi):
     assert rows(0, 24, 1, 16, 4, 64) == rows(1, 2000, 1, 32, 8, 128) == 64
     assert rows(0, 8192, 1, 64, 8, 128) == rows(1, 1 << 20, 65535, 1024, 1024, 256) == 128
     assert rows(0, 0, 1, 4, 2, 64) == rows(2, 9, 1, 4, 2, 64) == rows(0, 9, 1, 4, 3, 64) == rows(0, 9, -1, 4, 2, 64) == rows(0, 9, 1, 4, 2, 12) == 0
+
+
+def test_shares_of_few_items(capi):
+    """Between 128 and 256 items too few workgroups would run on an unsplit bound: their keys are shared by two."""
+    ws = capi.lib().fsw_attn_decode_workspace_bytes
+    for B in (15, 16, 20, 31):
+        assert ws(0, B, 64, 8, 128, 2300) > 0, B
+    assert ws(0, 32, 64, 8, 128, 2300) == ws(0, 64, 64, 8, 128, 2300) == ws(0, 16, 64, 8, 128, 512) == 0

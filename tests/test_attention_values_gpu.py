@@ -30,7 +30,9 @@ def put(cache, table, page, seq, key, channel, value):
     ([1300, 40, 700], None, 4, 2, 128, 16),        # shares that are joined
     ([1300, 40, 700], None, 2, 1, 256, 7),
     ([9000, 600], None, 2, 1, 64, 64),             # more than eight of them
-    ([70, 1, 130], None, 64, 64, 64, 16)])         # many items: four waves
+    ([70, 1, 130], None, 64, 64, 64, 16),
+    ([70, 1, 33, 130] * 3, None, 64, 64, 64, 16),  # many items: four waves
+    ([70, 1, 130], None, 200, 200, 128, 9)])
 @pytest.mark.parametrize("dtype", [BF, HF])
 def test_decode_infinities_that_are_seen(capi, lengths, max_len, Hq, Hkv, D, page, dtype):
     """What the weighted sum gives: the infinity, NaN where both signs or a NaN are seen; other channels and sequences as before."""
