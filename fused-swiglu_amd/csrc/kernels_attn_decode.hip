@@ -10,13 +10,15 @@
 // value rows that are read as they lie: 16 lanes with 8 consecutive channels each, four rows per lane, of which instruction j
 // takes the j-th channels, put side by side by two byte permutations. So neither P nor V crosses lanes, nothing goes through LDS before the end, and
 // the output is O^T: maximum, sum and rescaling of a head live in the lanes of its accumulators. P is not rounded to the element type but
-// split into two elements, whose products both are added (fp16, which has few exponents, takes them relative to the largest of 16 keys) (v_mfma_f32_16x16x4_f32 on fp32 values does the same at an eighth of the rate: 512 keys of
-// one sequence 12.5 against 10.6 us).
+// split into two elements, whose products both are added (v_mfma_f32_16x16x4_f32 on fp32 values does the same at an eighth of the rate: 512 keys of
+// one sequence 12.5 against 10.6 us). fp16, which has few exponents, takes them relative to the largest of 16 keys: 128 sequences of about 2000 keys 177.2 -> 179.0 us.
 // A wave takes 16 keys a turn, 8 KB, so 16 waves fit on a CU and keep 128 KB under way; tiles of 64 keys a wave, eight waves, were no faster on long
 // caches and slower on mixed ones (40 sequences of 1 .. 4096 keys: 153 against 113 us). A second set of registers for the next turn's keys and values costs
 // a quarter of the waves and gains nothing (112 against 100 us, 131071 keys). Loads are non-temporal, since every byte is read once: 100 -> 91 us. The page
 // number is looked up a turn ahead, and the first before the length is known. Measured: 131071 keys of 8 heads of 128 channels 86 us (6.2 TB/s) + 4.6 for the join;
-// 128 sequences of about 2000 keys 174 us (6.0 TB/s); HBM traffic is the keys and values once. A plain streaming read reaches 7.05 TB/s.
+// 128 sequences of about 2000 keys 174 us (6.0 TB/s); HBM traffic is the keys and values once. A plain streaming read reaches 7.05 TB/s. The same 128 sequences and 8
+// heads of 64 channels (half the bytes) 116 us (4.6 TB/s), of 96 154 (5.2); 64 sequences and 8 heads of 256 175 us (6.0). Pages of 9 or 24 tokens, which 16 keys do not fit, 188 and
+// 185 us where 16 and 64 take 181 and 184. 32 query heads on one, 128 sequences: 98 us (1.4 TB/s), since keys are walked once per 16 query heads and by too few workgroups.
 #include <float.h>
 
 #include <type_traits>

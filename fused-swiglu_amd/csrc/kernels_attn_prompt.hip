@@ -4,22 +4,27 @@
 // A workgroup owns 128 (or 64) rows of one sequence and key-value head. A row is a (token, query head of the group) pair: the group's
 // heads of a token are neighbouring rows, so they share the keys and values that the workgroup copies to LDS, short prompts fill their
 // tiles, and the triangle's edge cuts fewer tiles. Four waves own 32 (16) rows each and walk the same tiles of 64 keys, which come in by
-// LDS copies, two tiles of each kind in turn; workgroups with the longest walks start first, those of one key-value head on one XCD where
-// there are 8 heads.
+// LDS copies, two tiles of each kind in turn. Workgroups are dealt from the packed rows' end, so within a sequence the longest walks start first, and the
+// last sequence before the others: a long prompt behind short ones is met better than one before them (13 prompts of 32 heads on 8, twelve of 300 tokens and one
+// of 4000 at the end 153 us, at the start 169). Those of one key-value head are on one XCD where there are 8 heads.
 // The score tile is computed transposed, S^T = K Q^T (v_mfma_f32_16x16x32): lane l holds query row l % 16 and, of 16 keys, 4 (l / 16) + r in
 // register r, so a row's maximum and sum are in-lane ones and two lane swaps, and the registers of two blocks of 16 keys, rounded to the
 // element type, are the B operand of O^T = V^T P^T if its 32 keys are numbered {4 g .. 4 g + 3, 16 + 4 g .. 19 + 4 g} (g = l / 16). The A
 // operand has V's channels as rows and the same order of keys: two transposing reads of 4 keys x 16 channels (ds_read_b64_tr_b16) deliver
 // it from V as it lies. P never leaves its lanes.
 // The weights are rounded once, to the operand's type, as the matrix unit wants them; the sum is taken of the rounded ones (v_dot2), so the
-// normalisation is consistent: error against 64 bits 2.1e-3 on bf16 where one rounding of the output alone is 1.6e-3.
-// Bound: the matrix units, and the exponentials and moves that one instruction port per SIMD has to issue beside them. 8192 tokens of 64
-// heads of 128 on 8: 1017 .. 1100 us = 1.0 .. 1.08 PFLOP/s of what is under the diagonal, at the clock that the board's power leaves (about 1.9
-// GHz; a plain product of 8192 reaches 1.2); matrix units 48 % busy, no LDS bank conflicts. What that took: two waves a SIMD, by at most 256 registers
+// normalisation is consistent: error against 64 bits 2.1e-3 on bf16 where one rounding of the output alone is 1.6e-3, 2.2e-4 against 2.0e-4 on fp16.
+// Bound of long prompts: the matrix units, and the exponentials and moves that one instruction port per SIMD has to issue beside them. 8192 tokens of 64
+// heads of 128 on 8: 1000 .. 1060 us = 1.04 .. 1.10 PFLOP/s of what is under the diagonal, at the clock that the board's power leaves (2.1
+// GHz; a plain product of 8192 reaches 1.2); matrix units 48 % busy, vector instructions issue 54 % of the cycles, LDS 24 %, no bank conflicts.
+// Bound of middling ones: too little at once. 2000 tokens of 32 heads on 8, 49.6 us: matrix units and LDS 24 % busy each, vector instructions 33 %; a CU has work
+// 73 % of the time, and a SIMD 1.4 waves on average, each of which waits for its own chain of reads, products and exponentials.
+// Steps that were taken, each timed when it was (8192 tokens): two waves a SIMD, by at most 256 registers
 // instead of 276 (1582 -> 1150 us); 16 x 16 instead of 32 x 32 instructions, which move half the accumulators a flop (1127 -> 1104);
 // copies issued without a branch (1104 -> 1065). What did not pay: the scores of the next keys beside the weights of these (1172),
 // keys and values copied one and a half turns ahead with a barrier more (1162), wave priorities (1136), eight waves on every other tile of
-// the same rows (1243).
+// the same rows (1243). Limits in units of the scores come divided from the host: in the kernel they are vector registers, of which 256 channels have
+// none left (4000 tokens of fp16 234 us against 204).
 #include <float.h>
 
 #include "attn.h"
@@ -400,10 +405,10 @@ hipError_t launch(const PromptArgs& a, hipStream_t stream) {
 
 // 64 rows a workgroup (16 a wave) where workgroups of 128 (32 a wave) would (nearly) all be resident at once: half the rows are then not half the
 // rate, because no second round follows, and the longest workgroup's walk is what the launch takes. Above that 32 rows a wave
-// share each fragment that is read from LDS. 128 against 64 rows, us, 128 channels: 1000 tokens of 32 heads on 8 (252 workgroups of 128
-// rows) 27.4 | 22.2, 2000 (504) 56.2 | 53.5, 13 prompts of 1 .. 777 tokens and 40 heads (about 540) 25.3 | 22.4, 3000 tokens (752) 92 | 110, 8192 of 64
-// heads 1080 | 1425; 64 channels: 2000 tokens of 16
-// heads on 4 (252) 33.6 | 25.5, 6000 (752) 115 | 107; 256 channels: 1000 tokens of 16 heads on 8 (128) 49 | 34, 4000 (500) 199 | 250.
+// share each fragment that is read from LDS. us of 64 rows | 128 rows, by the estimated number of workgroups of 128 rows. 128 channels, 576 is the switch: 248 23.4 |
+// 29.1, 400 36.8 | 44.1, 496 50.0 | 52.0, 544 57.7 | 56.5, 600 66.8 | 62.3, 672 83 | 70, 744 98 | 82, 1000 161 | 142; 13 prompts of 1 .. 777 tokens (520) 22 | 33;
+// prompts of 500 tokens, 4 (512) 24.9 | 25.6, 6 (768) 34.0 | 33.4, 8 (1032) 42.6 | 39.3. 64 channels, 864: 248 26.6 | 35.6, 500 54 | 68, 748 107 | 105, 848 130 | 129, 936
+// 151 | 150, 1124 213 | 201. 256 channels, 288: 120 34 | 51, 200 50 | 79, 280 94 | 110, 320 117 | 121, 368 147 | 140, 496 232 | 201.
 int rows_of(int tq, int seqs, int hq, int hkv, int d) {
   const int resident = 256 * (d <= 64 ? 3 : d <= 128 ? 2 : 1);  // workgroups of 128 rows, by LDS and registers
   const long long rows = (long long)tq * (hq / hkv);

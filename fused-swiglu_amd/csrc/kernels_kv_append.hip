@@ -8,8 +8,9 @@
 // tokens are few. A thread owns one 16-byte vector of one head (interleaved), or the two that are each other's partners (halves). Four
 // heads a thread, which read the cosines and sines once, were as fast for many tokens (8192 tokens, 32 + 16 heads: 40.8 against 39.0 us) and slower for
 // few (one token: 4.8 against 3.0 us). Inputs are read once, so the loads are non-temporal: with four heads a thread 8192 tokens of 64 +
-// 16 heads of 128 channels went from 75 to 67 us by it. Stores are not (69 us): what is stored is read next. Now 60.7 us, 5.9 TB/s
-// (a copy of 2 GiB moves 4.9 TB/s).
+// 16 heads of 128 channels went from 75 to 67 us by it. Stores are not (69 us): what is stored is read next. Now 60.8 us, 5.9 TB/s
+// (a copy of 2 GiB moves 4.9 TB/s). 8192 tokens, 32 + 8 heads: 40.3 us at 128 channels (5.5 TB/s), 36.9 at 80 (3.8), half of 128 turned 52.7, half of 96 44.7. Where `rot` allows no
+// vectors (no multiple of 16, interleaved 8), everything goes by single elements, at a quarter of the rate: half of 80 channels 87 us, half of 112 142.
 #include "attn.h"
 #include "fsw_device.h"
 #include "fsw_internal.h"
