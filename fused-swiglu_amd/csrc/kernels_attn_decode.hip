@@ -50,33 +50,9 @@ template <>
 __device__ __forceinline__ f32x4 mfma_k16<Fp16>(u32x2 a, u32x2 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x16f16(__builtin_bit_cast(f16x4, a), __builtin_bit_cast(f16x4, b), c, 0, 0, 0);
 }
-template <class T>
-__device__ __forceinline__ void unpack2(unsigned u, float& lo, float& hi);
-template <>
-__device__ __forceinline__ void unpack2<Bf16>(unsigned u, float& lo, float& hi) {
-  lo = __builtin_bit_cast(float, u << 16);
-  hi = __builtin_bit_cast(float, u & 0xffff0000u);
-}
-template <>
-__device__ __forceinline__ void unpack2<Fp16>(unsigned u, float& lo, float& hi) {
-  const f16x2 v = __builtin_bit_cast(f16x2, u);
-  lo = (float)v[0];
-  hi = (float)v[1];
-}
 // the low (high) halves of a and b side by side
 __device__ __forceinline__ unsigned lows(unsigned a, unsigned b) { return __builtin_amdgcn_perm(b, a, 0x05040100u); }
 __device__ __forceinline__ unsigned highs(unsigned a, unsigned b) { return __builtin_amdgcn_perm(b, a, 0x07060302u); }
-
-__device__ __forceinline__ float sum_over_groups(float x) {
-  x += __shfl_xor(x, 16);
-  return x + __shfl_xor(x, 32);
-}
-
-// 2^(a - b) for a <= b, with -inf - -inf = 0 (nothing seen yet). Never zero, so that an infinity that has been summed up stays one; what
-// that adds to other sums is below 2^-126 of the values, in units in which all weights are 2^-38 at least.
-__device__ __forceinline__ float scale_of(float a, float b) {
-  return a == b ? 1.0f : fmaxf(__builtin_amdgcn_exp2f(a - b), FLT_MIN);
-}
 
 #define INLINE __attribute__((always_inline))
 
@@ -324,7 +300,7 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 2 : 4) void attn_decode_ker
     }
   }
   __syncthreads();
-  const bool parted = len > chunk && !bad_len;
+  const bool parted = a.before > 0 || (len > chunk && !bad_len);
   for (int t = threadIdx.x; t < here * WIDE; t += 64 * WAVES) {
     const int h = t / WIDE, ch = (t % WIDE) * 4;
     if (ch >= a.d) continue;
@@ -337,10 +313,11 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 2 : 4) void attn_decode_ker
 #pragma unroll
     for (int w = 0; w < WAVES; ++w) x += *(const f32x4*)(shares + (w * here + h) * ROW + ch);
     if (parted) {  // unnormalised sums, maximum and sum of this share: attn_join_kernel
-      const long long row = ((long long)seq * a.hq + head0 + h) * splits + split;
+      const int slots = a.before + splits;
+      const long long row = ((long long)seq * a.hq + head0 + h) * slots + a.before + split;
       *(f32x4*)(partial + row * a.d + ch) = x;
       if (ch == 0) {
-        float* ml = partial + (long long)a.seqs * a.hq * splits * a.d + row * 2;
+        float* ml = partial + (long long)a.seqs * a.hq * slots * a.d + row * 2;
         ml[0] = most;
         ml[1] = total;
       }
@@ -352,19 +329,21 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 2 : 4) void attn_decode_ker
   }
 }
 
-// The shares of one query head's keys, joined where there is more than one: weights 2^(m_i - m), one normalisation, one
+// The shares of one query head's keys, joined where there is more than one (those of a prefix, all of them, come first): weights 2^(m_i - m), one normalisation, one
 // rounding. TH threads per head: d / 4 of them stand side by side on a share's channels, TH / (d / 4) shares at a time, and
 // every thread keeps a running maximum of its own, so that all loads are one trip to memory.
 template <class T, int TH>
-__global__ __launch_bounds__(256) void attn_join_kernel(PagedAttnArgs a, int chunk, int splits, const float* partial) {
+__global__ __launch_bounds__(256) void attn_join_kernel(JoinArgs a, int chunk, int splits, const float* partial) {
   const int seq = blockIdx.y, lane = threadIdx.x % TH, first = threadIdx.x - lane;
   const int head = (int)blockIdx.x * (256 / TH) + (int)threadIdx.x / TH;
   const int width = a.d / 4, rows = TH / width, part = lane / width, at = lane % width;
   const int len = a.lengths[seq];
-  if (len <= chunk || len > a.max_len) return;
-  const int used = (len + chunk - 1) / chunk;  // <= splits: len <= max_len
-  const long long row = ((long long)seq * a.hq + head) * splits;
-  const float* ml = partial + (long long)a.seqs * a.hq * splits * a.d + row * 2;
+  const bool parted = len > chunk && len <= a.max_len;
+  if (!parted && a.before == 0) return;
+  const int used = a.before + (parted ? (len + chunk - 1) / chunk : 1);  // <= slots: len <= max_len
+  const int slots = a.before + splits;
+  const long long row = ((long long)seq * a.hq + head) * slots;
+  const float* ml = partial + (long long)a.seqs * a.hq * slots * a.d + row * 2;
   const float* po = partial + row * a.d + 4 * at;
 
   f32x4 o = {0, 0, 0, 0};
@@ -425,7 +404,16 @@ hipError_t launch_waves(const PagedAttnArgs& a, const PagedAttnPlan& p, float* p
   const dim3 grid(a.hkv * tiles, a.seqs, p.splits);
   const size_t lds = (size_t)WAVES * (group < 16 ? group : 16) * (DP + 4) * sizeof(float);
   const auto kernel = a.cache.page_size % 16 == 0 ? attn_decode_kernel<T, DP, true, WAVES> : attn_decode_kernel<T, DP, false, WAVES>;
-  kernel<<<grid, 64 * WAVES, lds, stream>>>(a, lift_of<T>(a.max_len), p.chunk, group, tiles, partial);
+  kernel<<<grid, 64 * WAVES, lds, stream>>>(a, lift_of<T>(a.keys), p.chunk, group, tiles, partial);
+  return hipGetLastError();
+}
+
+template <class T>
+hipError_t launch_join(const JoinArgs& a, int chunk, int splits, const float* partial, hipStream_t stream) {
+  if (a.before + splits > 8)
+    attn_join_kernel<T, 256><<<dim3(a.hq, a.seqs), 256, 0, stream>>>(a, chunk, splits, partial);
+  else
+    attn_join_kernel<T, 64><<<dim3((a.hq + 3) / 4, a.seqs), 256, 0, stream>>>(a, chunk, splits, partial);
   return hipGetLastError();
 }
 
@@ -436,12 +424,8 @@ template <class T, int DP>
 hipError_t launch_dp(const PagedAttnArgs& a, const PagedAttnPlan& p, float* partial, hipStream_t stream) {
   const hipError_t e = p.waves == 4 ? launch_waves<T, DP, 4>(a, p, partial, stream)
                                     : launch_waves<T, DP, MANY_WAVES<DP>>(a, p, partial, stream);
-  if (e != hipSuccess || p.splits == 1) return e;
-  if (p.splits > 8)
-    attn_join_kernel<T, 256><<<dim3(a.hq, a.seqs), 256, 0, stream>>>(a, p.chunk, p.splits, partial);
-  else
-    attn_join_kernel<T, 64><<<dim3((a.hq + 3) / 4, a.seqs), 256, 0, stream>>>(a, p.chunk, p.splits, partial);
-  return hipGetLastError();
+  if (e != hipSuccess || p.splits == 1 || a.before > 0) return e;  // who has a prefix joins all shares
+  return launch_join<T>(JoinArgs{a.seqs, a.hq, a.d, a.lengths, a.max_len, 0, a.o}, p.chunk, p.splits, partial, stream);
 }
 
 template <class T>
@@ -468,13 +452,13 @@ hipError_t launch_typed(const PagedAttnArgs& a, const PagedAttnPlan& p, float* p
 // 200 | 224, 2200 .. 3000 234 | 258, 3000 .. 4096 319 | 351. Which of them a batch is cannot be told here: 2560 is where the uneven one's gain begins to outgrow the even one's
 // loss. The farther the bound, the more shares, up to 8192 of all items together (32 x 8 items of 1 .. 32768 keys: 225 us in 8 shares, 150 in
 // 27): most of the short sequences' are empty and end at once. From 8192 items on the card's dynamic assignment levels them.
-PagedAttnPlan paged_attn_plan(int seqs, int hq, int hkv, int d, int max_len) {
+PagedAttnPlan paged_attn_plan(int seqs, int hq, int hkv, int d, int max_len, int turn) {
   const long long items = (long long)seqs * hkv * head_tiles(hq, hkv);
   PagedAttnPlan p;
   const bool whole = max_len <= 2560;  // not split where items are many
   const bool few = items < 128 || (whole && (items <= 256 ? max_len > 64 : items <= 512 && max_len > 512));
   p.waves = few ? (d > 128 ? 8 : 16) : 4;
-  const long long unit = 16 * p.waves;  // keys of a workgroup's turn
+  const long long unit = turn * p.waves;  // keys of a workgroup's turn
   long long wanted = 1;
   if (few)
     wanted = items > 0 ? (4096 / p.waves + items - 1) / items : 1;
@@ -488,8 +472,12 @@ PagedAttnPlan paged_attn_plan(int seqs, int hq, int hkv, int d, int max_len) {
   p.chunk = (int)(chunk < unit ? unit : chunk);
   p.splits = (int)((max_len + p.chunk - 1) / p.chunk);
   if (p.splits < 1) p.splits = 1;
-  p.workspace_bytes = p.splits > 1 ? (size_t)seqs * hq * p.splits * (size_t)(d + 2) * 4 : 0;
+  p.workspace_bytes = p.splits > 1 ? partial_bytes((long long)seqs * hq * p.splits, d) : 0;
   return p;
+}
+
+hipError_t launch_attn_join(int dtype, const JoinArgs& a, int chunk, int splits, const float* partial, hipStream_t stream) {
+  return dtype == FSW_BF16 ? launch_join<Bf16>(a, chunk, splits, partial, stream) : launch_join<Fp16>(a, chunk, splits, partial, stream);
 }
 
 hipError_t launch_attn_decode(int dtype, const PagedAttnArgs& a, const PagedAttnPlan& p, void* workspace, hipStream_t stream) {

@@ -1,0 +1,360 @@
+// Attention of one new token per sequence over a paged cache of e4m3 elements c and one power of two s per key and value row:
+//   o = sum_j p_j s'_j c'_j / sum_j p_j,  p_j = 2^(c s_j (q.c_j) - m),  c = scale log2(e),  j < length,
+// in one pass over the keys with a running maximum m and running sums (fp32).
+//
+// Memory bounds it, as it does the decode over 16-bit elements, whose arrangement this has (query heads are columns, keys rows, nothing crosses lanes or
+// goes through LDS before the end); the bytes of a key are half as many, so a wave takes 32 keys a turn, two blocks of 16. A key's channels are summed in any
+// order: a lane reads 16 elements side by side, which are two steps of the matrix instruction, with the queries' channels laid out alike. Scores
+// come out with head l % 16 and keys 4 (l / 16) + r of either block in lane l, which is what the B operand of the second product
+// wants if its 32 keys are numbered {4 g .. 4 g + 3, 16 + 4 g .. 19 + 4 g} (g = l / 16); its A operand's rows are value rows as they lie, DP / 16
+// channels a lane, whose elements of four keys are put side by side by four byte permutations for four channels.
+// Elements become 16-bit ones by v_cvt_scalef32_pk, two at a time, without loss in either type. Scales never meet them: a key's multiplies its score, a
+// value's its weight, both in fp32. The second product is bf16 for both types, since a weight times a power of two wants fp32's exponents; the weight is
+// split into two elements, 16 bits, whose products both are added.
+#include "attn.h"
+#include "attn_device.h"
+#include "fsw_device.h"
+#include "fsw_internal.h"
+
+namespace fsw {
+namespace {
+
+constexpr float NEG_INF = -__builtin_inff();
+constexpr float SLACK = 8.0f;  // a head's m moves when a score passes m - lift by it, and is that score plus the lift then
+constexpr int TURN = 32;       // keys of a wave at a time
+
+#define INLINE __attribute__((always_inline))
+
+// two elements as 16-bit ones
+template <class T, bool HIGH>
+__device__ __forceinline__ unsigned widen(unsigned x);
+template <>
+__device__ __forceinline__ unsigned widen<Bf16, false>(unsigned x) {
+  return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, false));
+}
+template <>
+__device__ __forceinline__ unsigned widen<Bf16, true>(unsigned x) {
+  return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, true));
+}
+template <>
+__device__ __forceinline__ unsigned widen<Fp16, false>(unsigned x) {
+  return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, false));
+}
+template <>
+__device__ __forceinline__ unsigned widen<Fp16, true>(unsigned x) {
+  return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, true));
+}
+
+// bits of the scale in byte r of four, as a float's; 255 gives an infinity, which the kernel looks for
+__device__ __forceinline__ unsigned scale_bits(unsigned four, int r) {
+  const unsigned b = (r < 3 ? four << (23 - 8 * r) : four >> 1) & 0x7f800000u;
+  return b > 0x00400000u ? b : 0x00400000u;
+}
+constexpr unsigned NO_NUMBER = 0x7f800000u;
+
+// DP: channels, padded to 64, 128 or 256; a row of values is VB elements on each of 16 lanes.
+// WHOLE: 16 keys in a row lie in one page, their scales in four aligned words.
+template <class T, int DP, bool WHOLE, int WAVES>
+__global__ __launch_bounds__(64 * WAVES, DP == 256 ? 2 : 4) void attn_decode8_kernel(PagedAttn8Args a, float lift, int chunk, int group, int head_tiles,
+                                                                                     float* partial) {
+  constexpr int VB = DP / 16, VW = VB / 4, KV = DP / 64;  // KV: vectors of a key
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, grp = lane >> 4;
+  const int split = blockIdx.z, splits = gridDim.z, seq = blockIdx.y;
+  int kvh = blockIdx.x, first = 0;
+  if (head_tiles > 1) {
+    kvh = (int)blockIdx.x / head_tiles;
+    first = ((int)blockIdx.x - kvh * head_tiles) * 16;
+  }
+  const int here = group - first < 16 ? group - first : 16;  // query heads of this workgroup
+  const int head0 = kvh * group + first, head = head0 + col;  // this lane's
+  const bool real = col < here;
+  const int begin = split * chunk;
+
+  const unsigned char* kc = a.cache.k + kvh * a.cache.head;
+  const unsigned char* vc = a.cache.v + kvh * a.cache.head;
+  const unsigned char* ksc = a.cache.k_scale + kvh * a.cache.scale_head;
+  const unsigned char* vsc = a.cache.v_scale + kvh * a.cache.scale_head;
+  const int* table = a.block_table + (long long)seq * a.table_ld;
+  // page and place of this lane's keys of the turn that begins at `at`; below max_len, whatever the length is. A second block that begins
+  // at max_len or behind it stands for the first once more: of its keys, none counts.
+  int page[2], place[2];
+  auto locate = [&](int at) INLINE {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      int key = (h == 1 && at + 16 >= a.max_len ? at : at + 16 * h) + col;
+      key = key < a.max_len ? key : a.max_len - 1;
+      const int idx = a.cache.per_page.quotient(key);
+      page[h] = table[idx];
+      place[h] = key - idx * a.cache.page_size;
+    }
+  };
+  int at = begin + wave * TURN;
+  if (at < a.max_len) locate(at);  // before the length is known
+
+  u32x4 qf[2 * KV];
+  const unsigned short* qp = (const unsigned short*)a.q.p + (long long)seq * a.q.token + (long long)head * a.q.head;
+#pragma unroll
+  for (int s = 0; s < 2 * KV; ++s) {
+    const int ch = (s / 2) * 64 + grp * 16 + (s % 2) * 8;
+    qf[s] = u32x4{0, 0, 0, 0};
+    if (real && ch < a.d) qf[s] = *(const u32x4*)(qp + ch);
+  }
+  const int len = a.lengths[seq];
+  const bool bad_len = len < 0 || len > a.max_len;
+  const int end = bad_len ? 0 : (len - begin < chunk ? len : begin + chunk);
+  if (split > 0 && begin >= end) return;
+
+  f32x4 acc[VB];
+#pragma unroll
+  for (int i = 0; i < VB; ++i) acc[i] = f32x4{0, 0, 0, 0};
+  float m = NEG_INF, sum = 0.0f;
+  bool bad_page = false;
+  unsigned worst = 0;  // largest scale
+
+  for (; at < end; at += TURN * WAVES) {
+    const bool part = at + TURN > end;
+    u32x4 kf[2][KV];
+    unsigned vf[2][4][VW], ks[2], vs[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      // a page outside the cache is an error where a key lies in it, and read as page 0
+      const bool inside = (unsigned)page[h] < (unsigned)a.cache.pages;
+      bad_page |= !inside && at + 16 * h + col < end;
+      const long long where = (inside ? page[h] : 0) * a.cache.page + place[h] * a.cache.token;
+      const long long mark = (inside ? page[h] : 0) * a.cache.scale_page + place[h] * a.cache.scale_token;
+#pragma unroll
+      for (int s = 0; s < KV; ++s) {
+        const int ch = s * 64 + grp * 16;
+        kf[h][s] = u32x4{0, 0, 0, 0};
+        if (ch < a.d) kf[h][s] = __builtin_nontemporal_load((const u32x4*)(kc + where + ch));
+      }
+      auto uniform = [](long long x) INLINE -> long long {
+        const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)x);
+        const unsigned hi = __builtin_amdgcn_readfirstlane((unsigned)((unsigned long long)x >> 32));
+        return (long long)(((unsigned long long)hi << 32) | lo);
+      };
+      const unsigned char* tile = vc;
+      if constexpr (WHOLE) {
+        tile += uniform(where);
+        const long long marks = uniform(mark) + 4 * grp;  // the page has room for all 16, keys or not
+        ks[h] = *(const unsigned*)(ksc + marks);
+        vs[h] = *(const unsigned*)(vsc + marks);
+      } else {
+        const int both = ksc[mark] | vsc[mark] << 8;
+        ks[h] = vs[h] = 0;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const unsigned x = (unsigned)__shfl(both, 4 * grp + r);
+          ks[h] |= (x & 255u) << (8 * r);
+          vs[h] |= (x >> 8) << (8 * r);
+        }
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const int k = 4 * grp + r;
+        const unsigned char* p;
+        if constexpr (WHOLE) {
+          p = tile + k * (int)a.cache.token;
+        } else {
+          p = vc + __shfl(where, k);
+        }
+#pragma unroll
+        for (int w = 0; w < VW; ++w) vf[h][r][w] = 0;
+        if (col * VB < a.d) {
+          if constexpr (VW == 4) {
+            const u32x4 x = __builtin_nontemporal_load((const u32x4*)(p + col * VB));
+#pragma unroll
+            for (int w = 0; w < VW; ++w) vf[h][r][w] = x[w];
+          } else if constexpr (VW == 2) {
+            const u32x2 x = __builtin_nontemporal_load((const u32x2*)(p + col * VB));
+            vf[h][r][0] = x[0], vf[h][r][1] = x[1];
+          } else {
+            vf[h][r][0] = __builtin_nontemporal_load((const unsigned*)(p + col * VB));
+          }
+        }
+      }
+    }
+    if (part) {  // what lies behind the end weighs nothing, whatever it holds
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int left = end - at - 16 * h - 4 * grp;  // keys of this lane
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          if (r < left) continue;
+          ks[h] = (ks[h] & ~(255u << 8 * r)) | 127u << 8 * r;
+          vs[h] = (vs[h] & ~(255u << 8 * r)) | 127u << 8 * r;
+#pragma unroll
+          for (int w = 0; w < VW; ++w) vf[h][r][w] = 0;
+        }
+      }
+    }
+    if (at + TURN * WAVES < end) locate(at + TURN * WAVES);
+
+    f32x4 s[2];
+    float top = NEG_INF;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      s[h] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < 2 * KV; ++i) {
+        const unsigned lo = kf[h][i / 2][i % 2 * 2], hi = kf[h][i / 2][i % 2 * 2 + 1];
+        s[h] = T::mfma16(u32x4{widen<T, false>(lo), widen<T, true>(lo), widen<T, false>(hi), widen<T, true>(hi)}, qf[i], s[h]);
+      }
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const unsigned bits = scale_bits(ks[h], r);
+        worst = worst > bits ? worst : bits;
+        s[h][r] *= __builtin_bit_cast(float, bits) * a.scale_log2;
+        if (part && at + 16 * h + 4 * grp + r >= end) s[h][r] = NEG_INF;
+        top = fmaxf(top, s[h][r]);
+      }
+    }
+    top = max_over_groups(top);
+    if (__any(top > m + (SLACK - lift))) {
+      const float now = fmaxf(m, top + lift), alpha = scale_of(m, now);
+      m = now;
+      sum *= alpha;
+#pragma unroll
+      for (int i = 0; i < VB; ++i)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) acc[i][r] *= alpha;
+    }
+    const float base = m == NEG_INF ? 0.0f : m;
+    u32x4 p1, p2;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float w[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) {
+        const float p = __builtin_amdgcn_exp2f(s[h][r] - base);
+        sum += p;
+        const unsigned bits = scale_bits(vs[h], r);
+        worst = worst > bits ? worst : bits;
+        w[r] = p * __builtin_bit_cast(float, bits);
+      }
+#pragma unroll
+      for (int r = 0; r < 4; r += 2) {
+        float lo, hi;
+        p1[2 * h + r / 2] = Bf16::pack2(w[r], w[r + 1]);
+        unpack2<Bf16>(p1[2 * h + r / 2], lo, hi);
+        p2[2 * h + r / 2] = Bf16::pack2(w[r] - lo, w[r + 1] - hi);
+      }
+    }
+#pragma unroll
+    for (int w = 0; w < VW; ++w) {
+      unsigned pair[2][2][2];  // [block][keys 0 and 1, 2 and 3][channels 0 and 1, 2 and 3]
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          pair[h][k][0] = __builtin_amdgcn_perm(vf[h][2 * k + 1][w], vf[h][2 * k][w], 0x05010400u);
+          pair[h][k][1] = __builtin_amdgcn_perm(vf[h][2 * k + 1][w], vf[h][2 * k][w], 0x07030602u);
+        }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        u32x4 v;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+            v[2 * h + k] = c % 2 == 0 ? widen<Bf16, false>(pair[h][k][c / 2]) : widen<Bf16, true>(pair[h][k][c / 2]);
+        acc[4 * w + c] = Bf16::mfma16(v, p1, acc[4 * w + c]);
+        acc[4 * w + c] = Bf16::mfma16(v, p2, acc[4 * w + c]);
+      }
+    }
+  }
+  if (__any(bad_page || worst == NO_NUMBER) || bad_len) sum = __builtin_nanf("");
+  sum = sum_over_groups(sum);
+
+  // The waves' shares of the keys, joined through LDS: rows of the real heads, each wave's scaled to the largest maximum. Four
+  // channels of padding spread the rows of 16 heads over the banks.
+  constexpr int ROW = DP + 4, WIDE = DP / 4;
+  extern __shared__ __align__(16) float shares[];  // [WAVES][here][ROW]
+  __shared__ float stats[WAVES][2][16];
+  if (grp == 0) {
+    stats[wave][0][col] = m;
+    stats[wave][1][col] = sum;
+  }
+  __syncthreads();
+  float top = NEG_INF;
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) top = fmaxf(top, stats[w][0][col]);
+  if (real) {
+    const float mine = scale_of(m, top);
+    float* row = shares + (wave * here + col) * ROW;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+      for (int j = 0; j < VB; j += 4) {
+        f32x4 x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = acc[j + i][r] * mine;
+        *(f32x4*)(row + (4 * grp + r) * VB + j) = x;
+      }
+  }
+  __syncthreads();
+  const bool parted = a.before > 0 || (len > chunk && !bad_len);
+  for (int t = threadIdx.x; t < here * WIDE; t += 64 * WAVES) {
+    const int h = t / WIDE, ch = (t % WIDE) * 4;
+    if (ch >= a.d) continue;
+    float most = NEG_INF, total = 0.0f;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) most = fmaxf(most, stats[w][0][h]);
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) total += stats[w][1][h] * scale_of(stats[w][0][h], most);
+    f32x4 x = {0, 0, 0, 0};
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) x += *(const f32x4*)(shares + (w * here + h) * ROW + ch);
+    if (parted) {  // unnormalised sums, maximum and sum of this share, to be joined
+      const int slots = a.before + splits;
+      const long long row = ((long long)seq * a.hq + head0 + h) * slots + a.before + split;
+      *(f32x4*)(partial + row * a.d + ch) = x;
+      if (ch == 0) {
+        float* ml = partial + (long long)a.seqs * a.hq * slots * a.d + row * 2;
+        ml[0] = most;
+        ml[1] = total;
+      }
+    } else {
+      const float inv = len == 0 ? 0.0f : 1.0f / total;
+      unsigned short* op = (unsigned short*)a.o.p + (long long)seq * a.o.token + (long long)(head0 + h) * a.o.head;
+      *(u32x2*)(op + ch) = u32x2{T::pack2(x[0] * inv, x[1] * inv), T::pack2(x[2] * inv, x[3] * inv)};
+    }
+  }
+}
+
+template <class T, int DP, int WAVES>
+hipError_t launch_waves(const PagedAttn8Args& a, const PagedAttnPlan& p, float* partial, hipStream_t stream) {
+  const int group = a.hq / a.hkv, tiles = (group + 15) / 16;
+  const dim3 grid(a.hkv * tiles, a.seqs, p.splits);
+  const size_t lds = (size_t)WAVES * (group < 16 ? group : 16) * (DP + 4) * sizeof(float);
+  const PagedKv8& c = a.cache;
+  const bool whole = c.page_size % 16 == 0 && c.scale_token == 1 && (c.scale_page | c.scale_head) % 4 == 0 &&
+                     (((uintptr_t)c.k_scale | (uintptr_t)c.v_scale) & 3) == 0;
+  const auto kernel = whole ? attn_decode8_kernel<T, DP, true, WAVES> : attn_decode8_kernel<T, DP, false, WAVES>;
+  // the weights of all keys together stay below 1, so that no sum of finite values overflows before it is normalised
+  kernel<<<grid, 64 * WAVES, lds, stream>>>(a, SLACK + ceil_log2(a.keys), p.chunk, group, tiles, partial);
+  return hipGetLastError();
+}
+
+template <class T, int DP>
+hipError_t launch_dp(const PagedAttn8Args& a, const PagedAttnPlan& p, float* partial, hipStream_t stream) {
+  return p.waves == 4 ? launch_waves<T, DP, 4>(a, p, partial, stream) : launch_waves<T, DP, DP == 256 ? 8 : 16>(a, p, partial, stream);
+}
+
+template <class T>
+hipError_t launch_typed(const PagedAttn8Args& a, const PagedAttnPlan& p, float* partial, hipStream_t stream) {
+  if (a.d <= 64) return launch_dp<T, 64>(a, p, partial, stream);
+  if (a.d <= 128) return launch_dp<T, 128>(a, p, partial, stream);
+  return launch_dp<T, 256>(a, p, partial, stream);
+}
+
+}  // namespace
+
+hipError_t launch_attn_decode8(int dtype, const PagedAttn8Args& a, const PagedAttnPlan& p, void* workspace, hipStream_t stream) {
+  float* partial = (float*)workspace;
+  const hipError_t e = dtype == FSW_BF16 ? launch_typed<Bf16>(a, p, partial, stream) : launch_typed<Fp16>(a, p, partial, stream);
+  if (e != hipSuccess || p.splits == 1 || a.before > 0) return e;  // who has a prefix joins all shares
+  return launch_attn_join(dtype, JoinArgs{a.seqs, a.hq, a.d, a.lengths, a.max_len, 0, a.o}, p.chunk, p.splits, partial, stream);
+}
+
+}  // namespace fsw

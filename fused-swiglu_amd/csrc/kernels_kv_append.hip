@@ -12,22 +12,13 @@
 // (a copy of 2 GiB moves 4.9 TB/s). 8192 tokens, 32 + 8 heads: 40.3 us at 128 channels (5.5 TB/s), 36.9 at 80 (3.8), half of 128 turned 52.7, half of 96 44.7. Where `rot` allows no
 // vectors (no multiple of 16, interleaved 8), everything goes by single elements, at a quarter of the rate: half of 80 channels 87 us, half of 112 142.
 #include "attn.h"
+#include "attn_device.h"
 #include "fsw_device.h"
 #include "fsw_internal.h"
 
 namespace fsw {
 namespace {
 
-template <class T>
-__device__ __forceinline__ float elem(unsigned short x);
-template <>
-__device__ __forceinline__ float elem<Bf16>(unsigned short x) {
-  return __builtin_bit_cast(float, (unsigned)x << 16);
-}
-template <>
-__device__ __forceinline__ float elem<Fp16>(unsigned short x) {
-  return (float)__builtin_bit_cast(_Float16, x);
-}
 template <class T>
 __device__ __forceinline__ void unpack8(u32x4 v, float (&f)[8]) {
 #pragma unroll

@@ -190,7 +190,9 @@ void meta_swiglu_fwd_bf16(int64_t, int64_t, int64_t, Tensor const&, int64_t, Ten
 
 }  // namespace
 
-void bind_attention(pybind11::module_& m);  // attn_bindings.cpp
+void bind_attention(pybind11::module_& m);   // attn_bindings.cpp
+void bind_attention8(pybind11::module_& m);  // attn8_bindings.cpp
+void bind_norms(pybind11::module_& m);       // norm_bindings.cpp
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("fused_swiglu_bf16", &fused_swiglu_bf16, "fused SwiGLU for bf16");
@@ -206,6 +208,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     return std::string(fsw_variant_name(family, FSW_BF16, M, n, k));
   }, "kernel variant the dispatcher picks (family 0 = gate/up, 1 = down)");
   bind_attention(m);
+  bind_attention8(m);
+  bind_norms(m);
 }
 
 TORCH_LIBRARY(ASMLLM, m) {

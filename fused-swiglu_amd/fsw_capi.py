@@ -25,7 +25,16 @@ class KvCache(ctypes.Structure):
                 ("token_stride", _i64)]
 
 
+class KvCache8(ctypes.Structure):
+    """fsw_kv_cache8 of include/fsw.h."""
+    _fields_ = [("k", _vp), ("v", _vp), ("k_scale", _vp), ("v_scale", _vp), ("pages", _i64), ("page_size", _i64), ("page_stride", _i64),
+                ("head_stride", _i64), ("token_stride", _i64), ("scale_page_stride", _i64), ("scale_head_stride", _i64),
+                ("scale_token_stride", _i64)]
+
+
 _kvp = ctypes.POINTER(KvCache)
+_kvp8 = ctypes.POINTER(KvCache8)
+_f = ctypes.c_float
 PROTOTYPES = {
     "fsw_validate_gateup": (_i, [_i, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64]),
     "fsw_gateup": (_i, [_i, _i64, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i64, _vp]),
@@ -54,6 +63,23 @@ PROTOTYPES = {
     "fsw_validate_attn_prompt": (_i, [_i] + [_i64] * 6 + _rows * 3 + [_vp, _vp, ctypes.c_float] + _rows),
     "fsw_attn_prompt_rows": (_i, [_i] + [_i64] * 5),
     "fsw_attn_prompt": (_i, [_i] + [_i64] * 6 + _rows * 3 + [_vp, _vp, ctypes.c_float] + _rows + [_vp]),
+    "fsw_validate_kv_append8": (_i, [_i] + [_i64] * 5 + _rows * 3 + [_vp, _i64, _vp, _vp] + _rows * 3 + [_kvp8]),
+    "fsw_kv_append8": (_i, [_i] + [_i64] * 5 + [_i] + _rows * 3 + [_vp, _i64, _vp, _vp] + _rows * 3 + [_kvp8, _vp]),
+    "fsw_validate_kv_read": (_i, [_i] + [_i64] * 4 + [_kvp, _vp, _i64, _i64, _vp] + _rows * 2),
+    "fsw_validate_kv_read8": (_i, [_i] + [_i64] * 4 + [_kvp8, _vp, _i64, _i64, _vp] + _rows * 2),
+    "fsw_kv_read": (_i, [_i] + [_i64] * 4 + [_kvp, _vp, _i64, _i64, _vp] + _rows * 2 + [_vp]),
+    "fsw_kv_read8": (_i, [_i] + [_i64] * 4 + [_kvp8, _vp, _i64, _i64, _vp] + _rows * 2 + [_vp]),
+    "fsw_validate_attn_decode8": (_i, [_i] + [_i64] * 4 + _rows + [_kvp8, _vp, _i64, _vp, _i64, _f] + _rows),
+    "fsw_attn_decode8_workspace_bytes": (_sz, [_i] + [_i64] * 5),
+    "fsw_attn_decode8": (_i, [_i] + [_i64] * 4 + _rows + [_kvp8, _vp, _i64, _vp, _i64, _f] + _rows + [_vp, _sz, _vp]),
+    "fsw_validate_attn_shared": (_i, [_i] + [_i64] * 4 + _rows + [_kvp, _vp, _i64, _vp, _i64, _vp, _i64, _f] + _rows),
+    "fsw_validate_attn_shared8": (_i, [_i] + [_i64] * 4 + _rows + [_kvp8, _vp, _i64, _vp, _i64, _vp, _i64, _f] + _rows),
+    "fsw_attn_shared_workspace_bytes": (_sz, [_i] + [_i64] * 6),
+    "fsw_attn_shared8_workspace_bytes": (_sz, [_i] + [_i64] * 6),
+    "fsw_attn_shared": (_i, [_i] + [_i64] * 4 + _rows + [_kvp, _vp, _i64, _vp, _i64, _vp, _i64, _f] + _rows + [_vp, _sz, _vp]),
+    "fsw_attn_shared8": (_i, [_i] + [_i64] * 4 + _rows + [_kvp8, _vp, _i64, _vp, _i64, _vp, _i64, _f] + _rows + [_vp, _sz, _vp]),
+    "fsw_validate_add_norm": (_i, [_i, _i64, _i64] + [_vp, _i64] * 3 + [_vp, _vp, _f, _f] + [_vp, _i64] * 2),
+    "fsw_add_norm": (_i, [_i, _i64, _i64] + [_vp, _i64] * 3 + [_vp, _vp, _f, _f] + [_vp, _i64] * 2 + [_vp]),
     "fsw_strerror": (_cp, [_i]),
     "fsw_last_hip_error": (_i, []),
     "fsw_decode_barrier_failures": (_i, []),
@@ -506,6 +532,169 @@ def attn_prompt(q, k, v, cu_q, cu_k, scale, out=None):
         check(lib().fsw_attn_prompt(code, Tq, Tk, cu_q.numel() - 1, Hq, Hkv, D, *_row_args(q), *_row_args(k), *_row_args(v),
                                     cu_q.data_ptr(), cu_k.data_ptr(), scale, *_row_args(out), _stream(q)))
     return out
+
+
+def kv_cache8(k_cache, v_cache, k_scale, v_scale):
+    """fsw_kv_cache8 of two float8_e4m3fn tensors [pages, heads, page_size, channels] and their float8_e8m0fnu scales [pages, heads,
+    page_size], each pair with the same strides."""
+    import torch
+    c = kv_cache(k_cache, v_cache)
+    if k_cache.dtype != torch.float8_e4m3fn or v_cache.dtype != k_cache.dtype or \
+            k_scale.dtype != torch.float8_e8m0fnu or v_scale.dtype != k_scale.dtype:
+        raise FswError(E_DTYPE, "fsw: the caches are float8_e4m3fn, their scales float8_e8m0fnu")
+    if k_scale.shape != k_cache.shape[:3] or v_scale.shape != k_scale.shape or any(_step(k_scale, i) != _step(v_scale, i) for i in range(3)):
+        raise FswError(E_SHAPE, "fsw: the scales must be [pages, heads, page_size] with the same strides")
+    return KvCache8(c.k, c.v, k_scale.data_ptr(), v_scale.data_ptr(), c.pages, c.page_size, c.page_stride, c.head_stride, c.token_stride,
+                    _step(k_scale, 0), _step(k_scale, 1), _step(k_scale, 2))
+
+
+def _cache_of(like, caches, dtype, heads, channels):
+    """A cache's structure from (k, v) or (k, v, k_scale, v_scale), checked against the rows it goes with."""
+    if any(not t.is_cuda or t.device != like.device for t in caches):
+        raise FswError(E_DEVICE, "fsw: operands must be device tensors on one device")
+    c = kv_cache(*caches) if len(caches) == 2 else kv_cache8(*caches)
+    if len(caches) == 2 and (caches[0].dtype != dtype or caches[1].dtype != dtype):
+        raise FswError(E_DTYPE, "fsw: the caches have the rows' element type")
+    if tuple(caches[0].shape[1::2]) != (heads, channels):
+        raise FswError(E_SHAPE, "fsw: the caches are [pages, Hkv, page_size, D]")
+    return ctypes.byref(c)
+
+
+def kv_append8(q, k, v, cos_sin, positions, slots, caches, interleaved=False, q_out=None, k_out=None, v_out=None):
+    """Rotated q, and k and v as the cache in 8 bits holds them; `caches` is (k, v, k_scale, v_scale) (fsw_kv_append8). k_out=False,
+    v_out=False: the cache only, the result is None."""
+    import torch
+    code = dtype_code(q)
+    _check_rows(q, k, v)
+    _check_int32(q, positions, slots)
+    T, Hq, D = q.shape
+    Hkv = k.shape[1]
+    if k.shape != (T, Hkv, D) or v.shape != k.shape or positions.shape != (T,) or slots.shape != (T,) or cos_sin.dim() != 2:
+        raise FswError(E_SHAPE, "fsw: q is [T, Hq, D], k and v are [T, Hkv, D], positions and slots [T], cos_sin [rows, rot]")
+    if cos_sin.dtype != torch.float32:
+        raise FswError(E_DTYPE, "fsw: cos_sin is float32")
+    if cos_sin.device != q.device:
+        raise FswError(E_DEVICE, "fsw: operands live on different devices")
+    if not cos_sin.is_contiguous():
+        raise FswError(E_LD, "fsw: cos_sin must be contiguous")
+    cache = _cache_of(q, caches, q.dtype, Hkv, D)
+    q_out, k_out, v_out = (None if o is False else torch.empty(r.shape, dtype=r.dtype, device=r.device) if o is None else o
+                           for o, r in ((q_out, q), (k_out, k), (v_out, v)))
+    for o, r in ((q_out, q), (k_out, k), (v_out, v)):
+        if o is not None:
+            _check_rows(q, o)
+            if o.shape != r.shape:
+                raise FswError(E_SHAPE, "fsw: q_out, k_out and v_out have the shapes of q, k and v")
+    outs = [_row_args(o) if o is not None else (None, 0, 0) for o in (q_out, k_out, v_out)]
+    with torch.cuda.device(q.device):
+        check(lib().fsw_kv_append8(code, T, Hq, Hkv, D, cos_sin.shape[1], int(interleaved), *_row_args(q), *_row_args(k), *_row_args(v),
+                                   cos_sin.data_ptr(), cos_sin.shape[0], positions.data_ptr(), slots.data_ptr(), *outs[0], *outs[1],
+                                   *outs[2], cache, _stream(q)))
+    return q_out, k_out, v_out
+
+
+def kv_read(caches, block_table, cu, tokens, dtype=None, k_out=None, v_out=None):
+    """Keys and values [tokens, Hkv, D] of sequences whose offsets are cu [B + 1], out of their pages (fsw_kv_read; with scales among
+    `caches` fsw_kv_read8, whose results are of `dtype`)."""
+    import torch
+    eight = len(caches) == 4
+    like = caches[0]
+    if like.dim() != 4:
+        raise FswError(E_SHAPE, "fsw: the caches are [pages, Hkv, page_size, D]")
+    dtype = dtype if eight else like.dtype
+    _check_int32(like, block_table, cu)
+    Hkv, D = like.shape[1::2]
+    cache = _cache_of(like, caches, dtype, Hkv, D)
+    if cu.dim() != 1 or cu.numel() < 1 or block_table.dim() != 2 or block_table.shape[0] != cu.numel() - 1:
+        raise FswError(E_SHAPE, "fsw: block_table is [B, width], offsets are [B + 1]")
+    k_out, v_out = (torch.empty((tokens, Hkv, D), dtype=dtype, device=like.device) if o is None else o for o in (k_out, v_out))
+    _check_rows(k_out, v_out)
+    if k_out.shape != (tokens, Hkv, D) or v_out.shape != k_out.shape or k_out.dtype != dtype or k_out.device != like.device:
+        raise FswError(E_SHAPE, "fsw: k_out and v_out are [tokens, Hkv, D]")
+    B, width = block_table.shape
+    f = lib().fsw_kv_read8 if eight else lib().fsw_kv_read
+    with torch.cuda.device(like.device):
+        check(f(dtype_code(k_out), tokens, B, Hkv, D, cache, block_table.data_ptr(), block_table.stride(0) if B > 1 else width, width,
+                cu.data_ptr(), *_row_args(k_out), *_row_args(v_out), _stream(like)))
+    return k_out, v_out
+
+
+def _attend(q, caches, prefix, prefix_len, block_table, lengths, max_len, scale, out, workspace):
+    import torch
+    code = dtype_code(q)
+    _check_rows(q)
+    _check_int32(q, block_table, lengths, *([] if prefix is None else [prefix]))
+    B, Hq, D = q.shape
+    if caches[0].dim() != 4 or block_table.dim() != 2 or block_table.shape[0] != B or lengths.shape != (B,):
+        raise FswError(E_SHAPE, "fsw: q is [B, Hq, D], the caches [pages, Hkv, page_size, D], block_table [B, width], lengths [B]")
+    Hkv, page = caches[0].shape[1:3]
+    cache = _cache_of(q, caches, q.dtype, Hkv, D)
+    if block_table.shape[1] * page < max_len:
+        raise FswError(E_LD, "fsw: block_table is narrower than max_len")
+    if prefix is not None and (prefix.dim() != 1 or prefix.numel() * page < prefix_len):
+        raise FswError(E_LD, "fsw: prefix has fewer pages than prefix_len needs")
+    out = torch.empty((B, Hq, D), dtype=q.dtype, device=q.device) if out is None else out
+    _check_rows(q, out)
+    if out.shape != q.shape:
+        raise FswError(E_SHAPE, "fsw: `out` has the shape of q")
+    L, head = lib(), [code, B, Hq, Hkv, D]
+    if prefix is None:
+        f, first, nbytes = L.fsw_attn_decode8, [], L.fsw_attn_decode8_workspace_bytes(*head, max_len)
+    else:
+        f, size = (L.fsw_attn_shared8, L.fsw_attn_shared8_workspace_bytes) if len(caches) == 4 else \
+            (L.fsw_attn_shared, L.fsw_attn_shared_workspace_bytes)
+        first, nbytes = [prefix.data_ptr(), prefix_len], size(*head, prefix_len, max_len)
+    if workspace is None and nbytes:
+        workspace = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    if workspace is not None and (workspace.dtype != torch.uint8 or workspace.device != q.device or not workspace.is_contiguous()):
+        raise FswError(E_WORKSPACE, "fsw: workspace must be a contiguous uint8 tensor on the operands' device")
+    with torch.cuda.device(q.device):
+        check(f(*head, *_row_args(q), cache, *first, block_table.data_ptr(), block_table.stride(0) if B > 1 else block_table.shape[1],
+                lengths.data_ptr(), max_len, scale, *_row_args(out), workspace.data_ptr() if workspace is not None else None,
+                workspace.numel() if workspace is not None else 0, _stream(q)))
+    return out
+
+
+def attn_decode8(q, caches, block_table, lengths, max_len, scale, out=None, workspace=None):
+    """Attention of one token per sequence over the caches (k, v, k_scale, v_scale) in 8 bits (fsw_attn_decode8)."""
+    if len(caches) != 4:
+        raise FswError(E_SHAPE, "fsw: the caches are (k, v, k_scale, v_scale)")
+    return _attend(q, caches, None, 0, block_table, lengths, max_len, scale, out, workspace)
+
+
+def attn_shared(q, caches, prefix, prefix_len, block_table, lengths, max_len, scale, out=None, workspace=None):
+    """Attention of one token per sequence over a prefix that all share, in pages prefix [n], and its own tokens, over (k, v) or
+    (k, v, k_scale, v_scale) (fsw_attn_shared, fsw_attn_shared8)."""
+    return _attend(q, caches, prefix, prefix_len, block_table, lengths, max_len, scale, out, workspace)
+
+
+def add_norm(x, y=None, gate=None, post=None, pre=None, scale=1.0, eps=1e-5, x_out=None, h=None):
+    """(x', h) of rows x, y [M, D]: x' = x + scale * gate * norm(y) * post, h = norm(x') * pre (fsw_add_norm). gate: [D] or [M, D].
+    Without y: (None, norm(x) * pre). x_out=False, h=False: not computed, None."""
+    import torch
+    code = dtype_code(x)
+    rows = [t for t in (y, gate if gate is not None and gate.dim() == 2 else None) if t is not None]
+    _check_operands(x, *rows)
+    M, D = x.shape
+    if any(t.shape != x.shape for t in rows):
+        raise FswError(E_SHAPE, "fsw: x, y and a gate of rows are [M, D]")
+    for t in (post, pre, gate if gate is not None and gate.dim() == 1 else None):
+        if t is not None and (t.shape != (D,) or (D > 1 and t.stride(0) != 1)):
+            raise FswError(E_SHAPE, "fsw: weights are [D], contiguous")
+    x_out, h = (None if o is False else torch.empty_like(x, memory_format=torch.contiguous_format) if o is None else o for o in (x_out, h))
+    x_out = None if y is None else x_out
+    for o in (x_out, h):
+        if o is not None:
+            _check_operands(x, out=o, out_shape=(M, D))
+    for t in (y, gate, post, pre):
+        if t is not None and (t.dtype != x.dtype or t.device != x.device):
+            raise FswError(E_DTYPE, "fsw: operands differ in element type or device")
+    two = lambda t: (t.data_ptr(), _ld(t)) if t is not None else (None, 0)  # noqa: E731
+    one = lambda t: t.data_ptr() if t is not None else None  # noqa: E731
+    gate_args = two(gate) if gate is not None and gate.dim() == 2 else (one(gate), 0)
+    with torch.cuda.device(x.device):
+        check(lib().fsw_add_norm(code, M, D, *two(x), *two(y), *gate_args, one(post), one(pre), scale, eps, *two(x_out), *two(h), _stream(x)))
+    return x_out, h
 
 
 def set_variant(family, variant):

@@ -23,7 +23,9 @@ OBJ_DIR = os.path.join(HERE, "build", "hip_obj")
 LIB_NAME = "libfsw_hip.so"
 HIP_SOURCES = ["kernels_pair16.hip", "kernels_mid_bf16_gateup.hip", "kernels_mid_bf16_down.hip",
                "kernels_mid_fp16_gateup.hip", "kernels_mid_fp16_down.hip", "kernels_mid.hip", "kernels_tiled.hip", "kernels_skinny.hip", "kernels_stream.hip", "kernels_decode.hip", "fsw_api.hip",
-               "kernels_kv_append.hip", "kernels_attn_decode.hip", "kernels_attn_prompt.hip", "attn_api.hip"]
+               "kernels_kv_append.hip", "kernels_attn_decode.hip", "kernels_attn_prompt.hip", "attn_api.hip",
+               "kernels_kv_append8.hip", "kernels_kv_read.hip", "kernels_attn_decode8.hip", "kernels_attn_prefix.hip", "attn8_api.hip",
+               "kernels_norm.hip", "norm_api.hip"]
 PROBE_LIB_NAME = "libfsw_probe.so"  # measurement kernels of the benchmark (include/fsw_probe.h): not part of the product
 PROBE_SOURCES = ["probes.hip"]
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
@@ -80,7 +82,8 @@ def main():
         ext_modules=[
             CppExtension(
                 name="fused_mlp_module",
-                sources=[os.path.join("csrc", "torch_bindings.cpp"), os.path.join("csrc", "attn_bindings.cpp")],
+                sources=[os.path.join("csrc", "torch_bindings.cpp"), os.path.join("csrc", "attn_bindings.cpp"),
+                         os.path.join("csrc", "attn8_bindings.cpp"), os.path.join("csrc", "norm_bindings.cpp")],
                 include_dirs=include_paths("cuda") + [INCLUDE, os.path.join(rocm, "include")],
                 define_macros=[("__HIP_PLATFORM_AMD__", "1"), ("USE_ROCM", "1")],
                 extra_compile_args=["-O3", "-Wall", "-std=c++17", "-Wno-unused-function"],

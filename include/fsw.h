@@ -267,12 +267,130 @@ FSW_API int fsw_attn_prompt(int dtype, int64_t Tq, int64_t Tk, int64_t B, int64_
  * there is nothing to launch. For tests and benchmarks. */
 FSW_API int fsw_attn_prompt_rows(int dtype, int64_t Tq, int64_t B, int64_t Hq, int64_t Hkv, int64_t D);
 
+/*
+ * The same cache in 8 bits. A row (one token, one head, keys or values) is D e4m3 elements c_i (four significant bits, 2^-9 .. 448, no
+ * infinities) and one power of two: it stands for c_i 2^e. Elements are addressed as in fsw_kv_cache (strides in elements, multiples of 16; D a
+ * multiple of 16); the scale of token t of a page's head h is byte page * scale_page_stride + h * scale_head_stride + t *
+ * scale_token_stride of k_scale (v_scale), e + 127 (e8m0; 255 is no number). Scales that 16 tokens have side by side, in aligned words, are read faster.
+ */
+typedef struct fsw_kv_cache8 {
+  void* k;
+  void* v;
+  uint8_t* k_scale;
+  uint8_t* v_scale;
+  int64_t pages, page_size;
+  int64_t page_stride, head_stride, token_stride;
+  int64_t scale_page_stride, scale_head_stride, scale_token_stride;
+} fsw_kv_cache8;
+
+/* Host-only validation of fsw_kv_append8: as for fsw_kv_append. */
+FSW_API int fsw_validate_kv_append8(int dtype, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t rot,
+                                    const void* Q, int64_t q_token, int64_t q_head, const void* K, int64_t k_token, int64_t k_head,
+                                    const void* V, int64_t v_token, int64_t v_head, const float* cos_sin, int64_t table_rows,
+                                    const int32_t* positions, const int32_t* slots, const void* Qout, int64_t qo_token,
+                                    int64_t qo_head, const void* Kout, int64_t ko_token, int64_t ko_head, const void* Vout,
+                                    int64_t vo_token, int64_t vo_head, const fsw_kv_cache8* cache);
+
+/*
+ * fsw_kv_append to a cache in 8 bits: e is the least integer, -126 at least, with max |x_i| <= 448 2^e over the row's finite values (0 for a row of
+ * zeros), c_i = x_i 2^-e rounded to nearest, ties to even. Infinities and NaN become NaN; a value that would round above the element type's
+ * largest becomes the largest below. Keys are rotated in 64 bits and rounded once. Kout and Vout (each may be NULL) receive the
+ * rows as the cache holds them, in the element type: what a prompt should attend to, so that it sees what later tokens will. Qout may be Q itself, Kout K itself, Vout V
+ * itself.
+ */
+FSW_API int fsw_kv_append8(int dtype, int64_t T, int64_t Hq, int64_t Hkv, int64_t D, int64_t rot, int interleaved,
+                           const void* Q, int64_t q_token, int64_t q_head, const void* K, int64_t k_token, int64_t k_head,
+                           const void* V, int64_t v_token, int64_t v_head, const float* cos_sin, int64_t table_rows,
+                           const int32_t* positions, const int32_t* slots, void* Qout, int64_t qo_token, int64_t qo_head,
+                           void* Kout, int64_t ko_token, int64_t ko_head, void* Vout, int64_t vo_token, int64_t vo_head,
+                           const fsw_kv_cache8* cache, void* stream);
+
+/* Host-only validation of fsw_kv_read and fsw_kv_read8. B <= 65535; width >= 0, table_ld >= width, or 0. */
+FSW_API int fsw_validate_kv_read(int dtype, int64_t T, int64_t B, int64_t Hkv, int64_t D, const fsw_kv_cache* cache, const int32_t* block_table,
+                                 int64_t table_ld, int64_t width, const int32_t* cu, const void* Kout, int64_t ko_token, int64_t ko_head,
+                                 const void* Vout, int64_t vo_token, int64_t vo_head);
+FSW_API int fsw_validate_kv_read8(int dtype, int64_t T, int64_t B, int64_t Hkv, int64_t D, const fsw_kv_cache8* cache, const int32_t* block_table,
+                                  int64_t table_ld, int64_t width, const int32_t* cu, const void* Kout, int64_t ko_token, int64_t ko_head,
+                                  const void* Vout, int64_t vo_token, int64_t vo_head);
+
+/*
+ * Keys and values of B sequences out of their pages, packed: row cu[b] + j of Kout and Vout (cu[b] <= row < cu[b + 1]; B + 1 offsets, ascending from
+ * 0) is token j of sequence b, which lies in page block_table[b * table_ld + j / page_size], j / page_size < width. For fsw_attn_prompt, whose prompts may continue
+ * what is in the cache. Rows behind the last sequence are zeros; a token behind the table's row, or in a page outside the cache, is NaN. Of a cache in 8 bits:
+ * c_i 2^e rounded to the element type.
+ */
+FSW_API int fsw_kv_read(int dtype, int64_t T, int64_t B, int64_t Hkv, int64_t D, const fsw_kv_cache* cache, const int32_t* block_table,
+                        int64_t table_ld, int64_t width, const int32_t* cu, void* Kout, int64_t ko_token, int64_t ko_head, void* Vout,
+                        int64_t vo_token, int64_t vo_head, void* stream);
+FSW_API int fsw_kv_read8(int dtype, int64_t T, int64_t B, int64_t Hkv, int64_t D, const fsw_kv_cache8* cache, const int32_t* block_table,
+                         int64_t table_ld, int64_t width, const int32_t* cu, void* Kout, int64_t ko_token, int64_t ko_head, void* Vout,
+                         int64_t vo_token, int64_t vo_head, void* stream);
+
+/* fsw_attn_decode over a cache in 8 bits: the same checks, scratch rules and answers to invalid sequences. A row whose scale is 255 is NaN. */
+FSW_API int fsw_validate_attn_decode8(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, const void* Q, int64_t q_seq,
+                                      int64_t q_head, const fsw_kv_cache8* cache, const int32_t* block_table, int64_t table_ld,
+                                      const int32_t* lengths, int64_t max_len, float scale, const void* O, int64_t o_seq,
+                                      int64_t o_head);
+FSW_API size_t fsw_attn_decode8_workspace_bytes(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t max_len);
+FSW_API int fsw_attn_decode8(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, const void* Q, int64_t q_seq, int64_t q_head,
+                             const fsw_kv_cache8* cache, const int32_t* block_table, int64_t table_ld, const int32_t* lengths,
+                             int64_t max_len, float scale, void* O, int64_t o_seq, int64_t o_head, void* workspace,
+                             size_t workspace_bytes, void* stream);
+
+/* Host-only validation of fsw_attn_shared and fsw_attn_shared8 (all but the workspace): as for fsw_attn_decode; prefix_len >= 0, prefix_len + max_len <= 2^30. */
+FSW_API int fsw_validate_attn_shared(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, const void* Q, int64_t q_seq,
+                                     int64_t q_head, const fsw_kv_cache* cache, const int32_t* prefix, int64_t prefix_len,
+                                     const int32_t* block_table, int64_t table_ld, const int32_t* lengths, int64_t max_len,
+                                     float scale, const void* O, int64_t o_seq, int64_t o_head);
+FSW_API int fsw_validate_attn_shared8(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, const void* Q, int64_t q_seq,
+                                      int64_t q_head, const fsw_kv_cache8* cache, const int32_t* prefix, int64_t prefix_len,
+                                      const int32_t* block_table, int64_t table_ld, const int32_t* lengths, int64_t max_len,
+                                      float scale, const void* O, int64_t o_seq, int64_t o_head);
+
+/* Bytes of device scratch fsw_attn_shared (fsw_attn_shared8) needs (FSW_E_WORKSPACE without them): float32 sums of the shares of the prefix and of
+ * the sequences' own keys. Need not be initialised. */
+FSW_API size_t fsw_attn_shared_workspace_bytes(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t prefix_len, int64_t max_len);
+FSW_API size_t fsw_attn_shared8_workspace_bytes(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t prefix_len, int64_t max_len);
+
+/*
+ * fsw_attn_decode for a batch whose sequences all begin with the same prefix_len tokens, which are read once for all of them: they lie in pages
+ * prefix[j / page_size], j < prefix_len. lengths, max_len and block_table are of each sequence's own tokens, which begin with a page of their own
+ * and follow the prefix. A length of 0 leaves the prefix alone. The weights of the prefix are rounded to the element type once, for the matrix product, and their
+ * sum is taken of the rounded values, as in fsw_attn_prompt; infinities, NaN, lengths and pages of own tokens are as for fsw_attn_decode; a
+ * page outside the cache among the prefix's gives NaN for all. fsw_attn_shared8 takes the prefix's keys and values rounded to the element type.
+ */
+FSW_API int fsw_attn_shared(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, const void* Q, int64_t q_seq, int64_t q_head,
+                            const fsw_kv_cache* cache, const int32_t* prefix, int64_t prefix_len, const int32_t* block_table,
+                            int64_t table_ld, const int32_t* lengths, int64_t max_len, float scale, void* O, int64_t o_seq,
+                            int64_t o_head, void* workspace, size_t workspace_bytes, void* stream);
+FSW_API int fsw_attn_shared8(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, const void* Q, int64_t q_seq, int64_t q_head,
+                             const fsw_kv_cache8* cache, const int32_t* prefix, int64_t prefix_len, const int32_t* block_table,
+                             int64_t table_ld, const int32_t* lengths, int64_t max_len, float scale, void* O, int64_t o_seq,
+                             int64_t o_head, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Host-only validation of fsw_add_norm. M <= 2^30; D a multiple of 8 up to 32768; leading dimensions multiples of 8, those of results at least D, pointers
+ * 16-byte aligned; scale finite, eps a positive normal number. */
+FSW_API int fsw_validate_add_norm(int dtype, int64_t M, int64_t D, const void* X, int64_t ldx, const void* Y, int64_t ldy, const void* gate,
+                                  int64_t ld_gate, const void* post, const void* pre, float scale, float eps, const void* Xout,
+                                  int64_t ldxo, const void* H, int64_t ldh);
+
+/*
+ * The norms around a block of a layer, its gate and its residual scale, a row at a time:
+ *   b = Y rms(Y) post,  Xout = X + scale gate b,  H = Xout rms(Xout) pre,  rms(z) = (mean z^2 + eps)^(-1/2)
+ * in fp32 (squares in 64 bits), Xout and H rounded once each, H from the unrounded Xout. post, pre: D weights. post NULL: b = Y. pre NULL: weights of 1. gate: a row for
+ * every row (ld_gate >= D) or one for all (ld_gate = 0); NULL: 1. Y NULL (then gate and post are, too): H alone of X, for the norm before the first block. One of Xout and H may
+ * be NULL. Xout may be X itself, H may be Y itself, with the same leading dimension.
+ */
+FSW_API int fsw_add_norm(int dtype, int64_t M, int64_t D, const void* X, int64_t ldx, const void* Y, int64_t ldy, const void* gate,
+                         int64_t ld_gate, const void* post, const void* pre, float scale, float eps, void* Xout, int64_t ldxo,
+                         void* H, int64_t ldh, void* stream);
+
 /* The hipError_t (as int) of the most recent failed launch on the calling thread, 0 if none. */
 FSW_API int fsw_last_hip_error(void);
 
 /* ABI version: major * 1000 + minor. 2000: the measurement kernels fsw_probe_* left this library (libfsw_probe.so,
  * fsw_probe.h); fsw_gateup_f32out and fsw_gateup_hblocked joined it; fsw_gateup_workspace_bytes returns 0. 2001: the attention
- * entry points. 2002: fsw_attn_prompt_rows. */
+ * entry points. 2002: fsw_attn_prompt_rows. 2003: the cache in 8 bits, fsw_kv_read, fsw_attn_shared, fsw_add_norm. */
 FSW_API int fsw_version(void);
 
 /*
