@@ -6,8 +6,8 @@
 // heads of its group, stand side by side: a workgroup owns 64 or 128 of them and a share of the keys, so the prefix is read once per 64 or 128 rows, from
 // the L2 of the head's XCD after the first. Four waves own 16 or 32 rows each and walk the same tiles of 64 keys through LDS, two tiles
 // of each kind in turn, as the prompts' kernel does (whose arrangement of the two products, with scores transposed and weights that stay in their lanes, this is);
-// there is no diagonal, and the keys come from pages. Elements of 16 bits are copied to LDS directly, 16 bytes a lane, each lane from an address of its own
-// (any page size); the page numbers of a tile are asked for a tile ahead. Elements of 8 bits pass through registers, where they
+// there is no diagonal, and the keys come from pages. Elements of 16 bits are copied to LDS directly, 16 bytes a lane;
+// the page numbers of a tile are asked for a tile ahead. Elements of 8 bits pass through registers, where they
 // become keys and values of the element type.
 #include <float.h>
 
@@ -22,12 +22,14 @@
 namespace fsw {
 namespace {
 
-template <class T, class CACHE, int DP, int NB>
+// WHOLE: the rows of a wave's load, ROWS of them, lie in one page, whose address is wave-uniform then.
+template <class T, class CACHE, int DP, int NB, bool WHOLE>
 __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prefix_kernel(PrefixOver<CACHE> a, Divisor by_group, Divisor by_hkv, int chunk,
                                                                               float lower, float limit) {
   constexpr bool EIGHT = std::is_same<CACHE, PagedKv8>::value;
   constexpr int RB = DP * 2, TILE = KEYS * RB;
-  constexpr int VECS = EIGHT ? KEYS * DP / 16 / 256 : TILE / 4096;  // 16-byte vectors of keys, and of values, that a thread moves per tile
+  constexpr int SIZE = EIGHT ? 1 : 2, PER_ROW = DP * SIZE / 16, ROWS = 64 / PER_ROW;  // 16-byte vectors of a row, rows of a wave's load
+  constexpr int VECS = KEYS / ROWS / 4;                                               // loads of keys, and of values, of a wave and tile
   constexpr int KSTEPS = DP / 32, DB = DP / 16, KB = KEYS / 16, WM = 16 * NB, BM = 4 * WM;
   constexpr bool AHEAD = DP < 256 || NB == 1;
   constexpr int VBUF = AHEAD ? 2 : 1, VG = AHEAD ? 4 : 1;
@@ -58,69 +60,70 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prefix_kernel(Pre
     }
   }
 
-  // Vector j of a thread is channels `channel` .. of key `key` of a tile. Keys behind the end are the last one once more: their scores are
-  // masked, and a weight of zero times a value that is seen anyway changes no sum that has no infinity (which is looked for below).
-  auto key_of = [&](int j) INLINE -> int { return EIGHT ? (j * 256 + tid) / (DP / 16) : ((j * 4 + wave) * 1024 + lane * 16) / RB; };
-  int page[VECS];
+  // Load j of a wave is rows first_row(j) .. + ROWS - 1 of a tile, PER_ROW lanes each. Lane l knows the page of the tile's key l.
+  const int lrow = lane / PER_ROW, lvec = lane % PER_ROW;
+  auto first_row = [&](int j) INLINE -> int { return (j * 4 + wave) * ROWS; };
+  int pages;
   bool bad = false;
   auto locate = [&](int at) INLINE {
-#pragma unroll
-    for (int j = 0; j < VECS; ++j) {
-      const int key = at + key_of(j) < end ? at + key_of(j) : end - 1;
-      page[j] = a.pages[a.cache.per_page.quotient(key)];
-    }
+    const int key = at + lane < end ? at + lane : end - 1;
+    pages = a.pages[a.cache.per_page.quotient(key)];
   };
-  const unsigned char *kc, *vc, *ksc = nullptr, *vsc = nullptr;
-  if constexpr (EIGHT) {
-    kc = a.cache.k + kvh * a.cache.head, vc = a.cache.v + kvh * a.cache.head;
-    ksc = a.cache.k_scale + kvh * a.cache.scale_head, vsc = a.cache.v_scale + kvh * a.cache.scale_head;
-  } else {
-    kc = (const unsigned char*)a.cache.k + kvh * a.cache.head * 2, vc = (const unsigned char*)a.cache.v + kvh * a.cache.head * 2;
-  }
+  const unsigned char* kc = (const unsigned char*)a.cache.k + kvh * a.cache.head * SIZE;
+  const unsigned char* vc = (const unsigned char*)a.cache.v + kvh * a.cache.head * SIZE;
   u32x4 kr[EIGHT ? VECS : 1], vr[EIGHT ? VECS : 1];  // a tile under way
-  unsigned km[EIGHT ? VECS : 1], vm[EIGHT ? VECS : 1];
-  // asks for the tile at `at`, whose pages are known, and for the next one's pages
+  unsigned marks[EIGHT ? VECS : 1];                  // its scales: keys' and values' bytes
+  // Asks for the tile at `at`, whose pages are known, and for the next one's pages. Rows behind the end are rows of the last load once more, or, in it,
+  // whatever its page holds: their scores are masked, their values replaced by zeros.
   auto ask = [&](int at, unsigned char* kto, unsigned char* vto) INLINE {
+    bad |= (unsigned)pages >= (unsigned)a.cache.pages;
+    if constexpr (!WHOLE) asm volatile("" : "+v"(pages));
 #pragma unroll
     for (int j = 0; j < VECS; ++j) {
-      const int key = at + key_of(j) < end ? at + key_of(j) : end - 1;
+      const int last = WHOLE ? (end - 1) & ~(ROWS - 1) : end - 1;
+      int key = at + first_row(j) + (WHOLE ? 0 : lrow);
+      key = key < last ? key : last;
+      const int n = WHOLE ? __builtin_amdgcn_readlane(pages, key < at ? 0 : key - at) : __shfl(pages, key < at ? 0 : key - at);
       const int place = key - a.cache.per_page.quotient(key) * a.cache.page_size;
-      const bool inside = (unsigned)page[j] < (unsigned)a.cache.pages;
-      bad |= !inside;
-      const long long n = inside ? page[j] : 0, where = n * a.cache.page + place * a.cache.token;
+      const long long page = (unsigned)n < (unsigned)a.cache.pages ? n : 0;
+      const long long where = (page * a.cache.page + place * a.cache.token) * SIZE;
+      const unsigned from = WHOLE ? (unsigned)(lrow * (int)a.cache.token * SIZE) : 0u;
       if constexpr (EIGHT) {
-        const int ch = (j * 256 + tid) % (DP / 16) * 16;
-        const long long mark = n * a.cache.scale_page + place * a.cache.scale_token;
-        km[j] = ksc[mark], vm[j] = vsc[mark];
+        const long long mark = kvh * a.cache.scale_head + page * a.cache.scale_page + place * a.cache.scale_token;
+        const unsigned more = WHOLE ? (unsigned)(lrow * (int)a.cache.scale_token) : 0u;
+        marks[j] = (a.cache.k_scale + mark)[more] | (a.cache.v_scale + mark)[more] << 8;
         kr[j] = vr[j] = u32x4{0, 0, 0, 0};
-        if (ch < a.d) kr[j] = *(const u32x4*)(kc + where + ch), vr[j] = *(const u32x4*)(vc + where + ch);
+        if (lvec * 16 < a.d) {
+          kr[j] = *(const u32x4*)(kc + where + (from + lvec * 16));
+          vr[j] = *(const u32x4*)(vc + where + (from + lvec * 16));
+        }
       } else {
-        const int pos = (((j * 4 + wave) * 1024 + lane * 16) % RB) / 16, row = key_of(j);
-        const int kch = (pos ^ k_swizzle<DP>(row)) * 8, vch = (pos ^ v_swizzle<DP>(row)) * 8;
+        const int row = first_row(j) + lrow, kch = (lvec ^ k_swizzle<DP>(row)) * 8, vch = (lvec ^ v_swizzle<DP>(row)) * 8;
         // (channels that the head has not: their places hold zeros from the beginning)
         if (kch < a.d)
-          __builtin_amdgcn_global_load_lds((const global_void*)(kc + (where + kch) * 2), (lds_void*)(kto + (j * 4 + wave) * 1024), 16, 0, 0);
+          __builtin_amdgcn_global_load_lds((const global_void*)(kc + where + (from + kch * 2)), (lds_void*)(kto + (j * 4 + wave) * 1024), 16, 0, 0);
         if (vch < a.d)
-          __builtin_amdgcn_global_load_lds((const global_void*)(vc + (where + vch) * 2), (lds_void*)(vto + (j * 4 + wave) * 1024), 16, 0, 0);
+          __builtin_amdgcn_global_load_lds((const global_void*)(vc + where + (from + vch * 2)), (lds_void*)(vto + (j * 4 + wave) * 1024), 16, 0, 0);
       }
     }
-    if (at + KEYS < end) locate(at + KEYS);
+    locate(at + KEYS);
   };
-  // 8 bits: the tile that was asked for, as the element type
-  auto put = [&](unsigned char* kto, unsigned char* vto) INLINE {
+  // 8 bits: the tile at `at`, that was asked for, as the element type
+  auto put = [&](int at, unsigned char* kto, unsigned char* vto) INLINE {
     if constexpr (EIGHT) {
 #pragma unroll
       for (int j = 0; j < VECS; ++j) {
-        const int row = key_of(j), vec = (j * 256 + tid) % (DP / 16) * 2;
+        const int row = first_row(j) + lrow;
         auto store = [&](u32x4 x, float up, unsigned char* to, int swizzle) INLINE {
 #pragma unroll
           for (int i = 0; i < 2; ++i)
-            *(u32x4*)(to + row * RB + ((vec + i) ^ swizzle) * 16) =
+            *(u32x4*)(to + row * RB + ((2 * lvec + i) ^ swizzle) * 16) =
                 u32x4{value_of<T, false>(x[2 * i], up), value_of<T, true>(x[2 * i], up), value_of<T, false>(x[2 * i + 1], up),
                       value_of<T, true>(x[2 * i + 1], up)};
         };
-        store(kr[j], scale_value(km[j]), kto, k_swizzle<DP>(row));
-        store(vr[j], scale_value(vm[j]), vto, v_swizzle<DP>(row));
+        if (at + row >= end) vr[j] = u32x4{0, 0, 0, 0}, marks[j] = 127u << 8;
+        store(kr[j], scale_value(marks[j] & 255u), kto, k_swizzle<DP>(row));
+        store(vr[j], scale_value(marks[j] >> 8), vto, v_swizzle<DP>(row));
       }
     }
   };
@@ -129,6 +132,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prefix_kernel(Pre
   float m[NB], sum[NB];
   const float c = a.scale_log2;
   auto attend = [&](int at, const unsigned char* ks, const unsigned char* vs) INLINE {
+    if (wrow >= rows) return;  // a wave without rows helps with the copies
     f32x4 s[KB][NB];
     u32x4 kf[2][KSTEPS];
     auto key_fragment = [&](int kb, int st) INLINE -> u32x4 {
@@ -233,14 +237,21 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prefix_kernel(Pre
     }
     __syncthreads();
   };
+  // values of rows behind the end
+  auto clear = [&](int at, unsigned char* vs) INLINE {
+#pragma unroll 1
+    for (int byte = (end - at) * RB + tid * 16; byte < TILE; byte += 4096) *(u32x4*)(vs + byte) = u32x4{0, 0, 0, 0};
+    __syncthreads();
+  };
   bool again = false;
   // Tile t is in buffer t % 2. At the barrier the tile has landed, and every wave has read the one before.
   auto turn = [&](int at, const unsigned char* ks, unsigned char* vs, unsigned char* knext, unsigned char* vnext) INLINE {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (at + KEYS < end) ask(at + KEYS, knext, vnext);
+    ask(at + KEYS, knext, vnext);
+    if (!EIGHT && at + KEYS > end) clear(at, vs);
     if (__builtin_expect(again, 0)) silence(vs);
     attend(at, ks, vs);
-    if (at + KEYS < end) put(knext, vnext);
+    put(at + KEYS, knext, vnext);
   };
   if (!EIGHT && a.d < DP) {
     for (int byte = tid * 16; byte < TILE; byte += 4096) {
@@ -259,7 +270,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prefix_kernel(Pre
     }
     locate(begin);
     ask(begin, k0s, v0s);
-    put(k0s, v0s);
+    put(begin, k0s, v0s);
     for (int at = begin; at < end; at += 2 * KEYS) {
       turn(at, k0s, v0s, k1s, v1s);
       if (at + KEYS >= end) break;
@@ -314,7 +325,8 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prefix_kernel(Pre
       const long long at = (unsigned)n < (unsigned)a.cache.pages ? n : 0;
       if constexpr (EIGHT) {
         const unsigned code = vc[at * a.cache.page + place * a.cache.token + ch];
-        seen.add((unsigned short)value_of<T, false>(code, scale_value(vsc[at * a.cache.scale_page + place * a.cache.scale_token])));
+        const long long mark = kvh * a.cache.scale_head + at * a.cache.scale_page + place * a.cache.scale_token;
+        seen.add((unsigned short)value_of<T, false>(code, scale_value(a.cache.v_scale[mark])));
       } else {
         seen.add(((const unsigned short*)vc)[at * a.cache.page + place * a.cache.token + ch]);
       }
@@ -325,19 +337,22 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prefix_kernel(Pre
   }
 }
 
-template <class T, class CACHE, int DP, int NB>
+template <class T, class CACHE, int DP, int NB, bool WHOLE>
 hipError_t launch(const PrefixOver<CACHE>& a, const PrefixPlan& p, hipStream_t stream) {
   const int group = a.hq / a.hkv;
   const float shift = shift_of<T>(a.keys);
   const float lower = fmaxf(shift / a.scale_log2, -FLT_MAX / 4), limit = fmaxf((shift + SLACK<T>) / a.scale_log2, -FLT_MAX / 4);
   const dim3 grid(a.hkv * ((a.seqs * group + 64 * NB - 1) / (64 * NB)), p.splits);
-  attn_prefix_kernel<T, CACHE, DP, NB><<<grid, 256, 0, stream>>>(a, Divisor(group), Divisor(a.hkv), p.chunk, lower, limit);
+  attn_prefix_kernel<T, CACHE, DP, NB, WHOLE><<<grid, 256, 0, stream>>>(a, Divisor(group), Divisor(a.hkv), p.chunk, lower, limit);
   return hipGetLastError();
 }
 
 template <class T, class CACHE, int DP>
 hipError_t launch_dp(const PrefixOver<CACHE>& a, const PrefixPlan& p, hipStream_t stream) {
-  return p.rows == 64 ? launch<T, CACHE, DP, 1>(a, p, stream) : launch<T, CACHE, DP, 2>(a, p, stream);
+  constexpr int ROWS = 1024 / (DP * (std::is_same<CACHE, PagedKv8>::value ? 1 : 2));
+  if (a.cache.page_size % ROWS != 0)
+    return p.rows == 64 ? launch<T, CACHE, DP, 1, false>(a, p, stream) : launch<T, CACHE, DP, 2, false>(a, p, stream);
+  return p.rows == 64 ? launch<T, CACHE, DP, 1, true>(a, p, stream) : launch<T, CACHE, DP, 2, true>(a, p, stream);
 }
 
 template <class T, class CACHE>
