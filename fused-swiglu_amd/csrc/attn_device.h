@@ -44,6 +44,26 @@ template <bool HIGH>
 __device__ __forceinline__ f32x2 unpack_e4m3(unsigned x) {
   return __builtin_bit_cast(f32x2, __builtin_amdgcn_cvt_pk_f32_fp8((int)x, HIGH));
 }
+// Two elements times the power of two whose exponent `scale` has, as 16-bit ones (v_cvt_scalef32_pk)
+template <class T, bool HIGH>
+__device__ __forceinline__ unsigned widen(unsigned x, float scale);
+template <>
+__device__ __forceinline__ unsigned widen<Bf16, false>(unsigned x, float scale) {
+  return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, scale, false));
+}
+template <>
+__device__ __forceinline__ unsigned widen<Bf16, true>(unsigned x, float scale) {
+  return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, scale, true));
+}
+template <>
+__device__ __forceinline__ unsigned widen<Fp16, false>(unsigned x, float scale) {
+  return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, scale, false));
+}
+template <>
+__device__ __forceinline__ unsigned widen<Fp16, true>(unsigned x, float scale) {
+  return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, scale, true));
+}
+
 // the scale of a byte: 255 is no number
 __device__ __forceinline__ float scale_value(unsigned byte) {
   return byte == 255 ? __builtin_nanf("") : byte == 0 ? __builtin_bit_cast(float, 0x00400000u) : __builtin_bit_cast(float, byte << 23);

@@ -12,7 +12,6 @@ namespace {
 
 typedef __attribute__((ext_vector_type(4))) short s16x4;
 typedef __attribute__((address_space(3))) void lds_void;
-typedef __attribute__((address_space(1))) void global_void;
 typedef __attribute__((address_space(3))) unsigned char lds_byte;
 
 constexpr float NEG_INF = -__builtin_inff();
@@ -73,13 +72,6 @@ __device__ __forceinline__ u32x4 value_fragment(const unsigned char* vs, int st,
   const u32x2 lo = read_tr(vs + key * RB + (ch ^ v_swizzle<DP>(key)) * 16 + (col & 1) * 8);
   const u32x2 hi = read_tr(vs + (key + 16) * RB + (ch ^ v_swizzle<DP>(key + 16)) * 16 + (col & 1) * 8);
   return u32x4{lo[0], lo[1], hi[0], hi[1]};
-}
-
-// two e4m3 elements times a power of two as elements of the type
-template <class T, bool HIGH>
-__device__ __forceinline__ unsigned value_of(unsigned x, float scale) {
-  const f32x2 v = unpack_e4m3<HIGH>(x);
-  return T::pack2(v[0] * scale, v[1] * scale);
 }
 
 }  // namespace

@@ -8,9 +8,10 @@
 // come out with head l % 16 and keys 4 (l / 16) + r of either block in lane l, which is what the B operand of the second product
 // wants if its 32 keys are numbered {4 g .. 4 g + 3, 16 + 4 g .. 19 + 4 g} (g = l / 16); its A operand's rows are value rows as they lie, DP / 16
 // channels a lane, whose elements of four keys are put side by side by four byte permutations for four channels.
-// Elements become 16-bit ones by v_cvt_scalef32_pk, two at a time, without loss in either type. Scales never meet them: a key's multiplies its score, a
-// value's its weight, both in fp32. The second product is bf16 for both types, since a weight times a power of two wants fp32's exponents; the weight is
-// split into two elements, 16 bits, whose products both are added.
+// Elements become 16-bit ones by v_cvt_scalef32_pk, two at a time: keys, of which a lane has one in either block, with their scale, values without
+// (theirs multiplies the weight, in fp32), so the second product is bf16 for both types, since a weight times a power of two wants fp32's exponents; the
+// weight is split into two elements, 16 bits, whose products both are added. Where 16 keys lie in one page its descriptor ends with the sequence: rows behind
+// it read as zeros.
 #include "attn.h"
 #include "attn_device.h"
 #include "fsw_device.h"
@@ -25,40 +26,13 @@ constexpr int TURN = 32;       // keys of a wave at a time
 
 #define INLINE __attribute__((always_inline))
 
-// two elements as 16-bit ones
-template <class T, bool HIGH>
-__device__ __forceinline__ unsigned widen(unsigned x);
-template <>
-__device__ __forceinline__ unsigned widen<Bf16, false>(unsigned x) {
-  return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, false));
-}
-template <>
-__device__ __forceinline__ unsigned widen<Bf16, true>(unsigned x) {
-  return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(x, 1.0f, true));
-}
-template <>
-__device__ __forceinline__ unsigned widen<Fp16, false>(unsigned x) {
-  return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, false));
-}
-template <>
-__device__ __forceinline__ unsigned widen<Fp16, true>(unsigned x) {
-  return __builtin_bit_cast(unsigned, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, 1.0f, true));
-}
-
-// bits of the scale in byte r of four, as a float's; 255 gives an infinity, which the kernel looks for
-__device__ __forceinline__ unsigned scale_bits(unsigned four, int r) {
-  const unsigned b = (r < 3 ? four << (23 - 8 * r) : four >> 1) & 0x7f800000u;
-  return b > 0x00400000u ? b : 0x00400000u;
-}
-constexpr unsigned NO_NUMBER = 0x7f800000u;
-
 // DP: channels, padded to 64, 128 or 256; a row of values is VB elements on each of 16 lanes.
 // WHOLE: 16 keys in a row lie in one page, their scales in four aligned words.
 template <class T, int DP, bool WHOLE, int WAVES>
 __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 2 : 4) void attn_decode8_kernel(PagedAttn8Args a, float lift, int chunk, int group, int head_tiles,
                                                                                      float* partial) {
   constexpr int VB = DP / 16, VW = VB / 4, KV = DP / 64;  // KV: vectors of a key
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, grp = lane >> 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, grp = lane >> 4;
   const int split = blockIdx.z, splits = gridDim.z, seq = blockIdx.y;
   int kvh = blockIdx.x, first = 0;
   if (head_tiles > 1) {
@@ -75,13 +49,13 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 2 : 4) void attn_decode8_ke
   const unsigned char* ksc = a.cache.k_scale + kvh * a.cache.scale_head;
   const unsigned char* vsc = a.cache.v_scale + kvh * a.cache.scale_head;
   const int* table = a.block_table + (long long)seq * a.table_ld;
-  // page and place of this lane's keys of the turn that begins at `at`; below max_len, whatever the length is. A second block that begins
-  // at max_len or behind it stands for the first once more: of its keys, none counts.
+  // Pages of the turn that begins at `at`, below max_len, whatever the length is. WHOLE: of its two blocks of 16 keys; a block that begins
+  // at max_len or behind it has none. Else of this lane's keys, and their places; keys from max_len on stand for the last before it.
   int page[2], place[2];
   auto locate = [&](int at) INLINE {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      int key = (h == 1 && at + 16 >= a.max_len ? at : at + 16 * h) + col;
+      int key = at + 16 * h + (WHOLE ? 0 : col);
       key = key < a.max_len ? key : a.max_len - 1;
       const int idx = a.cache.per_page.quotient(key);
       page[h] = table[idx];
@@ -104,88 +78,91 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 2 : 4) void attn_decode8_ke
   const int end = bad_len ? 0 : (len - begin < chunk ? len : begin + chunk);
   if (split > 0 && begin >= end) return;
 
+  // places of a lane's vectors in a block of 16 keys; channels that the head has not are behind every end
+  const int stride = (int)a.cache.token;
+  unsigned koff[KV], voff[4];
+#pragma unroll
+  for (int s = 0; s < KV; ++s) koff[s] = s * 64 + grp * 16 < a.d ? (unsigned)(col * stride + s * 64 + grp * 16) : OOB_OFFSET;
+#pragma unroll
+  for (int r = 0; r < 4; ++r) voff[r] = col * VB < a.d ? (unsigned)((4 * grp + r) * stride + col * VB) : OOB_OFFSET;
+
   f32x4 acc[VB];
 #pragma unroll
   for (int i = 0; i < VB; ++i) acc[i] = f32x4{0, 0, 0, 0};
   float m = NEG_INF, sum = 0.0f;
   bool bad_page = false;
-  unsigned worst = 0;  // largest scale
+  int most = -127;  // largest exponent of a value's scale; 128 is no number
 
   for (; at < end; at += TURN * WAVES) {
     const bool part = at + TURN > end;
     u32x4 kf[2][KV];
-    unsigned vf[2][4][VW], ks[2], vs[2];
+    unsigned vf[2][4][VW], ks[2], vs[2];  // ks: of this lane's key, vs: of the four that its scores are of
+    if constexpr (WHOLE) {
+      // the keys of a block are rows of one page: those behind the end are zeros and touch no memory
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      // a page outside the cache is an error where a key lies in it, and read as page 0
-      const bool inside = (unsigned)page[h] < (unsigned)a.cache.pages;
-      bad_page |= !inside && at + 16 * h + col < end;
-      const long long where = (inside ? page[h] : 0) * a.cache.page + place[h] * a.cache.token;
-      const long long mark = (inside ? page[h] : 0) * a.cache.scale_page + place[h] * a.cache.scale_token;
+      for (int h = 0; h < 2; ++h) {
+        const int left = end - at - 16 * h, keys = left < 16 ? left : 16;
+        const int n = __builtin_amdgcn_readfirstlane(page[h]), first_row = __builtin_amdgcn_readfirstlane(place[h]);
+        // a page outside the cache is an error where a key lies in it, and read as page 0
+        const bool inside = (unsigned)n < (unsigned)a.cache.pages;
+        bad_page |= !inside && keys > 0;
+        const long long known = inside ? n : 0, where = known * a.cache.page + first_row * a.cache.token;
+        const int span = keys > 0 ? (keys - 1) * stride + a.d : 0;
+        const auto krsrc = make_rsrc(kc + where, span), vrsrc = make_rsrc(vc + where, span);
+        const long long mark = known * a.cache.scale_page + first_row;  // the page has room for all 16, keys or not
+        const unsigned four = keys > 0 ? 4 * grp : OOB_OFFSET;
+        ks[h] = __builtin_amdgcn_raw_buffer_load_b8(make_rsrc(ksc + mark, 16), keys > 0 ? col : (int)OOB_OFFSET, 0, 0);
+        vs[h] = __builtin_amdgcn_raw_buffer_load_b32(make_rsrc(vsc + mark, 16), (int)four, 0, 0);
 #pragma unroll
-      for (int s = 0; s < KV; ++s) {
-        const int ch = s * 64 + grp * 16;
-        kf[h][s] = u32x4{0, 0, 0, 0};
-        if (ch < a.d) kf[h][s] = __builtin_nontemporal_load((const u32x4*)(kc + where + ch));
-      }
-      auto uniform = [](long long x) INLINE -> long long {
-        const unsigned lo = __builtin_amdgcn_readfirstlane((unsigned)x);
-        const unsigned hi = __builtin_amdgcn_readfirstlane((unsigned)((unsigned long long)x >> 32));
-        return (long long)(((unsigned long long)hi << 32) | lo);
-      };
-      const unsigned char* tile = vc;
-      if constexpr (WHOLE) {
-        tile += uniform(where);
-        const long long marks = uniform(mark) + 4 * grp;  // the page has room for all 16, keys or not
-        ks[h] = *(const unsigned*)(ksc + marks);
-        vs[h] = *(const unsigned*)(vsc + marks);
-      } else {
-        const int both = ksc[mark] | vsc[mark] << 8;
-        ks[h] = vs[h] = 0;
+        for (int s = 0; s < KV; ++s) kf[h][s] = buf_load16_stream(krsrc, koff[s]);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-          const unsigned x = (unsigned)__shfl(both, 4 * grp + r);
-          ks[h] |= (x & 255u) << (8 * r);
-          vs[h] |= (x >> 8) << (8 * r);
-        }
-      }
-#pragma unroll
-      for (int r = 0; r < 4; ++r) {
-        const int k = 4 * grp + r;
-        const unsigned char* p;
-        if constexpr (WHOLE) {
-          p = tile + k * (int)a.cache.token;
-        } else {
-          p = vc + __shfl(where, k);
-        }
-#pragma unroll
-        for (int w = 0; w < VW; ++w) vf[h][r][w] = 0;
-        if (col * VB < a.d) {
           if constexpr (VW == 4) {
-            const u32x4 x = __builtin_nontemporal_load((const u32x4*)(p + col * VB));
+            const u32x4 x = buf_load16_stream(vrsrc, voff[r]);
 #pragma unroll
             for (int w = 0; w < VW; ++w) vf[h][r][w] = x[w];
           } else if constexpr (VW == 2) {
-            const u32x2 x = __builtin_nontemporal_load((const u32x2*)(p + col * VB));
+            const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(vrsrc, (int)voff[r], 0, 2);
             vf[h][r][0] = x[0], vf[h][r][1] = x[1];
           } else {
-            vf[h][r][0] = __builtin_nontemporal_load((const unsigned*)(p + col * VB));
+            vf[h][r][0] = __builtin_amdgcn_raw_buffer_load_b32(vrsrc, (int)voff[r], 0, 2);
+          }
+        }
+      }
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const bool inside = (unsigned)page[h] < (unsigned)a.cache.pages;
+        bad_page |= !inside && at + 16 * h + col < end;
+        const long long where = (inside ? page[h] : 0) * a.cache.page + place[h] * a.cache.token;
+        const long long mark = (inside ? page[h] : 0) * a.cache.scale_page + place[h] * a.cache.scale_token;
+#pragma unroll
+        for (int s = 0; s < KV; ++s) {
+          const int ch = s * 64 + grp * 16;
+          kf[h][s] = u32x4{0, 0, 0, 0};
+          if (ch < a.d) kf[h][s] = __builtin_nontemporal_load((const u32x4*)(kc + where + ch));
+        }
+        const int value_mark = vsc[mark];
+        ks[h] = ksc[mark], vs[h] = 0;
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          vs[h] |= (unsigned)__shfl(value_mark, 4 * grp + r) << (8 * r);
+          const unsigned* p = (const unsigned*)(vc + __shfl(where, 4 * grp + r) + col * VB);
+#pragma unroll
+          for (int w = 0; w < VW; ++w) vf[h][r][w] = 0;
+          if (col * VB < a.d && at + 16 * h + 4 * grp + r < end) {
+#pragma unroll
+            for (int w = 0; w < VW; ++w) vf[h][r][w] = p[w];
           }
         }
       }
     }
-    if (part) {  // what lies behind the end weighs nothing, whatever it holds
+    if (part) {  // what lies behind the end weighs nothing, whatever its scale
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const int left = end - at - 16 * h - 4 * grp;  // keys of this lane
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-          if (r < left) continue;
-          ks[h] = (ks[h] & ~(255u << 8 * r)) | 127u << 8 * r;
-          vs[h] = (vs[h] & ~(255u << 8 * r)) | 127u << 8 * r;
-#pragma unroll
-          for (int w = 0; w < VW; ++w) vf[h][r][w] = 0;
-        }
+        const unsigned keep = left >= 4 ? ~0u : left <= 0 ? 0u : (1u << 8 * left) - 1;
+        vs[h] = (vs[h] & keep) | (0x7f7f7f7fu & ~keep);
       }
     }
     if (at + TURN * WAVES < end) locate(at + TURN * WAVES);
@@ -195,16 +172,15 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 2 : 4) void attn_decode8_ke
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       s[h] = f32x4{0, 0, 0, 0};
+      const float up = __builtin_bit_cast(float, ks[h] << 23);
 #pragma unroll
       for (int i = 0; i < 2 * KV; ++i) {
         const unsigned lo = kf[h][i / 2][i % 2 * 2], hi = kf[h][i / 2][i % 2 * 2 + 1];
-        s[h] = T::mfma16(u32x4{widen<T, false>(lo), widen<T, true>(lo), widen<T, false>(hi), widen<T, true>(hi)}, qf[i], s[h]);
+        s[h] = T::mfma16(u32x4{widen<T, false>(lo, up), widen<T, true>(lo, up), widen<T, false>(hi, up), widen<T, true>(hi, up)}, qf[i], s[h]);
       }
 #pragma unroll
       for (int r = 0; r < 4; ++r) {
-        const unsigned bits = scale_bits(ks[h], r);
-        worst = worst > bits ? worst : bits;
-        s[h][r] *= __builtin_bit_cast(float, bits) * a.scale_log2;
+        s[h][r] *= a.scale_log2;
         if (part && at + 16 * h + 4 * grp + r >= end) s[h][r] = NEG_INF;
         top = fmaxf(top, s[h][r]);
       }
@@ -228,9 +204,9 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 2 : 4) void attn_decode8_ke
       for (int r = 0; r < 4; ++r) {
         const float p = __builtin_amdgcn_exp2f(s[h][r] - base);
         sum += p;
-        const unsigned bits = scale_bits(vs[h], r);
-        worst = worst > bits ? worst : bits;
-        w[r] = p * __builtin_bit_cast(float, bits);
+        const int e = (int)(vs[h] >> 8 * r & 255u) - 127;
+        most = most > e ? most : e;
+        w[r] = __builtin_amdgcn_ldexpf(p, e);
       }
 #pragma unroll
       for (int r = 0; r < 4; r += 2) {
@@ -257,13 +233,13 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 2 : 4) void attn_decode8_ke
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int k = 0; k < 2; ++k)
-            v[2 * h + k] = c % 2 == 0 ? widen<Bf16, false>(pair[h][k][c / 2]) : widen<Bf16, true>(pair[h][k][c / 2]);
+            v[2 * h + k] = c % 2 == 0 ? widen<Bf16, false>(pair[h][k][c / 2], 1.0f) : widen<Bf16, true>(pair[h][k][c / 2], 1.0f);
         acc[4 * w + c] = Bf16::mfma16(v, p1, acc[4 * w + c]);
         acc[4 * w + c] = Bf16::mfma16(v, p2, acc[4 * w + c]);
       }
     }
   }
-  if (__any(bad_page || worst == NO_NUMBER) || bad_len) sum = __builtin_nanf("");
+  if (__any(bad_page || most == 128) || bad_len) sum = __builtin_nanf("");
   sum = sum_over_groups(sum);
 
   // The waves' shares of the keys, joined through LDS: rows of the real heads, each wave's scaled to the largest maximum. Four

@@ -10,6 +10,7 @@
 // the page numbers of a tile are asked for a tile ahead. Elements of 8 bits pass through registers, where they
 // become keys and values of the element type.
 #include <float.h>
+#include <stdlib.h>
 
 #include <type_traits>
 
@@ -22,22 +23,29 @@
 namespace fsw {
 namespace {
 
+struct Scales {
+  const unsigned char *k, *v;
+  long long page, head, token;
+};
+__device__ __forceinline__ Scales scales_of(const PagedKv8& c) { return {c.k_scale, c.v_scale, c.scale_page, c.scale_head, c.scale_token}; }
+__device__ __forceinline__ Scales scales_of(const PagedKv&) { return {nullptr, nullptr, 0, 0, 0}; }
+
 // WHOLE: the rows of a wave's load, ROWS of them, lie in one page, whose address is wave-uniform then.
-template <class T, class CACHE, int DP, int NB, bool WHOLE>
-__global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prefix_kernel(PrefixOver<CACHE> a, Divisor by_group, Divisor by_hkv, int chunk,
+template <class T, class CACHE, int DP, int NB, int WAVES, bool WHOLE>
+__global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) void attn_prefix_kernel(PrefixOver<CACHE> a, Divisor by_group, Divisor by_hkv, int chunk,
                                                                               float lower, float limit) {
-  constexpr bool EIGHT = std::is_same<CACHE, PagedKv8>::value;
+  constexpr bool EIGHT = std::is_same<CACHE, PagedKv8>::value, STAGED = EIGHT || !WHOLE;
   constexpr int RB = DP * 2, TILE = KEYS * RB;
   constexpr int SIZE = EIGHT ? 1 : 2, PER_ROW = DP * SIZE / 16, ROWS = 64 / PER_ROW;  // 16-byte vectors of a row, rows of a wave's load
-  constexpr int VECS = KEYS / ROWS / 4;                                               // loads of keys, and of values, of a wave and tile
-  constexpr int KSTEPS = DP / 32, DB = DP / 16, KB = KEYS / 16, WM = 16 * NB, BM = 4 * WM;
+  constexpr int VECS = KEYS / ROWS / WAVES;                                           // loads of keys, and of values, of a wave and tile
+  constexpr int KSTEPS = DP / 32, DB = DP / 16, KB = KEYS / 16, WM = 16 * NB, BM = WAVES * WM;
   constexpr bool AHEAD = DP < 256 || NB == 1;
   constexpr int VBUF = AHEAD ? 2 : 1, VG = AHEAD ? 4 : 1;
   __shared__ __align__(1024) unsigned char k0s[TILE];
   __shared__ __align__(1024) unsigned char k1s[TILE];
   __shared__ __align__(1024) unsigned char v0s[TILE];
   __shared__ __align__(1024) unsigned char v1s[TILE];
-  __shared__ int odd_sums[4], bad_pages[4];
+  __shared__ int odd_sums[WAVES], bad_pages[WAVES];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 15, grp = lane >> 4;
@@ -45,6 +53,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prefix_kernel(Pre
   const int split = blockIdx.y, group = (int)by_group.d, rows = a.seqs * group;  // < 2^26
   const int begin = split * chunk, end = a.len - begin < chunk ? a.len : begin + chunk;
   const int wrow = row_tile * BM + wave * WM;
+  const Scales scales = scales_of(a.cache);
 
   u32x4 qf[NB][KSTEPS];
 #pragma unroll
@@ -62,7 +71,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prefix_kernel(Pre
 
   // Load j of a wave is rows first_row(j) .. + ROWS - 1 of a tile, PER_ROW lanes each. Lane l knows the page of the tile's key l.
   const int lrow = lane / PER_ROW, lvec = lane % PER_ROW;
-  auto first_row = [&](int j) INLINE -> int { return (j * 4 + wave) * ROWS; };
+  auto first_row = [&](int j) INLINE -> int { return (j * WAVES + wave) * ROWS; };
   int pages;
   bool bad = false;
   auto locate = [&](int at) INLINE {
@@ -71,59 +80,68 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prefix_kernel(Pre
   };
   const unsigned char* kc = (const unsigned char*)a.cache.k + kvh * a.cache.head * SIZE;
   const unsigned char* vc = (const unsigned char*)a.cache.v + kvh * a.cache.head * SIZE;
-  u32x4 kr[EIGHT ? VECS : 1], vr[EIGHT ? VECS : 1];  // a tile under way
-  unsigned marks[EIGHT ? VECS : 1];                  // its scales: keys' and values' bytes
-  // Asks for the tile at `at`, whose pages are known, and for the next one's pages. Rows behind the end are rows of the last load once more, or, in it,
-  // whatever its page holds: their scores are masked, their values replaced by zeros.
+  const int stride = (int)a.cache.token * SIZE;
+  u32x4 kr[STAGED ? VECS : 1], vr[STAGED ? VECS : 1];   // a tile under way
+  unsigned km[EIGHT ? VECS : 1], vm[EIGHT ? VECS : 1];  // its scales
+  // Asks for the tile at `at`, whose pages are known, and for the next one's pages. Rows behind the end are zeros and touch no memory.
   auto ask = [&](int at, unsigned char* kto, unsigned char* vto) INLINE {
     bad |= (unsigned)pages >= (unsigned)a.cache.pages;
-    if constexpr (!WHOLE) asm volatile("" : "+v"(pages));
 #pragma unroll
     for (int j = 0; j < VECS; ++j) {
-      const int last = WHOLE ? (end - 1) & ~(ROWS - 1) : end - 1;
-      int key = at + first_row(j) + (WHOLE ? 0 : lrow);
-      key = key < last ? key : last;
-      const int n = WHOLE ? __builtin_amdgcn_readlane(pages, key < at ? 0 : key - at) : __shfl(pages, key < at ? 0 : key - at);
-      const int place = key - a.cache.per_page.quotient(key) * a.cache.page_size;
+      const int row = first_row(j) + lrow, key = at + first_row(j) + (WHOLE ? 0 : lrow);
+      const int n = WHOLE ? __builtin_amdgcn_readlane(pages, first_row(j)) : __shfl(pages, row);
       const long long page = (unsigned)n < (unsigned)a.cache.pages ? n : 0;
+      const int known = key < end ? key : end - 1, place = known - a.cache.per_page.quotient(known) * a.cache.page_size;
       const long long where = (page * a.cache.page + place * a.cache.token) * SIZE;
-      const unsigned from = WHOLE ? (unsigned)(lrow * (int)a.cache.token * SIZE) : 0u;
-      if constexpr (EIGHT) {
-        const long long mark = kvh * a.cache.scale_head + page * a.cache.scale_page + place * a.cache.scale_token;
-        const unsigned more = WHOLE ? (unsigned)(lrow * (int)a.cache.scale_token) : 0u;
-        marks[j] = (a.cache.k_scale + mark)[more] | (a.cache.v_scale + mark)[more] << 8;
-        kr[j] = vr[j] = u32x4{0, 0, 0, 0};
-        if (lvec * 16 < a.d) {
-          kr[j] = *(const u32x4*)(kc + where + (from + lvec * 16));
-          vr[j] = *(const u32x4*)(vc + where + (from + lvec * 16));
+      const long long mark = EIGHT ? kvh * scales.head + page * scales.page + place * scales.token : 0;
+      if constexpr (WHOLE) {
+        const int real = end - key < ROWS ? end - key : ROWS, span = real > 0 ? (real - 1) * stride + a.d * SIZE : 0;
+        const auto krsrc = make_rsrc(kc + where, span), vrsrc = make_rsrc(vc + where, span);
+        if constexpr (EIGHT) {
+          const unsigned off = lvec * 16 < a.d ? (unsigned)(lrow * stride + lvec * 16) : OOB_OFFSET;
+          const int marks = real > 0 ? (real - 1) * (int)scales.token + 1 : 0;
+          km[j] = __builtin_amdgcn_raw_buffer_load_b8(make_rsrc(scales.k + mark, marks), lrow * (int)scales.token, 0, 0);
+          vm[j] = __builtin_amdgcn_raw_buffer_load_b8(make_rsrc(scales.v + mark, marks), lrow * (int)scales.token, 0, 0);
+          kr[j] = buf_load16(krsrc, off);
+          vr[j] = buf_load16(vrsrc, off);
+        } else {
+          const int kch = (lvec ^ k_swizzle<DP>(row)) * 8, vch = (lvec ^ v_swizzle<DP>(row)) * 8;
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(krsrc, (lds_void*)(kto + (j * WAVES + wave) * 1024), 16,
+                                                   (int)(kch < a.d ? (unsigned)(lrow * stride + kch * 2) : OOB_OFFSET), 0, 0, 0);
+          __builtin_amdgcn_raw_ptr_buffer_load_lds(vrsrc, (lds_void*)(vto + (j * WAVES + wave) * 1024), 16,
+                                                   (int)(vch < a.d ? (unsigned)(lrow * stride + vch * 2) : OOB_OFFSET), 0, 0, 0);
         }
       } else {
-        const int row = first_row(j) + lrow, kch = (lvec ^ k_swizzle<DP>(row)) * 8, vch = (lvec ^ v_swizzle<DP>(row)) * 8;
-        // (channels that the head has not: their places hold zeros from the beginning)
-        if (kch < a.d)
-          __builtin_amdgcn_global_load_lds((const global_void*)(kc + where + (from + kch * 2)), (lds_void*)(kto + (j * 4 + wave) * 1024), 16, 0, 0);
-        if (vch < a.d)
-          __builtin_amdgcn_global_load_lds((const global_void*)(vc + where + (from + vch * 2)), (lds_void*)(vto + (j * 4 + wave) * 1024), 16, 0, 0);
+        kr[j] = vr[j] = u32x4{0, 0, 0, 0};
+        if (key < end && lvec * (16 / SIZE) < a.d) {
+          kr[j] = *(const u32x4*)(kc + where + lvec * 16);
+          vr[j] = *(const u32x4*)(vc + where + lvec * 16);
+        }
+        if constexpr (EIGHT) km[j] = key < end ? scales.k[mark] : 127, vm[j] = key < end ? scales.v[mark] : 127;
       }
     }
     locate(at + KEYS);
   };
-  // 8 bits: the tile at `at`, that was asked for, as the element type
-  auto put = [&](int at, unsigned char* kto, unsigned char* vto) INLINE {
-    if constexpr (EIGHT) {
+  // what passes through registers: the tile that was asked for, as the element type
+  auto put = [&](unsigned char* kto, unsigned char* vto) INLINE {
+    if constexpr (STAGED) {
 #pragma unroll
       for (int j = 0; j < VECS; ++j) {
         const int row = first_row(j) + lrow;
-        auto store = [&](u32x4 x, float up, unsigned char* to, int swizzle) INLINE {
+        auto store = [&](u32x4 x, unsigned byte, unsigned char* to, int swizzle) INLINE {
+          if constexpr (EIGHT) {
+            const float up = __builtin_bit_cast(float, byte << 23);
 #pragma unroll
-          for (int i = 0; i < 2; ++i)
-            *(u32x4*)(to + row * RB + ((2 * lvec + i) ^ swizzle) * 16) =
-                u32x4{value_of<T, false>(x[2 * i], up), value_of<T, true>(x[2 * i], up), value_of<T, false>(x[2 * i + 1], up),
-                      value_of<T, true>(x[2 * i + 1], up)};
+            for (int i = 0; i < 2; ++i)
+              *(u32x4*)(to + row * RB + ((2 * lvec + i) ^ swizzle) * 16) =
+                  u32x4{widen<T, false>(x[2 * i], up), widen<T, true>(x[2 * i], up), widen<T, false>(x[2 * i + 1], up),
+                        widen<T, true>(x[2 * i + 1], up)};
+          } else {
+            *(u32x4*)(to + row * RB + (lvec ^ swizzle) * 16) = x;
+          }
         };
-        if (at + row >= end) vr[j] = u32x4{0, 0, 0, 0}, marks[j] = 127u << 8;
-        store(kr[j], scale_value(marks[j] & 255u), kto, k_swizzle<DP>(row));
-        store(vr[j], scale_value(marks[j] >> 8), vto, v_swizzle<DP>(row));
+        store(kr[j], EIGHT ? km[j] : 0, kto, k_swizzle<DP>(row));
+        store(vr[j], EIGHT ? vm[j] : 0, vto, v_swizzle<DP>(row));
       }
     }
   };
@@ -229,7 +247,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prefix_kernel(Pre
   // of them), and what their weighted sum is, the same for every row since every row sees every key, is written over the sums below.
   auto silence = [&](unsigned char* vs) INLINE {
 #pragma unroll 1
-    for (int byte = tid * 16; byte < TILE; byte += 4096) {
+    for (int byte = tid * 16; byte < TILE; byte += 1024 * WAVES) {
       u32x4 x = *(u32x4*)(vs + byte);
 #pragma unroll
       for (int j = 0; j < 4; ++j) x[j] = finite2<T>(x[j]);
@@ -237,29 +255,15 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prefix_kernel(Pre
     }
     __syncthreads();
   };
-  // values of rows behind the end
-  auto clear = [&](int at, unsigned char* vs) INLINE {
-#pragma unroll 1
-    for (int byte = (end - at) * RB + tid * 16; byte < TILE; byte += 4096) *(u32x4*)(vs + byte) = u32x4{0, 0, 0, 0};
-    __syncthreads();
-  };
   bool again = false;
   // Tile t is in buffer t % 2. At the barrier the tile has landed, and every wave has read the one before.
   auto turn = [&](int at, const unsigned char* ks, unsigned char* vs, unsigned char* knext, unsigned char* vnext) INLINE {
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
     ask(at + KEYS, knext, vnext);
-    if (!EIGHT && at + KEYS > end) clear(at, vs);
     if (__builtin_expect(again, 0)) silence(vs);
     attend(at, ks, vs);
-    put(at + KEYS, knext, vnext);
+    put(knext, vnext);
   };
-  if (!EIGHT && a.d < DP) {
-    for (int byte = tid * 16; byte < TILE; byte += 4096) {
-      const u32x4 zero = {0, 0, 0, 0};
-      *(u32x4*)(k0s + byte) = zero, *(u32x4*)(k1s + byte) = zero, *(u32x4*)(v0s + byte) = zero, *(u32x4*)(v1s + byte) = zero;
-    }
-    __syncthreads();
-  }
   while (true) {
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
@@ -270,7 +274,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prefix_kernel(Pre
     }
     locate(begin);
     ask(begin, k0s, v0s);
-    put(begin, k0s, v0s);
+    put(k0s, v0s);
     for (int at = begin; at < end; at += 2 * KEYS) {
       turn(at, k0s, v0s, k1s, v1s);
       if (at + KEYS >= end) break;
@@ -287,11 +291,15 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prefix_kernel(Pre
     if (lane == 0) odd_sums[wave] = odd, bad_pages[wave] = wrong;
     // also: every wave has read the last tile when the LDS is filled again
     asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (again || __builtin_expect(!(odd_sums[0] | odd_sums[1] | odd_sums[2] | odd_sums[3]), 1)) break;
+    int any = 0;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) any |= odd_sums[w];
+    if (again || __builtin_expect(!any, 1)) break;
     again = true;
     __syncthreads();  // every wave has read them
   }
-  bad = bad_pages[0] | bad_pages[1] | bad_pages[2] | bad_pages[3];
+#pragma unroll
+  for (int w = 0; w < WAVES; ++w) bad |= bad_pages[w] != 0;
 
   float* ml = a.partial + (long long)a.seqs * a.hq * a.slots * a.d;
   auto out_row = [&](int row) INLINE -> long long {
@@ -325,8 +333,8 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prefix_kernel(Pre
       const long long at = (unsigned)n < (unsigned)a.cache.pages ? n : 0;
       if constexpr (EIGHT) {
         const unsigned code = vc[at * a.cache.page + place * a.cache.token + ch];
-        const long long mark = kvh * a.cache.scale_head + at * a.cache.scale_page + place * a.cache.scale_token;
-        seen.add((unsigned short)value_of<T, false>(code, scale_value(a.cache.v_scale[mark])));
+        const unsigned byte = scales.v[kvh * scales.head + at * scales.page + place * scales.token];
+        seen.add((unsigned short)widen<T, false>(code, __builtin_bit_cast(float, byte << 23)));
       } else {
         seen.add(((const unsigned short*)vc)[at * a.cache.page + place * a.cache.token + ch]);
       }
@@ -337,22 +345,25 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prefix_kernel(Pre
   }
 }
 
-template <class T, class CACHE, int DP, int NB, bool WHOLE>
+template <class T, class CACHE, int DP, int NB, int WAVES, bool WHOLE>
 hipError_t launch(const PrefixOver<CACHE>& a, const PrefixPlan& p, hipStream_t stream) {
   const int group = a.hq / a.hkv;
   const float shift = shift_of<T>(a.keys);
   const float lower = fmaxf(shift / a.scale_log2, -FLT_MAX / 4), limit = fmaxf((shift + SLACK<T>) / a.scale_log2, -FLT_MAX / 4);
-  const dim3 grid(a.hkv * ((a.seqs * group + 64 * NB - 1) / (64 * NB)), p.splits);
-  attn_prefix_kernel<T, CACHE, DP, NB, WHOLE><<<grid, 256, 0, stream>>>(a, Divisor(group), Divisor(a.hkv), p.chunk, lower, limit);
+  constexpr int BM = 16 * NB * WAVES;
+  const dim3 grid(a.hkv * ((a.seqs * group + BM - 1) / BM), p.splits);
+  attn_prefix_kernel<T, CACHE, DP, NB, WAVES, WHOLE><<<grid, 64 * WAVES, 0, stream>>>(a, Divisor(group), Divisor(a.hkv), p.chunk, lower, limit);
   return hipGetLastError();
 }
 
 template <class T, class CACHE, int DP>
 hipError_t launch_dp(const PrefixOver<CACHE>& a, const PrefixPlan& p, hipStream_t stream) {
   constexpr int ROWS = 1024 / (DP * (std::is_same<CACHE, PagedKv8>::value ? 1 : 2));
-  if (a.cache.page_size % ROWS != 0)
-    return p.rows == 64 ? launch<T, CACHE, DP, 1, false>(a, p, stream) : launch<T, CACHE, DP, 2, false>(a, p, stream);
-  return p.rows == 64 ? launch<T, CACHE, DP, 1, true>(a, p, stream) : launch<T, CACHE, DP, 2, true>(a, p, stream);
+  if (a.cache.page_size % ROWS) return launch<T, CACHE, DP, 1, 4, false>(a, p, stream);
+  if constexpr (DP > 64) {
+    if (p.rows == 256) return launch<T, CACHE, DP, 2, 8, true>(a, p, stream);
+  }
+  return p.rows == 128 ? launch<T, CACHE, DP, 2, 4, true>(a, p, stream) : launch<T, CACHE, DP, 1, 4, true>(a, p, stream);
 }
 
 template <class T, class CACHE>
@@ -367,10 +378,12 @@ hipError_t launch_typed(const PrefixOver<CACHE>& a, const PrefixPlan& p, hipStre
 PrefixPlan prefix_plan(int seqs, int hq, int hkv, int d, int len) {
   PrefixPlan p;
   const long long rows = (long long)seqs * (hq / hkv);
-  p.rows = rows > 64 ? 128 : 64;
+  p.rows = rows > 128 && d > 64 ? 256 : rows > 64 ? 128 : 64;
+  if (getenv("X_ROWS")) p.rows = atoi(getenv("X_ROWS"));
   const long long items = hkv * ((rows + p.rows - 1) / p.rows), tiles = (len + KEYS - 1) / KEYS;
   long long splits = (512 + items - 1) / items;
   if (splits > (tiles + 3) / 4) splits = (tiles + 3) / 4;
+  if (getenv("X_SPLITS")) splits = atoi(getenv("X_SPLITS"));
   if (splits < 1) splits = 1;
   p.chunk = (int)((tiles + splits - 1) / splits) * KEYS;
   p.splits = (len + p.chunk - 1) / p.chunk;
