@@ -123,6 +123,8 @@ struct PagedAttnPlan {
 };
 // turn: keys of a wave at a time, 16 or 32
 PagedAttnPlan paged_attn_plan(int seqs, int hq, int hkv, int d, int max_len, int turn);
+// of the keys behind a shared prefix, whose shares are joined anyway
+PagedAttnPlan paged_attn_tail_plan(int seqs, int hq, int hkv, int max_len, int turn);
 // The sums of a share, a row per (sequence, query head, share): d floats each, behind all rows the maximum and sum of each.
 inline size_t partial_bytes(long long rows, int d) { return (size_t)rows * (size_t)(d + 2) * 4; }
 hipError_t launch_attn_decode(int dtype, const PagedAttnArgs& a, const PagedAttnPlan& p, void* workspace, hipStream_t stream);

@@ -147,7 +147,8 @@ SharedPlan shared_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t pr
   SharedPlan p;
   p.prefix = fsw::PrefixPlan{0, 0, 0};
   if (prefix_len > 0) p.prefix = fsw::prefix_plan((int)B, (int)Hq, (int)Hkv, (int)D, (int)prefix_len);
-  p.own = fsw::paged_attn_plan((int)B, (int)Hq, (int)Hkv, (int)D, (int)max_len, turn);
+  p.own = prefix_len > 0 ? fsw::paged_attn_tail_plan((int)B, (int)Hq, (int)Hkv, (int)max_len, turn)
+                         : fsw::paged_attn_plan((int)B, (int)Hq, (int)Hkv, (int)D, (int)max_len, turn);
   p.slots = p.prefix.splits + p.own.splits;
   p.bytes = prefix_len > 0 ? fsw::partial_bytes(B * Hq * p.slots, (int)D) : p.own.workspace_bytes;
   return p;

@@ -476,6 +476,21 @@ PagedAttnPlan paged_attn_plan(int seqs, int hq, int hkv, int d, int max_len, int
   return p;
 }
 
+// Four waves; shares of 128 keys while there are few, since a join follows in any case, but not many more workgroups than 4096, since empty ones are not
+// free. us, shares of 128 | 256 | 512 | 1024 keys: 512 items of 1 .. 900 keys of 16 bits 16.5 | 18.4 | 27 | 39; 1600 items of 1 .. 1500 keys of 8 bits 47 | 35 | 33 | 38.
+PagedAttnPlan paged_attn_tail_plan(int seqs, int hq, int hkv, int max_len, int turn) {
+  const long long items = (long long)seqs * hkv * head_tiles(hq, hkv), unit = 4 * turn;
+  const long long wanted = (4096 + items - 1) / items, most = (max_len + 127) / 128;
+  const long long splits = most < 1 ? 1 : wanted < most ? wanted : most;
+  PagedAttnPlan p;
+  p.waves = 4;
+  const long long chunk = ((max_len + splits - 1) / splits + unit - 1) / unit * unit;
+  p.chunk = (int)(chunk < unit ? unit : chunk);
+  p.splits = max_len > 0 ? (int)((max_len + p.chunk - 1) / p.chunk) : 1;
+  p.workspace_bytes = 0;
+  return p;
+}
+
 hipError_t launch_attn_join(int dtype, const JoinArgs& a, int chunk, int splits, const float* partial, hipStream_t stream) {
   return dtype == FSW_BF16 ? launch_join<Bf16>(a, chunk, splits, partial, stream) : launch_join<Fp16>(a, chunk, splits, partial, stream);
 }

@@ -10,7 +10,6 @@
 // the page numbers of a tile are asked for a tile ahead. Elements of 8 bits pass through registers, where they
 // become keys and values of the element type.
 #include <float.h>
-#include <stdlib.h>
 
 #include <type_traits>
 
@@ -375,19 +374,29 @@ hipError_t launch_typed(const PrefixOver<CACHE>& a, const PrefixPlan& p, hipStre
 
 }  // namespace
 
+// Rows of a workgroup, and shares of the keys. A turn of 64 keys takes 2.7 us with 256 rows on a CU (eight waves), 3.0 with two workgroups of 128 rows, 2.2
+// with one of them; a workgroup's first keys and its sums take about two turns more. Each share costs its sums' way to memory and back, in the join. The plan of least
+// estimated time: more shares fill the card's last round better, and are more to join. us of the whole call, 64 sequences of 32 heads on 8 (256 rows a head) behind
+// 16384 keys in 16, 24, 32, 64 shares: 59, 60, 56, 72 with 256 rows, 58, 58, 56, 73 with 128; 200 sequences of 64 heads on 8 (1600 rows) behind 8000 keys of 8 bits in
+// 2, 3, 4, 5, 8 shares 180, 140, 121, 145, 138 with 256 rows, 155, 151, 131, 146, 139 with 128.
 PrefixPlan prefix_plan(int seqs, int hq, int hkv, int d, int len) {
-  PrefixPlan p;
-  const long long rows = (long long)seqs * (hq / hkv);
-  p.rows = rows > 128 && d > 64 ? 256 : rows > 64 ? 128 : 64;
-  if (getenv("X_ROWS")) p.rows = atoi(getenv("X_ROWS"));
-  const long long items = hkv * ((rows + p.rows - 1) / p.rows), tiles = (len + KEYS - 1) / KEYS;
-  long long splits = (512 + items - 1) / items;
-  if (splits > (tiles + 3) / 4) splits = (tiles + 3) / 4;
-  if (getenv("X_SPLITS")) splits = atoi(getenv("X_SPLITS"));
-  if (splits < 1) splits = 1;
-  p.chunk = (int)((tiles + splits - 1) / splits) * KEYS;
-  p.splits = (len + p.chunk - 1) / p.chunk;
-  return p;
+  const long long rows = (long long)seqs * (hq / hkv), tiles = (len + KEYS - 1) / KEYS;
+  const double join = 2.0 * (double)seqs * hq * d * 4 / 4e6;  // us a share, written and read
+  PrefixPlan best = {0, 0, 0};
+  double least = 0.0;
+  for (const int size : {64, 128, 256}) {
+    if (size == 256 && d <= 64) continue;  // (tiles too small for eight waves' copies)
+    if (size == 64 && rows > 64) continue;
+    const long long items = hkv * ((rows + size - 1) / size), resident = 256 * (size == 256 || d > 128 ? 1 : 2);
+    const long long most = tiles < 64 ? tiles : 64;
+    for (long long splits = 1; splits <= most; ++splits) {
+      const long long per = (tiles + splits - 1) / splits, work = items * ((tiles + per - 1) / per);
+      const double turn = size == 256 ? 2.7 : work <= 256 ? 2.2 : 3.0;
+      const double us = (double)((work + resident - 1) / resident) * (double)(per + 2) * turn + join * (double)splits;
+      if (best.rows == 0 || us < least * (size > best.rows ? 0.95 : 1.0)) least = us, best = {(int)((tiles + per - 1) / per), (int)(per * KEYS), size};
+    }
+  }
+  return best;
 }
 
 hipError_t launch_attn_prefix(int dtype, const PrefixOver<PagedKv>& a, const PrefixPlan& p, hipStream_t stream) {
