@@ -326,7 +326,8 @@ FSW_API int fsw_kv_read8(int dtype, int64_t T, int64_t B, int64_t Hkv, int64_t D
                          int64_t table_ld, int64_t width, const int32_t* cu, void* Kout, int64_t ko_token, int64_t ko_head, void* Vout,
                          int64_t vo_token, int64_t vo_head, void* stream);
 
-/* fsw_attn_decode over a cache in 8 bits: the same checks, scratch rules and answers to invalid sequences. A row whose scale is 255 is NaN. */
+/* fsw_attn_decode over a cache in 8 bits: the same checks, scratch rules and answers to invalid sequences. A row whose scale is 255 is NaN. Keys are
+ * taken rounded to the queries' type. Values below 2^-100 lose bits (their weights times their scales are held in numbers from 2^-133 on). */
 FSW_API int fsw_validate_attn_decode8(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, const void* Q, int64_t q_seq,
                                       int64_t q_head, const fsw_kv_cache8* cache, const int32_t* block_table, int64_t table_ld,
                                       const int32_t* lengths, int64_t max_len, float scale, const void* O, int64_t o_seq,

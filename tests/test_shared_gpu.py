@@ -1,0 +1,297 @@
+"""Attention of single tokens over a prefix that a batch shares and their own keys, on the device, against the float64 restatement of
+attention over both together (oracle/attention.py): both caches, all forms of the kernels, edges, invalid input, graphs."""
+import pytest
+import torch
+
+from oracle import attention
+from test_attention_gpu import BF, DEV, HF, NAN, angles, inside, int32, randn, untouched
+from test_cache8_gpu import codes_of, paged8, rows_of
+
+pytestmark = pytest.mark.gpu
+INF = float("inf")
+
+
+def setup(gen, prefix, lengths, Hkv, D, page, dtype, bits, **kw):
+    """-> (cache on the device, its rows in float64, table, prefix pages). 16 bits: elements of the type, NaN where no key lies."""
+    cache, table, pages = paged8(gen, lengths, Hkv, D, page, dtype, prefix=prefix, **kw)
+    rows = rows_of(cache)
+    if bits == 16:
+        cache = [r.to(dtype).to(DEV) for r in rows]
+    return cache, rows, table, pages
+
+
+def reference(q, rows, pages, prefix, table, lengths, page, scale):
+    """Every sequence's pages, the prefix's and its own, as one list of cells."""
+    o, mag = torch.zeros(q.shape, dtype=torch.float64), torch.zeros(q.shape, dtype=torch.float64)
+    group = q.shape[1] // rows[0].shape[1]
+    first = [torch.stack([r[int(pages[j // page]), :, j % page] for j in range(prefix)]) if prefix else r[0, :, 0][None][:0] for r in rows]
+    for b, n in enumerate(lengths):
+        k, v = (torch.cat([f] + [r[int(table[b, j // page]), :, j % page][None] for j in range(n)]) for f, r in zip(first, rows))
+        for h in range(q.shape[1]):
+            o[b, h:h + 1], mag[b, h:h + 1] = attention.attend(q[b, h:h + 1], k[:, h // group], v[:, h // group], scale, [prefix + n])
+    return o, mag
+
+
+def widened(table, most, page):
+    width = -(-most // page)
+    return torch.cat([table, table[:, -1:].expand(-1, max(0, width - table.shape[1]))], 1)
+
+
+def check(capi, gen, prefix, lengths, Hq, Hkv, D, page, dtype, bits, max_len=None, q_scale=1.5, **kw):
+    cache, rows, table, pages = setup(gen, prefix, lengths, Hkv, D, page, dtype, bits, **kw)
+    B, most, scale = len(lengths), max_len if max_len is not None else max(lengths), D ** -0.5
+    table = widened(table, most, page)
+    q = randn(gen, B, Hq, D, dtype=dtype, scale=q_scale)
+    out, wide = inside(torch.zeros(B, Hq, D, dtype=dtype))
+    q_dev = inside(q)[0]
+    capi.attn_shared(q_dev, cache, pages.to(DEV), prefix, table.to(DEV), int32(lengths), most, scale, out=out)
+    ref, mag = reference(q, rows, pages, prefix, table, lengths, page, scale)
+    err, tol = (out.cpu().double() - ref).abs(), attention.tolerance(ref, mag, dtype, True, prefix + most)
+    assert (err <= tol).all(), (err - tol).max().item()
+    assert untouched(wide, out.shape)
+    return q_dev, cache, pages.to(DEV), table.to(DEV), most, scale
+
+
+@pytest.mark.parametrize("prefix", [1, 63, 64, 65, 130])
+@pytest.mark.parametrize("Hq,Hkv,D,page", [(4, 2, 64, 16), (8, 2, 128, 16), (3, 1, 80, 24), (5, 5, 128, 3), (6, 2, 96, 8), (2, 1, 256, 4)])
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_shared(capi, prefix, Hq, Hkv, D, page, bits, dtype):
+    """64 rows a workgroup. Lengths of own keys from none; pages that end inside a tile and pages of any size."""
+    gen = torch.Generator().manual_seed(prefix * 7 + D)
+    check(capi, gen, prefix, [1, 0, 17, 33, 5], Hq, Hkv, D, page, dtype, bits)
+
+
+@pytest.mark.parametrize("B,Hq,Hkv,D,page,prefix", [
+    (17, 5, 1, 128, 16, 200),      # 85 rows: 128 a workgroup, three waves with rows
+    (33, 8, 2, 64, 8, 333),        # 132 rows of 64 channels: two of them
+    (40, 8, 1, 128, 32, 500),      # 320 rows: 256 a workgroup, or 128
+    (70, 4, 1, 112, 64, 129),
+    (20, 16, 1, 256, 16, 190),     # 256 channels
+    (9, 16, 1, 256, 2, 70),
+    (40, 8, 1, 128, 5, 300)])      # pages that a load's rows do not fit
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_shared_by_many_rows(capi, B, Hq, Hkv, D, page, prefix, bits, dtype):
+    gen = torch.Generator().manual_seed(B + D)
+    check(capi, gen, prefix, [(7 * b) % 40 for b in range(B)], Hq, Hkv, D, page, dtype, bits)
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("prefix,lengths,max_len", [(4000, [3, 0], 2000), (2500, [700, 1, 130], None), (70, [0, 0, 0], 0), (300, [1], 1)])
+def test_shared_in_many_shares(capi, prefix, lengths, max_len, bits):
+    """Long prefixes of few rows, own keys in several shares, none at all."""
+    gen = torch.Generator().manual_seed(prefix)
+    check(capi, gen, prefix, lengths, 4, 2, 128, 16, BF, bits, max_len)
+    check(capi, gen, prefix, lengths, 2, 1, 64, 24, HF, bits, max_len)
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+def test_without_a_prefix_it_is_the_decode(capi, bits):
+    gen = torch.Generator().manual_seed(4)
+    cache, _, table, pages = setup(gen, 0, [40, 0, 700], 2, 64, 16, BF, bits)
+    q = randn(gen, 3, 4, 64).to(DEV)
+    args = (table.to(DEV), int32([40, 0, 700]), 700, 0.125)
+    want = capi.attn_decode8(q, cache, *args) if bits == 8 else capi.attn_decode(q, *cache, *args)
+    assert torch.equal(capi.attn_shared(q, cache, pages.to(DEV), 0, *args), want)
+
+
+@pytest.mark.parametrize("page", [16, 5])
+@pytest.mark.parametrize("bits", [8, 16])
+def test_what_lies_in_no_page_is_nan(capi, bits, page):
+    gen = torch.Generator().manual_seed(6)
+    prefix, lengths = 150, [20, 33, 40, 7]
+    q, cache, pages, table, most, scale = check(capi, gen, prefix, lengths, 4, 2, 64, page, BF, bits, max_len=60)
+    args = (int32(lengths), most, scale)
+    good = capi.attn_shared(q, cache, pages, prefix, table, *args)
+    bad = table.clone()
+    bad[1, 0], bad[2, 1] = -1, cache[0].shape[0]
+    out = capi.attn_shared(q, cache, pages, prefix, bad, int32([20, 33, 40, most + 1]), most, scale)
+    assert torch.equal(out[0], good[0]) and torch.isnan(out[1:]).all()
+    out = capi.attn_shared(q, cache, pages, prefix, table, int32([20, -1, 40, 7]), most, scale)
+    assert torch.equal(out[[0, 2, 3]], good[[0, 2, 3]]) and torch.isnan(out[1]).all()
+    wrong = torch.cat([pages, int32([1 << 30])])
+    assert torch.equal(capi.attn_shared(q, cache, wrong, prefix, table, *args), good)          # behind the prefix's pages
+    wrong[-(-prefix // page) - 1] = 1 << 30
+    assert torch.isnan(capi.attn_shared(q, cache, wrong, prefix, table, *args)).all()
+    wrong[-(-prefix // page) - 1], wrong[0] = pages[-1], -1
+    assert torch.isnan(capi.attn_shared(q, cache, wrong, prefix, table, *args)).all()
+
+
+@pytest.mark.parametrize("B,Hq,Hkv,D,page,prefix", [(3, 4, 2, 64, 16, 100), (40, 8, 1, 128, 32, 500), (17, 5, 1, 128, 16, 3000), (3, 2, 2, 96, 5, 100),
+                                                    (5, 2, 1, 256, 64, 70)])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_infinities_in_a_prefix(capi, B, Hq, Hkv, D, page, prefix, dtype):
+    """What the weighted sum gives, in every sequence: the infinity, NaN where both signs or a NaN are among the values."""
+    gen = torch.Generator().manual_seed(D + prefix)
+    lengths = [(5 * b) % 30 for b in range(B)]
+    cache, rows, table, pages = setup(gen, prefix, lengths, Hkv, D, page, dtype, 16)
+    for key, channel, value in ((prefix // 2, 3, INF), (prefix - 1, 4, -INF), (0, 5, NAN), (prefix // 3, 6, INF), (prefix - 2, 6, -INF),
+                                (1, D - 1, INF), (prefix - 3, D - 1, INF)):
+        rows[1][int(pages[key // page]), 0, key % page, channel] = value
+    cache = [r.to(dtype).to(DEV) for r in rows]
+    q = randn(gen, B, Hq, D, dtype=dtype)
+    out = capi.attn_shared(q.to(DEV), cache, pages.to(DEV), prefix, table.to(DEV), int32(lengths), max(lengths), D ** -0.5).cpu().double()
+    ref, mag = reference(q, rows, pages, prefix, table, lengths, page, D ** -0.5)
+    finite = torch.isfinite(ref)
+    assert ((out - ref).abs() <= attention.tolerance(ref, mag, dtype, True, prefix + 30))[finite].all()
+    assert torch.equal(out[~finite].nan_to_num(7.0, INF, -INF), ref[~finite].nan_to_num(7.0, INF, -INF)) and not finite[:, 0, 3].any()
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+def test_one_side_outweighs_the_other(capi, bits):
+    """Scores of the prefix far above or below the own keys': the join keeps what weighs."""
+    gen = torch.Generator().manual_seed(8)
+    for q_scale in (0.0, 60.0):
+        check(capi, gen, 200, [1, 40, 90], 4, 2, 128, 16, BF, bits, q_scale=q_scale)
+        check(capi, gen, 200, [1, 40, 90], 4, 2, 128, 16, HF, bits, q_scale=q_scale)
+
+
+@pytest.mark.parametrize("dtype,size", [(BF, 3.0e38), (HF, 65504.0)])
+def test_values_as_large_as_the_type_has(capi, dtype, size):
+    gen = torch.Generator().manual_seed(9)
+    prefix, lengths = 700, [100, 3]
+    cache, rows, table, pages = setup(gen, prefix, lengths, 1, 64, 16, dtype, 16)
+    rows = (rows[0], torch.where(torch.isnan(rows[1]), rows[1], torch.full_like(rows[1], size)))
+    cache = [r.to(dtype).to(DEV) for r in rows]
+    q = randn(gen, 2, 4, 64, dtype=dtype)
+    out = capi.attn_shared(q.to(DEV), cache, pages.to(DEV), prefix, table.to(DEV), int32(lengths), 100, 0.125).cpu().double()
+    assert torch.isfinite(out).all() and ((out - size).abs() <= 2.0 ** -6 * size).all()
+
+
+def test_workspace_and_refusals(capi):
+    gen = torch.Generator().manual_seed(1)
+    cache, _, table, pages = setup(gen, 100, [5, 7], 2, 64, 16, BF, 8)
+    q, pages, table, lengths = randn(gen, 2, 4, 64).to(DEV), pages.to(DEV), table.to(DEV), int32([5, 7])
+    need = capi.lib().fsw_attn_shared8_workspace_bytes(0, 2, 4, 2, 64, 100, 7)
+    want = capi.attn_shared(q, cache, pages, 100, table, lengths, 7, 0.125)
+    # room for no more than it asks for, uninitialised
+    wide = torch.full((need + 64,), 255, dtype=torch.uint8, device=DEV)
+    assert torch.equal(capi.attn_shared(q, cache, pages, 100, table, lengths, 7, 0.125, workspace=wide[:need]), want)
+    assert (wide[need:] == 255).all()
+    for bad, code in ((dict(workspace=wide[:need - 16]), capi.E_WORKSPACE), (dict(out=torch.empty(2, 4, 32, dtype=BF, device=DEV)), capi.E_SHAPE)):
+        with pytest.raises(capi.FswError) as e:
+            capi.attn_shared(q, cache, pages, 100, table, lengths, 7, 0.125, **bad)
+        assert e.value.code == code
+    for args in ((pages, 113), (pages[:1], 17)):
+        with pytest.raises(capi.FswError) as e:
+            capi.attn_shared(q, cache, *args, table, lengths, 7, 0.125)
+        assert e.value.code == capi.E_LD
+    with pytest.raises(capi.FswError) as e:
+        capi.attn_shared(q, [cache[0].view(torch.uint8), *cache[1:]], pages, 100, table, lengths, 7, 0.125)
+    assert e.value.code == capi.E_DTYPE
+    with pytest.raises(capi.FswError) as e:
+        capi.attn_shared(q, [*cache[:3], cache[3][:, :1]], pages, 100, table, lengths, 7, 0.125)
+    assert e.value.code == capi.E_SHAPE
+
+
+# ---------------------------------------------------------------------------------------------- together
+
+@pytest.mark.parametrize("dtype,name", [(BF, "bf16"), (HF, "fp16")])
+def test_torch_operators_equal_the_c_entry_points(capi, ext, dtype, name):
+    gen = torch.Generator().manual_seed(21)
+    op = lambda n: getattr(ext, "%s_%s" % (n, name))  # noqa: E731
+    ops = lambda n: getattr(torch.ops.ASMLLM, "%s_%s" % (n, name))  # noqa: E731
+    q, k, v = (randn(gen, 50, h, 64, dtype=dtype).to(DEV) for h in (4, 2, 2))
+    table, at = angles(gen, 50, 64).to(DEV), int32(list(range(50)))
+    a, b = (paged8(gen, [64], 2, 64, 16, dtype)[0] for _ in range(2))
+    for x, y in zip(a, b):
+        y.view(torch.uint8).copy_(x.view(torch.uint8))
+    got = op("kv_append8")(q, k, v, table, at, at, *a, interleaved=True)
+    want = capi.kv_append8(q, k, v, table, at, at, b, True)
+    assert all(torch.equal(x, y) for x, y in zip(got, want)) and all(torch.equal(x, y) for x, y in zip(codes_of(a), codes_of(b)))
+    assert all(torch.equal(x, y) for x, y in zip(ops("kv_append8")(q, k, v, table, at, at, *b, True), want))
+    pages, lengths, cu = int32([[0, 1, 2, 3], [3, 2, 1, 0]]), int32([50, 3]), int32([0, 20, 23])
+    sixteen = [torch.randn(4, 2, 16, 64, generator=gen).to(dtype).to(DEV) for _ in range(2)]
+    for cache, s in ((a, "8"), (sixteen, "")):
+        for f in (op, ops):
+            got = f("kv_read" + s)(*cache, pages, cu, 25)
+            assert all(torch.equal(x, y) for x, y in zip(got, capi.kv_read(cache, pages, cu, 25, dtype)))
+            got = f("attn_shared" + s)(q[:2], *cache, int32([2, 0]), 19, pages, lengths, 50, 0.125)
+            assert torch.equal(got, capi.attn_shared(q[:2], cache, int32([2, 0]), 19, pages, lengths, 50, 0.125))
+    for f in (op, ops):
+        assert torch.equal(f("attn_decode8")(q[:2], *a, pages, lengths, 50, 0.125), capi.attn_decode8(q[:2], a, pages, lengths, 50, 0.125))
+    empty = q[:0]
+    assert op("attn_decode8")(empty, *a, pages[:0], lengths[:0], 50, 0.125).shape == (0, 4, 64)
+    assert op("attn_shared8")(empty, *a, int32([2, 0]), 19, pages[:0], lengths[:0], 50, 0.125).shape == (0, 4, 64)
+    assert op("kv_append8")(empty, k[:0], v[:0], table, at[:0], at[:0], *a)[2].shape == (0, 2, 64)
+    other = ext.attn_decode8_bf16 if dtype == HF else ext.attn_decode8_fp16
+    with pytest.raises(RuntimeError, match="type"):
+        other(q[:2], *a, pages, lengths, 50, 0.125)
+    with pytest.raises(RuntimeError, match="type"):
+        op("attn_decode8")(q[:2], *a[:2], a[2].view(torch.uint8), a[3], pages, lengths, 50, 0.125)
+
+
+@pytest.mark.parametrize("bits", [8, 16])
+def test_a_step_replays_from_a_hip_graph(ext, bits):
+    """Append, attention behind a prefix and over own keys, norm: captured once, with inputs, slots and lengths that change; two graphs of one
+    program alternate. Another stream's work goes on beside."""
+    gen = torch.Generator().manual_seed(22)
+    B, Hq, Hkv, D, page, most, prefix = 3, 8, 2, 128, 16, 300, 200
+    lens = [100, 0, 260]
+    cache, _, block, pages = setup(gen, prefix, [most] * B, Hkv, D, page, BF, bits)
+    block, pages, table = block.to(DEV), pages.to(DEV), angles(gen, prefix + most, D).to(DEV)
+    weight = randn(gen, Hq * D).to(DEV)
+
+    def make():
+        return dict(q=randn(gen, B, Hq, D).to(DEV), k=randn(gen, B, Hkv, D).to(DEV), v=randn(gen, B, Hkv, D).to(DEV),
+                    positions=int32([0] * B), lengths=int32([1] * B), slots=int32([0] * B))
+
+    def place(st, step):
+        n = [x + step for x in lens]
+        st["positions"].copy_(int32([prefix + x for x in n]))
+        st["lengths"].copy_(int32([x + 1 for x in n]))
+        st["slots"].copy_(int32([int(block[b, x // page]) * page + x % page for b, x in enumerate(n)]))
+        for name in "qkv":
+            st[name].copy_(randn(gen, *st[name].shape).to(DEV))
+
+    def run(st, caches):
+        s = "8" if bits == 8 else ""
+        qr = getattr(ext, "kv_append%s_bf16" % s)(st["q"], st["k"], st["v"], table, st["positions"], st["slots"], *caches)[0]
+        o = getattr(ext, "attn_shared%s_bf16" % s)(qr, *caches, pages, prefix, block, st["lengths"], most, D ** -0.5).view(B, -1)
+        return ext.add_norm_bf16(st["q"].view(B, -1), o, None, weight, weight, 0.5)
+
+    sts = [make(), make()]
+    for st in sts:
+        place(st, 0)
+        run(st, cache)
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for st in sts:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(run(st, cache))
+    side = torch.cuda.Stream()
+    for step in range(1, 6):
+        for st, graph, out in zip(sts, graphs, outs):
+            place(st, step)
+            copies = [c.clone() if bits == 16 else c.view(torch.uint8).clone().view(c.dtype) for c in cache]
+            eager = run(st, copies)
+            torch.cuda.synchronize()
+            for o in out:
+                o.zero_()
+            torch.cuda.synchronize()
+            with torch.cuda.stream(side):
+                busy = torch.randn(512, 512, device=DEV) @ torch.randn(512, 512, device=DEV)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(x, y) for x, y in zip(out, eager)), "replay %d" % step
+            assert all(torch.equal(x, y) for x, y in zip(codes_of(cache), codes_of(copies)))
+            del busy
+
+
+def test_calls_on_other_streams_at_once(capi):
+    """Scratch is each call's own: two streams' calls give what they give one after the other."""
+    gen = torch.Generator().manual_seed(30)
+    cache, _, table, pages = setup(gen, 2000, [40, 300], 2, 128, 16, BF, 16)
+    pages, table, lengths = pages.to(DEV), table.to(DEV), int32([40, 300])
+    qs = [randn(gen, 2, 8, 128).to(DEV) for _ in range(6)]
+    want = [capi.attn_shared(q, cache, pages, 2000, table, lengths, 300, 0.1) for q in qs]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for i, q in enumerate(qs):
+        with torch.cuda.stream(streams[i % 2]):
+            got.append(capi.attn_shared(q, cache, pages, 2000, table, lengths, 300, 0.1))
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(got, want))
