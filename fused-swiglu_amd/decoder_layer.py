@@ -7,6 +7,10 @@
 The projections are `swiglu_down_*` (a row-major product with a [out, in] weight), the MLP is `fused_swiglu_mlp_*`; the norm is
 elementary torch. Random weights. `python decoder_layer.py` runs a batch of prompts, then decodes some tokens of each, and
 compares the decoded tokens' outputs with those of the whole sequences taken as prompts.
+
+`--eight`: the cache holds e4m3 elements (`kv_append8_*`, `attn_decode8_*`). `--prefix N`: all sequences begin with the same N tokens, which are
+taken once and attended to together (`attn_shared_*`). `--turns N`: prompts come in N parts, each of which attends to what the cache holds of
+the ones before (`kv_read_*`). `--sandwich`: norms with weights before and after both blocks, gates and a residual scale (`add_norm_*`).
 """
 import argparse
 import math
@@ -21,15 +25,29 @@ class PagedCache:
     """Keys and values of one layer in pages of `page` tokens, and which pages each sequence has. Pages are handed out as
     tokens arrive; the table and the lengths are kept on the device, where the kernels read them."""
 
-    def __init__(self, seqs, longest, kv_heads, channels, page, dtype, device):
-        per_seq = -(-longest // page)
-        self.page, self.longest, self.device = page, longest, device
-        self.k = torch.empty(seqs * per_seq, kv_heads, page, channels, dtype=dtype, device=device)
+    def __init__(self, seqs, longest, kv_heads, channels, page, dtype, device, eight=False, prefix=0):
+        """eight: e4m3 elements and their rows' scales. prefix: tokens that all sequences begin with, whole pages; longest, lengths and pages are of a
+        sequence's own tokens behind them."""
+        if prefix % page:
+            raise ValueError("a shared prefix of %d tokens does not fill pages of %d" % (prefix, page))
+        per_seq, shared = -(-longest // page), prefix // page
+        self.page, self.longest, self.device, self.eight, self.prefix = page, longest, device, eight, prefix
+        cells = (seqs * per_seq + shared, kv_heads, page)
+        self.k = torch.empty(*cells, channels, dtype=torch.float8_e4m3fn if eight else dtype, device=device)
         self.v = torch.empty_like(self.k)
-        self.free = list(range(seqs * per_seq))
+        self.arrays = [self.k, self.v]
+        if eight:
+            self.arrays += [torch.empty(cells, dtype=torch.float8_e8m0fnu, device=device) for _ in range(2)]
+        self.free = list(range(seqs * per_seq + shared))
+        self.prefix_pages = [self.free.pop() for _ in range(shared)]
         self.pages = [[] for _ in range(seqs)]
         self.lengths = [0] * seqs
         self.per_seq = per_seq
+
+    def prefix_slots(self):
+        """Positions and slots of the shared tokens."""
+        slots = [p * self.page + t for p in self.prefix_pages for t in range(self.page)]
+        return self._int32(range(self.prefix)), self._int32(slots)
 
     def grow(self, counts):
         """Room for counts[b] more tokens of sequence b -> positions and slots of the new tokens, packed, on the device."""
@@ -41,7 +59,7 @@ class PagedCache:
             for t in range(self.lengths[b], self.lengths[b] + n):
                 if t // self.page == len(self.pages[b]):
                     self.pages[b].append(self.free.pop())
-                positions.append(t)
+                positions.append(self.prefix + t)
                 slots.append(self.pages[b][t // self.page] * self.page + t % self.page)
             self.lengths[b] += n
         return self._int32(positions), self._int32(slots)
@@ -50,16 +68,23 @@ class PagedCache:
         """(block table, lengths, longest) for attn_decode."""
         return (self._int32([p + [0] * (self.per_seq - len(p)) for p in self.pages]), self._int32(self.lengths), max(self.lengths))
 
+    def whole_table(self):
+        """Pages of every sequence from its first token on, those of the prefix among them, for kv_read."""
+        return self._int32([self.prefix_pages + p + [0] * (self.per_seq - len(p)) for p in self.pages])
+
     def _int32(self, values):
-        return torch.tensor(values, dtype=torch.int32).to(self.device)
+        return torch.tensor(list(values), dtype=torch.int32).to(self.device)
 
 
 class DecoderLayer:
-    def __init__(self, d, ff, heads, kv_heads, longest, dtype=torch.bfloat16, device="cuda:0", seed=0):
+    def __init__(self, d, ff, heads, kv_heads, longest, dtype=torch.bfloat16, device="cuda:0", seed=0, sandwich=False):
         import fused_mlp_module as m
         name = "bf16" if dtype == torch.bfloat16 else "fp16"
         self.append, self.decode, self.prompt, self.project, self.mlp = (
             getattr(m, op + name) for op in ("kv_append_", "attn_decode_", "attn_prompt_", "swiglu_down_", "fused_swiglu_mlp_"))
+        self.append8, self.decode8, self.shared, self.shared8, self.read, self.read8, self.add_norm, self.rms_norm = (
+            getattr(m, op + name) for op in ("kv_append8_", "attn_decode8_", "attn_shared_", "attn_shared8_", "kv_read_", "kv_read8_", "add_norm_",
+                                             "rms_norm_"))
         self.heads, self.kv_heads, self.channels = heads, kv_heads, d // heads
         w = fsw_weights.make_inputs(1, d, ff, dtype, seed)
         self.w13, self.w2 = w["W13"].to(device), w["W2"].to(device)
@@ -73,6 +98,11 @@ class DecoderLayer:
         rate = 10000.0 ** (-torch.arange(0, self.channels, 2, dtype=torch.float64) / self.channels)
         angle = torch.outer(torch.arange(longest, dtype=torch.float64), rate)
         self.cos_sin = torch.cat([angle.cos(), angle.sin()], 1).float().to(device)
+        self.sandwich = sandwich
+        if sandwich:  # weights of the norms before and after attention and MLP, and both gates
+            vectors = (1 + 0.1 * torch.randn(6, d, generator=gen)).to(dtype).to(device)
+            self.before_attn, self.after_attn, self.before_mlp, self.after_mlp, self.attn_gate, self.mlp_gate = vectors
+            self.residual_scale = 0.5
 
     @staticmethod
     def norm(x):
@@ -80,54 +110,98 @@ class DecoderLayer:
         return (y * torch.rsqrt(y.square().mean(-1, keepdim=True) + 1e-5)).to(x.dtype)
 
     def _qkv(self, x):
-        rows = self.project(self.norm(x), self.w_qkv).view(x.shape[0], -1, self.channels)
+        h = self.rms_norm(x, self.before_attn) if self.sandwich else self.norm(x)
+        rows = self.project(h, self.w_qkv).view(x.shape[0], -1, self.channels)
         return rows.split([self.heads, self.kv_heads, self.kv_heads], 1)
 
     def _finish(self, x, attended):
-        x = x + self.project(attended.reshape(x.shape[0], -1), self.w_out)
+        y = self.project(attended.reshape(x.shape[0], -1), self.w_out)
+        if self.sandwich:
+            x, h = self.add_norm(x, y, self.attn_gate, self.after_attn, self.before_mlp, self.residual_scale)
+            return self.add_norm(x, self.mlp(h, self.w13, self.w2), self.mlp_gate, self.after_mlp, None, self.residual_scale)[0]
+        x = x + y
         return x + self.mlp(self.norm(x), self.w13, self.w2)
+
+    def _append(self, q, k, v, positions, slots, cache):
+        """Rotated queries, and keys and values as later tokens will see them."""
+        if cache.eight:
+            return self.append8(q, k, v, self.cos_sin, positions, slots, *cache.arrays)
+        return (*self.append(q, k, v, self.cos_sin, positions, slots, cache.k, cache.v), v)
+
+    def _prompts(self, x, lengths, positions, slots, cache):
+        q, k, v = self._append(*self._qkv(x), positions, slots, cache)
+        starts = self._starts(lengths, x.device)
+        return self._finish(x, self.prompt(q, k, v, starts, starts, self.channels ** -0.5))
+
+    @staticmethod
+    def _starts(lengths, device):
+        starts = [0]
+        for n in lengths:
+            starts.append(starts[-1] + n)
+        return torch.tensor(starts, dtype=torch.int32).to(device)
 
     def prefill(self, x, lengths, cache):
         """x: the packed rows of new sequences' prompts."""
         for b, n in enumerate(lengths):
             if n and cache.lengths[b]:
                 raise ValueError("sequence %d has tokens in the cache already" % b)
+        if cache.prefix:
+            raise ValueError("prompts behind a shared prefix extend what the cache holds: extend()")
+        return self._prompts(x, lengths, *cache.grow(lengths), cache)
+
+    def prefill_shared(self, x, cache):
+        """x: the rows of the prefix that all of the cache's sequences begin with."""
+        return self._prompts(x, [cache.prefix], *cache.prefix_slots(), cache)
+
+    def extend(self, x, lengths, cache):
+        """x: the packed rows of prompts that continue what the cache holds of their sequences."""
         q, k, v = self._qkv(x)
         positions, slots = cache.grow(lengths)
-        q, k = self.append(q, k, v, self.cos_sin, positions, slots, cache.k, cache.v)
-        starts = [0]
-        for n in lengths:
-            starts.append(starts[-1] + n)
-        starts = torch.tensor(starts, dtype=torch.int32).to(x.device)
-        return self._finish(x, self.prompt(q, k, v, starts, starts, self.channels ** -0.5))
+        q = self._append(q, k, v, positions, slots, cache)[0]
+        held = [cache.prefix + n for n in cache.lengths]
+        starts = self._starts(held, x.device)
+        k, v = (self.read8 if cache.eight else self.read)(*cache.arrays, cache.whole_table(), starts, sum(held))
+        return self._finish(x, self.prompt(q, k, v, self._starts(lengths, x.device), starts, self.channels ** -0.5))
 
     def step(self, x, cache):
         """x: one row per sequence, its next token."""
         q, k, v = self._qkv(x)
         positions, slots = cache.grow([1] * x.shape[0])
-        q, _ = self.append(q, k, v, self.cos_sin, positions, slots, cache.k, cache.v)
+        q = self._append(q, k, v, positions, slots, cache)[0]
         table, lengths, longest = cache.table()
-        return self._finish(x, self.decode(q, cache.k, cache.v, table, lengths, longest, self.channels ** -0.5))
+        own = (table, lengths, longest, self.channels ** -0.5)
+        if cache.prefix:
+            pages = cache._int32(cache.prefix_pages)
+            return self._finish(x, (self.shared8 if cache.eight else self.shared)(q, *cache.arrays, pages, cache.prefix, *own))
+        return self._finish(x, (self.decode8 if cache.eight else self.decode)(q, *cache.arrays, *own))
 
 
-def run(d=1024, ff=2816, heads=16, kv_heads=4, prompts=(37, 5, 130), steps=9, page=16, dtype=torch.bfloat16, seed=0):
+def run(d=1024, ff=2816, heads=16, kv_heads=4, prompts=(37, 5, 130), steps=9, page=16, dtype=torch.bfloat16, seed=0, eight=False, prefix=0, turns=1,
+        sandwich=False):
     """Largest difference, over the root mean square of the outputs, between tokens decoded one by one and the same tokens
     inside their whole sequences."""
-    longest = max(prompts) + steps
-    layer = DecoderLayer(d, ff, heads, kv_heads, longest, dtype, seed=seed)
+    longest = prefix + max(prompts) + steps
+    layer = DecoderLayer(d, ff, heads, kv_heads, longest, dtype, seed=seed, sandwich=sandwich)
     gen = torch.Generator().manual_seed(seed + 2)
     whole = [torch.randn(n + steps, d, generator=gen).to(dtype).to("cuda:0") for n in prompts]
+    first = torch.randn(prefix, d, generator=gen).to(dtype).to("cuda:0")
 
-    def new_cache():
-        return PagedCache(len(prompts), longest, kv_heads, d // heads, page, dtype, "cuda:0")
+    def new_cache(shared):
+        return PagedCache(len(prompts), longest, kv_heads, d // heads, page, dtype, "cuda:0", eight, shared)
 
-    cache = new_cache()
-    layer.prefill(torch.cat([x[:n] for x, n in zip(whole, prompts)]), list(prompts), cache)
+    cache = new_cache(prefix)
+    if prefix:
+        layer.prefill_shared(first, cache)
+    for turn in range(turns):  # the prompts' parts of about the same length
+        parts = [x[n * turn // turns:n * (turn + 1) // turns] for x, n in zip(whole, prompts)]
+        take = layer.prefill if turn == 0 and not prefix else layer.extend
+        take(torch.cat(parts), [p.shape[0] for p in parts], cache)
     decoded = [layer.step(torch.stack([x[n + i] for x, n in zip(whole, prompts)]), cache) for i in range(steps)]
-    want = layer.prefill(torch.cat(whole), [n + steps for n in prompts], new_cache()).split([n + steps for n in prompts])
+    lengths = [prefix + n + steps for n in prompts]
+    want = layer.prefill(torch.cat([torch.cat([first, x]) for x in whole]), lengths, new_cache(0)).split(lengths)
     worst = 0.0
     for b, n in enumerate(prompts):
-        got, ref = torch.stack([y[b] for y in decoded]).float(), want[b][n:].float()
+        got, ref = torch.stack([y[b] for y in decoded]).float(), want[b][prefix + n:].float()
         worst = max(worst, ((got - ref).abs().max() / ref.square().mean().sqrt()).item())
     return worst
 
@@ -141,10 +215,15 @@ def main(argv=None):
     ap.add_argument("--prompts", type=int, nargs="+", default=[37, 5, 130])
     ap.add_argument("--steps", type=int, default=9)
     ap.add_argument("--page", type=int, default=16)
+    ap.add_argument("--eight", action="store_true", help="a cache of 8 bits")
+    ap.add_argument("--prefix", type=int, default=0, help="tokens that all sequences begin with, whole pages")
+    ap.add_argument("--turns", type=int, default=1, help="parts that prompts come in")
+    ap.add_argument("--sandwich", action="store_true", help="norms before and after both blocks, with gates")
     args = ap.parse_args(argv)
     if not torch.cuda.is_available():
         sys.exit("decoder_layer.py needs the GPU: the extension has no CPU path")
-    worst = run(args.d, args.ff, args.heads, args.kv_heads, tuple(args.prompts), args.steps, args.page)
+    worst = run(args.d, args.ff, args.heads, args.kv_heads, tuple(args.prompts), args.steps, args.page, eight=args.eight, prefix=args.prefix,
+                turns=args.turns, sandwich=args.sandwich)
     print("%d prompts, %d steps each: decoded tokens differ from whole sequences by %.1e of the outputs' size" %
           (len(args.prompts), args.steps, worst))
 
