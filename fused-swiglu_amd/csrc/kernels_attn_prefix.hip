@@ -3,12 +3,17 @@
 // over a share of the prefix's keys, unnormalised, to be joined with those of the other shares and of the sequence's own keys.
 //
 // A decode batch has one row per sequence, and taken by itself each would read the whole prefix. Here the rows of a key-value head, all sequences' query
-// heads of its group, stand side by side: a workgroup owns 64 or 128 of them and a share of the keys, so the prefix is read once per 64 or 128 rows, from
-// the L2 of the head's XCD after the first. Four waves own 16 or 32 rows each and walk the same tiles of 64 keys through LDS, two tiles
+// heads of its group, stand side by side: a workgroup owns 64, 128 or 256 of them and a share of the keys, so the prefix is read once per 64 to 256 rows,
+// from the L2 of the head's XCD after the first. Four or eight waves own 16 or 32 rows each and walk the same tiles of 64 keys through LDS, two tiles
 // of each kind in turn, as the prompts' kernel does (whose arrangement of the two products, with scores transposed and weights that stay in their lanes, this is);
 // there is no diagonal, and the keys come from pages. Elements of 16 bits are copied to LDS directly, 16 bytes a lane;
 // the page numbers of a tile are asked for a tile ahead. Elements of 8 bits pass through registers, where they
-// become keys and values of the element type.
+// become keys and values of the element type. The sum of the weights is a product too, with values that are all 1.
+//
+// Measured, 128 channels: 1024 sequences of 32 heads on 8 (4096 rows a key-value head) behind 4096 keys 82 us, 840 TFLOP/s, in 16 bits and in 8; 64 sequences
+// behind 16384 keys (256 rows, 32 shares of 512 keys) 31 us, 560 TFLOP/s; 200 sequences of 64 heads on 8 behind 8000 keys of 8 bits (1600 rows in 7 groups, 4
+// shares: 224 workgroups on 256 CUs) 78 us, 670. What bounds it: the matrix instructions alone take 38 of the 82, and reading LDS, the softmax and asking for
+// tiles each add 14 to 18 to them, since the waves of a SIMD, two, wait at the same barrier and do the same at the same time.
 #include <float.h>
 
 #include <type_traits>
@@ -22,6 +27,27 @@
 namespace fsw {
 namespace {
 
+template <class T>
+constexpr unsigned ONES = 0x3f803f80u;
+template <>
+inline constexpr unsigned ONES<Fp16> = 0x3c003c00u;
+
+// Largest value of lanes l, l ^ 16, l ^ 32, l ^ 48 (max_over_groups), NaN if one is: v_maximum3 takes scores as they come, where v_max wants them
+// made canonical first, an instruction each.
+__device__ __forceinline__ float maximum_over_groups(float x) {
+  float y = x;
+  asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1\n\ts_nop 1" : "+v"(x), "+v"(y));
+  x = __builtin_elementwise_maximum(x, y);
+  y = x;
+  asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1\n\ts_nop 1" : "+v"(x), "+v"(y));
+  return __builtin_elementwise_maximum(x, y);
+}
+
+// 16 bytes a lane, to LDS from `to` on
+__device__ __forceinline__ void copy_to_lds(__amdgpu_buffer_rsrc_t from, unsigned offset, unsigned char* to) {
+  __builtin_amdgcn_raw_ptr_buffer_load_lds(from, (lds_void*)to, 16, (int)offset, 0, 0, 0);
+}
+
 struct Scales {
   const unsigned char *k, *v;
   long long page, head, token;
@@ -32,18 +58,16 @@ __device__ __forceinline__ Scales scales_of(const PagedKv&) { return {nullptr, n
 // WHOLE: the rows of a wave's load, ROWS of them, lie in one page, whose address is wave-uniform then.
 template <class T, class CACHE, int DP, int NB, int WAVES, bool WHOLE>
 __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) void attn_prefix_kernel(PrefixOver<CACHE> a, Divisor by_group, Divisor by_hkv, int chunk,
-                                                                              float lower, float limit) {
+                                                                                     float lower, float limit) {
   constexpr bool EIGHT = std::is_same<CACHE, PagedKv8>::value, STAGED = EIGHT || !WHOLE;
   constexpr int RB = DP * 2, TILE = KEYS * RB;
   constexpr int SIZE = EIGHT ? 1 : 2, PER_ROW = DP * SIZE / 16, ROWS = 64 / PER_ROW;  // 16-byte vectors of a row, rows of a wave's load
   constexpr int VECS = KEYS / ROWS / WAVES;                                           // loads of keys, and of values, of a wave and tile
   constexpr int KSTEPS = DP / 32, DB = DP / 16, KB = KEYS / 16, WM = 16 * NB, BM = WAVES * WM;
-  constexpr bool AHEAD = DP < 256 || NB == 1;
+  constexpr bool AHEAD = DP < 256 || WHOLE;  // fragments are read from LDS a step ahead, if registers allow
   constexpr int VBUF = AHEAD ? 2 : 1, VG = AHEAD ? 4 : 1;
-  __shared__ __align__(1024) unsigned char k0s[TILE];
-  __shared__ __align__(1024) unsigned char k1s[TILE];
-  __shared__ __align__(1024) unsigned char v0s[TILE];
-  __shared__ __align__(1024) unsigned char v1s[TILE];
+  __shared__ __align__(1024) unsigned char k0s[TILE], k1s[TILE];
+  __shared__ __align__(1024) unsigned char v0s[TILE], v1s[TILE];
   __shared__ int odd_sums[WAVES], bad_pages[WAVES];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -52,6 +76,7 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) void attn_prefix_ker
   const int split = blockIdx.y, group = (int)by_group.d, rows = a.seqs * group;  // < 2^26
   const int begin = split * chunk, end = a.len - begin < chunk ? a.len : begin + chunk;
   const int wrow = row_tile * BM + wave * WM;
+  const bool idle = wrow >= rows;  // a wave without rows helps with the copies
   const Scales scales = scales_of(a.cache);
 
   u32x4 qf[NB][KSTEPS];
@@ -61,30 +86,30 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) void attn_prefix_ker
     const int seq = by_group.quotient(row);
     const unsigned short* p = (const unsigned short*)a.q.p + seq * a.q.token + (kvh * group + row - seq * group) * a.q.head;
 #pragma unroll
-    for (int s = 0; s < KSTEPS; ++s) {
-      const int ch = s * 32 + grp * 8;
-      qf[n][s] = u32x4{0, 0, 0, 0};
-      if (ch < a.d) qf[n][s] = *(const u32x4*)(p + ch);
+    for (int st = 0; st < KSTEPS; ++st) {
+      const int ch = st * 32 + grp * 8;
+      qf[n][st] = u32x4{0, 0, 0, 0};
+      if (ch < a.d) qf[n][st] = *(const u32x4*)(p + ch);
     }
   }
 
   // Load j of a wave is rows first_row(j) .. + ROWS - 1 of a tile, PER_ROW lanes each. Lane l knows the page of the tile's key l.
   const int lrow = lane / PER_ROW, lvec = lane % PER_ROW;
   auto first_row = [&](int j) INLINE -> int { return (j * WAVES + wave) * ROWS; };
-  int pages;
-  bool bad = false;
-  auto locate = [&](int at) INLINE {
+  auto locate = [&](int at) INLINE -> int {
     const int key = at + lane < end ? at + lane : end - 1;
-    pages = a.pages[a.cache.per_page.quotient(key)];
+    return a.pages[a.cache.per_page.quotient(key)];
   };
   const unsigned char* kc = (const unsigned char*)a.cache.k + kvh * a.cache.head * SIZE;
   const unsigned char* vc = (const unsigned char*)a.cache.v + kvh * a.cache.head * SIZE;
   const int stride = (int)a.cache.token * SIZE;
   u32x4 kr[STAGED ? VECS : 1], vr[STAGED ? VECS : 1];   // a tile under way
   unsigned km[EIGHT ? VECS : 1], vm[EIGHT ? VECS : 1];  // its scales
-  // Asks for the tile at `at`, whose pages are known, and for the next one's pages. Rows behind the end are zeros and touch no memory.
-  auto ask = [&](int at, unsigned char* kto, unsigned char* vto) INLINE {
-    bad |= (unsigned)pages >= (unsigned)a.cache.pages;
+  bool bad = false;
+  // Asks for the keys or the values of the tile at `at`, whose pages are known. Rows behind the end are zeros and touch no memory.
+  auto ask = [&](bool value, int at, int pages, unsigned char* to) INLINE {
+    if (!value) bad |= (unsigned)pages >= (unsigned)a.cache.pages;
+    const unsigned char* cells = value ? vc : kc;
 #pragma unroll
     for (int j = 0; j < VECS; ++j) {
       const int row = first_row(j) + lrow, key = at + first_row(j) + (WHOLE ? 0 : lrow);
@@ -93,64 +118,63 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) void attn_prefix_ker
       const int known = key < end ? key : end - 1, place = known - a.cache.per_page.quotient(known) * a.cache.page_size;
       const long long where = (page * a.cache.page + place * a.cache.token) * SIZE;
       const long long mark = EIGHT ? kvh * scales.head + page * scales.page + place * scales.token : 0;
+      const unsigned char* marks = value ? scales.v : scales.k;
       if constexpr (WHOLE) {
-        const int real = end - key < ROWS ? end - key : ROWS, span = real > 0 ? (real - 1) * stride + a.d * SIZE : 0;
-        const auto krsrc = make_rsrc(kc + where, span), vrsrc = make_rsrc(vc + where, span);
+        const int real = end - key < ROWS ? end - key : ROWS;
+        const auto rsrc = make_rsrc(cells + where, real > 0 ? (real - 1) * stride + a.d * SIZE : 0);
         if constexpr (EIGHT) {
-          const unsigned off = lvec * 16 < a.d ? (unsigned)(lrow * stride + lvec * 16) : OOB_OFFSET;
-          const int marks = real > 0 ? (real - 1) * (int)scales.token + 1 : 0;
-          km[j] = __builtin_amdgcn_raw_buffer_load_b8(make_rsrc(scales.k + mark, marks), lrow * (int)scales.token, 0, 0);
-          vm[j] = __builtin_amdgcn_raw_buffer_load_b8(make_rsrc(scales.v + mark, marks), lrow * (int)scales.token, 0, 0);
-          kr[j] = buf_load16(krsrc, off);
-          vr[j] = buf_load16(vrsrc, off);
+          const auto mrsrc = make_rsrc(marks + mark, real > 0 ? (real - 1) * (int)scales.token + 1 : 0);
+          (value ? vm : km)[j] = __builtin_amdgcn_raw_buffer_load_b8(mrsrc, lrow * (int)scales.token, 0, 0);
+          (value ? vr : kr)[j] = buf_load16(rsrc, lvec * 16 < a.d ? (unsigned)(lrow * stride + lvec * 16) : OOB_OFFSET);
         } else {
-          const int kch = (lvec ^ k_swizzle<DP>(row)) * 8, vch = (lvec ^ v_swizzle<DP>(row)) * 8;
-          __builtin_amdgcn_raw_ptr_buffer_load_lds(krsrc, (lds_void*)(kto + (j * WAVES + wave) * 1024), 16,
-                                                   (int)(kch < a.d ? (unsigned)(lrow * stride + kch * 2) : OOB_OFFSET), 0, 0, 0);
-          __builtin_amdgcn_raw_ptr_buffer_load_lds(vrsrc, (lds_void*)(vto + (j * WAVES + wave) * 1024), 16,
-                                                   (int)(vch < a.d ? (unsigned)(lrow * stride + vch * 2) : OOB_OFFSET), 0, 0, 0);
+          const int ch = (lvec ^ (value ? v_swizzle<DP>(row) : k_swizzle<DP>(row))) * 8;
+          copy_to_lds(rsrc, ch < a.d ? (unsigned)(lrow * stride + ch * 2) : OOB_OFFSET, to + (j * WAVES + wave) * 1024);
         }
       } else {
-        kr[j] = vr[j] = u32x4{0, 0, 0, 0};
-        if (key < end && lvec * (16 / SIZE) < a.d) {
-          kr[j] = *(const u32x4*)(kc + where + lvec * 16);
-          vr[j] = *(const u32x4*)(vc + where + lvec * 16);
-        }
-        if constexpr (EIGHT) km[j] = key < end ? scales.k[mark] : 127, vm[j] = key < end ? scales.v[mark] : 127;
+        u32x4 x = {0, 0, 0, 0};
+        if (key < end && lvec * (16 / SIZE) < a.d) x = *(const u32x4*)(cells + where + lvec * 16);
+        (value ? vr : kr)[j] = x;
+        if constexpr (EIGHT) (value ? vm : km)[j] = key < end ? marks[mark] : 127;
       }
     }
-    locate(at + KEYS);
   };
-  // what passes through registers: the tile that was asked for, as the element type
-  auto put = [&](unsigned char* kto, unsigned char* vto) INLINE {
+  constexpr bool KEY = false, VALUE = true;
+  // what passes through registers: keys or values that were asked for, as the element type
+  auto put = [&](bool value, unsigned char* to) INLINE {
     if constexpr (STAGED) {
 #pragma unroll
       for (int j = 0; j < VECS; ++j) {
-        const int row = first_row(j) + lrow;
-        auto store = [&](u32x4 x, unsigned byte, unsigned char* to, int swizzle) INLINE {
-          if constexpr (EIGHT) {
-            const float up = __builtin_bit_cast(float, byte << 23);
+        const int row = first_row(j) + lrow, swizzle = value ? v_swizzle<DP>(row) : k_swizzle<DP>(row);
+        const u32x4 x = (value ? vr : kr)[j];
+        if constexpr (EIGHT) {
+          const float up = __builtin_bit_cast(float, (value ? vm : km)[j] << 23);
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-              *(u32x4*)(to + row * RB + ((2 * lvec + i) ^ swizzle) * 16) =
-                  u32x4{widen<T, false>(x[2 * i], up), widen<T, true>(x[2 * i], up), widen<T, false>(x[2 * i + 1], up),
-                        widen<T, true>(x[2 * i + 1], up)};
-          } else {
-            *(u32x4*)(to + row * RB + (lvec ^ swizzle) * 16) = x;
-          }
-        };
-        store(kr[j], EIGHT ? km[j] : 0, kto, k_swizzle<DP>(row));
-        store(vr[j], EIGHT ? vm[j] : 0, vto, v_swizzle<DP>(row));
+          for (int i = 0; i < 2; ++i)
+            *(u32x4*)(to + row * RB + ((2 * lvec + i) ^ swizzle) * 16) =
+                u32x4{widen<T, false>(x[2 * i], up), widen<T, true>(x[2 * i], up), widen<T, false>(x[2 * i + 1], up),
+                      widen<T, true>(x[2 * i + 1], up)};
+        } else {
+          *(u32x4*)(to + row * RB + (lvec ^ swizzle) * 16) = x;
+        }
       }
     }
   };
 
-  f32x4 o[DB][NB];
-  float m[NB], sum[NB];
+  f32x4 o[DB][NB], s[KB][NB];
+  f32x4 sum[NB];  // the same in all four: a channel of values that are all 1
+  float m[NB];
+  unsigned p[NB][KB][2];
   const float c = a.scale_log2;
-  auto attend = [&](int at, const unsigned char* ks, const unsigned char* vs) INLINE {
-    if (wrow >= rows) return;  // a wave without rows helps with the copies
-    f32x4 s[KB][NB];
+  auto clear = [&]() INLINE {
+#pragma unroll
+    for (int n = 0; n < NB; ++n) {
+      m[n] = NEG_INF;
+      sum[n] = f32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < DB; ++i) o[i][n] = f32x4{0, 0, 0, 0};
+    }
+  };
+  auto scores = [&](const unsigned char* ks) INLINE {
     u32x4 kf[2][KSTEPS];
     auto key_fragment = [&](int kb, int st) INLINE -> u32x4 {
       const int key = kb * 16 + col;
@@ -174,7 +198,10 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) void attn_prefix_ker
         for (int n = 0; n < NB; ++n) s[kb][n] = T::mfma16(f, qf[n][st], s[kb][n]);
       }
     }
-    if (at + KEYS > end) {
+  };
+  auto weights = [&](int at) INLINE {
+    if (__builtin_expect(at + KEYS > end, 0)) {
+      asm volatile("");  // (a branch, not 45 selections in every tile)
       const int left = end - at - 4 * grp;
 #pragma unroll
       for (int n = 0; n < NB; ++n)
@@ -188,10 +215,10 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) void attn_prefix_ker
     bool above = false;
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
-      float t[KB];
+      float t = s[0][n][0];
 #pragma unroll
-      for (int kb = 0; kb < KB; ++kb) t[kb] = fmaxf(fmaxf(s[kb][n][0], s[kb][n][1]), fmaxf(s[kb][n][2], s[kb][n][3]));
-      top[n] = max_over_groups(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])));
+      for (int i = 1; i < 4 * KB; ++i) t = __builtin_elementwise_maximum(t, s[i / 4][n][i % 4]);
+      top[n] = maximum_over_groups(t);
       above |= top[n] > m[n] + limit;
     }
     if (__any(above)) {
@@ -207,20 +234,21 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) void attn_prefix_ker
           for (int r = 0; r < 4; ++r) o[i][n][r] *= alpha;
       }
     }
-    unsigned p[NB][KB][2];
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
       const float mc = m[n] == NEG_INF ? 0.0f : m[n] * c;
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
-        for (int r = 0; r < 4; r += 2) {
-          const float lo = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][n][r], c, -mc));
-          const float hi = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][n][r + 1], c, -mc));
-          p[n][kb][r / 2] = T::pack2(lo, hi);
-          sum[n] = add2<T>(p[n][kb][r / 2], sum[n]);
-        }
+        for (int r = 0; r < 4; r += 2)
+          p[n][kb][r / 2] = T::pack2(__builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][n][r], c, -mc)),
+                                     __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][n][r + 1], c, -mc)));
     }
+  };
+  auto values = [&](const unsigned char* vs) INLINE {
+    auto weight = [&](int n, int st) INLINE -> u32x4 {
+      return u32x4{p[n][2 * st][0], p[n][2 * st][1], p[n][2 * st + 1][0], p[n][2 * st + 1][1]};
+    };
     constexpr int GROUPS = KB / 2 * DB / VG;
     u32x4 vf[VBUF][VG];
     auto value_group = [&](int g) INLINE {
@@ -229,6 +257,10 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) void attn_prefix_ker
     };
     if (AHEAD) value_group(0);
 #pragma unroll
+    for (int st = 0; st < KB / 2; ++st)
+#pragma unroll
+      for (int n = 0; n < NB; ++n) sum[n] = T::mfma16(u32x4{ONES<T>, ONES<T>, ONES<T>, ONES<T>}, weight(n, st), sum[n]);
+#pragma unroll
     for (int g = 0; g < GROUPS; ++g) {
       if (g + VBUF - 1 < GROUPS) value_group(g + VBUF - 1);
       if (AHEAD) __builtin_amdgcn_sched_barrier(0);
@@ -236,44 +268,47 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) void attn_prefix_ker
       for (int x = 0; x < VG; ++x) {
         const int st = (g * VG + x) / DB, i = (g * VG + x) % DB;
 #pragma unroll
-        for (int n = 0; n < NB; ++n)
-          o[i][n] = T::mfma16(vf[g % VBUF][x], u32x4{p[n][2 * st][0], p[n][2 * st][1], p[n][2 * st + 1][0], p[n][2 * st + 1][1]}, o[i][n]);
+        for (int n = 0; n < NB; ++n) o[i][n] = T::mfma16(vf[g % VBUF][x], weight(n, st), o[i][n]);
       }
     }
   };
 
   // A sum that is not finite: all keys are taken once more with zeros in place of infinities and NaN among the values (8 bits: of what came out
   // of them), and what their weighted sum is, the same for every row since every row sees every key, is written over the sums below.
-  auto silence = [&](unsigned char* vs) INLINE {
-#pragma unroll 1
-    for (int byte = tid * 16; byte < TILE; byte += 1024 * WAVES) {
-      u32x4 x = *(u32x4*)(vs + byte);
+  auto silence = [&](unsigned char* p) INLINE {
+    u32x4 x = *(u32x4*)p;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = finite2<T>(x[j]);
-      *(u32x4*)(vs + byte) = x;
-    }
-    __syncthreads();
+    for (int j = 0; j < 4; ++j) x[j] = finite2<T>(x[j]);
+    *(u32x4*)p = x;
   };
   bool again = false;
-  // Tile t is in buffer t % 2. At the barrier the tile has landed, and every wave has read the one before.
-  auto turn = [&](int at, const unsigned char* ks, unsigned char* vs, unsigned char* knext, unsigned char* vnext) INLINE {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    ask(at + KEYS, knext, vnext);
-    if (__builtin_expect(again, 0)) silence(vs);
-    attend(at, ks, vs);
-    put(knext, vnext);
-  };
   while (true) {
-#pragma unroll
-    for (int n = 0; n < NB; ++n) {
-      m[n] = NEG_INF;
-      sum[n] = 0.0f;
-#pragma unroll
-      for (int i = 0; i < DB; ++i) o[i][n] = f32x4{0, 0, 0, 0};
-    }
-    locate(begin);
-    ask(begin, k0s, v0s);
-    put(k0s, v0s);
+    clear();
+    int pages = locate(begin);
+    // Tile t is in buffer t % 2. At the barrier the tile has landed, and every wave has read the one before.
+    auto turn = [&](int at, const unsigned char* ks, unsigned char* vs, unsigned char* knext, unsigned char* vnext) INLINE {
+      asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      ask(KEY, at + KEYS, pages, knext);
+      ask(VALUE, at + KEYS, pages, vnext);
+      pages = locate(at + 2 * KEYS);
+      if (__builtin_expect(again, 0)) {
+#pragma unroll 1
+        for (int byte = tid * 16; byte < TILE; byte += 1024 * WAVES) silence(vs + byte);
+        __syncthreads();
+      }
+      if (!idle) {
+        scores(ks);
+        weights(at);
+        values(vs);
+      }
+      put(KEY, knext);
+      put(VALUE, vnext);
+    };
+    ask(KEY, begin, pages, k0s);
+    ask(VALUE, begin, pages, v0s);
+    pages = locate(begin + KEYS);
+    put(KEY, k0s);
+    put(VALUE, v0s);
     for (int at = begin; at < end; at += 2 * KEYS) {
       turn(at, k0s, v0s, k1s, v1s);
       if (at + KEYS >= end) break;
@@ -307,7 +342,7 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) void attn_prefix_ker
   };
 #pragma unroll
   for (int n = 0; n < NB; ++n) {
-    float total = sum_over_groups(sum[n]);
+    const float total = sum[n][0];
     const int row = wrow + 16 * n + col;
     if (row >= rows) continue;
     const long long at = out_row(row);
@@ -346,10 +381,10 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) void attn_prefix_ker
 
 template <class T, class CACHE, int DP, int NB, int WAVES, bool WHOLE>
 hipError_t launch(const PrefixOver<CACHE>& a, const PrefixPlan& p, hipStream_t stream) {
+  constexpr int BM = 16 * NB * WAVES;
   const int group = a.hq / a.hkv;
   const float shift = shift_of<T>(a.keys);
   const float lower = fmaxf(shift / a.scale_log2, -FLT_MAX / 4), limit = fmaxf((shift + SLACK<T>) / a.scale_log2, -FLT_MAX / 4);
-  constexpr int BM = 16 * NB * WAVES;
   const dim3 grid(a.hkv * ((a.seqs * group + BM - 1) / BM), p.splits);
   attn_prefix_kernel<T, CACHE, DP, NB, WAVES, WHOLE><<<grid, 64 * WAVES, 0, stream>>>(a, Divisor(group), Divisor(a.hkv), p.chunk, lower, limit);
   return hipGetLastError();
@@ -359,10 +394,13 @@ template <class T, class CACHE, int DP>
 hipError_t launch_dp(const PrefixOver<CACHE>& a, const PrefixPlan& p, hipStream_t stream) {
   constexpr int ROWS = 1024 / (DP * (std::is_same<CACHE, PagedKv8>::value ? 1 : 2));
   if (a.cache.page_size % ROWS) return launch<T, CACHE, DP, 1, 4, false>(a, p, stream);
-  if constexpr (DP > 64) {
+  if constexpr (DP == 128) {
     if (p.rows == 256) return launch<T, CACHE, DP, 2, 8, true>(a, p, stream);
   }
-  return p.rows == 128 ? launch<T, CACHE, DP, 2, 4, true>(a, p, stream) : launch<T, CACHE, DP, 1, 4, true>(a, p, stream);
+  if constexpr (DP < 256) {
+    if (p.rows == 128) return launch<T, CACHE, DP, 2, 4, true>(a, p, stream);
+  }
+  return launch<T, CACHE, DP, 1, 4, true>(a, p, stream);
 }
 
 template <class T, class CACHE>
@@ -385,8 +423,9 @@ PrefixPlan prefix_plan(int seqs, int hq, int hkv, int d, int len) {
   PrefixPlan best = {0, 0, 0};
   double least = 0.0;
   for (const int size : {64, 128, 256}) {
-    if (size == 256 && d <= 64) continue;  // (tiles too small for eight waves' copies)
-    if (size == 64 && rows > 64) continue;
+    if (size == 256 && (d <= 64 || d > 128)) continue;  // (tiles too small for eight waves' copies; registers)
+    if (size == 128 && d > 128) continue;               // (registers)
+    if (size == 64 && rows > 64 && d <= 128) continue;
     const long long items = hkv * ((rows + size - 1) / size), resident = 256 * (size == 256 || d > 128 ? 1 : 2);
     const long long most = tiles < 64 ? tiles : 64;
     for (long long splits = 1; splits <= most; ++splits) {
