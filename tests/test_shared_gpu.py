@@ -65,7 +65,7 @@ def test_shared(capi, prefix, Hq, Hkv, D, page, bits, dtype):
 @pytest.mark.parametrize("B,Hq,Hkv,D,page,prefix", [
     (17, 5, 1, 128, 16, 200),      # 85 rows: 128 a workgroup, three waves with rows
     (33, 8, 2, 64, 8, 333),        # 132 rows of 64 channels: two of them
-    (40, 8, 1, 128, 32, 500),      # 320 rows: 256 a workgroup, or 128
+    (40, 8, 1, 128, 32, 500),      # 320 rows
     (70, 4, 1, 112, 64, 129),
     (20, 16, 1, 256, 16, 190),     # 256 channels
     (9, 16, 1, 256, 2, 70),
@@ -75,6 +75,41 @@ def test_shared(capi, prefix, Hq, Hkv, D, page, bits, dtype):
 def test_shared_by_many_rows(capi, B, Hq, Hkv, D, page, prefix, bits, dtype):
     gen = torch.Generator().manual_seed(B + D)
     check(capi, gen, prefix, [(7 * b) % 40 for b in range(B)], Hq, Hkv, D, page, dtype, bits)
+
+
+def joined(q, rows, pages, prefix, table, lengths, page, scale):
+    """reference() for one key-value head and many rows: a sequence's heads in one product, the prefix gathered once."""
+    o, mag = torch.zeros(q.shape, dtype=torch.float64), torch.zeros(q.shape, dtype=torch.float64)
+    at = torch.arange(prefix)
+    first = [r[pages[at // page].long(), 0, at % page] for r in rows]
+    for b, n in enumerate(lengths):
+        own = torch.arange(n)
+        k, v = (torch.cat([f, r[table[b, own // page].long(), 0, own % page]]) for f, r in zip(first, rows))
+        w = torch.softmax(q[b].double() @ k.T * scale, -1)
+        o[b], mag[b] = w @ v, w @ v.abs()
+    return o, mag
+
+
+@pytest.mark.parametrize("D", [112, 128])
+@pytest.mark.parametrize("bits,dtype,infinities", [(8, BF, False), (8, HF, False), (16, BF, False), (16, HF, False), (16, BF, True), (16, HF, True)])
+def test_shared_by_thousands_of_rows(capi, bits, dtype, D, infinities):
+    """256 rows a workgroup, the last with 192 of them, in nine shares, the last of which ends inside a tile."""
+    gen = torch.Generator().manual_seed(D + bits)
+    B, Hq, page, prefix = 99, 64, 16, 4000
+    lengths = [(7 * b) % 23 for b in range(B)]
+    cache, rows, table, pages = setup(gen, prefix, lengths, 1, D, page, dtype, bits)
+    if infinities:
+        for key, channel, value in ((2000, 3, INF), (3999, 4, -INF), (0, 5, NAN), (77, 6, INF), (3998, 6, -INF)):
+            rows[1][int(pages[key // page]), 0, key % page, channel] = value
+        cache = [r.to(dtype).to(DEV) for r in rows]
+    q = randn(gen, B, Hq, D, dtype=dtype, scale=1.5)
+    out, wide = inside(torch.zeros(B, Hq, D, dtype=dtype))
+    capi.attn_shared(q.to(DEV), cache, pages.to(DEV), prefix, table.to(DEV), int32(lengths), max(lengths), D ** -0.5, out=out)
+    ref, mag = joined(q, rows, pages, prefix, table, lengths, page, D ** -0.5)
+    got, finite = out.cpu().double(), torch.isfinite(ref)
+    assert ((got - ref).abs() <= attention.tolerance(ref, mag, dtype, True, prefix + 23))[finite].all()
+    assert torch.equal(got[~finite].nan_to_num(7.0, INF, -INF), ref[~finite].nan_to_num(7.0, INF, -INF)) and finite.all() == (not infinities)
+    assert untouched(wide, out.shape)
 
 
 @pytest.mark.parametrize("bits", [8, 16])
@@ -278,6 +313,38 @@ def test_a_step_replays_from_a_hip_graph(ext, bits):
             assert all(torch.equal(x, y) for x, y in zip(out, eager)), "replay %d" % step
             assert all(torch.equal(x, y) for x, y in zip(codes_of(cache), codes_of(copies)))
             del busy
+
+
+@pytest.mark.parametrize("backend", ["eager", "aot_eager"])
+def test_operators_under_torch_compile_fullgraph(ext, backend):
+    """A function of the operators traces whole, with the caches it writes, and gives what the operators give."""
+    import torch._dynamo
+    torch._dynamo.reset()
+    gen = torch.Generator().manual_seed(31)
+    ops, D, page, prefix = torch.ops.ASMLLM, 64, 16, 50
+    cache, rows, block, pages = setup(gen, prefix, [40, 40], 2, D, page, BF, 8)
+    sixteen = [r.to(BF).to(DEV) for r in rows]
+    block, pages, table, weight = block.to(DEV), pages.to(DEV), angles(gen, 100, D).to(DEV), randn(gen, 4 * D).to(DEV)
+    at = [0, 7]
+    slots = int32([int(block[b, x // page]) * page + x % page for b, x in enumerate(at)])
+    where, lengths, cu = int32([prefix + x for x in at]), int32([x + 1 for x in at]), int32([0, 1, 9])
+
+    def step(q, k, v, a, b, a_s, b_s, c, d):
+        qr, ka, va = ops.kv_append8_bf16(q, k, v, table, where, slots, a, b, a_s, b_s, False)
+        o = ops.attn_shared8_bf16(qr, a, b, a_s, b_s, pages, prefix, block, lengths, 40, 0.125)
+        p = ops.attn_shared_bf16(qr, c, d, pages, prefix, block, lengths, 40, 0.125)
+        o = o + p + ops.attn_decode8_bf16(qr, a, b, a_s, b_s, block, lengths, 40, 0.125)
+        x, y = ops.add_norm_bf16(q.flatten(1), o.flatten(1), None, weight, weight, 0.5)
+        return (x, y, ops.rms_norm_bf16(y, weight), ka, va, *ops.kv_read8_bf16(a, b, a_s, b_s, block, cu, 9), *ops.kv_read_bf16(c, d, block, cu, 9))
+
+    q, k, v = (randn(gen, 2, h, D).to(DEV) for h in (4, 2, 2))
+    copy = lambda c: [x.view(torch.uint8).clone().view(x.dtype) for x in c]  # noqa: E731
+    ones, others = copy(cache), copy(cache)
+    want = step(q, k, v, *ones, *sixteen)
+    got = torch.compile(step, fullgraph=True, backend=backend)(q, k, v, *others, *sixteen)
+    assert len(want) == len(got) and all(torch.equal(x, y) for x, y in zip(got, want))
+    assert all(torch.equal(x, y) for x, y in zip(codes_of(others), codes_of(ones)))
+    assert not torch.equal(codes_of(cache)[0], codes_of(ones)[0])
 
 
 def test_calls_on_other_streams_at_once(capi):
