@@ -125,4 +125,67 @@ __device__ __forceinline__ float scale_of(float a, float b) {
   return a == b ? 1.0f : fmaxf(__builtin_amdgcn_exp2f(a - b), FLT_MIN);
 }
 
+// Unnormalised sums of four channels over some keys, and the maximum and sum of their weights.
+struct Share {
+  f32x4 o = {0, 0, 0, 0};
+  float m = -__builtin_inff(), sum = 0.0f;
+  __device__ __forceinline__ void add(float other_m, float other_sum, f32x4 other) {
+    const float now = fmaxf(m, other_m), old = scale_of(m, now), w = scale_of(other_m, now);
+    m = now;
+    sum = sum * old + other_sum * w;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] = o[j] * old + other[j] * w;
+  }
+  // shares first, first + step .. below `used`, at these channels of them (d floats each) and their maxima and sums
+  __device__ __forceinline__ void add_all(const float* sums, const float* ml, int first, int step, int used, int d) {
+    constexpr int BATCH = 4;  // under way at a time
+    for (int i = first; i < used; i += step * BATCH) {
+      f32x4 x[BATCH];
+      float xm[BATCH], xs[BATCH];
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k) {
+        const int n = i + k * step < used ? i + k * step : i;
+        x[k] = *(const f32x4*)(sums + (long long)n * d);
+        xm[k] = ml[2 * n];
+        xs[k] = ml[2 * n + 1];
+      }
+#pragma unroll
+      for (int k = 0; k < BATCH; ++k)
+        if (i + k * step < used) add(xm[k], xs[k], x[k]);
+    }
+  }
+};
+
+// The end of a workgroup that has all of its sequence's own keys behind a shared prefix: adds the prefix's shares to what `own(h, ch)` gives for
+// query head h < here and four channels from ch on, and hands each result to `out(h, ch, share)`. Where there are more threads than results, groups of
+// threads take the shares in turn. All of the workgroup's threads come here; `room`: THREADS f32x4 and 2 THREADS floats of LDS.
+template <int THREADS, int WIDE, class Own, class Out>
+__device__ __forceinline__ void finish_prefix(const float* partial, long long row0, long long rows, int before, int d, int here, float* room, Own own, Out out) {
+  const int items = here * WIDE, parts = items < THREADS ? THREADS / items : 1;
+  const float* ml = partial + rows * before * d;
+  f32x4* os = (f32x4*)room;
+  float* ms = room + 4 * THREADS;
+  for (int from = 0; from < items; from += THREADS) {  // once, if parts > 1
+    const int t = from + (int)threadIdx.x, part = parts > 1 ? t / items : 0, item = t - part * items;
+    const int h = item / WIDE, ch = item % WIDE * 4;
+    const bool mine = part < parts && item < items && ch < d;
+    Share s;
+    if (mine) s.add_all(partial + (row0 + h) * before * d + ch, ml + (row0 + h) * before * 2, part, parts, before, d);
+    if (parts > 1) {
+      if (mine && part > 0) {
+        os[t] = s.o;
+        ms[2 * t] = s.m;
+        ms[2 * t + 1] = s.sum;
+      }
+      __syncthreads();
+    }
+    if (!mine || part > 0) continue;
+    for (int n = t + items; n < parts * items; n += items) s.add(ms[2 * n], ms[2 * n + 1], os[n]);
+    const Share last = own(h, ch);
+    s.add(last.m, last.sum, last.o);
+    out(h, ch, s);
+  }
+}
+constexpr int finish_bytes(int threads) { return threads * 24; }
+
 }  // namespace fsw

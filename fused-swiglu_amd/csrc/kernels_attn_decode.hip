@@ -300,31 +300,42 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 2 : 4) void attn_decode_ker
     }
   }
   __syncthreads();
+  const auto joined = [&](int h, int ch) INLINE -> Share {
+    Share s;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) s.m = fmaxf(s.m, stats[w][0][h]);
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) s.sum += stats[w][1][h] * scale_of(stats[w][0][h], s.m);
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) s.o += *(const f32x4*)(shares + (w * here + h) * ROW + ch);
+    return s;
+  };
+  const auto write = [&](int h, int ch, const Share& s) INLINE {
+    const float inv = len == 0 && a.before == 0 ? 0.0f : 1.0f / s.sum;
+    unsigned short* op = (unsigned short*)a.o.p + (long long)seq * a.o.token + (long long)(head0 + h) * a.o.head;
+    *(u32x2*)(op + ch) = u32x2{T::pack2(s.o[0] * inv, s.o[1] * inv), T::pack2(s.o[2] * inv, s.o[3] * inv)};
+  };
+  const long long rows = (long long)a.seqs * a.hq, row0 = (long long)seq * a.hq + head0;
+  if (a.before > 0 && splits == 1) {
+    finish_prefix<64 * WAVES, WIDE>(partial, row0, rows, a.before, a.d, here, shares + WAVES * here * ROW, joined, write);
+    return;
+  }
   const bool parted = a.before > 0 || (len > chunk && !bad_len);
   for (int t = threadIdx.x; t < here * WIDE; t += 64 * WAVES) {
     const int h = t / WIDE, ch = (t % WIDE) * 4;
     if (ch >= a.d) continue;
-    float most = NEG_INF, total = 0.0f;
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) most = fmaxf(most, stats[w][0][h]);
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) total += stats[w][1][h] * scale_of(stats[w][0][h], most);
-    f32x4 x = {0, 0, 0, 0};
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) x += *(const f32x4*)(shares + (w * here + h) * ROW + ch);
-    if (parted) {  // unnormalised sums, maximum and sum of this share: attn_join_kernel
+    const Share s = joined(h, ch);
+    if (parted) {  // unnormalised sums, maximum and sum of this share, to be joined
       const int slots = a.before + splits;
-      const long long row = ((long long)seq * a.hq + head0 + h) * slots + a.before + split;
-      *(f32x4*)(partial + row * a.d + ch) = x;
+      const long long row = (row0 + h) * slots + a.before + split;
+      *(f32x4*)(partial + row * a.d + ch) = s.o;
       if (ch == 0) {
-        float* ml = partial + (long long)a.seqs * a.hq * slots * a.d + row * 2;
-        ml[0] = most;
-        ml[1] = total;
+        float* ml = partial + rows * slots * a.d + row * 2;
+        ml[0] = s.m;
+        ml[1] = s.sum;
       }
     } else {
-      const float inv = len == 0 ? 0.0f : 1.0f / total;
-      unsigned short* op = (unsigned short*)a.o.p + (long long)seq * a.o.token + (long long)(head0 + h) * a.o.head;
-      *(u32x2*)(op + ch) = u32x2{T::pack2(x[0] * inv, x[1] * inv), T::pack2(x[2] * inv, x[3] * inv)};
+      write(h, ch, s);
     }
   }
 }
@@ -346,46 +357,22 @@ __global__ __launch_bounds__(256) void attn_join_kernel(JoinArgs a, int chunk, i
   const float* ml = partial + (long long)a.seqs * a.hq * slots * a.d + row * 2;
   const float* po = partial + row * a.d + 4 * at;
 
-  f32x4 o = {0, 0, 0, 0};
-  float top = NEG_INF, total = 0.0f;
-  auto add = [&](float m, float sum, f32x4 x) {
-    const float now = fmaxf(top, m), old = scale_of(top, now), w = scale_of(m, now);
-    top = now;
-    total = total * old + sum * w;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) o[j] = o[j] * old + x[j] * w;
-  };
-  constexpr int BATCH = 4;
-  if (part < rows && head < a.hq) {
-    for (int i = part; i < used; i += rows * BATCH) {
-      f32x4 x[BATCH];
-      float m[BATCH], s[BATCH];
-#pragma unroll
-      for (int k = 0; k < BATCH; ++k) {
-        const int n = i + k * rows < used ? i + k * rows : i;
-        x[k] = *(const f32x4*)(po + (long long)n * a.d);
-        m[k] = ml[2 * n];
-        s[k] = ml[2 * n + 1];
-      }
-#pragma unroll
-      for (int k = 0; k < BATCH; ++k)
-        if (i + k * rows < used) add(m[k], s[k], x[k]);
-    }
-  }
+  Share s;
+  if (part < rows && head < a.hq) s.add_all(po, ml, part, rows, used, a.d);
   __shared__ f32x4 os[256];
   __shared__ float ms[256], ts[256];
-  os[threadIdx.x] = o;
-  ms[threadIdx.x] = top;
-  ts[threadIdx.x] = total;
+  os[threadIdx.x] = s.o;
+  ms[threadIdx.x] = s.m;
+  ts[threadIdx.x] = s.sum;
   __syncthreads();
   if (part > 0 || head >= a.hq) return;
   for (int i = 1; i < rows && i < used; ++i) {
     const int n = first + i * width + at;
-    add(ms[n], ts[n], os[n]);
+    s.add(ms[n], ts[n], os[n]);
   }
-  const float inv = 1.0f / total;
+  const float inv = 1.0f / s.sum;
   unsigned short* op = (unsigned short*)a.o.p + (long long)seq * a.o.token + (long long)head * a.o.head;
-  *(u32x2*)(op + 4 * at) = u32x2{T::pack2(o[0] * inv, o[1] * inv), T::pack2(o[2] * inv, o[3] * inv)};
+  *(u32x2*)(op + 4 * at) = u32x2{T::pack2(s.o[0] * inv, s.o[1] * inv), T::pack2(s.o[2] * inv, s.o[3] * inv)};
 }
 
 // bf16 has values as large as fp32's: there the weights of all keys together stay below 1, so that no sum of finite values overflows before it is
@@ -402,7 +389,7 @@ hipError_t launch_waves(const PagedAttnArgs& a, const PagedAttnPlan& p, float* p
   const int tiles = head_tiles(a.hq, a.hkv);
   const int group = a.hq / a.hkv;
   const dim3 grid(a.hkv * tiles, a.seqs, p.splits);
-  const size_t lds = (size_t)WAVES * (group < 16 ? group : 16) * (DP + 4) * sizeof(float);
+  const size_t lds = (size_t)WAVES * (group < 16 ? group : 16) * (DP + 4) * sizeof(float) + (a.before > 0 && p.splits == 1 ? finish_bytes(64 * WAVES) : 0);
   const auto kernel = a.cache.page_size % 16 == 0 ? attn_decode_kernel<T, DP, true, WAVES> : attn_decode_kernel<T, DP, false, WAVES>;
   kernel<<<grid, 64 * WAVES, lds, stream>>>(a, lift_of<T>(a.keys), p.chunk, group, tiles, partial);
   return hipGetLastError();
@@ -476,12 +463,17 @@ PagedAttnPlan paged_attn_plan(int seqs, int hq, int hkv, int d, int max_len, int
   return p;
 }
 
-// Four waves; shares of 128 keys while there are few, since a join follows in any case, but not many more workgroups than 4096, since empty ones are not
-// free. us, shares of 128 | 256 | 512 | 1024 keys: 512 items of 1 .. 900 keys of 16 bits 16.5 | 18.4 | 27 | 39; 1600 items of 1 .. 1500 keys of 8 bits 47 | 35 | 33 | 38.
+// Four waves (sixteen, unsplit: 15.3 against 7.8 us with 512 items of 1 .. 60 keys of 8 bits, 42 against 28 with 4000). Unsplit, a workgroup adds the prefix's shares itself
+// and there is no join, 5 to 9 us; that pays while its turns are few, or items many. us, unsplit | in shares and joined, up to 400, 1500, 4000 keys: of 8 bits (128
+// a turn), 128 items 12.6 | 10.8, 24.8 | 13.5, 50 | 20; 512 items 12.1 | 13.8, 23.4 | 18.9, 50 | 28; 1600 items 18.3 | 23.5, 34 | 38, 75 | 70; of 16 (64 a turn), 512 items
+// 19.4 | 16.9, 54 | 26, 157 | 46; 1600 items 28.6 | 33.6, 75 | 62, 178 | 122.
+// Else shares of 128 keys while there are few, but not many more workgroups than 4096, since empty ones are not free. us without the join, shares of 128 | 256 |
+// 512 | 1024 keys: 512 items of 1 .. 900 keys of 16 bits 16.5 | 18.4 | 27 | 39; 1600 items of 1 .. 1500 keys of 8 bits 47 | 35 | 33 | 38.
 PagedAttnPlan paged_attn_tail_plan(int seqs, int hq, int hkv, int max_len, int turn) {
   const long long items = (long long)seqs * hkv * head_tiles(hq, hkv), unit = 4 * turn;
-  const long long wanted = (4096 + items - 1) / items, most = (max_len + 127) / 128;
-  const long long splits = most < 1 ? 1 : wanted < most ? wanted : most;
+  const long long wanted = (4096 + items - 1) / items, most = (max_len + 127) / 128, turns = (max_len + unit - 1) / unit;
+  const bool one = turns <= 1 + items / 160;
+  const long long splits = one ? 1 : wanted < most ? wanted : most;
   PagedAttnPlan p;
   p.waves = 4;
   const long long chunk = ((max_len + splits - 1) / splits + unit - 1) / unit * unit;

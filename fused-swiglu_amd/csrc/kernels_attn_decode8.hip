@@ -269,31 +269,42 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 2 : 4) void attn_decode8_ke
       }
   }
   __syncthreads();
+  const auto joined = [&](int h, int ch) INLINE -> Share {
+    Share s;
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) s.m = fmaxf(s.m, stats[w][0][h]);
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) s.sum += stats[w][1][h] * scale_of(stats[w][0][h], s.m);
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) s.o += *(const f32x4*)(shares + (w * here + h) * ROW + ch);
+    return s;
+  };
+  const auto write = [&](int h, int ch, const Share& s) INLINE {
+    const float inv = len == 0 && a.before == 0 ? 0.0f : 1.0f / s.sum;
+    unsigned short* op = (unsigned short*)a.o.p + (long long)seq * a.o.token + (long long)(head0 + h) * a.o.head;
+    *(u32x2*)(op + ch) = u32x2{T::pack2(s.o[0] * inv, s.o[1] * inv), T::pack2(s.o[2] * inv, s.o[3] * inv)};
+  };
+  const long long rows = (long long)a.seqs * a.hq, row0 = (long long)seq * a.hq + head0;
+  if (a.before > 0 && splits == 1) {
+    finish_prefix<64 * WAVES, WIDE>(partial, row0, rows, a.before, a.d, here, shares + WAVES * here * ROW, joined, write);
+    return;
+  }
   const bool parted = a.before > 0 || (len > chunk && !bad_len);
   for (int t = threadIdx.x; t < here * WIDE; t += 64 * WAVES) {
     const int h = t / WIDE, ch = (t % WIDE) * 4;
     if (ch >= a.d) continue;
-    float most = NEG_INF, total = 0.0f;
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) most = fmaxf(most, stats[w][0][h]);
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) total += stats[w][1][h] * scale_of(stats[w][0][h], most);
-    f32x4 x = {0, 0, 0, 0};
-#pragma unroll
-    for (int w = 0; w < WAVES; ++w) x += *(const f32x4*)(shares + (w * here + h) * ROW + ch);
+    const Share s = joined(h, ch);
     if (parted) {  // unnormalised sums, maximum and sum of this share, to be joined
       const int slots = a.before + splits;
-      const long long row = ((long long)seq * a.hq + head0 + h) * slots + a.before + split;
-      *(f32x4*)(partial + row * a.d + ch) = x;
+      const long long row = (row0 + h) * slots + a.before + split;
+      *(f32x4*)(partial + row * a.d + ch) = s.o;
       if (ch == 0) {
-        float* ml = partial + (long long)a.seqs * a.hq * slots * a.d + row * 2;
-        ml[0] = most;
-        ml[1] = total;
+        float* ml = partial + rows * slots * a.d + row * 2;
+        ml[0] = s.m;
+        ml[1] = s.sum;
       }
     } else {
-      const float inv = len == 0 ? 0.0f : 1.0f / total;
-      unsigned short* op = (unsigned short*)a.o.p + (long long)seq * a.o.token + (long long)(head0 + h) * a.o.head;
-      *(u32x2*)(op + ch) = u32x2{T::pack2(x[0] * inv, x[1] * inv), T::pack2(x[2] * inv, x[3] * inv)};
+      write(h, ch, s);
     }
   }
 }
@@ -302,7 +313,7 @@ template <class T, int DP, int WAVES>
 hipError_t launch_waves(const PagedAttn8Args& a, const PagedAttnPlan& p, float* partial, hipStream_t stream) {
   const int group = a.hq / a.hkv, tiles = (group + 15) / 16;
   const dim3 grid(a.hkv * tiles, a.seqs, p.splits);
-  const size_t lds = (size_t)WAVES * (group < 16 ? group : 16) * (DP + 4) * sizeof(float);
+  const size_t lds = (size_t)WAVES * (group < 16 ? group : 16) * (DP + 4) * sizeof(float) + (a.before > 0 && p.splits == 1 ? finish_bytes(64 * WAVES) : 0);
   const PagedKv8& c = a.cache;
   const bool whole = c.page_size % 16 == 0 && c.scale_token == 1 && (c.scale_page | c.scale_head) % 4 == 0 &&
                      (((uintptr_t)c.k_scale | (uintptr_t)c.v_scale) & 3) == 0;

@@ -173,6 +173,26 @@ def test_infinities_in_a_prefix(capi, B, Hq, Hkv, D, page, prefix, dtype):
     assert torch.equal(out[~finite].nan_to_num(7.0, INF, -INF), ref[~finite].nan_to_num(7.0, INF, -INF)) and not finite[:, 0, 3].any()
 
 
+@pytest.mark.parametrize("lengths", [[20, 0, 33], [300, 0, 700]])  # own keys in one share, whose workgroup ends the work, and in several
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_infinities_on_both_sides(capi, lengths, dtype):
+    gen = torch.Generator().manual_seed(len(lengths) + lengths[0])
+    prefix, page, D = 200, 16, 64
+    cache, rows, table, pages = setup(gen, prefix, lengths, 1, D, page, dtype, 16)
+    for key, channel, value in ((7, 0, INF), (199, 1, -INF), (60, 2, INF)):
+        rows[1][int(pages[key // page]), 0, key % page, channel] = value
+    for key, channel, value in ((5, 0, INF), (19, 1, INF), (0, 3, -INF), (11, 4, NAN)):
+        rows[1][int(table[0, key // page]), 0, key % page, channel] = value
+    cache = [r.to(dtype).to(DEV) for r in rows]
+    q = randn(gen, 3, 4, D, dtype=dtype)
+    out = capi.attn_shared(q.to(DEV), cache, pages.to(DEV), prefix, table.to(DEV), int32(lengths), max(lengths), D ** -0.5).cpu().double()
+    ref, mag = reference(q, rows, pages, prefix, table, lengths, page, D ** -0.5)
+    finite = torch.isfinite(ref)
+    assert ((out - ref).abs() <= attention.tolerance(ref, mag, dtype, True, prefix + max(lengths)))[finite].all()
+    assert torch.equal(out[~finite].nan_to_num(7.0, INF, -INF), ref[~finite].nan_to_num(7.0, INF, -INF))
+    assert torch.equal((~finite).sum(-1), torch.tensor([[5] * 4, [3] * 4, [3] * 4]))
+
+
 @pytest.mark.parametrize("bits", [8, 16])
 def test_one_side_outweighs_the_other(capi, bits):
     """Scores of the prefix far above or below the own keys': the join keeps what weighs."""
