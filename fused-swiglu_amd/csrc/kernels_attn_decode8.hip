@@ -11,7 +11,9 @@
 // Elements become 16-bit ones by v_cvt_scalef32_pk, two at a time: keys, of which a lane has one in either block, with their scale, values without
 // (theirs multiplies the weight, in fp32), so the second product is bf16 for both types, since a weight times a power of two wants fp32's exponents; the
 // weight is split into two elements, 16 bits, whose products both are added. Where 16 keys lie in one page its descriptor ends with the sequence: rows behind
-// it read as zeros.
+// it read as zeros. Measured: 131071 keys of 8 heads of 128 channels 48 us (5.6 TB/s) + 4.6 for the join (16-bit elements 86 + 4.6); 128 sequences of about 2000 keys, 64
+// heads on 8, 93 us (5.7 TB/s), of 64 channels 51, of 96 81, of 256 171 (6.2); pages of 24 or 9 tokens 102 and 109. Asking for the next keys and values while these are
+// in use is no faster (48 -> 51 us), since other waves' loads fill the time.
 #include "attn.h"
 #include "attn_device.h"
 #include "fsw_device.h"

@@ -12,7 +12,8 @@
 //
 // Measured, 128 channels: 1024 sequences of 32 heads on 8 (4096 rows a key-value head) behind 4096 keys 82 us, 840 TFLOP/s, in 16 bits and in 8; 64 sequences
 // behind 16384 keys (256 rows, 32 shares of 512 keys) 31 us, 560 TFLOP/s; 200 sequences of 64 heads on 8 behind 8000 keys of 8 bits (1600 rows in 7 groups, 4
-// shares: 224 workgroups on 256 CUs) 78 us, 670. What bounds it: the matrix instructions alone take 38 of the 82, and reading LDS, the softmax and asking for
+// shares: 224 workgroups on 256 CUs) 78 us, 670. 256 channels, 4096 rows behind 4096 keys 109 us, 630 (64 rows a workgroup 188), 64 channels, 64 sequences behind
+// 16384 keys 22 us, 390. Eight waves of 16 rows at 128 channels, four a SIMD, read LDS twice as much: 97 us where eight of 32 take 82. What bounds it: the matrix instructions alone take 38 of the 82, and reading LDS, the softmax and asking for
 // tiles each add 14 to 18 to them, since the waves of a SIMD, two, wait at the same barrier and do the same at the same time.
 #include <float.h>
 
@@ -57,14 +58,14 @@ __device__ __forceinline__ Scales scales_of(const PagedKv&) { return {nullptr, n
 
 // WHOLE: the rows of a wave's load, ROWS of them, lie in one page, whose address is wave-uniform then.
 template <class T, class CACHE, int DP, int NB, int WAVES, bool WHOLE>
-__global__ __launch_bounds__(64 * WAVES, DP == 256 ? 1 : 2) void attn_prefix_kernel(PrefixOver<CACHE> a, Divisor by_group, Divisor by_hkv, int chunk,
+__global__ __launch_bounds__(64 * WAVES, DP == 256 && WAVES == 4 ? 1 : 2) void attn_prefix_kernel(PrefixOver<CACHE> a, Divisor by_group, Divisor by_hkv, int chunk,
                                                                                      float lower, float limit) {
   constexpr bool EIGHT = std::is_same<CACHE, PagedKv8>::value, STAGED = EIGHT || !WHOLE;
   constexpr int RB = DP * 2, TILE = KEYS * RB;
   constexpr int SIZE = EIGHT ? 1 : 2, PER_ROW = DP * SIZE / 16, ROWS = 64 / PER_ROW;  // 16-byte vectors of a row, rows of a wave's load
   constexpr int VECS = KEYS / ROWS / WAVES;                                           // loads of keys, and of values, of a wave and tile
   constexpr int KSTEPS = DP / 32, DB = DP / 16, KB = KEYS / 16, WM = 16 * NB, BM = WAVES * WM;
-  constexpr bool AHEAD = DP < 256 || WHOLE;  // fragments are read from LDS a step ahead, if registers allow
+  constexpr bool AHEAD = DP < 256 || (WHOLE && WAVES == 4);  // fragments are read from LDS a step ahead, if registers allow
   constexpr int VBUF = AHEAD ? 2 : 1, VG = AHEAD ? 4 : 1;
   __shared__ __align__(1024) unsigned char k0s[TILE], k1s[TILE];
   __shared__ __align__(1024) unsigned char v0s[TILE], v1s[TILE];
@@ -397,9 +398,7 @@ hipError_t launch_dp(const PrefixOver<CACHE>& a, const PrefixPlan& p, hipStream_
   if constexpr (DP == 128) {
     if (p.rows == 256) return launch<T, CACHE, DP, 2, 8, true>(a, p, stream);
   }
-  if constexpr (DP < 256) {
-    if (p.rows == 128) return launch<T, CACHE, DP, 2, 4, true>(a, p, stream);
-  }
+  if (p.rows == 128) return launch<T, CACHE, DP, DP == 256 ? 1 : 2, DP == 256 ? 8 : 4, true>(a, p, stream);
   return launch<T, CACHE, DP, 1, 4, true>(a, p, stream);
 }
 
@@ -412,8 +411,8 @@ hipError_t launch_typed(const PrefixOver<CACHE>& a, const PrefixPlan& p, hipStre
 
 }  // namespace
 
-// Rows of a workgroup, and shares of the keys. A turn of 64 keys takes 2.7 us with 256 rows on a CU (eight waves), 3.0 with two workgroups of 128 rows, 2.2
-// with one of them; a workgroup's first keys and its sums take about two turns more. Each share costs its sums' way to memory and back, in the join. The plan of least
+// Rows of a workgroup, and shares of the keys. A turn of 64 keys takes 2.7 us with 256 rows on a CU (eight waves of 32), 3.0 with two workgroups of 128 rows (four), 2.2
+// with one of them; of more than 128 channels 3.2 with 128 rows (eight waves of 16, one workgroup on a CU) and 2.85 with 64 (four); a workgroup's first keys and its sums take about two turns more. Each share costs its sums' way to memory and back, in the join. The plan of least
 // estimated time: more shares fill the card's last round better, and are more to join. us of the whole call, 64 sequences of 32 heads on 8 (256 rows a head) behind
 // 16384 keys in 16, 24, 32, 64 shares: 59, 60, 56, 72 with 256 rows, 58, 58, 56, 73 with 128; 200 sequences of 64 heads on 8 (1600 rows) behind 8000 keys of 8 bits in
 // 2, 3, 4, 5, 8 shares 180, 140, 121, 145, 138 with 256 rows, 155, 151, 131, 146, 139 with 128.
@@ -423,14 +422,13 @@ PrefixPlan prefix_plan(int seqs, int hq, int hkv, int d, int len) {
   PrefixPlan best = {0, 0, 0};
   double least = 0.0;
   for (const int size : {64, 128, 256}) {
-    if (size == 256 && (d <= 64 || d > 128)) continue;  // (tiles too small for eight waves' copies; registers)
-    if (size == 128 && d > 128) continue;               // (registers)
-    if (size == 64 && rows > 64 && d <= 128) continue;
+    if (size == 256 && (d <= 64 || d > 128)) continue;  // tiles too small for eight waves' copies; registers
+    if (size == 64 && rows > 64) continue;
     const long long items = hkv * ((rows + size - 1) / size), resident = 256 * (size == 256 || d > 128 ? 1 : 2);
     const long long most = tiles < 64 ? tiles : 64;
     for (long long splits = 1; splits <= most; ++splits) {
       const long long per = (tiles + splits - 1) / splits, work = items * ((tiles + per - 1) / per);
-      const double turn = size == 256 ? 2.7 : work <= 256 ? 2.2 : 3.0;
+      const double turn = d > 128 ? (size == 128 ? 3.2 : 2.85) : size == 256 ? 2.7 : work <= 256 ? 2.2 : 3.0;
       const double us = (double)((work + resident - 1) / resident) * (double)(per + 2) * turn + join * (double)splits;
       if (best.rows == 0 || us < least * (size > best.rows ? 0.95 : 1.0)) least = us, best = {(int)((tiles + per - 1) / per), (int)(per * KEYS), size};
     }

@@ -2,7 +2,9 @@
 // attends to together with itself (attn_prompt). From a cache of 16-bit elements, or of e4m3 elements with a power of two per row.
 //
 // Memory traffic bounds it: every cell is read and every row written once. A workgroup owns some rows in a row; its waves find the
-// sequence and the page of each (a search of 64 offsets at a time), then its threads move 16-byte vectors of the cache.
+// sequence and the page of each (a search of 64 offsets at a time), then its threads move 16-byte vectors of the cache. Measured: 24 sequences of 100 .. 8192
+// tokens, 8 heads of 128 channels, from 8 bits 70 us (4.4 TB/s, two thirds of it written), from 16 bits 65 us (6.0 TB/s); pages of 9 tokens no slower. Four
+// vectors of a thread under way at a time, and stores past the caches, change nothing (71, 69).
 #include "attn.h"
 #include "attn_device.h"
 #include "fsw_device.h"

@@ -71,6 +71,15 @@ def test_append(capi, T, Hq, Hkv, D, rot, interleaved, page, dtype):
     check_append(capi, qkv, Hq, Hkv, rot, interleaved, page, dtype, slots, positions, table, pages, token_major=T % 2 == 1)
 
 
+@pytest.mark.parametrize("T,Hq,Hkv,D,rot,page", [(21, 6, 2, 80, 40, 8), (9, 4, 4, 112, 56, 16), (5, 2, 1, 32, 24, 3), (3, 1, 1, 256, 248, 16), (70, 3, 1, 16, 8, 16)])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_append_of_halves_that_are_multiples_of_four(capi, T, Hq, Hkv, D, rot, page, dtype):
+    gen = torch.Generator().manual_seed(T + D)
+    qkv = randn(gen, T, Hq + 2 * Hkv, D, dtype=dtype)
+    table, positions, pages = angles(gen, T + 7, rot), torch.randperm(T + 7, generator=gen)[:T], T // page + 2
+    check_append(capi, qkv, Hq, Hkv, rot, False, page, dtype, torch.randperm(pages * page, generator=gen)[:T], positions, table, pages, token_major=T % 2 == 1)
+
+
 @pytest.mark.parametrize("dtype", [BF, HF])
 def test_append_rows_at_the_edges_of_the_types(capi, dtype):
     """Zeros of both signs, the smallest and the largest numbers, largest elements next to 448 scales, ties, infinities and NaN among the others."""

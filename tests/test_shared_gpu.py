@@ -90,10 +90,10 @@ def joined(q, rows, pages, prefix, table, lengths, page, scale):
     return o, mag
 
 
-@pytest.mark.parametrize("D", [112, 128])
+@pytest.mark.parametrize("D", [112, 128, 256])
 @pytest.mark.parametrize("bits,dtype,infinities", [(8, BF, False), (8, HF, False), (16, BF, False), (16, HF, False), (16, BF, True), (16, HF, True)])
 def test_shared_by_thousands_of_rows(capi, bits, dtype, D, infinities):
-    """256 rows a workgroup, the last with 192 of them, in nine shares, the last of which ends inside a tile."""
+    """256 rows a workgroup (128 of 256 channels), the last with 192 (64) of them, in several shares, the last of which ends inside a tile."""
     gen = torch.Generator().manual_seed(D + bits)
     B, Hq, page, prefix = 99, 64, 16, 4000
     lengths = [(7 * b) % 23 for b in range(B)]
