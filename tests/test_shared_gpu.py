@@ -173,6 +173,28 @@ def test_infinities_in_a_prefix(capi, B, Hq, Hkv, D, page, prefix, dtype):
     assert torch.equal(out[~finite].nan_to_num(7.0, INF, -INF), ref[~finite].nan_to_num(7.0, INF, -INF)) and not finite[:, 0, 3].any()
 
 
+@pytest.mark.parametrize("B,Hq,Hkv,D,page,prefix", [(3, 4, 2, 64, 16, 150), (3, 4, 2, 80, 5, 150), (40, 16, 2, 128, 32, 500), (20, 16, 2, 256, 16, 190)])
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_what_is_no_number_in_a_prefix_of_8_bits(capi, B, Hq, Hkv, D, page, prefix, dtype):
+    """An element, or a row's scale: NaN in its channel, or in all, of the heads that read it, in every sequence. A scale of 2^-127 is a number."""
+    gen = torch.Generator().manual_seed(D + prefix)
+    lengths = [(5 * b) % 30 for b in range(B)]
+    cache, rows, table, pages = setup(gen, prefix, lengths, Hkv, D, page, dtype, 8)
+    args = (pages.to(DEV), prefix, table.to(DEV), int32(lengths), max(lengths), D ** -0.5)
+    q = randn(gen, B, Hq, D, dtype=dtype)
+    for which, value, key, channel in ((1, 127, 7, 3), (1, 255, prefix - 1, D - 1), (0, 127, 20, 7), (3, 255, 66, None), (2, 255, 0, None), (3, 0, 9, None), (2, 0, 9, None)):
+        raw = cache[which].view(torch.uint8)
+        at = (int(pages[key // page]), Hkv - 1, key % page) + (() if channel is None else (channel,))
+        kept = int(raw[at])
+        raw[at] = value
+        ref, mag = reference(q, rows_of(cache), pages, prefix, table, lengths, page, D ** -0.5)
+        out = capi.attn_shared(q.to(DEV), cache, *args).cpu().double()
+        finite = torch.isfinite(ref)
+        assert ((out - ref).abs() <= attention.tolerance(ref, mag, dtype, True, prefix + 30))[finite].all()
+        assert torch.isnan(out[~finite]).all() and finite[:, 0].all() and finite.all() == (value == 0)
+        raw[at] = kept
+
+
 @pytest.mark.parametrize("lengths", [[20, 0, 33], [300, 0, 700]])  # own keys in one share, whose workgroup ends the work, and in several
 @pytest.mark.parametrize("dtype", [BF, HF])
 def test_infinities_on_both_sides(capi, lengths, dtype):
