@@ -109,7 +109,9 @@ def test_attn_shared_codes_and_scratch(capi, cache, eight):
     assert v(ld=3) == capi.E_LD and v(prefix=P + 2) == v(table=P + 1) == capi.E_ALIGN
     assert ws(0, 3, 4, 2, 64, -1, 64) == ws(0, 0, 4, 2, 64, 40, 64) == ws(0, 3, 4, 2, 64, 0, 64) == ws(0, 3, 5, 2, 64, 40, 64) == 0
     need = ws(0, 3, 4, 2, 64, 40, 64)
-    assert need % (3 * 4 * (64 + 2) * 4) == 0 and need >= 2 * 3 * 4 * 66 * 4          # a share of the prefix, one of own keys
+    share = 3 * 4 * (64 + 2) * 4
+    assert need % share == 0 and need >= share                                       # a share of the prefix; few own keys need none
+    assert ws(0, 3, 4, 2, 64, 40, 2000) % share == 0 and ws(0, 3, 4, 2, 64, 40, 2000) >= need + 2 * share
     for work, size, code in ((None, 0, capi.E_WORKSPACE), (P, need - 1, capi.E_WORKSPACE), (P + 4, need, capi.E_ALIGN)):
         assert call(0, 3, 4, 2, 64, P, 256, 64, sound, P, 40, P, 4, P, 64, 0.125, P, 256, 64, work, size, None) == code
     for B, Hq, plen, n in ((1, 1024, 1 << 29, 1 << 29), (65535, 1024, 1 << 20, 100), (7, 14, 12345, 0), (200, 64, 8000, 1500)):
