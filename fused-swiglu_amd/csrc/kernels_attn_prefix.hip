@@ -385,7 +385,9 @@ hipError_t launch(const PrefixOver<CACHE>& a, const PrefixPlan& p, hipStream_t s
   constexpr int BM = 16 * NB * WAVES;
   const int group = a.hq / a.hkv;
   const float shift = shift_of<T>(a.keys);
-  const float lower = fmaxf(shift / a.scale_log2, -FLT_MAX / 4), limit = fmaxf((shift + SLACK<T>) / a.scale_log2, -FLT_MAX / 4);
+  // in units of the scores; finite for the least scales too, or no share would have a maximum to be joined by
+  auto bounded = [](float x) { return fminf(fmaxf(x, -FLT_MAX / 4), FLT_MAX / 4); };
+  const float lower = bounded(shift / a.scale_log2), limit = bounded((shift + SLACK<T>) / a.scale_log2);
   const dim3 grid(a.hkv * ((a.seqs * group + BM - 1) / BM), p.splits);
   attn_prefix_kernel<T, CACHE, DP, NB, WAVES, WHOLE><<<grid, 64 * WAVES, 0, stream>>>(a, Divisor(group), Divisor(a.hkv), p.chunk, lower, limit);
   return hipGetLastError();

@@ -224,6 +224,33 @@ def test_one_side_outweighs_the_other(capi, bits):
         check(capi, gen, 200, [1, 40, 90], 4, 2, 128, 16, HF, bits, q_scale=q_scale)
 
 
+@pytest.mark.parametrize("bits", [8, 16])
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("scale", [1.2e-38, 2.0e-38, 1e-30])
+def test_scales_that_leave_all_weights_alike(capi, bits, dtype, scale):
+    """Scores times the scale are nothing: means over prefix and own keys, none of which is lost whatever the units of the maximum."""
+    gen = torch.Generator().manual_seed(bits)
+    prefix, lengths = 150, [100, 0, 700]
+    cache, rows, table, pages = setup(gen, prefix, lengths, 2, 64, 16, dtype, bits)
+    q = randn(gen, 3, 4, 64, dtype=dtype)
+    out = capi.attn_shared(q.to(DEV), cache, pages.to(DEV), prefix, table.to(DEV), int32(lengths), 700, scale)
+    ref, mag = reference(q, rows, pages, prefix, table, lengths, 16, scale)
+    assert ((out.cpu().double() - ref).abs() <= attention.tolerance(ref, mag, dtype, True, prefix + 700)).all()
+
+
+@pytest.mark.parametrize("kw", [dict(token_major=True), dict(wide_scales=True), dict(token_major=True, wide_scales=True)])
+@pytest.mark.parametrize("Hq,Hkv,D,page", [(4, 2, 64, 16), (6, 3, 128, 8), (4, 2, 80, 5), (4, 4, 256, 16)])
+def test_caches_in_any_order(capi, Hq, Hkv, D, page, kw):
+    gen = torch.Generator().manual_seed(D)
+    check(capi, gen, 150, [1, 0, 40], Hq, Hkv, D, page, BF, 8, **kw)
+    cache, rows, table, pages = setup(gen, 150, [1, 0, 40], Hkv, D, page, HF, 16, **kw)
+    cache = [c.transpose(1, 2).contiguous().transpose(1, 2) for c in cache]
+    q = randn(gen, 1, Hq, D, dtype=HF).expand(3, -1, -1)                                # one query for all
+    out = capi.attn_shared(q.to(DEV), cache, pages.to(DEV), 150, table.to(DEV), int32([1, 0, 40]), 40, 0.1)
+    ref, mag = reference(q, rows, pages, 150, table, [1, 0, 40], page, 0.1)
+    assert ((out.cpu().double() - ref).abs() <= attention.tolerance(ref, mag, HF, True, 190)).all()
+
+
 @pytest.mark.parametrize("dtype,size", [(BF, 3.0e38), (HF, 65504.0)])
 def test_values_as_large_as_the_type_has(capi, dtype, size):
     gen = torch.Generator().manual_seed(9)
