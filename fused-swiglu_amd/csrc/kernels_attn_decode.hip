@@ -426,7 +426,8 @@ hipError_t launch_typed(const PagedAttnArgs& a, const PagedAttnPlan& p, float* p
 
 // Shares of the keys, and waves of a workgroup.
 // Few (sequence, key-value head, 16 query heads) items: workgroups of many waves, of which a CU holds one; as many shares as give every CU one, of
-// at least 512 keys, because the launch that joins them costs 4.5 us. (One sequence of 131071 keys, 8 key-value heads: 87 + 4.6 us; four
+// at least 512 keys, because the launch that joins them costs 4.5 us; a turn and a half of 8-bit elements, 768 keys, is still one (12 items of 700 keys 10.4 us,
+// in two shares 12.0; of 1024 keys 13.1 and 12.5). (One sequence of 131071 keys, 8 key-value heads: 87 + 4.6 us; four
 // waves a workgroup and 128 shares 91 + 5.5.) Empty shares cost more there than they level (four sequences of 20 .. 32000 keys: 68 us in 8
 // shares, 81 in 32, 96 in 63).
 // Many items: four waves, of which a CU holds four workgroups, so 1024 fill the card. Below that they do so only if they are split, and
@@ -454,6 +455,7 @@ PagedAttnPlan paged_attn_plan(int seqs, int hq, int hkv, int d, int max_len, int
   const long long least = few ? 512 : 1024;
   long long splits = (max_len + least - 1) / least;
   if (splits > wanted) splits = wanted;
+  if (2 * (long long)max_len <= 3 * unit) splits = 1;
   if (splits < 1) splits = 1;
   const long long chunk = ((max_len + splits - 1) / splits + unit - 1) / unit * unit;
   p.chunk = (int)(chunk < unit ? unit : chunk);
