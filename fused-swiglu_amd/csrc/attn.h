@@ -112,6 +112,7 @@ struct PagedAttnOver {
   RowsOut o;
   int keys;    // bound of all keys of a query, those of a shared prefix among them
   int before;  // shares of the prefix, whose sums lie before those of the sequences' own keys
+  bool ends;   // a workgroup has all of a sequence's own keys, and adds the prefix's shares itself
 };
 using PagedAttnArgs = PagedAttnOver<PagedKv>;
 using PagedAttn8Args = PagedAttnOver<PagedKv8>;
@@ -120,11 +121,12 @@ struct PagedAttnPlan {
   int chunk;   // keys of each
   int waves;   // of a workgroup
   size_t workspace_bytes;
+  bool ends;  // of own keys behind a prefix: no join follows
 };
 // turn: keys of a wave at a time, 16 or 32
 PagedAttnPlan paged_attn_plan(int seqs, int hq, int hkv, int d, int max_len, int turn);
 // of the keys behind a shared prefix, whose shares are joined anyway
-PagedAttnPlan paged_attn_tail_plan(int seqs, int hq, int hkv, int max_len, int turn);
+PagedAttnPlan paged_attn_tail_plan(int seqs, int hq, int hkv, int d, int max_len, int turn, int before);
 // The sums of a share, a row per (sequence, query head, share): d floats each, behind all rows the maximum and sum of each.
 inline size_t partial_bytes(long long rows, int d) { return (size_t)rows * (size_t)(d + 2) * 4; }
 hipError_t launch_attn_decode(int dtype, const PagedAttnArgs& a, const PagedAttnPlan& p, void* workspace, hipStream_t stream);
@@ -152,7 +154,7 @@ struct PrefixOver {
 struct PrefixPlan {
   int splits, chunk, rows;  // rows: of a workgroup
 };
-PrefixPlan prefix_plan(int seqs, int hq, int hkv, int d, int len);
+PrefixPlan prefix_plan(int seqs, int hq, int hkv, int d, int len, int element_bytes);
 hipError_t launch_attn_prefix(int dtype, const PrefixOver<PagedKv>& a, const PrefixPlan& p, hipStream_t stream);
 hipError_t launch_attn_prefix8(int dtype, const PrefixOver<PagedKv8>& a, const PrefixPlan& p, hipStream_t stream);
 

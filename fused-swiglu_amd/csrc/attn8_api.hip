@@ -46,7 +46,7 @@ struct Of;
 template <>
 struct Of<fsw_kv_cache> {
   typedef fsw::PagedKv Paged;
-  static constexpr int TURN = 16;
+  static constexpr int TURN = 16, BYTES = 2;
   static int heads(int dtype, int64_t hq, int64_t hkv, int64_t d) { return check_heads(dtype, hq, hkv, d); }
   static int cache(const fsw_kv_cache* c, int64_t d, int64_t heads) { return fsw::checks::check_cache(c, d, heads); }
   static fsw::PagedKv kernel(const fsw_kv_cache* c) { return fsw::checks::paged(c); }
@@ -55,7 +55,7 @@ struct Of<fsw_kv_cache> {
 template <>
 struct Of<fsw_kv_cache8> {
   typedef fsw::PagedKv8 Paged;
-  static constexpr int TURN = 32;
+  static constexpr int TURN = 32, BYTES = 1;
   static int heads(int dtype, int64_t hq, int64_t hkv, int64_t d) { return check_heads8(dtype, hq, hkv, d); }
   static int cache(const fsw_kv_cache8* c, int64_t d, int64_t heads) { return check_cache(c, d, heads); }
   static fsw::PagedKv8 kernel(const fsw_kv_cache8* c) { return paged(c); }
@@ -143,13 +143,13 @@ struct SharedPlan {
   int slots;
   size_t bytes;
 };
-SharedPlan shared_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t prefix_len, int64_t max_len, int turn) {
+SharedPlan shared_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t prefix_len, int64_t max_len, int turn, int element_bytes) {
   SharedPlan p;
   p.prefix = fsw::PrefixPlan{0, 0, 0};
-  if (prefix_len > 0) p.prefix = fsw::prefix_plan((int)B, (int)Hq, (int)Hkv, (int)D, (int)prefix_len);
-  p.own = prefix_len > 0 ? fsw::paged_attn_tail_plan((int)B, (int)Hq, (int)Hkv, (int)max_len, turn)
+  if (prefix_len > 0) p.prefix = fsw::prefix_plan((int)B, (int)Hq, (int)Hkv, (int)D, (int)prefix_len, element_bytes);
+  p.own = prefix_len > 0 ? fsw::paged_attn_tail_plan((int)B, (int)Hq, (int)Hkv, (int)D, (int)max_len, turn, p.prefix.splits)
                          : fsw::paged_attn_plan((int)B, (int)Hq, (int)Hkv, (int)D, (int)max_len, turn);
-  p.slots = p.prefix.splits + (p.own.splits > 1 ? p.own.splits : 0);  // a workgroup that has all own keys joins the prefix's shares itself
+  p.slots = p.prefix.splits + (p.own.ends ? 0 : p.own.splits);  // a workgroup that has all own keys joins the prefix's shares itself
   p.bytes = prefix_len > 0 ? fsw::partial_bytes(B * Hq * p.slots, (int)D) : p.own.workspace_bytes;
   return p;
 }
@@ -159,7 +159,7 @@ size_t shared_bytes(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, in
   if (Of<CACHE>::heads(dtype, Hq, Hkv, D) != FSW_OK || B < 1 || B > MAX_SEQS || prefix_len < 0 || prefix_len > MAX_LEN || max_len < 0 ||
       max_len > MAX_LEN - prefix_len)
     return 0;
-  return shared_plan(B, Hq, Hkv, D, prefix_len, max_len, Of<CACHE>::TURN).bytes;
+  return shared_plan(B, Hq, Hkv, D, prefix_len, max_len, Of<CACHE>::TURN, Of<CACHE>::BYTES).bytes;
 }
 
 template <class CACHE>
@@ -167,7 +167,7 @@ int attend(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, const void*
            const int32_t* prefix_pages, int64_t prefix_len, const int32_t* block_table, int64_t table_ld, const int32_t* lengths,
            int64_t max_len, float scale, void* O, int64_t o_seq, int64_t o_head, void* workspace, size_t workspace_bytes, void* stream) {
   if (B == 0) return FSW_OK;
-  const SharedPlan plan = shared_plan(B, Hq, Hkv, D, prefix_len, max_len, Of<CACHE>::TURN);
+  const SharedPlan plan = shared_plan(B, Hq, Hkv, D, prefix_len, max_len, Of<CACHE>::TURN, Of<CACHE>::BYTES);
   if (plan.bytes > 0 && (!workspace || workspace_bytes < plan.bytes)) return FSW_E_WORKSPACE;
   if (plan.bytes > 0 && !aligned(workspace, 16)) return FSW_E_ALIGN;
   CHECK(fsw::device_status());
@@ -186,9 +186,9 @@ int attend(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, const void*
   a.q = {Q, q_seq, q_head}, a.cache = paged_cache;
   a.block_table = block_table, a.table_ld = table_ld, a.lengths = lengths, a.max_len = (int)max_len;
   a.scale_log2 = scale * LOG2E;
-  a.o = {O, o_seq, o_head}, a.keys = (int)(prefix_len + max_len), a.before = plan.prefix.splits;
+  a.o = {O, o_seq, o_head}, a.keys = (int)(prefix_len + max_len), a.before = plan.prefix.splits, a.ends = plan.own.ends;
   CHECK(fsw::launch_status(decode(dtype, a, plan.own, workspace, (hipStream_t)stream)));
-  if (prefix_len == 0 || plan.own.splits == 1) return FSW_OK;
+  if (prefix_len == 0 || plan.own.ends) return FSW_OK;
   return fsw::launch_status(fsw::launch_attn_join(dtype, fsw::JoinArgs{a.seqs, a.hq, a.d, lengths, a.max_len, a.before, a.o}, plan.own.chunk,
                                                   plan.own.splits, (const float*)workspace, (hipStream_t)stream));
 }

@@ -85,7 +85,7 @@ int fsw_attn_decode(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, co
   a.cache = max_len > 0 ? paged(cache) : fsw::PagedKv{nullptr, nullptr, 0, 16, 0, 0, 0, fsw::Divisor(16)};
   a.block_table = block_table, a.table_ld = table_ld, a.lengths = lengths, a.max_len = (int)max_len;
   a.scale_log2 = scale * LOG2E;
-  a.o = {O, o_seq, o_head}, a.keys = a.max_len, a.before = 0;
+  a.o = {O, o_seq, o_head}, a.keys = a.max_len, a.before = 0, a.ends = false;
   const fsw::PagedAttnPlan plan = fsw::paged_attn_plan(a.seqs, a.hq, a.hkv, a.d, a.max_len, 16);
   if (plan.workspace_bytes > 0 && (!workspace || workspace_bytes < plan.workspace_bytes)) return FSW_E_WORKSPACE;
   if (plan.workspace_bytes > 0 && !aligned(workspace, 16)) return FSW_E_ALIGN;

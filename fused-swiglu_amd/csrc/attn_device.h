@@ -138,7 +138,7 @@ struct Share {
   }
   // shares first, first + step .. below `used`, at these channels of them (d floats each) and their maxima and sums
   __device__ __forceinline__ void add_all(const float* sums, const float* ml, int first, int step, int used, int d) {
-    constexpr int BATCH = 4;  // under way at a time
+    constexpr int BATCH = 8;  // under way at a time
     for (int i = first; i < used; i += step * BATCH) {
       f32x4 x[BATCH];
       float xm[BATCH], xs[BATCH];

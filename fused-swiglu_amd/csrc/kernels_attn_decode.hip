@@ -316,7 +316,7 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 2 : 4) void attn_decode_ker
     *(u32x2*)(op + ch) = u32x2{T::pack2(s.o[0] * inv, s.o[1] * inv), T::pack2(s.o[2] * inv, s.o[3] * inv)};
   };
   const long long rows = (long long)a.seqs * a.hq, row0 = (long long)seq * a.hq + head0;
-  if (a.before > 0 && splits == 1) {
+  if (a.ends) {
     finish_prefix<64 * WAVES, WIDE>(partial, row0, rows, a.before, a.d, here, shares + WAVES * here * ROW, joined, write);
     return;
   }
@@ -389,7 +389,7 @@ hipError_t launch_waves(const PagedAttnArgs& a, const PagedAttnPlan& p, float* p
   const int tiles = head_tiles(a.hq, a.hkv);
   const int group = a.hq / a.hkv;
   const dim3 grid(a.hkv * tiles, a.seqs, p.splits);
-  const size_t lds = (size_t)WAVES * (group < 16 ? group : 16) * (DP + 4) * sizeof(float) + (a.before > 0 && p.splits == 1 ? finish_bytes(64 * WAVES) : 0);
+  const size_t lds = (size_t)WAVES * (group < 16 ? group : 16) * (DP + 4) * sizeof(float) + (a.ends ? finish_bytes(64 * WAVES) : 0);
   const auto kernel = a.cache.page_size % 16 == 0 ? attn_decode_kernel<T, DP, true, WAVES> : attn_decode_kernel<T, DP, false, WAVES>;
   kernel<<<grid, 64 * WAVES, lds, stream>>>(a, lift_of<T>(a.keys), p.chunk, group, tiles, partial);
   return hipGetLastError();
@@ -443,6 +443,7 @@ hipError_t launch_typed(const PagedAttnArgs& a, const PagedAttnPlan& p, float* p
 PagedAttnPlan paged_attn_plan(int seqs, int hq, int hkv, int d, int max_len, int turn) {
   const long long items = (long long)seqs * hkv * head_tiles(hq, hkv);
   PagedAttnPlan p;
+  p.ends = false;
   const bool whole = max_len <= 2560;  // not split where items are many
   const bool few = items < 128 || (whole && (items <= 256 ? max_len > 64 : items <= 512 && max_len > 512));
   p.waves = few ? (d > 128 ? 8 : 16) : 4;
@@ -471,16 +472,20 @@ PagedAttnPlan paged_attn_plan(int seqs, int hq, int hkv, int d, int max_len, int
 // 19.4 | 16.9, 54 | 26, 157 | 46; 1600 items 28.6 | 33.6, 75 | 62, 178 | 122.
 // Else shares of 128 keys while there are few, but not many more workgroups than 4096, since empty ones are not free. us without the join, shares of 128 | 256 |
 // 512 | 1024 keys: 512 items of 1 .. 900 keys of 16 bits 16.5 | 18.4 | 27 | 39; 1600 items of 1 .. 1500 keys of 8 bits 47 | 35 | 33 | 38.
-PagedAttnPlan paged_attn_tail_plan(int seqs, int hq, int hkv, int max_len, int turn) {
+PagedAttnPlan paged_attn_tail_plan(int seqs, int hq, int hkv, int d, int max_len, int turn, int before) {
   const long long items = (long long)seqs * hkv * head_tiles(hq, hkv), unit = 4 * turn;
   const long long wanted = (4096 + items - 1) / items, most = (max_len + 127) / 128, turns = (max_len + unit - 1) / unit;
   const bool one = turns <= 1 + items / 160;
+  // threads that take the shares of four channels in turn: with more than 16 shares each, the join is faster, which has more threads (2 sequences of 16 heads on 2
+  // behind 26064 keys in 64 shares 30.7 | 23.9 us, 64 of 32 on 8 in 32, 16 a thread, 40.3 | 43.6)
+  const int group = hq / hkv < 16 ? hq / hkv : 16, results = group * (d <= 64 ? 16 : d <= 128 ? 32 : 64), parts = results < 256 ? 256 / results : 1;
   const long long splits = one ? 1 : wanted < most ? wanted : most;
   PagedAttnPlan p;
   p.waves = 4;
   const long long chunk = ((max_len + splits - 1) / splits + unit - 1) / unit * unit;
   p.chunk = (int)(chunk < unit ? unit : chunk);
   p.splits = max_len > 0 ? (int)((max_len + p.chunk - 1) / p.chunk) : 1;
+  p.ends = p.splits == 1 && before <= 16 * parts;
   p.workspace_bytes = 0;
   return p;
 }

@@ -287,7 +287,7 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 2 : 4) void attn_decode8_ke
     *(u32x2*)(op + ch) = u32x2{T::pack2(s.o[0] * inv, s.o[1] * inv), T::pack2(s.o[2] * inv, s.o[3] * inv)};
   };
   const long long rows = (long long)a.seqs * a.hq, row0 = (long long)seq * a.hq + head0;
-  if (a.before > 0 && splits == 1) {
+  if (a.ends) {
     finish_prefix<64 * WAVES, WIDE>(partial, row0, rows, a.before, a.d, here, shares + WAVES * here * ROW, joined, write);
     return;
   }
@@ -315,7 +315,7 @@ template <class T, int DP, int WAVES>
 hipError_t launch_waves(const PagedAttn8Args& a, const PagedAttnPlan& p, float* partial, hipStream_t stream) {
   const int group = a.hq / a.hkv, tiles = (group + 15) / 16;
   const dim3 grid(a.hkv * tiles, a.seqs, p.splits);
-  const size_t lds = (size_t)WAVES * (group < 16 ? group : 16) * (DP + 4) * sizeof(float) + (a.before > 0 && p.splits == 1 ? finish_bytes(64 * WAVES) : 0);
+  const size_t lds = (size_t)WAVES * (group < 16 ? group : 16) * (DP + 4) * sizeof(float) + (a.ends ? finish_bytes(64 * WAVES) : 0);
   const PagedKv8& c = a.cache;
   const bool whole = c.page_size % 16 == 0 && c.scale_token == 1 && (c.scale_page | c.scale_head) % 4 == 0 &&
                      (((uintptr_t)c.k_scale | (uintptr_t)c.v_scale) & 3) == 0;

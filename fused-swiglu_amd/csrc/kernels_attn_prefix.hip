@@ -417,21 +417,24 @@ hipError_t launch_typed(const PrefixOver<CACHE>& a, const PrefixPlan& p, hipStre
 // with one of them; of more than 128 channels 3.2 with 128 rows (eight waves of 16, one workgroup on a CU) and 2.85 with 64 (four); a workgroup's first keys and its sums take about two turns more. Each share costs its sums' way to memory and back, in the join. The plan of least
 // estimated time: more shares fill the card's last round better, and are more to join. us of the whole call, 64 sequences of 32 heads on 8 (256 rows a head) behind
 // 16384 keys in 16, 24, 32, 64 shares: 59, 60, 56, 72 with 256 rows, 58, 58, 56, 73 with 128; 200 sequences of 64 heads on 8 (1600 rows) behind 8000 keys of 8 bits in
-// 2, 3, 4, 5, 8 shares 180, 140, 121, 145, 138 with 256 rows, 155, 151, 131, 146, 139 with 128.
-PrefixPlan prefix_plan(int seqs, int hq, int hkv, int d, int len) {
+// 2, 3, 4, 5, 8 shares 180, 140, 121, 145, 138 with 256 rows, 155, 151, 131, 146, 139 with 128. Few rows want many shares, as long as memory is not what bounds them: one
+// sequence of 8 heads on one behind 65536 keys in 32, 64, 128 shares 52, 34, 26, 8 of 32 on 4 58, 42, 45.
+PrefixPlan prefix_plan(int seqs, int hq, int hkv, int d, int len, int element_bytes) {
   const long long rows = (long long)seqs * (hq / hkv), tiles = (len + KEYS - 1) / KEYS;
-  const double join = 2.0 * (double)seqs * hq * d * 4 / 4e6;  // us a share, written and read
+  const double join = 0.05 + 2.0 * (double)seqs * hq * d * 4 / 4e6;              // us a share: a step of the join, written and read
+  const double memory = 2.0 * (double)len * hkv * d * element_bytes / 4e6;
   PrefixPlan best = {0, 0, 0};
   double least = 0.0;
   for (const int size : {64, 128, 256}) {
     if (size == 256 && (d <= 64 || d > 128)) continue;  // tiles too small for eight waves' copies; registers
     if (size == 64 && rows > 64) continue;
     const long long items = hkv * ((rows + size - 1) / size), resident = 256 * (size == 256 || d > 128 ? 1 : 2);
-    const long long most = tiles < 64 ? tiles : 64;
+    const long long most = tiles < 128 ? tiles : 128;
     for (long long splits = 1; splits <= most; ++splits) {
       const long long per = (tiles + splits - 1) / splits, work = items * ((tiles + per - 1) / per);
       const double turn = d > 128 ? (size == 128 ? 3.2 : 2.85) : size == 256 ? 2.7 : work <= 256 ? 2.2 : 3.0;
-      const double us = (double)((work + resident - 1) / resident) * (double)(per + 2) * turn + join * (double)splits;
+      const double turns = (double)((work + resident - 1) / resident) * (double)(per + 2) * turn;
+      const double us = (turns > memory ? turns : memory) + join * (double)splits;
       if (best.rows == 0 || us < least * (size > best.rows ? 0.95 : 1.0)) least = us, best = {(int)((tiles + per - 1) / per), (int)(per * KEYS), size};
     }
   }
