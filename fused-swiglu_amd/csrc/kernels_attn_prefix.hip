@@ -94,7 +94,7 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 && WAVES == 4 ? 1 : 2) void a
     }
   }
 
-  // Load j of a wave is rows first_row(j) .. + ROWS - 1 of a tile, PER_ROW lanes each. Lane l knows the page of the tile's key l.
+  // Load j of a wave is rows first_row(j) .. + ROWS - 1 of a tile, PER_ROW lanes each. Lane l knows the page of the tile's key l, and its cell.
   const int lrow = lane / PER_ROW, lvec = lane % PER_ROW;
   auto first_row = [&](int j) INLINE -> int { return (j * WAVES + wave) * ROWS; };
   auto locate = [&](int at) INLINE -> int {
@@ -103,39 +103,71 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 && WAVES == 4 ? 1 : 2) void a
   };
   const unsigned char* kc = (const unsigned char*)a.cache.k + kvh * a.cache.head * SIZE;
   const unsigned char* vc = (const unsigned char*)a.cache.v + kvh * a.cache.head * SIZE;
-  const int stride = (int)a.cache.token * SIZE;
+  const int stride = (int)a.cache.token * SIZE, span = (ROWS - 1) * stride + a.d * SIZE;
+  unsigned koff[STAGED ? 1 : VECS], voff[STAGED ? 1 : VECS];  // a lane's vectors, in the cells of a load
+#pragma unroll
+  for (int j = 0; j < (STAGED ? 1 : VECS); ++j) {
+    const int row = first_row(j) + lrow, kch = (lvec ^ k_swizzle<DP>(row)) * 8, vch = (lvec ^ v_swizzle<DP>(row)) * 8;
+    koff[j] = STAGED ? (lvec * 16 < a.d * SIZE ? (unsigned)(lrow * stride + lvec * 16) : OOB_OFFSET)
+                     : (kch < a.d ? (unsigned)(lrow * stride + kch * 2) : OOB_OFFSET);
+    voff[j] = STAGED ? koff[j] : (vch < a.d ? (unsigned)(lrow * stride + vch * 2) : OOB_OFFSET);
+  }
   u32x4 kr[STAGED ? VECS : 1], vr[STAGED ? VECS : 1];   // a tile under way
   unsigned km[EIGHT ? VECS : 1], vm[EIGHT ? VECS : 1];  // its scales
   bool bad = false;
-  // Asks for the keys or the values of the tile at `at`, whose pages are known. Rows behind the end are zeros and touch no memory.
-  auto ask = [&](bool value, int at, int pages, unsigned char* to) INLINE {
-    if (!value) bad |= (unsigned)pages >= (unsigned)a.cache.pages;
-    const unsigned char* cells = value ? vc : kc;
+  // Asks for the keys and values of the tile at `at`, whose pages are known. Rows behind the end are zeros and touch no memory. Places are the lanes' work,
+  // all keys' at once, since a CU's four SIMDs share one scalar unit.
+  auto ask = [&](int at, int pages, unsigned char* kto, unsigned char* vto) INLINE {
+    const bool inside = (unsigned)pages < (unsigned)a.cache.pages;
+    bad |= !inside;
+    const int own = at + lane < end ? at + lane : end - 1, place = own - a.cache.per_page.quotient(own) * a.cache.page_size;
+    const long long page = inside ? pages : 0, cell = (page * a.cache.page + place * a.cache.token) * SIZE;
+    const long long mark = EIGHT ? page * scales.page + place * scales.token : 0;
+    auto of_row = [&](long long x, int row) INLINE -> long long {  // wave-uniform
+      const unsigned lo = __builtin_amdgcn_readlane((unsigned)x, row), hi = __builtin_amdgcn_readlane((unsigned)((unsigned long long)x >> 32), row);
+      return (long long)(((unsigned long long)hi << 32) | lo);
+    };
+    auto of_lane = [&](long long x, int row) INLINE -> long long {
+      const unsigned lo = __shfl((unsigned)x, row), hi = __shfl((unsigned)((unsigned long long)x >> 32), row);
+      return (long long)(((unsigned long long)hi << 32) | lo);
+    };
 #pragma unroll
     for (int j = 0; j < VECS; ++j) {
-      const int row = first_row(j) + lrow, key = at + first_row(j) + (WHOLE ? 0 : lrow);
-      const int n = WHOLE ? __builtin_amdgcn_readlane(pages, first_row(j)) : __shfl(pages, row);
-      const long long page = (unsigned)n < (unsigned)a.cache.pages ? n : 0;
-      const int known = key < end ? key : end - 1, place = known - a.cache.per_page.quotient(known) * a.cache.page_size;
-      const long long where = (page * a.cache.page + place * a.cache.token) * SIZE;
-      const long long mark = EIGHT ? kvh * scales.head + page * scales.page + place * scales.token : 0;
-      const unsigned char* marks = value ? scales.v : scales.k;
       if constexpr (WHOLE) {
-        const int real = end - key < ROWS ? end - key : ROWS;
-        const auto rsrc = make_rsrc(cells + where, real > 0 ? (real - 1) * stride + a.d * SIZE : 0);
+        const long long where = of_row(cell, first_row(j));
+        int size = span, real = ROWS;
+        if (__builtin_expect(at + KEYS > end, 0)) {
+          asm volatile("");
+          real = end - at - first_row(j);
+          real = real < 0 ? 0 : real < ROWS ? real : ROWS;
+          size = real > 0 ? (real - 1) * stride + a.d * SIZE : 0;
+        }
+        const auto krsrc = make_rsrc(kc + where, size), vrsrc = make_rsrc(vc + where, size);
         if constexpr (EIGHT) {
-          const auto mrsrc = make_rsrc(marks + mark, real > 0 ? (real - 1) * (int)scales.token + 1 : 0);
-          (value ? vm : km)[j] = __builtin_amdgcn_raw_buffer_load_b8(mrsrc, lrow * (int)scales.token, 0, 0);
-          (value ? vr : kr)[j] = buf_load16(rsrc, lvec * 16 < a.d ? (unsigned)(lrow * stride + lvec * 16) : OOB_OFFSET);
+          const long long at_mark = of_row(mark, first_row(j)) + kvh * scales.head;
+          const int marks = real > 0 ? (real - 1) * (int)scales.token + 1 : 0, mine = lrow * (int)scales.token;
+          km[j] = __builtin_amdgcn_raw_buffer_load_b8(make_rsrc(scales.k + at_mark, marks), mine, 0, 0);
+          vm[j] = __builtin_amdgcn_raw_buffer_load_b8(make_rsrc(scales.v + at_mark, marks), mine, 0, 0);
+          kr[j] = buf_load16(krsrc, koff[0]);
+          vr[j] = buf_load16(vrsrc, koff[0]);
         } else {
-          const int ch = (lvec ^ (value ? v_swizzle<DP>(row) : k_swizzle<DP>(row))) * 8;
-          copy_to_lds(rsrc, ch < a.d ? (unsigned)(lrow * stride + ch * 2) : OOB_OFFSET, to + (j * WAVES + wave) * 1024);
+          copy_to_lds(krsrc, koff[j], kto + (j * WAVES + wave) * 1024);
+          copy_to_lds(vrsrc, voff[j], vto + (j * WAVES + wave) * 1024);
         }
       } else {
-        u32x4 x = {0, 0, 0, 0};
-        if (key < end && lvec * (16 / SIZE) < a.d) x = *(const u32x4*)(cells + where + lvec * 16);
-        (value ? vr : kr)[j] = x;
-        if constexpr (EIGHT) (value ? vm : km)[j] = key < end ? marks[mark] : 127;
+        const int row = first_row(j) + lrow;
+        const long long where = of_lane(cell, row);
+        const bool real = at + row < end;
+        kr[j] = vr[j] = u32x4{0, 0, 0, 0};
+        if (real && koff[0] != OOB_OFFSET) {
+          kr[j] = *(const u32x4*)(kc + where + lvec * 16);
+          vr[j] = *(const u32x4*)(vc + where + lvec * 16);
+        }
+        if constexpr (EIGHT) {
+          const long long at_mark = of_lane(mark, row) + kvh * scales.head;
+          km[j] = real ? scales.k[at_mark] : 127;
+          vm[j] = real ? scales.v[at_mark] : 127;
+        }
       }
     }
   };
@@ -289,8 +321,7 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 && WAVES == 4 ? 1 : 2) void a
     // Tile t is in buffer t % 2. At the barrier the tile has landed, and every wave has read the one before.
     auto turn = [&](int at, const unsigned char* ks, unsigned char* vs, unsigned char* knext, unsigned char* vnext) INLINE {
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-      ask(KEY, at + KEYS, pages, knext);
-      ask(VALUE, at + KEYS, pages, vnext);
+      ask(at + KEYS, pages, knext, vnext);
       pages = locate(at + 2 * KEYS);
       if (__builtin_expect(again, 0)) {
 #pragma unroll 1
@@ -305,8 +336,7 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 && WAVES == 4 ? 1 : 2) void a
       put(KEY, knext);
       put(VALUE, vnext);
     };
-    ask(KEY, begin, pages, k0s);
-    ask(VALUE, begin, pages, v0s);
+    ask(begin, pages, k0s, v0s);
     pages = locate(begin + KEYS);
     put(KEY, k0s);
     put(VALUE, v0s);
