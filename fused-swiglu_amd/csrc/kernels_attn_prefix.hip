@@ -10,11 +10,12 @@
 // the page numbers of a tile are asked for a tile ahead. Elements of 8 bits pass through registers, where they
 // become keys and values of the element type. The sum of the weights is a product too, with values that are all 1.
 //
-// Measured, 128 channels: 1024 sequences of 32 heads on 8 (4096 rows a key-value head) behind 4096 keys 82 us, 840 TFLOP/s, in 16 bits and in 8; 64 sequences
-// behind 16384 keys (256 rows, 32 shares of 512 keys) 31 us, 560 TFLOP/s; 200 sequences of 64 heads on 8 behind 8000 keys of 8 bits (1600 rows in 7 groups, 4
+// Measured, 128 channels: 1024 sequences of 32 heads on 8 (4096 rows a key-value head) behind 4096 keys 78 us, 880 TFLOP/s, in 8 bits 84; 64 sequences
+// behind 16384 keys (256 rows, 32 shares of 512 keys) 29.5 us, 580 TFLOP/s; 200 sequences of 64 heads on 8 behind 8000 keys of 8 bits (1600 rows in 7 groups, 4
 // shares: 224 workgroups on 256 CUs) 78 us, 670. 256 channels, 4096 rows behind 4096 keys 109 us, 630 (64 rows a workgroup 188), 64 channels, 64 sequences behind
-// 16384 keys 22 us, 390. Eight waves of 16 rows at 128 channels, four a SIMD, read LDS twice as much: 97 us where eight of 32 take 82. What bounds it: the matrix instructions alone take 38 of the 82, and reading LDS, the softmax and asking for
-// tiles each add 14 to 18 to them, since the waves of a SIMD, two, wait at the same barrier and do the same at the same time.
+// 16384 keys 22 us, 390. Eight waves of 16 rows at 128 channels, four a SIMD, read LDS twice as much: 97 us where eight of 32 take 82. What bounds it: the matrix
+// instructions alone take 38 of the 78; the softmax, LDS reads and asking for tiles add 10 to 14 each. Two halves of the waves half a tile apart, so that a SIMD has matrix and
+// vector instructions at the same time (rings of four tiles), take the same 78: the vector work alone is 57 us there, the matrix work alone 44.
 #include <float.h>
 
 #include <type_traits>
@@ -33,15 +34,34 @@ constexpr unsigned ONES = 0x3f803f80u;
 template <>
 inline constexpr unsigned ONES<Fp16> = 0x3c003c00u;
 
-// Largest value of lanes l, l ^ 16, l ^ 32, l ^ 48 (max_over_groups), NaN if one is: v_maximum3 takes scores as they come, where v_max wants them
-// made canonical first, an instruction each.
-__device__ __forceinline__ float maximum_over_groups(float x) {
-  float y = x;
-  asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1\n\ts_nop 1" : "+v"(x), "+v"(y));
-  x = __builtin_elementwise_maximum(x, y);
-  y = x;
-  asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1\n\ts_nop 1" : "+v"(x), "+v"(y));
-  return __builtin_elementwise_maximum(x, y);
+// Largest of each x over lanes l, l ^ 16, l ^ 32, l ^ 48, NaN if one is: v_maximum3 takes scores as they come, where v_max wants them made canonical
+// first, an instruction each. Two at a time share the waits.
+__device__ __forceinline__ void maximum_over_groups(float (&x)[1]) {
+  float y = x[0];
+  asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1\n\ts_nop 1" : "+v"(x[0]), "+v"(y));
+  x[0] = y = __builtin_elementwise_maximum(x[0], y);
+  asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1\n\ts_nop 1" : "+v"(x[0]), "+v"(y));
+  x[0] = __builtin_elementwise_maximum(x[0], y);
+}
+__device__ __forceinline__ void maximum_over_groups(float (&x)[2]) {
+  float y[2] = {x[0], x[1]};
+  asm volatile("s_nop 1\n\tv_permlane16_swap_b32 %0, %1\n\tv_permlane16_swap_b32 %2, %3\n\ts_nop 1" : "+v"(x[0]), "+v"(y[0]), "+v"(x[1]), "+v"(y[1]));
+  for (int n = 0; n < 2; ++n) x[n] = y[n] = __builtin_elementwise_maximum(x[n], y[n]);
+  asm volatile("s_nop 1\n\tv_permlane32_swap_b32 %0, %1\n\tv_permlane32_swap_b32 %2, %3\n\ts_nop 1" : "+v"(x[0]), "+v"(y[0]), "+v"(x[1]), "+v"(y[1]));
+  for (int n = 0; n < 2; ++n) x[n] = __builtin_elementwise_maximum(x[n], y[n]);
+}
+
+// A lane's place in a tile of values, for channels 16 i on of the first 32 keys (16 keys more have the same swizzle), and the fragment of 16 channels x 32 keys
+// there: keys 4 g .. 4 g + 3 and 16 + 4 g .. 19 + 4 g of lane group g.
+template <int DP>
+__device__ __forceinline__ int value_place(int i, int col, int grp) {
+  const int key = 4 * grp + (col >> 2), ch = i * 2 + ((col & 3) >> 1);
+  return key * DP * 2 + (ch ^ v_swizzle<DP>(key)) * 16 + (col & 1) * 8;
+}
+template <int DP>
+__device__ __forceinline__ u32x4 value_fragment(const unsigned char* place, int st) {
+  const u32x2 lo = read_tr(place + st * 64 * DP), hi = read_tr(place + (st * 64 + 32) * DP);
+  return u32x4{lo[0], lo[1], hi[0], hi[1]};
 }
 
 // 16 bytes a lane, to LDS from `to` on
@@ -193,6 +213,19 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 && WAVES == 4 ? 1 : 2) void a
     }
   };
 
+  // Places of a lane's fragments in a tile: of the first 16 keys, by 32 channels, and of the first 32 values, by 16 channels.
+  unsigned kfrag[KSTEPS], vfrag[DB];
+#pragma unroll
+  for (int st = 0; st < KSTEPS; ++st) kfrag[st] = col * RB + ((4 * st + grp) ^ k_swizzle<DP>(col)) * 16;
+#pragma unroll
+  for (int i = 0; i < DB; ++i) vfrag[i] = value_place<DP>(i, col, grp);
+  // a turn's own, or each is added to each buffer's address ahead of the loop, a register for every sum
+  auto keep = [&]() INLINE {
+#pragma unroll
+    for (int st = 0; st < KSTEPS; ++st) asm volatile("" : "+v"(kfrag[st]));
+#pragma unroll
+    for (int i = 0; i < DB; ++i) asm volatile("" : "+v"(vfrag[i]));
+  };
   f32x4 o[DB][NB], s[KB][NB];
   f32x4 sum[NB];  // the same in all four: a channel of values that are all 1
   float m[NB];
@@ -210,8 +243,7 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 && WAVES == 4 ? 1 : 2) void a
   auto scores = [&](const unsigned char* ks) INLINE {
     u32x4 kf[2][KSTEPS];
     auto key_fragment = [&](int kb, int st) INLINE -> u32x4 {
-      const int key = kb * 16 + col;
-      return *(const u32x4*)(ks + key * RB + ((4 * st + grp) ^ k_swizzle<DP>(key)) * 16);
+      return *(const u32x4*)(ks + kfrag[st] + kb * 16 * RB);
     };
     auto key_fragments = [&](int kb) INLINE {
 #pragma unroll
@@ -251,9 +283,11 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 && WAVES == 4 ? 1 : 2) void a
       float t = s[0][n][0];
 #pragma unroll
       for (int i = 1; i < 4 * KB; ++i) t = __builtin_elementwise_maximum(t, s[i / 4][n][i % 4]);
-      top[n] = maximum_over_groups(t);
-      above |= top[n] > m[n] + limit;
+      top[n] = t;
     }
+    maximum_over_groups(top);
+#pragma unroll
+    for (int n = 0; n < NB; ++n) above |= top[n] > m[n] + limit;
     if (__any(above)) {
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
@@ -286,7 +320,7 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 && WAVES == 4 ? 1 : 2) void a
     u32x4 vf[VBUF][VG];
     auto value_group = [&](int g) INLINE {
 #pragma unroll
-      for (int x = 0; x < VG; ++x) vf[g % VBUF][x] = value_fragment<DP>(vs, (g * VG + x) / DB, (g * VG + x) % DB, col, grp);
+      for (int x = 0; x < VG; ++x) vf[g % VBUF][x] = value_fragment<DP>(vs + vfrag[(g * VG + x) % DB], (g * VG + x) / DB);
     };
     if (AHEAD) value_group(0);
 #pragma unroll
@@ -321,6 +355,7 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 && WAVES == 4 ? 1 : 2) void a
     // Tile t is in buffer t % 2. At the barrier the tile has landed, and every wave has read the one before.
     auto turn = [&](int at, const unsigned char* ks, unsigned char* vs, unsigned char* knext, unsigned char* vnext) INLINE {
       asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+      keep();
       ask(at + KEYS, pages, knext, vnext);
       pages = locate(at + 2 * KEYS);
       if (__builtin_expect(again, 0)) {
