@@ -112,7 +112,7 @@ struct PagedAttnOver {
   RowsOut o;
   int keys;    // bound of all keys of a query, those of a shared prefix among them
   int before;  // shares of the prefix, whose sums lie before those of the sequences' own keys
-  bool ends;   // a workgroup has all of a sequence's own keys, and adds the prefix's shares itself
+  bool ends;   // a workgroup that has all of a sequence's own keys adds the prefix's shares itself
 };
 using PagedAttnArgs = PagedAttnOver<PagedKv>;
 using PagedAttn8Args = PagedAttnOver<PagedKv8>;
@@ -121,7 +121,7 @@ struct PagedAttnPlan {
   int chunk;   // keys of each
   int waves;   // of a workgroup
   size_t workspace_bytes;
-  bool ends;  // of own keys behind a prefix: no join follows
+  bool ends;  // of own keys behind a prefix: the join is for sequences of more than one share
 };
 // turn: keys of a wave at a time, 16 or 32
 PagedAttnPlan paged_attn_plan(int seqs, int hq, int hkv, int d, int max_len, int turn);
@@ -135,6 +135,7 @@ struct JoinArgs {
   int seqs, hq, d;
   const int* lengths;
   int max_len, before;
+  bool ends;  // sequences of one share are done
   RowsOut o;
 };
 hipError_t launch_attn_join(int dtype, const JoinArgs& a, int chunk, int splits, const float* partial, hipStream_t stream);

@@ -149,7 +149,7 @@ SharedPlan shared_plan(int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t pr
   if (prefix_len > 0) p.prefix = fsw::prefix_plan((int)B, (int)Hq, (int)Hkv, (int)D, (int)prefix_len, element_bytes);
   p.own = prefix_len > 0 ? fsw::paged_attn_tail_plan((int)B, (int)Hq, (int)Hkv, (int)D, (int)max_len, turn, p.prefix.splits)
                          : fsw::paged_attn_plan((int)B, (int)Hq, (int)Hkv, (int)D, (int)max_len, turn);
-  p.slots = p.prefix.splits + (p.own.ends ? 0 : p.own.splits);  // a workgroup that has all own keys joins the prefix's shares itself
+  p.slots = p.prefix.splits + p.own.splits;
   p.bytes = prefix_len > 0 ? fsw::partial_bytes(B * Hq * p.slots, (int)D) : p.own.workspace_bytes;
   return p;
 }
@@ -188,8 +188,8 @@ int attend(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, const void*
   a.scale_log2 = scale * LOG2E;
   a.o = {O, o_seq, o_head}, a.keys = (int)(prefix_len + max_len), a.before = plan.prefix.splits, a.ends = plan.own.ends;
   CHECK(fsw::launch_status(decode(dtype, a, plan.own, workspace, (hipStream_t)stream)));
-  if (prefix_len == 0 || plan.own.ends) return FSW_OK;
-  return fsw::launch_status(fsw::launch_attn_join(dtype, fsw::JoinArgs{a.seqs, a.hq, a.d, lengths, a.max_len, a.before, a.o}, plan.own.chunk,
+  if (prefix_len == 0 || (plan.own.ends && plan.own.splits == 1)) return FSW_OK;
+  return fsw::launch_status(fsw::launch_attn_join(dtype, fsw::JoinArgs{a.seqs, a.hq, a.d, lengths, a.max_len, a.before, a.ends, a.o}, plan.own.chunk,
                                                   plan.own.splits, (const float*)workspace, (hipStream_t)stream));
 }
 

@@ -156,13 +156,13 @@ struct Share {
   }
 };
 
-// The end of a workgroup that has all of its sequence's own keys behind a shared prefix: adds the prefix's shares to what `own(h, ch)` gives for
+// The end of a workgroup that has all of its sequence's own keys behind a shared prefix: adds the prefix's shares, the first of `slots` a row, to what `own(h, ch)` gives for
 // query head h < here and four channels from ch on, and hands each result to `out(h, ch, share)`. Where there are more threads than results, groups of
 // threads take the shares in turn. All of the workgroup's threads come here; `room`: THREADS f32x4 and 2 THREADS floats of LDS.
 template <int THREADS, int WIDE, class Own, class Out>
-__device__ __forceinline__ void finish_prefix(const float* partial, long long row0, long long rows, int before, int d, int here, float* room, Own own, Out out) {
+__device__ __forceinline__ void finish_prefix(const float* partial, long long row0, long long rows, int before, int slots, int d, int here, float* room, Own own, Out out) {
   const int items = here * WIDE, parts = items < THREADS ? THREADS / items : 1;
-  const float* ml = partial + rows * before * d;
+  const float* ml = partial + rows * slots * d;
   f32x4* os = (f32x4*)room;
   float* ms = room + 4 * THREADS;
   for (int from = 0; from < items; from += THREADS) {  // once, if parts > 1
@@ -170,7 +170,7 @@ __device__ __forceinline__ void finish_prefix(const float* partial, long long ro
     const int h = item / WIDE, ch = item % WIDE * 4;
     const bool mine = part < parts && item < items && ch < d;
     Share s;
-    if (mine) s.add_all(partial + (row0 + h) * before * d + ch, ml + (row0 + h) * before * 2, part, parts, before, d);
+    if (mine) s.add_all(partial + (row0 + h) * slots * d + ch, ml + (row0 + h) * slots * 2, part, parts, before, d);
     if (parts > 1) {
       if (mine && part > 0) {
         os[t] = s.o;

@@ -316,17 +316,17 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 2 : 4) void attn_decode_ker
     *(u32x2*)(op + ch) = u32x2{T::pack2(s.o[0] * inv, s.o[1] * inv), T::pack2(s.o[2] * inv, s.o[3] * inv)};
   };
   const long long rows = (long long)a.seqs * a.hq, row0 = (long long)seq * a.hq + head0;
-  if (a.ends) {
-    finish_prefix<64 * WAVES, WIDE>(partial, row0, rows, a.before, a.d, here, shares + WAVES * here * ROW, joined, write);
+  const int slots = a.before + splits;
+  const bool parted = len > chunk && !bad_len;
+  if (a.ends && !parted) {
+    finish_prefix<64 * WAVES, WIDE>(partial, row0, rows, a.before, slots, a.d, here, shares + WAVES * here * ROW, joined, write);
     return;
   }
-  const bool parted = a.before > 0 || (len > chunk && !bad_len);
   for (int t = threadIdx.x; t < here * WIDE; t += 64 * WAVES) {
     const int h = t / WIDE, ch = (t % WIDE) * 4;
     if (ch >= a.d) continue;
     const Share s = joined(h, ch);
-    if (parted) {  // unnormalised sums, maximum and sum of this share, to be joined
-      const int slots = a.before + splits;
+    if (parted || a.before > 0) {  // unnormalised sums, maximum and sum of this share, to be joined
       const long long row = (row0 + h) * slots + a.before + split;
       *(f32x4*)(partial + row * a.d + ch) = s.o;
       if (ch == 0) {
@@ -350,7 +350,7 @@ __global__ __launch_bounds__(256) void attn_join_kernel(JoinArgs a, int chunk, i
   const int width = a.d / 4, rows = TH / width, part = lane / width, at = lane % width;
   const int len = a.lengths[seq];
   const bool parted = len > chunk && len <= a.max_len;
-  if (!parted && a.before == 0) return;
+  if (!parted && (a.before == 0 || a.ends)) return;
   const int used = a.before + (parted ? (len + chunk - 1) / chunk : 1);  // <= slots: len <= max_len
   const int slots = a.before + splits;
   const long long row = ((long long)seq * a.hq + head) * slots;
@@ -412,7 +412,7 @@ hipError_t launch_dp(const PagedAttnArgs& a, const PagedAttnPlan& p, float* part
   const hipError_t e = p.waves == 4 ? launch_waves<T, DP, 4>(a, p, partial, stream)
                                     : launch_waves<T, DP, MANY_WAVES<DP>>(a, p, partial, stream);
   if (e != hipSuccess || p.splits == 1 || a.before > 0) return e;  // who has a prefix joins all shares
-  return launch_join<T>(JoinArgs{a.seqs, a.hq, a.d, a.lengths, a.max_len, 0, a.o}, p.chunk, p.splits, partial, stream);
+  return launch_join<T>(JoinArgs{a.seqs, a.hq, a.d, a.lengths, a.max_len, 0, false, a.o}, p.chunk, p.splits, partial, stream);
 }
 
 template <class T>
@@ -485,7 +485,7 @@ PagedAttnPlan paged_attn_tail_plan(int seqs, int hq, int hkv, int d, int max_len
   const long long chunk = ((max_len + splits - 1) / splits + unit - 1) / unit * unit;
   p.chunk = (int)(chunk < unit ? unit : chunk);
   p.splits = max_len > 0 ? (int)((max_len + p.chunk - 1) / p.chunk) : 1;
-  p.ends = p.splits == 1 && before <= 16 * parts;
+  p.ends = before <= 16 * parts;
   p.workspace_bytes = 0;
   return p;
 }

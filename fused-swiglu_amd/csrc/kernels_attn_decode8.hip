@@ -287,17 +287,17 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 2 : 4) void attn_decode8_ke
     *(u32x2*)(op + ch) = u32x2{T::pack2(s.o[0] * inv, s.o[1] * inv), T::pack2(s.o[2] * inv, s.o[3] * inv)};
   };
   const long long rows = (long long)a.seqs * a.hq, row0 = (long long)seq * a.hq + head0;
-  if (a.ends) {
-    finish_prefix<64 * WAVES, WIDE>(partial, row0, rows, a.before, a.d, here, shares + WAVES * here * ROW, joined, write);
+  const int slots = a.before + splits;
+  const bool parted = len > chunk && !bad_len;
+  if (a.ends && !parted) {
+    finish_prefix<64 * WAVES, WIDE>(partial, row0, rows, a.before, slots, a.d, here, shares + WAVES * here * ROW, joined, write);
     return;
   }
-  const bool parted = a.before > 0 || (len > chunk && !bad_len);
   for (int t = threadIdx.x; t < here * WIDE; t += 64 * WAVES) {
     const int h = t / WIDE, ch = (t % WIDE) * 4;
     if (ch >= a.d) continue;
     const Share s = joined(h, ch);
-    if (parted) {  // unnormalised sums, maximum and sum of this share, to be joined
-      const int slots = a.before + splits;
+    if (parted || a.before > 0) {  // unnormalised sums, maximum and sum of this share, to be joined
       const long long row = (row0 + h) * slots + a.before + split;
       *(f32x4*)(partial + row * a.d + ch) = s.o;
       if (ch == 0) {
@@ -343,7 +343,7 @@ hipError_t launch_attn_decode8(int dtype, const PagedAttn8Args& a, const PagedAt
   float* partial = (float*)workspace;
   const hipError_t e = dtype == FSW_BF16 ? launch_typed<Bf16>(a, p, partial, stream) : launch_typed<Fp16>(a, p, partial, stream);
   if (e != hipSuccess || p.splits == 1 || a.before > 0) return e;  // who has a prefix joins all shares
-  return launch_attn_join(dtype, JoinArgs{a.seqs, a.hq, a.d, a.lengths, a.max_len, 0, a.o}, p.chunk, p.splits, partial, stream);
+  return launch_attn_join(dtype, JoinArgs{a.seqs, a.hq, a.d, a.lengths, a.max_len, 0, false, a.o}, p.chunk, p.splits, partial, stream);
 }
 
 }  // namespace fsw
