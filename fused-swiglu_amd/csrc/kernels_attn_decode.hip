@@ -469,7 +469,8 @@ PagedAttnPlan paged_attn_plan(int seqs, int hq, int hkv, int d, int max_len, int
 // Four waves (sixteen, unsplit: 15.3 against 7.8 us with 512 items of 1 .. 60 keys of 8 bits, 42 against 28 with 4000). Unsplit, a workgroup adds the prefix's shares itself
 // and there is no join, 5 to 9 us; that pays while its turns are few, or items many. us, unsplit | in shares and joined, up to 400, 1500, 4000 keys: of 8 bits (128
 // a turn), 128 items 12.6 | 10.8, 24.8 | 13.5, 50 | 20; 512 items 12.1 | 13.8, 23.4 | 18.9, 50 | 28; 1600 items 18.3 | 23.5, 34 | 38, 75 | 70; of 16 (64 a turn), 512 items
-// 19.4 | 16.9, 54 | 26, 157 | 46; 1600 items 28.6 | 33.6, 75 | 62, 178 | 122.
+// 19.4 | 16.9, 54 | 26, 157 | 46; 1600 items 28.6 | 33.6, 75 | 62, 178 | 122. In shares, sequences of one share end there as well, and the join is the others' (200
+// sequences of up to 1500 keys of 8 bits, in shares of 512, 112.6 -> 110.9 for the whole call).
 // Else shares of 128 keys while there are few, but not many more workgroups than 4096, since empty ones are not free. us without the join, shares of 128 | 256 |
 // 512 | 1024 keys: 512 items of 1 .. 900 keys of 16 bits 16.5 | 18.4 | 27 | 39; 1600 items of 1 .. 1500 keys of 8 bits 47 | 35 | 33 | 38.
 PagedAttnPlan paged_attn_tail_plan(int seqs, int hq, int hkv, int d, int max_len, int turn, int before) {
