@@ -27,20 +27,19 @@ struct Cells16 {
 };
 template <class T>
 struct Cells8 {
-  static constexpr int VEC = 16;
+  static constexpr int VEC = 8;
   PagedKv8 c;
   __device__ __forceinline__ void move(bool value, long long page, int place, int head, int ch, unsigned short* to) const {
-    const u32x4 x = __builtin_nontemporal_load((const u32x4*)((value ? c.v : c.k) + page * c.page + head * c.head + place * c.token + ch));
+    const u32x2 x = __builtin_nontemporal_load((const u32x2*)((value ? c.v : c.k) + page * c.page + head * c.head + place * c.token + ch));
     const float up = scale_value((value ? c.v_scale : c.k_scale)[page * c.scale_page + head * c.scale_head + place * c.scale_token]);
-    u32x4 o[2];
+    u32x4 o;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < 2; ++i) {
       const f32x2 lo = unpack_e4m3<false>(x[i]), hi = unpack_e4m3<true>(x[i]);
-      o[i / 2][i % 2 * 2] = T::pack2(lo[0] * up, lo[1] * up);
-      o[i / 2][i % 2 * 2 + 1] = T::pack2(hi[0] * up, hi[1] * up);
+      o[2 * i] = T::pack2(lo[0] * up, lo[1] * up);
+      o[2 * i + 1] = T::pack2(hi[0] * up, hi[1] * up);
     }
-    *(u32x4*)to = o[0];
-    *(u32x4*)(to + 8) = o[1];
+    *(u32x4*)to = o;
   }
 };
 
