@@ -11,9 +11,10 @@
 // Elements become 16-bit ones by v_cvt_scalef32_pk, two at a time: keys, of which a lane has one in either block, with their scale, values without
 // (theirs multiplies the weight, in fp32), so the second product is bf16 for both types, since a weight times a power of two wants fp32's exponents; the
 // weight is split into two elements, 16 bits, whose products both are added. Where 16 keys lie in one page its descriptor ends with the sequence: rows behind
-// it read as zeros. Measured: 131071 keys of 8 heads of 128 channels 48 us (5.6 TB/s) + 4.6 for the join (16-bit elements 86 + 4.6); 128 sequences of about 2000 keys, 64
-// heads on 8, 93 us (5.7 TB/s), of 64 channels 51, of 96 81, of 256 171 (6.2); pages of 24 or 9 tokens 102 and 109. Asking for the next keys and values while these are
-// in use is no faster (48 -> 51 us), since other waves' loads fill the time.
+// it read as zeros. Measured: 131071 keys of 8 heads of 128 channels 46 us (5.8 TB/s) + 4.6 for the join (16-bit elements 86 + 4.6); 128 sequences of about 2000 keys, 64
+// heads on 8, 91 us (5.8 TB/s), of 64 channels 52, of 96 77, of 256 171 (6.2); pages of 24 or 9 tokens 101 and 104. Loads are non-temporal, but for keys of 65 .. 128
+// channels, whose lines two loads share half and half (non-temporal | not: 128 channels 93.2 | 91.0 us, 96 81 | 77, pages of 9 109 | 104; 64 51.6 | 52.8, 256 171.5 | 174.4). Asking for the next keys and values while these are
+// in use is no faster (48 -> 51 us then), since other waves' loads fill the time.
 #include "attn.h"
 #include "attn_device.h"
 #include "fsw_device.h"
@@ -116,7 +117,7 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 2 : 4) void attn_decode8_ke
         ks[h] = __builtin_amdgcn_raw_buffer_load_b8(make_rsrc(ksc + mark, 16), keys > 0 ? col : (int)OOB_OFFSET, 0, 0);
         vs[h] = __builtin_amdgcn_raw_buffer_load_b32(make_rsrc(vsc + mark, 16), (int)four, 0, 0);
 #pragma unroll
-        for (int s = 0; s < KV; ++s) kf[h][s] = buf_load16_stream(krsrc, koff[s]);
+        for (int s = 0; s < KV; ++s) kf[h][s] = DP == 128 ? buf_load16(krsrc, koff[s]) : buf_load16_stream(krsrc, koff[s]);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           if constexpr (VW == 4) {
@@ -142,7 +143,8 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 2 : 4) void attn_decode8_ke
         for (int s = 0; s < KV; ++s) {
           const int ch = s * 64 + grp * 16;
           kf[h][s] = u32x4{0, 0, 0, 0};
-          if (ch < a.d) kf[h][s] = __builtin_nontemporal_load((const u32x4*)(kc + where + ch));
+          const u32x4* p = (const u32x4*)(kc + where + ch);
+          if (ch < a.d) kf[h][s] = DP == 128 ? *p : __builtin_nontemporal_load(p);
         }
         const int value_mark = vsc[mark];
         ks[h] = ksc[mark], vs[h] = 0;
