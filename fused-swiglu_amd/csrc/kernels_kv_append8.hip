@@ -10,7 +10,8 @@
 // the cache: 2^n threads, the least that hold the head, are a group that finds its largest element by lane exchanges. Where halves of a head are
 // turned into each other a thread's channels are two times 8, partners of each other; halves of 4 channels more than that find partners in memory, 4 at a time, and others
 // one by one. Measured: one token of 32 + 8 heads of 128 channels 4.2 .. 5.2 us, 8192 tokens of 64 + 8 74 us (4.8 TB/s, half of it written; a copy reaches 4.9), of
-// 32 + 8 51 us; of 80 channels, all rotated, 44 us, half of them 56 (one by one 110), interleaved or in halves alike.
+// 32 + 8 51 us; of 80 channels, all rotated, 41 us, half of them 53 (one by one 110), interleaved or in halves alike. Loads are non-temporal where heads are whole
+// lines (64 + 8 heads of 128 channels 76 | 81 us, 32 + 8 of 256 89 | 98), and not where lines are shared (of 80 44 | 41, of 96 47 | 45, of 112, half rotated, 69 | 61).
 #include <float.h>
 
 #include "attn.h"
@@ -58,7 +59,8 @@ __device__ __forceinline__ float to_odd(double x) {
 
 enum { HALVES = 0, INTERLEAVED = 1, SCALAR = 2, QUARTERS = 3 };
 
-template <class T, int STYLE>
+// LINES: heads share no line of 128 bytes, and none is asked for twice.
+template <class T, int STYLE, bool LINES>
 __global__ __launch_bounds__(256) void kv_append8_kernel(Append8Args a, Divisor per_token, int tokens_per_block, int lanes_log2) {
   // blockIdx.y = 256 threads of a token that needs more, else the block has several tokens
   const int local = gridDim.y == 1 ? per_token.quotient(threadIdx.x) : 0;
@@ -86,8 +88,9 @@ __global__ __launch_bounds__(256) void kv_append8_kernel(Append8Args a, Divisor 
 #pragma unroll
   for (int i = 0; i < 16; ++i) x[i] = 0.0f;
   if (here) {
-    unpack8<T>(__builtin_nontemporal_load((const u32x4*)(p + ca)), x);
-    unpack8<T>(__builtin_nontemporal_load((const u32x4*)(p + cb)), x + 8);
+    const u32x4 *pa = (const u32x4*)(p + ca), *pb = (const u32x4*)(p + cb);
+    unpack8<T>(LINES ? __builtin_nontemporal_load(pa) : *pa, x);
+    unpack8<T>(LINES ? __builtin_nontemporal_load(pb) : *pb, x + 8);
     // pairs of the thread's channels turned by (c, s); keys in 64 bits
     auto turn = [&](float& u, float& v, float c, float s) __attribute__((always_inline)) {
       if (is_q) {
@@ -215,20 +218,22 @@ __global__ __launch_bounds__(256) void kv_append8_kernel(Append8Args a, Divisor 
   *(u32x4*)(out + cb) = pack8<T>(x + 8);
 }
 
-template <class T, int STYLE>
+template <class T, int STYLE, bool LINES>
 hipError_t launch(const Append8Args& a, hipStream_t stream) {
   const int lanes_log2 = ceil_log2(a.d / 16), per_token = (a.hq + 2 * a.hkv) << lanes_log2;
   const int per_block = per_token <= 256 ? 256 / per_token : 1;
   const dim3 grid((a.tokens + per_block - 1) / per_block, (per_token + 255) / 256);
-  kv_append8_kernel<T, STYLE><<<grid, 256, 0, stream>>>(a, Divisor(per_token), per_block, lanes_log2);
+  kv_append8_kernel<T, STYLE, LINES><<<grid, 256, 0, stream>>>(a, Divisor(per_token), per_block, lanes_log2);
   return hipGetLastError();
 }
 
 template <class T>
 hipError_t launch_typed(const Append8Args& a, hipStream_t stream) {
-  if (a.rot % 8 != 0) return launch<T, SCALAR>(a, stream);
-  if (!a.interleaved && a.rot % 16 != 0) return launch<T, QUARTERS>(a, stream);
-  return a.interleaved ? launch<T, INTERLEAVED>(a, stream) : launch<T, HALVES>(a, stream);
+  if (a.rot % 8 != 0) return launch<T, SCALAR, false>(a, stream);
+  if (!a.interleaved && a.rot % 16 != 0) return launch<T, QUARTERS, false>(a, stream);
+  const bool lines = a.d % 64 == 0;
+  if (a.interleaved) return lines ? launch<T, INTERLEAVED, true>(a, stream) : launch<T, INTERLEAVED, false>(a, stream);
+  return lines ? launch<T, HALVES, true>(a, stream) : launch<T, HALVES, false>(a, stream);
 }
 
 }  // namespace
