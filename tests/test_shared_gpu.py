@@ -289,6 +289,21 @@ def test_workspace_and_refusals(capi):
     assert e.value.code == capi.E_SHAPE
 
 
+@pytest.mark.parametrize("bits", [8, 16])
+def test_scratch_may_hold_anything(capi, bits):
+    """Sequences of one share of own keys beside longer ones, NaN all over the scratch; one row of pages for all."""
+    gen = torch.Generator().manual_seed(11)
+    lengths = [5, 700, 0, 64, 300, 128]
+    cache, rows, table, pages = setup(gen, 1000, [700], 2, 64, 16, BF, bits)
+    q, table = randn(gen, 6, 8, 64), table.expand(6, -1)
+    L = capi.lib()
+    need = (L.fsw_attn_shared8_workspace_bytes if bits == 8 else L.fsw_attn_shared_workspace_bytes)(0, 6, 8, 2, 64, 1000, 700)
+    scratch = torch.full((need,), 255, dtype=torch.uint8, device=DEV)
+    out = capi.attn_shared(q.to(DEV), cache, pages.to(DEV), 1000, table[:1].to(DEV).expand(6, -1), int32(lengths), 700, 0.125, workspace=scratch)
+    ref, mag = reference(q, rows, pages, 1000, table, lengths, 16, 0.125)
+    assert ((out.cpu().double() - ref).abs() <= attention.tolerance(ref, mag, BF, True, 1700)).all()
+
+
 # ---------------------------------------------------------------------------------------------- together
 
 @pytest.mark.parametrize("dtype,name", [(BF, "bf16"), (HF, "fp16")])
