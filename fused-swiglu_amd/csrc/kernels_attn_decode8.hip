@@ -291,7 +291,7 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 ? 2 : 4) void attn_decode8_ke
   const long long rows = (long long)a.seqs * a.hq, row0 = (long long)seq * a.hq + head0;
   const int slots = a.before + splits;
   const bool parted = len > chunk && !bad_len;
-  if (a.ends && !parted) {
+  if (WAVES == 4 && a.ends && !parted) {
     finish_prefix<64 * WAVES, WIDE>(partial, row0, rows, a.before, slots, a.d, here, shares + WAVES * here * ROW, joined, write);
     return;
   }
