@@ -13,12 +13,15 @@ taken once and attended to together (`attn_shared_*`). `--turns N`: prompts come
 the ones before (`kv_read_*`). `--sandwich`: norms with weights before and after both blocks, gates and a residual scale (`add_norm_*`).
 """
 import argparse
+import contextlib
 import math
 import sys
 
 import torch
 
 import fsw_weights
+
+MOST_ROWS = 1 << 20  # of a call
 
 
 class PagedCache:
@@ -63,6 +66,20 @@ class PagedCache:
                 slots.append(self.pages[b][t // self.page] * self.page + t % self.page)
             self.lengths[b] += n
         return self._int32(positions), self._int32(slots)
+
+    @contextlib.contextmanager
+    def growing(self, counts):
+        """grow() for the length of a block: what is raised inside, a refused call say, gives the tokens' places back, so that the cache still has the
+        tokens that it had."""
+        lengths, pages = list(self.lengths), [len(p) for p in self.pages]
+        try:
+            yield self.grow(counts)
+        except BaseException:
+            self.lengths = lengths
+            for own, n in zip(self.pages, pages):
+                while len(own) > n:
+                    self.free.append(own.pop())
+            raise
 
     def table(self):
         """(block table, lengths, longest) for attn_decode."""
@@ -147,33 +164,35 @@ class DecoderLayer:
                 raise ValueError("sequence %d has tokens in the cache already" % b)
         if cache.prefix:
             raise ValueError("prompts behind a shared prefix extend what the cache holds: extend()")
-        return self._prompts(x, lengths, *cache.grow(lengths), cache)
+        with cache.growing(lengths) as (positions, slots):
+            return self._prompts(x, lengths, positions, slots, cache)
 
     def prefill_shared(self, x, cache):
         """x: the rows of the prefix that all of the cache's sequences begin with."""
         return self._prompts(x, [cache.prefix], *cache.prefix_slots(), cache)
 
     def extend(self, x, lengths, cache):
-        """x: the packed rows of prompts that continue what the cache holds of their sequences."""
-        q, k, v = self._qkv(x)
-        positions, slots = cache.grow(lengths)
-        q = self._append(q, k, v, positions, slots, cache)[0]
-        held = [cache.prefix + n for n in cache.lengths]
-        starts = self._starts(held, x.device)
-        k, v = (self.read8 if cache.eight else self.read)(*cache.arrays, cache.whole_table(), starts, sum(held))
-        return self._finish(x, self.prompt(q, k, v, self._starts(lengths, x.device), starts, self.channels ** -0.5))
+        """x: the packed rows of prompts that continue what the cache holds of their sequences. Every sequence's tokens are packed, those of the prefix
+        once for each, so all sequences together have at most MOST_ROWS of them."""
+        with cache.growing(lengths) as (positions, slots):
+            held = [cache.prefix + n for n in cache.lengths]
+            if sum(held) > MOST_ROWS:
+                raise ValueError("%d cached tokens of all sequences together, kv_read takes %d" % (sum(held), MOST_ROWS))
+            q = self._append(*self._qkv(x), positions, slots, cache)[0]
+            starts = self._starts(held, x.device)
+            k, v = (self.read8 if cache.eight else self.read)(*cache.arrays, cache.whole_table(), starts, sum(held))
+            return self._finish(x, self.prompt(q, k, v, self._starts(lengths, x.device), starts, self.channels ** -0.5))
 
     def step(self, x, cache):
         """x: one row per sequence, its next token."""
-        q, k, v = self._qkv(x)
-        positions, slots = cache.grow([1] * x.shape[0])
-        q = self._append(q, k, v, positions, slots, cache)[0]
-        table, lengths, longest = cache.table()
-        own = (table, lengths, longest, self.channels ** -0.5)
-        if cache.prefix:
-            pages = cache._int32(cache.prefix_pages)
-            return self._finish(x, (self.shared8 if cache.eight else self.shared)(q, *cache.arrays, pages, cache.prefix, *own))
-        return self._finish(x, (self.decode8 if cache.eight else self.decode)(q, *cache.arrays, *own))
+        with cache.growing([1] * x.shape[0]) as (positions, slots):
+            q = self._append(*self._qkv(x), positions, slots, cache)[0]
+            table, lengths, longest = cache.table()
+            own = (table, lengths, longest, self.channels ** -0.5)
+            if cache.prefix:
+                pages = cache._int32(cache.prefix_pages)
+                return self._finish(x, (self.shared8 if cache.eight else self.shared)(q, *cache.arrays, pages, cache.prefix, *own))
+            return self._finish(x, (self.decode8 if cache.eight else self.decode)(q, *cache.arrays, *own))
 
 
 def run(d=1024, ff=2816, heads=16, kv_heads=4, prompts=(37, 5, 130), steps=9, page=16, dtype=torch.bfloat16, seed=0, eight=False, prefix=0, turns=1,
