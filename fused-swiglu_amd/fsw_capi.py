@@ -673,6 +673,8 @@ def add_norm(x, y=None, gate=None, post=None, pre=None, scale=1.0, eps=1e-5, x_o
     Without y: (None, norm(x) * pre). x_out=False, h=False: not computed, None."""
     import torch
     code = dtype_code(x)
+    if gate is not None and gate.dim() not in (1, 2):
+        raise FswError(E_SHAPE, "fsw: gate is [D] or [M, D]")
     rows = [t for t in (y, gate if gate is not None and gate.dim() == 2 else None) if t is not None]
     _check_operands(x, *rows)
     M, D = x.shape
