@@ -548,6 +548,12 @@ def kv_cache8(k_cache, v_cache, k_scale, v_scale):
                     _step(k_scale, 0), _step(k_scale, 1), _step(k_scale, 2))
 
 
+def _check_caches(caches, *kinds):
+    """`caches` are two tensors of the rows' type, or four of 8 bits and their scales, where `kinds` has that number."""
+    if len(caches) not in kinds:
+        raise FswError(E_SHAPE, "fsw: the caches are %s" % " or ".join({2: "(k, v)", 4: "(k, v, k_scale, v_scale)"}[n] for n in kinds))
+
+
 def _cache_of(like, caches, dtype, heads, channels):
     """A cache's structure from (k, v) or (k, v, k_scale, v_scale), checked against the rows it goes with."""
     if any(not t.is_cuda or t.device != like.device for t in caches):
@@ -564,6 +570,7 @@ def kv_append8(q, k, v, cos_sin, positions, slots, caches, interleaved=False, q_
     """Rotated q, and k and v as the cache in 8 bits holds them; `caches` is (k, v, k_scale, v_scale) (fsw_kv_append8). k_out=False,
     v_out=False: the cache only, the result is None."""
     import torch
+    _check_caches(caches, 4)
     code = dtype_code(q)
     _check_rows(q, k, v)
     _check_int32(q, positions, slots)
@@ -597,6 +604,7 @@ def kv_read(caches, block_table, cu, tokens, dtype=None, k_out=None, v_out=None)
     """Keys and values [tokens, Hkv, D] of sequences whose offsets are cu [B + 1], out of their pages (fsw_kv_read; with scales among
     `caches` fsw_kv_read8, whose results are of `dtype`)."""
     import torch
+    _check_caches(caches, 2, 4)
     eight = len(caches) == 4
     like = caches[0]
     if like.dim() != 4:
@@ -657,14 +665,16 @@ def _attend(q, caches, prefix, prefix_len, block_table, lengths, max_len, scale,
 
 def attn_decode8(q, caches, block_table, lengths, max_len, scale, out=None, workspace=None):
     """Attention of one token per sequence over the caches (k, v, k_scale, v_scale) in 8 bits (fsw_attn_decode8)."""
-    if len(caches) != 4:
-        raise FswError(E_SHAPE, "fsw: the caches are (k, v, k_scale, v_scale)")
+    _check_caches(caches, 4)
     return _attend(q, caches, None, 0, block_table, lengths, max_len, scale, out, workspace)
 
 
 def attn_shared(q, caches, prefix, prefix_len, block_table, lengths, max_len, scale, out=None, workspace=None):
     """Attention of one token per sequence over a prefix that all share, in pages prefix [n], and its own tokens, over (k, v) or
     (k, v, k_scale, v_scale) (fsw_attn_shared, fsw_attn_shared8)."""
+    _check_caches(caches, 2, 4)
+    if prefix is None:
+        raise FswError(E_NULL, "fsw: prefix is an int32 tensor of pages; without one there is attn_decode, attn_decode8")
     return _attend(q, caches, prefix, prefix_len, block_table, lengths, max_len, scale, out, workspace)
 
 
