@@ -128,11 +128,11 @@ class DecoderLayer:
 
     def _qkv(self, x):
         h = self.rms_norm(x, self.before_attn) if self.sandwich else self.norm(x)
-        rows = self.project(h, self.w_qkv).view(x.shape[0], -1, self.channels)
+        rows = self.project(h, self.w_qkv).view(x.shape[0], self.heads + 2 * self.kv_heads, self.channels)
         return rows.split([self.heads, self.kv_heads, self.kv_heads], 1)
 
     def _finish(self, x, attended):
-        y = self.project(attended.reshape(x.shape[0], -1), self.w_out)
+        y = self.project(attended.flatten(1), self.w_out)
         if self.sandwich:
             x, h = self.add_norm(x, y, self.attn_gate, self.after_attn, self.before_mlp, self.residual_scale)
             return self.add_norm(x, self.mlp(h, self.w13, self.w2), self.mlp_gate, self.after_mlp, None, self.residual_scale)[0]
@@ -199,6 +199,8 @@ def run(d=1024, ff=2816, heads=16, kv_heads=4, prompts=(37, 5, 130), steps=9, pa
         sandwich=False):
     """Largest difference, over the root mean square of the outputs, between tokens decoded one by one and the same tokens
     inside their whole sequences."""
+    if turns < 1:
+        raise ValueError("prompts come in one part at least, not in %d" % turns)
     longest = prefix + max(prompts) + steps
     layer = DecoderLayer(d, ff, heads, kv_heads, longest, dtype, seed=seed, sandwich=sandwich)
     gen = torch.Generator().manual_seed(seed + 2)

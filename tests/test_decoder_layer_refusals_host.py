@@ -83,3 +83,21 @@ def test_more_cached_rows_than_a_call_takes_are_refused_before_the_cache_grows(m
     monkeypatch.setattr(decoder_layer, "MOST_ROWS", 147)
     layer_that_fails_at(None).extend(torch.zeros(30, 64), [12, 1, 17], cache)
     assert cache.lengths == [12, 17, 22]
+
+
+@pytest.mark.parametrize("prefix", [0, 32])
+def test_no_rows_are_an_answer_of_no_rows(prefix):
+    """Prompts in more parts than the longest has tokens: some parts have none."""
+    cache, layer = new(prefix), layer_that_fails_at(None)
+    cache.grow([0, 16, 5])
+    assert layer.extend(torch.zeros(0, 64), [0, 0, 0], cache).shape == (0, 64)
+    if not prefix:
+        assert layer.prefill(torch.zeros(0, 64), [0, 0, 0], cache).shape == (0, 64)
+    assert cache.lengths == [0, 16, 5]
+
+
+@pytest.mark.parametrize("turns", [0, -1])
+def test_prompts_come_in_parts(turns):
+    """Without any, tokens would be decoded behind nothing."""
+    with pytest.raises(ValueError, match="part"):
+        decoder_layer.run(turns=turns)
