@@ -156,6 +156,7 @@ struct PrefixPlan {
   int splits, chunk, rows;  // rows: of a workgroup
 };
 PrefixPlan prefix_plan(int seqs, int hq, int hkv, int d, int len, int element_bytes);
+int prefix_rows(const PrefixPlan& p, int d, int page_size, int element_bytes);  // of a workgroup, as it is launched
 hipError_t launch_attn_prefix(int dtype, const PrefixOver<PagedKv>& a, const PrefixPlan& p, hipStream_t stream);
 hipError_t launch_attn_prefix8(int dtype, const PrefixOver<PagedKv8>& a, const PrefixPlan& p, hipStream_t stream);
 

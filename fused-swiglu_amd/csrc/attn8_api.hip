@@ -163,6 +163,13 @@ size_t shared_bytes(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, in
 }
 
 template <class CACHE>
+int shared_rows(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t prefix_len, int64_t page_size) {
+  if (Of<CACHE>::heads(dtype, Hq, Hkv, D) != FSW_OK || B < 1 || B > MAX_SEQS || prefix_len < 1 || prefix_len > MAX_LEN || page_size < 1 || page_size > MAX_LEN)
+    return 0;
+  return fsw::prefix_rows(fsw::prefix_plan((int)B, (int)Hq, (int)Hkv, (int)D, (int)prefix_len, Of<CACHE>::BYTES), (int)D, (int)page_size, Of<CACHE>::BYTES);
+}
+
+template <class CACHE>
 int attend(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, const void* Q, int64_t q_seq, int64_t q_head, const CACHE* cache,
            const int32_t* prefix_pages, int64_t prefix_len, const int32_t* block_table, int64_t table_ld, const int32_t* lengths,
            int64_t max_len, float scale, void* O, int64_t o_seq, int64_t o_head, void* workspace, size_t workspace_bytes, void* stream) {
@@ -312,6 +319,14 @@ size_t fsw_attn_shared_workspace_bytes(int dtype, int64_t B, int64_t Hq, int64_t
 
 size_t fsw_attn_shared8_workspace_bytes(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t prefix_len, int64_t max_len) {
   return shared_bytes<fsw_kv_cache8>(dtype, B, Hq, Hkv, D, prefix_len, max_len);
+}
+
+int fsw_attn_shared_rows(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t prefix_len, int64_t page_size) {
+  return shared_rows<fsw_kv_cache>(dtype, B, Hq, Hkv, D, prefix_len, page_size);
+}
+
+int fsw_attn_shared8_rows(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t prefix_len, int64_t page_size) {
+  return shared_rows<fsw_kv_cache8>(dtype, B, Hq, Hkv, D, prefix_len, page_size);
 }
 
 int fsw_attn_shared(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, const void* Q, int64_t q_seq, int64_t q_head,

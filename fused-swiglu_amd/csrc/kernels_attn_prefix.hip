@@ -458,10 +458,16 @@ hipError_t launch(const PrefixOver<CACHE>& a, const PrefixPlan& p, hipStream_t s
   return hipGetLastError();
 }
 
+// Do the keys that a wave loads at a time, 1 KB of them, lie in one page?
+bool whole_pages(int d, int page_size, int element_bytes) {
+  const int padded = d <= 64 ? 64 : d <= 128 ? 128 : 256;
+  return page_size % (1024 / (padded * element_bytes)) == 0;
+}
+
 template <class T, class CACHE, int DP>
 hipError_t launch_dp(const PrefixOver<CACHE>& a, const PrefixPlan& p, hipStream_t stream) {
-  constexpr int ROWS = 1024 / (DP * (std::is_same<CACHE, PagedKv8>::value ? 1 : 2));
-  if (a.cache.page_size % ROWS) return launch<T, CACHE, DP, 1, 4, false>(a, p, stream);
+  constexpr int BYTES = std::is_same<CACHE, PagedKv8>::value ? 1 : 2;
+  if (!whole_pages(DP, a.cache.page_size, BYTES)) return launch<T, CACHE, DP, 1, 4, false>(a, p, stream);
   if constexpr (DP == 128) {
     if (p.rows == 256) return launch<T, CACHE, DP, 2, 8, true>(a, p, stream);
   }
@@ -505,6 +511,8 @@ PrefixPlan prefix_plan(int seqs, int hq, int hkv, int d, int len, int element_by
   }
   return best;
 }
+
+int prefix_rows(const PrefixPlan& p, int d, int page_size, int element_bytes) { return whole_pages(d, page_size, element_bytes) ? p.rows : 64; }
 
 hipError_t launch_attn_prefix(int dtype, const PrefixOver<PagedKv>& a, const PrefixPlan& p, hipStream_t stream) {
   return dtype == FSW_BF16 ? launch_typed<Bf16>(a, p, stream) : launch_typed<Fp16>(a, p, stream);

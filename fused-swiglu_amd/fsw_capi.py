@@ -76,6 +76,8 @@ PROTOTYPES = {
     "fsw_validate_attn_shared8": (_i, [_i] + [_i64] * 4 + _rows + [_kvp8, _vp, _i64, _vp, _i64, _vp, _i64, _f] + _rows),
     "fsw_attn_shared_workspace_bytes": (_sz, [_i] + [_i64] * 6),
     "fsw_attn_shared8_workspace_bytes": (_sz, [_i] + [_i64] * 6),
+    "fsw_attn_shared_rows": (_i, [_i] + [_i64] * 6),
+    "fsw_attn_shared8_rows": (_i, [_i] + [_i64] * 6),
     "fsw_attn_shared": (_i, [_i] + [_i64] * 4 + _rows + [_kvp, _vp, _i64, _vp, _i64, _vp, _i64, _f] + _rows + [_vp, _sz, _vp]),
     "fsw_attn_shared8": (_i, [_i] + [_i64] * 4 + _rows + [_kvp8, _vp, _i64, _vp, _i64, _vp, _i64, _f] + _rows + [_vp, _sz, _vp]),
     "fsw_validate_add_norm": (_i, [_i, _i64, _i64] + [_vp, _i64] * 3 + [_vp, _vp, _f, _f] + [_vp, _i64] * 2),

@@ -369,6 +369,12 @@ FSW_API int fsw_attn_shared8(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int6
                              int64_t table_ld, const int32_t* lengths, int64_t max_len, float scale, void* O, int64_t o_seq,
                              int64_t o_head, void* workspace, size_t workspace_bytes, void* stream);
 
+/* Rows, (sequence, query head of a key-value head) pairs, of a workgroup over the prefix of fsw_attn_shared (fsw_attn_shared8): 64, 128 or 256 by the plan of
+ * least estimated time, but 64 where the page size is no multiple of the keys that a wave loads at a time; 0 for what is refused or where there is no prefix. For
+ * tests and benchmarks. */
+FSW_API int fsw_attn_shared_rows(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t prefix_len, int64_t page_size);
+FSW_API int fsw_attn_shared8_rows(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, int64_t prefix_len, int64_t page_size);
+
 /* Host-only validation of fsw_add_norm. M <= 2^30; D a multiple of 8 up to 32768; leading dimensions multiples of 8, those of results at least D, pointers
  * 16-byte aligned; scale finite, eps a positive normal number. */
 FSW_API int fsw_validate_add_norm(int dtype, int64_t M, int64_t D, const void* X, int64_t ldx, const void* Y, int64_t ldy, const void* gate,
@@ -391,7 +397,8 @@ FSW_API int fsw_last_hip_error(void);
 
 /* ABI version: major * 1000 + minor. 2000: the measurement kernels fsw_probe_* left this library (libfsw_probe.so,
  * fsw_probe.h); fsw_gateup_f32out and fsw_gateup_hblocked joined it; fsw_gateup_workspace_bytes returns 0. 2001: the attention
- * entry points. 2002: fsw_attn_prompt_rows. 2003: the cache in 8 bits, fsw_kv_read, fsw_attn_shared, fsw_add_norm. */
+ * entry points. 2002: fsw_attn_prompt_rows. 2003: the cache in 8 bits, fsw_kv_read, fsw_attn_shared, fsw_add_norm. 2004:
+ * fsw_attn_shared_rows, fsw_attn_shared8_rows. */
 FSW_API int fsw_version(void);
 
 /*
