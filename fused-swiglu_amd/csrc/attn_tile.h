@@ -2,6 +2,7 @@
 // prefixes).
 #pragma once
 #include <hip/hip_runtime.h>
+#include <math.h>
 
 #include "attn.h"
 #include "attn_device.h"
@@ -34,6 +35,19 @@ float shift_of<Fp16>(int) {
   return 11.0f;
 }
 constexpr int KEYS = 64;       // of a tile
+
+// Both limits in units of the scores, for scores that weigh 2^(c s): m is set `lower` below a score, and moves when one is `limit` above it. Bounded, since the least
+// c would make them infinite, and no row would have a maximum; what the bound takes from a shift, `rest` gives back to the exponent: a weight is 2^(c s - (c m + rest)).
+struct Limits {
+  float lower, limit, rest;
+};
+template <class T>
+Limits limits_of(int keys, float c) {
+  const float shift = shift_of<T>(keys), most = 0x1p96f;  // below what the largest score is rounded to
+  const auto bounded = [&](float x) { return fminf(fmaxf(x, -most), most); };
+  const float lower = bounded(shift / c);
+  return {lower, bounded((shift + SLACK<T>) / c), fabsf(lower) < most ? 0.0f : lower * c - shift};
+}
 
 #define INLINE __attribute__((always_inline))
 

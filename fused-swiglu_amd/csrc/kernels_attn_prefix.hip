@@ -79,7 +79,7 @@ __device__ __forceinline__ Scales scales_of(const PagedKv&) { return {nullptr, n
 // WHOLE: the rows of a wave's load, ROWS of them, lie in one page, whose address is wave-uniform then.
 template <class T, class CACHE, int DP, int NB, int WAVES, bool WHOLE>
 __global__ __launch_bounds__(64 * WAVES, DP == 256 && WAVES == 4 ? 1 : 2) void attn_prefix_kernel(PrefixOver<CACHE> a, Divisor by_group, Divisor by_hkv, int chunk,
-                                                                                     float lower, float limit) {
+                                                                                     Limits limits) {
   constexpr bool EIGHT = std::is_same<CACHE, PagedKv8>::value, STAGED = EIGHT || !WHOLE;
   constexpr int RB = DP * 2, TILE = KEYS * RB;
   constexpr int SIZE = EIGHT ? 1 : 2, PER_ROW = DP * SIZE / 16, ROWS = 64 / PER_ROW;  // 16-byte vectors of a row, rows of a wave's load
@@ -287,11 +287,11 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 && WAVES == 4 ? 1 : 2) void a
     }
     maximum_over_groups(top);
 #pragma unroll
-    for (int n = 0; n < NB; ++n) above |= top[n] > m[n] + limit;
+    for (int n = 0; n < NB; ++n) above |= top[n] > m[n] + limits.limit;
     if (__any(above)) {
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
-        const float now = fmaxf(m[n], top[n] - lower);
+        const float now = fmaxf(m[n], top[n] - limits.lower);
         const float alpha = now == m[n] ? 1.0f : __builtin_amdgcn_exp2f((m[n] - now) * c);
         m[n] = now;
         sum[n] *= alpha;
@@ -303,7 +303,7 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 && WAVES == 4 ? 1 : 2) void a
     }
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
-      const float mc = m[n] == NEG_INF ? 0.0f : m[n] * c;
+      const float mc = m[n] == NEG_INF ? 0.0f : __builtin_fmaf(m[n], c, limits.rest);
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -413,7 +413,7 @@ __global__ __launch_bounds__(64 * WAVES, DP == 256 && WAVES == 4 ? 1 : 2) void a
     if (row >= rows) continue;
     const long long at = out_row(row);
     if (grp == 0) {
-      ml[2 * at] = m[n] * c;
+      ml[2 * at] = __builtin_fmaf(m[n], c, limits.rest);
       ml[2 * at + 1] = bad ? __builtin_nanf("") : total;
     }
 #pragma unroll
@@ -449,12 +449,8 @@ template <class T, class CACHE, int DP, int NB, int WAVES, bool WHOLE>
 hipError_t launch(const PrefixOver<CACHE>& a, const PrefixPlan& p, hipStream_t stream) {
   constexpr int BM = 16 * NB * WAVES;
   const int group = a.hq / a.hkv;
-  const float shift = shift_of<T>(a.keys);
-  // in units of the scores; finite for the least scales too, or no share would have a maximum to be joined by
-  auto bounded = [](float x) { return fminf(fmaxf(x, -FLT_MAX / 4), FLT_MAX / 4); };
-  const float lower = bounded(shift / a.scale_log2), limit = bounded((shift + SLACK<T>) / a.scale_log2);
   const dim3 grid(a.hkv * ((a.seqs * group + BM - 1) / BM), p.splits);
-  attn_prefix_kernel<T, CACHE, DP, NB, WAVES, WHOLE><<<grid, 64 * WAVES, 0, stream>>>(a, Divisor(group), Divisor(a.hkv), p.chunk, lower, limit);
+  attn_prefix_kernel<T, CACHE, DP, NB, WAVES, WHOLE><<<grid, 64 * WAVES, 0, stream>>>(a, Divisor(group), Divisor(a.hkv), p.chunk, limits_of<T>(a.keys, a.scale_log2));
   return hipGetLastError();
 }
 
