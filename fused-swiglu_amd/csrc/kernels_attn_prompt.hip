@@ -25,8 +25,6 @@
 // keys and values copied one and a half turns ahead with a barrier more (1162), wave priorities (1136), eight waves on every other tile of
 // the same rows (1243). Limits in units of the scores come divided from the host: in the kernel they are vector registers, of which 256 channels have
 // none left (4000 tokens of fp16 234 us against 204).
-#include <float.h>
-
 #include "attn.h"
 #include "attn_device.h"
 #include "attn_tile.h"
@@ -38,7 +36,7 @@ namespace {
 
 template <class T, int DP, int NB>
 __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prompt_kernel(PromptArgs a, Divisor by_group, Divisor by_hkv,
-                                                                                  int slots, float lower, float limit) {
+                                                                                  int slots, Limits limits) {
   constexpr int RB = DP * 2, TILE = KEYS * RB, LOADS = TILE / 4096;  // copies per wave and tile
   constexpr int KSTEPS = DP / 32, DB = DP / 16, KB = KEYS / 16, WM = 16 * NB, BM = 4 * WM;
   // Fragments of keys and values are read ahead of the matrix instructions that take them, a block of 16 keys and four value fragments
@@ -189,12 +187,12 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prompt_kernel(Pro
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb) t[kb] = fmaxf(fmaxf(s[kb][n][0], s[kb][n][1]), fmaxf(s[kb][n][2], s[kb][n][3]));
       top[n] = max_over_groups(fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3])));
-      above |= top[n] > m[n] + limit;
+      above |= top[n] > m[n] + limits.limit;
     }
     if (__any(above)) {
 #pragma unroll
       for (int n = 0; n < NB; ++n) {
-        const float now = fmaxf(m[n], top[n] - lower);
+        const float now = fmaxf(m[n], top[n] - limits.lower);
         const float alpha = now == m[n] ? 1.0f : __builtin_amdgcn_exp2f((m[n] - now) * c);
         m[n] = now;
         sum[n] *= alpha;
@@ -207,7 +205,7 @@ __global__ __launch_bounds__(256, DP == 256 ? 1 : 2) void attn_prompt_kernel(Pro
     unsigned p[NB][KB][2];
 #pragma unroll
     for (int n = 0; n < NB; ++n) {
-      const float mc = m[n] == NEG_INF ? 0.0f : m[n] * c;
+      const float mc = m[n] == NEG_INF ? 0.0f : __builtin_fmaf(m[n], c, limits.rest);
 #pragma unroll
       for (int kb = 0; kb < KB; ++kb)
 #pragma unroll
@@ -335,11 +333,9 @@ template <class T, int DP, int NB>
 hipError_t launch(const PromptArgs& a, hipStream_t stream) {
   const long long rows = (long long)a.tq * (a.hq / a.hkv);
   const long long slots = rows / (64 * NB) + a.seqs + 1;
-  // (the smallest scales do without: a score that is no finite number is none)
-  const float shift = shift_of<T>(a.tk), lower = fmaxf(shift / a.scale_log2, -FLT_MAX / 4), limit = fmaxf((shift + SLACK<T>) / a.scale_log2, -FLT_MAX / 4);
   const long long blocks = slots * a.hkv, most = 1 << 22;  // a launch has less than 2^32 threads along x
   const dim3 grid((unsigned)(blocks < most ? blocks : most), (unsigned)((blocks + most - 1) / most));
-  attn_prompt_kernel<T, DP, NB><<<grid, 256, 0, stream>>>(a, Divisor(a.hq / a.hkv), Divisor(a.hkv), (int)slots, lower, limit);
+  attn_prompt_kernel<T, DP, NB><<<grid, 256, 0, stream>>>(a, Divisor(a.hq / a.hkv), Divisor(a.hkv), (int)slots, limits_of<T>(a.tk, a.scale_log2));
   return hipGetLastError();
 }
 

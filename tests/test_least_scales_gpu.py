@@ -50,3 +50,24 @@ def test_shared_of_scores_as_large_as_a_float_holds(capi):
     out = capi.attn_shared(q.to(DEV), [c.to(DEV) for c in cache], pages.to(DEV), prefix, table.to(DEV), int32([5, 0]), 5, 1.2e-38).cpu().double()
     ref, mag = reference(q, rows, pages, prefix, table, [5, 0], 16, 1.2e-38)
     assert ((out - ref).abs() <= attention.tolerance(ref, mag, BF, True, 133)).all()
+
+
+@pytest.mark.parametrize("scale", SCALES)
+@pytest.mark.parametrize("dtype,size", [(BF, 3.0e38), (HF, 65504.0)])
+@pytest.mark.parametrize("n,Hq,D", [(300, 4, 64), (900, 8, 128), (200, 2, 256)])
+def test_prompts_of_values_as_large_as_the_type_has(capi, n, Hq, D, dtype, size, scale):
+    gen = torch.Generator().manual_seed(n)
+    q, k = (randn(gen, n, h, D, dtype=dtype).to(DEV) for h in (Hq, 1))
+    out = capi.attn_prompt(q, k, torch.full_like(k, size), int32([0, n]), int32([0, n]), scale).cpu().double()
+    assert torch.isfinite(out).all() and ((out - size).abs() <= 2.0 ** -6 * size).all()
+
+
+@pytest.mark.parametrize("scale", SCALES)
+@pytest.mark.parametrize("dtype", [BF, HF])
+def test_prompts_are_means(capi, dtype, scale):
+    gen = torch.Generator().manual_seed(2)
+    cu = [0, 1, 70, 200]
+    q, k, v = (randn(gen, 200, h, 64, dtype=dtype) for h in (4, 2, 2))
+    out = capi.attn_prompt(q.to(DEV), k.to(DEV), v.to(DEV), int32(cu), int32(cu), scale)
+    ref, mag = attention.prompt(q, k, v, cu, cu, scale)
+    assert ((out.cpu().double() - ref).abs() <= attention.tolerance(ref, mag, dtype, True, 130)).all()
