@@ -140,7 +140,11 @@ class DecoderLayer:
         return x + self.mlp(self.norm(x), self.w13, self.w2)
 
     def _append(self, q, k, v, positions, slots, cache):
-        """Rotated queries, and keys and values as later tokens will see them."""
+        """Rotated queries, and keys and values as later tokens will see them. Own tokens' positions go on behind the prefix's: a cache for as many tokens as
+        the layer has angles, and a prefix beside them, would come to positions that have none, and keys that are NaN."""
+        reach = cache.prefix + max(cache.lengths)
+        if reach > self.cos_sin.shape[0]:
+            raise ValueError("%d tokens in a row, the layer was made for %d" % (reach, self.cos_sin.shape[0]))
         if cache.eight:
             return self.append8(q, k, v, self.cos_sin, positions, slots, *cache.arrays)
         return (*self.append(q, k, v, self.cos_sin, positions, slots, cache.k, cache.v), v)

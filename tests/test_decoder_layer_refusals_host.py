@@ -12,7 +12,7 @@ class Refused(RuntimeError):
 def layer_that_fails_at(name):
     """A layer whose operator `name` refuses its call; the others return rows of the right sizes."""
     layer = decoder_layer.DecoderLayer.__new__(decoder_layer.DecoderLayer)
-    layer.heads, layer.kv_heads, layer.channels, layer.sandwich, layer.cos_sin = 4, 2, 16, False, None
+    layer.heads, layer.kv_heads, layer.channels, layer.sandwich, layer.cos_sin = 4, 2, 16, False, torch.zeros(69, 16)
     layer.w_qkv, layer.w_out, layer.w13, layer.w2 = (torch.zeros(n, 64) for n in (128, 64, 8, 64))
 
     def stand_in(op, result):
@@ -101,3 +101,20 @@ def test_prompts_come_in_parts(turns):
     """Without any, tokens would be decoded behind nothing."""
     with pytest.raises(ValueError, match="part"):
         decoder_layer.run(turns=turns)
+
+
+def test_positions_behind_a_prefix_have_angles():
+    """The cache was made for 37 tokens behind 32, the layer for 40 in a row: refused, not NaN."""
+    cache, layer = new(32), layer_that_fails_at(None)
+    layer.cos_sin = torch.zeros(40, 16)
+    layer.extend(torch.zeros(7, 64), [7, 0, 0], cache)
+    before = state(cache)
+    assert layer.step(torch.zeros(3, 64), cache).shape == (3, 64)
+    with pytest.raises(ValueError, match="made for 40"):
+        layer.step(torch.zeros(3, 64), cache)
+    with pytest.raises(ValueError, match="made for 40"):
+        layer.extend(torch.zeros(9, 64), [0, 0, 9], cache)
+    assert cache.lengths == [8, 1, 1] and before[0] == [7, 0, 0]
+    layer.cos_sin = torch.zeros(31, 16)
+    with pytest.raises(ValueError, match="made for 31"):
+        layer.prefill_shared(torch.zeros(32, 64), new(32))
