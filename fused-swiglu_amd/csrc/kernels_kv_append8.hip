@@ -10,7 +10,8 @@
 // the cache: 2^n threads, the least that hold the head, are a group that finds its largest element by lane exchanges. Where halves of a head are
 // turned into each other a thread's channels are two times 8, partners of each other; halves of 4 channels more than that find partners in memory, 4 at a time, and others
 // one by one. Measured: one token of 32 + 8 heads of 128 channels 4.2 .. 5.2 us, 8192 tokens of 64 + 8 74 us (4.8 TB/s, half of it written; a copy reaches 4.9), of
-// 32 + 8 51 us; of 80 channels, all rotated, 41 us, half of them 53 (one by one 110), interleaved or in halves alike. Loads are non-temporal where heads are whole
+// 32 + 8 51 us; of 80 channels, all rotated, 41 us, half of them 53 (one by one 110), interleaved or in halves alike (floors 28; five of a head's eight threads have
+// channels, and halves of 4 more are read twice). Loads are non-temporal where heads are whole
 // lines (64 + 8 heads of 128 channels 76 | 81 us, 32 + 8 of 256 89 | 98), and not where lines are shared (of 80 44 | 41, of 96 47 | 45, of 112, half rotated, 69 | 61).
 #include <float.h>
 

@@ -6,7 +6,8 @@
 // keeps it in registers between the two sums, so the row is never read again; workgroups of many rows keep the weights of
 // their channels in registers as well. Squares are summed in 64 bits: they are exact there and neither overflow nor vanish for any values that the types
 // have, and beside the memory traffic they cost nothing. Measured, both norms: 8192 rows of 8192 channels with a gate of their own 130 us (5.2 TB/s, two fifths of it written; a
-// copy reaches 4.9), of 4096 with one gate for all 49 (5.5), of 1024 17 (3.9); 2048 of 16384 66 (4.1); one row of 4096 3.4 us on the device.
+// copy reaches 4.9), of 4096 with one gate for all 49 (5.5), of 1024 17 (3.9); 2048 of 16384 66 (4.1: bf16 holds 130 registers there, so a CU has one
+// workgroup of eight waves, not two; of 1024 half of the threads have nothing to do); one row of 4096 3.4 us on the device.
 #include "attn_device.h"
 #include "fsw.h"
 #include "fsw_device.h"
@@ -170,6 +171,7 @@ hipError_t launch(const NormArgs& a, hipStream_t stream) {
   return hipGetLastError();
 }
 
+// The least form that holds a row: one vector a thread up to 256 threads, then up to four of 256 threads, and more threads beyond.
 template <class T>
 hipError_t launch_typed(const NormArgs& a, hipStream_t stream) {
   const int vecs = a.d / 8;

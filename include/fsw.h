@@ -238,7 +238,8 @@ FSW_API size_t fsw_attn_decode_workspace_bytes(int dtype, int64_t B, int64_t Hq,
  * that hold 16 bits (bf16) or 22 (fp16) of them, one rounding. max_len: the host's bound of the lengths, which sets
  * the launch's shape. A length of 0 gives zeros; a length below 0 or above max_len, or a page outside the cache among a sequence's pages, gives NaN for that
  * sequence. What the cache holds behind a length is never used. Every key before it weighs more than nothing: an infinity among their values gives that
- * infinity, both signs or a NaN give NaN, in their channel. Finite values give finite sums, however large they are.
+ * infinity, both signs or a NaN give NaN, in their channel. Finite values give finite sums, however large they are; in bf16 a weight
+ * below 2^-88 of the largest may count as none or as that much, which values 2^80 times as large as the result would show.
  */
 FSW_API int fsw_attn_decode(int dtype, int64_t B, int64_t Hq, int64_t Hkv, int64_t D, const void* Q, int64_t q_seq, int64_t q_head,
                             const fsw_kv_cache* cache, const int32_t* block_table, int64_t table_ld, const int32_t* lengths,
